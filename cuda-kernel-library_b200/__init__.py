@@ -295,6 +295,136 @@ def stream_copy(dst, src, nbytes: int, stream=None) -> None:
     _check(_lib.ckl_stream_copy(_ptr(dst), _ptr(src), nbytes, _stream(stream)))
 
 
+# --- products whose weight is chosen per row: experts and low-rank adapters -------------------
+
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
+
+_ll, _sz = ctypes.c_longlong, ctypes.c_size_t
+_lib.ckl_group_rows.argtypes = [_vp, _i, _i, _i, _vp, _vp, _vp, _vp]
+_lib.ckl_moe_route.argtypes = [_i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _vp]
+_lib.ckl_moe_route_backward.argtypes = [_i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp]
+_lib.ckl_gemm_grouped.argtypes = [_i, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _ll, _i, _i,
+                                  _f, _f, _vp]
+_lib.ckl_gemm_grouped_wgrad.argtypes = [_i, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _ll,
+                                        _f, _f, _vp]
+_lib.ckl_moe_combine.argtypes = [_i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]
+_lib.ckl_moe_combine_backward.argtypes = [_i, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i,
+                                          _vp]
+_lib.ckl_gemm_lora_workspace_bytes.argtypes = [_i, _i, _i]
+_lib.ckl_gemm_lora.argtypes = [_i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i,
+                               _ll, _i, _ll, _i, _f, _vp, _sz, _vp]
+_lib.ckl_gemm_lora_backward.argtypes = [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _vp, _i,
+                                        _i, _i, _i, _i, _i, _i, _i, _i, _ll, _i, _ll, _i, _i, _ll, _i, _ll, _f,
+                                        _vp, _sz, _vp]
+for _name in ("ckl_group_rows", "ckl_moe_route", "ckl_moe_route_backward", "ckl_gemm_grouped",
+              "ckl_gemm_grouped_wgrad", "ckl_moe_combine", "ckl_moe_combine_backward", "ckl_gemm_lora",
+              "ckl_gemm_lora_backward"):
+    getattr(_lib, _name).restype = ctypes.c_int
+_lib.ckl_gemm_lora_workspace_bytes.restype = _sz
+
+
+def group_rows(ids, slots, groups, offsets, rows, positions, slots_per_row=1, stream=None) -> None:
+    """Stable order of ``slots`` int32 group ids: ``offsets`` (groups + 1), ``rows`` and ``positions``
+    (slots each), all int32 on the device.  Ids outside [0, groups) come last."""
+    _check(_lib.ckl_group_rows(_ptr(ids), slots, groups, slots_per_row, _ptr(offsets), _ptr(rows),
+                               _ptr(positions), _stream(stream)))
+
+
+def moe_route(logit_dtype, logits, weights, experts, tokens, n_experts, top_k, ldl=None, bias=None,
+              score=SCORE_SOFTMAX, groups=1, top_groups=1, renormalise=False, scale=1.0, stream=None) -> None:
+    """top_k experts (int32) and weights (FP32), tokens x top_k, for each row of logits."""
+    _check(_lib.ckl_moe_route(logit_dtype, _ptr(logits), n_experts if ldl is None else ldl, _ptr(bias),
+                              _ptr(weights), _ptr(experts), tokens, n_experts, top_k, score, groups, top_groups,
+                              1 if renormalise else 0, scale, _stream(stream)))
+
+
+def moe_route_backward(logit_dtype, logits, experts, dweights, dlogits, tokens, n_experts, top_k, ldl=None,
+                       ldd=None, score=SCORE_SOFTMAX, renormalise=False, scale=1.0, stream=None) -> None:
+    """dlogits (the logits' type) from the gradient of moe_route's weights."""
+    _check(_lib.ckl_moe_route_backward(logit_dtype, _ptr(logits), n_experts if ldl is None else ldl,
+                                       _ptr(experts), _ptr(dweights), _ptr(dlogits),
+                                       n_experts if ldd is None else ldd, tokens, n_experts, top_k, score,
+                                       1 if renormalise else 0, scale, _stream(stream)))
+
+
+def gemm_grouped(ab_dtype, a, b, c, c_dtype, offsets, groups, rows, n, k, lda=None, ldb=None, ldc=None,
+                 stride_b=None, a_rows=None, a_count=None, trans_b=False, alpha=1.0, beta=0.0,
+                 stream=None) -> None:
+    """C[p] = alpha * A[a_rows[p]] * op(B_g) + beta * C[p] for the positions p of each group g."""
+    if a_rows is not None and a_count is None:
+        raise ValueError("gemm_grouped: a_rows needs a_count, the number of rows of a")
+    ldb = (k if trans_b else n) if ldb is None else ldb
+    _check(_lib.ckl_gemm_grouped(ab_dtype, _ptr(a), _ptr(a_rows), rows if a_count is None else a_count, _ptr(b),
+                                 _ptr(c), c_dtype, _ptr(offsets), groups, rows, n, k, k if lda is None else lda,
+                                 ldb, ldb * (n if trans_b else k) if stride_b is None else stride_b,
+                                 n if ldc is None else ldc, 1 if trans_b else 0, alpha, beta, _stream(stream)))
+
+
+def gemm_grouped_wgrad(ab_dtype, a, g, dw, dw_dtype, offsets, groups, rows, m, n, lda=None, ldg=None, lddw=None,
+                       stride_dw=None, a_rows=None, a_count=None, alpha=1.0, beta=0.0, stream=None) -> None:
+    """dW_g = alpha * sum over group g of A[a_rows[p]]^T G[p] + beta * dW_g (each m x n)."""
+    if a_rows is not None and a_count is None:
+        raise ValueError("gemm_grouped_wgrad: a_rows needs a_count, the number of rows of a")
+    lddw = n if lddw is None else lddw
+    _check(_lib.ckl_gemm_grouped_wgrad(ab_dtype, _ptr(a), _ptr(a_rows), rows if a_count is None else a_count,
+                                       _ptr(g), _ptr(dw), dw_dtype, _ptr(offsets), groups, rows, m, n,
+                                       m if lda is None else lda, n if ldg is None else ldg, lddw,
+                                       lddw * m if stride_dw is None else stride_dw, alpha, beta,
+                                       _stream(stream)))
+
+
+def moe_combine(y_dtype, y, positions, weights, out, out_dtype, tokens, top_k, n, y_rows, ldy=None, ldo=None,
+                stream=None) -> None:
+    """out[t] = sum_j weights[t][j] * y[positions[t][j]]."""
+    _check(_lib.ckl_moe_combine(y_dtype, _ptr(y), _ptr(positions), _ptr(weights), _ptr(out), out_dtype, tokens,
+                                top_k, n, y_rows, n if ldy is None else ldy, n if ldo is None else ldo,
+                                _stream(stream)))
+
+
+def moe_combine_backward(y_dtype, y, positions, weights, dout, dout_dtype, dy, dweights, tokens, top_k, n,
+                         y_rows, ldy=None, ldo=None, lddy=None, stream=None) -> None:
+    """dy (y's type) and dweights (FP32) from the gradient of moe_combine's output."""
+    _check(_lib.ckl_moe_combine_backward(y_dtype, _ptr(y), _ptr(positions), _ptr(weights), _ptr(dout), dout_dtype,
+                                         _ptr(dy), _ptr(dweights), tokens, top_k, n, y_rows,
+                                         n if ldy is None else ldy, n if ldo is None else ldo,
+                                         n if lddy is None else lddy, _stream(stream)))
+
+
+def gemm_lora_workspace_bytes(m: int, rank: int, backward: bool = False) -> int:
+    """Bytes of the workspace of gemm_lora, or of gemm_lora_backward."""
+    return int(_lib.ckl_gemm_lora_workspace_bytes(m, rank, 1 if backward else 0))
+
+
+def gemm_lora(ab_dtype, x, w, lora_a, lora_b, scales, y, y_dtype, offsets, rows, adapters, m, n, k, rank,
+              workspace, workspace_bytes, ldx=None, ldw=None, ldla=None, stride_a=None, ldlb=None, stride_b=None,
+              ldy=None, beta=0.0, stream=None) -> None:
+    """y[i] = x[i] W + scales[g] * (x[i] A_g) B_g + beta * y[i], g the adapter of row i (or none).
+    ``offsets`` and ``rows`` are group_rows of the rows' adapter ids."""
+    ldla, ldlb = rank if ldla is None else ldla, n if ldlb is None else ldlb
+    _check(_lib.ckl_gemm_lora(ab_dtype, _ptr(x), _ptr(w), _ptr(lora_a), _ptr(lora_b), _ptr(scales), _ptr(y),
+                              y_dtype, _ptr(offsets), _ptr(rows), adapters, m, n, k, rank,
+                              k if ldx is None else ldx, n if ldw is None else ldw, ldla,
+                              ldla * k if stride_a is None else stride_a, ldlb,
+                              ldlb * rank if stride_b is None else stride_b, n if ldy is None else ldy, beta,
+                              _ptr(workspace), workspace_bytes, _stream(stream)))
+
+
+def gemm_lora_backward(ab_dtype, dy, x, w, lora_a, lora_b, scales, dx, dx_dtype, da, db, dab_dtype, offsets, rows,
+                       adapters, m, n, k, rank, workspace, workspace_bytes, lddy=None, ldx=None, ldw=None,
+                       ldla=None, stride_a=None, ldlb=None, stride_b=None, lddx=None, ldda=None, stride_da=None,
+                       lddb=None, stride_db=None, beta=0.0, stream=None) -> None:
+    """dx, da and db (any may be None) of gemm_lora with a frozen W; beta applies to da and db."""
+    ldla, ldlb = rank if ldla is None else ldla, n if ldlb is None else ldlb
+    ldda, lddb = rank if ldda is None else ldda, n if lddb is None else lddb
+    _check(_lib.ckl_gemm_lora_backward(
+        ab_dtype, _ptr(dy), _ptr(x), _ptr(w), _ptr(lora_a), _ptr(lora_b), _ptr(scales), _ptr(dx), dx_dtype, _ptr(da),
+        _ptr(db), dab_dtype, _ptr(offsets), _ptr(rows), adapters, m, n, k, rank, n if lddy is None else lddy,
+        k if ldx is None else ldx, n if ldw is None else ldw, ldla, ldla * k if stride_a is None else stride_a,
+        ldlb, ldlb * rank if stride_b is None else stride_b, k if lddx is None else lddx, ldda,
+        ldda * k if stride_da is None else stride_da, lddb, lddb * rank if stride_db is None else stride_db, beta,
+        _ptr(workspace), workspace_bytes, _stream(stream)))
+
+
 # --- several GPUs of one box: communicator, host-buffer sharded GEMM, gathered GEMM -----------
 
 COMM_ID_BYTES = 128

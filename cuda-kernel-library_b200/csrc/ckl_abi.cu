@@ -616,6 +616,66 @@ int get_workspace(DeviceCtx* ctx, cudaStream_t stream, size_t bytes, float** slo
     return CKL_OK;
 }
 
+}  // namespace
+
+namespace ckl {
+
+int device_view(DeviceView* out) {
+    DeviceCtx* ctx = nullptr;
+    if (const int rc = get_ctx(&ctx); rc != CKL_OK) {
+        return rc;
+    }
+    out->device = ctx->device;
+    out->sm_count = ctx->sm_count;
+    out->status = ctx->status;
+    return CKL_OK;
+}
+
+int encode_operand(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uint64_t outer,
+                   uint64_t pitch, uint64_t depth, uint64_t stack, uint32_t box_inner,
+                   uint32_t box_outer) {
+    std::memset(map, 0, sizeof *map);
+    if (inner == 0 || outer == 0) {
+        return CKL_OK;
+    }
+    DeviceCtx* ctx = nullptr;
+    if (const int rc = get_ctx(&ctx); rc != CKL_OK) {
+        return rc;
+    }
+    g_tensor_map_encodes.fetch_add(1, std::memory_order_relaxed);
+    const cuuint32_t rank = depth == 0 ? 2 : 3;
+    const cuuint64_t dims[3] = {inner, outer, depth};
+    const cuuint64_t strides[2] = {pitch * 2, stack * 2};
+    const cuuint32_t box[3] = {box_inner, box_outer, 1};
+    const cuuint32_t elem_strides[3] = {1, 1, 1};
+    const CUresult r = ctx->encode(
+        map, dtype == CKL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
+        const_cast<void*>(base), dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        return fail(CKL_ERR_CUDA,
+                    "cuTensorMapEncodeTiled failed with CUresult %d (base=%p dims=%llu x %llu x %llu "
+                    "pitch=%llu stack=%llu box=%u x %u)",
+                    static_cast<int>(r), base, static_cast<unsigned long long>(inner),
+                    static_cast<unsigned long long>(outer), static_cast<unsigned long long>(depth),
+                    static_cast<unsigned long long>(pitch), static_cast<unsigned long long>(stack),
+                    box_inner, box_outer);
+    }
+    return CKL_OK;
+}
+
+int take_wait_fault(unsigned long long* limit_ns) {
+    const WaitFault fault = g_wait_fault;
+    g_wait_fault = WaitFault{};
+    *limit_ns = fault.limit_ns;
+    return fault.kind;
+}
+
+}  // namespace ckl
+
+namespace {
+
 // ---- launches --------------------------------------------------------------------
 
 template <int kMode, typename OutT>

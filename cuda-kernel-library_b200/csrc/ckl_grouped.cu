@@ -1,0 +1,496 @@
+// C entry points of the products whose weight is chosen per row (gemm_grouped.cuh): experts'
+// products with their gradients, and low-rank adapters beside a shared projection.
+
+#include <algorithm>
+#include <cstring>
+#include <mutex>
+
+#include "ckl_gemm.h"
+#include "ckl_internal.h"
+#include "gemm_grouped.cuh"
+
+namespace {
+
+using namespace ckl;
+
+#define GRP_TRY_CUDA(expr)                                                                  \
+    do {                                                                                    \
+        const cudaError_t err__ = (expr);                                                   \
+        if (err__ != cudaSuccess) {                                                         \
+            return set_error(CKL_ERR_CUDA, "%s failed: %s (%s)", #expr,                     \
+                             cudaGetErrorName(err__), cudaGetErrorString(err__));           \
+        }                                                                                   \
+    } while (0)
+#define GRP_TRY(expr)                                       \
+    do {                                                    \
+        if (const int rc__ = (expr); rc__ != CKL_OK) {      \
+            return rc__;                                    \
+        }                                                   \
+    } while (0)
+
+int size_of(int dtype) { return dtype == CKL_F32 ? 4 : 2; }
+bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
+
+// An operand that TMA reads: base on 16 bytes, pitch and stack distance multiples of 8 elements.
+int check_operand(const char* what, const char* name, const void* ptr, int pitch, int columns,
+                  long long stack) {
+    if (ptr == nullptr || pitch < columns || pitch < 1 || stack < 0) {
+        return set_error(CKL_ERR_INVALID_ARG, "%s: %s is %p, leading dimension %d for %d columns, stride %lld",
+                         what, name, ptr, pitch, columns, stack);
+    }
+    if (misaligned(ptr, 16) || pitch % 8 != 0 || stack % 8 != 0) {
+        return set_error(CKL_ERR_UNSUPPORTED,
+                         "%s: %s must be 16-byte aligned with a leading dimension (%d) and a stride (%lld) "
+                         "that are multiples of 8 elements",
+                         what, name, pitch, stack);
+    }
+    return CKL_OK;
+}
+
+int check_types(const char* what, int ab_dtype, int c_dtype) {
+    if ((ab_dtype != CKL_F16 && ab_dtype != CKL_BF16) ||
+        (c_dtype != CKL_F32 && c_dtype != CKL_F16 && c_dtype != CKL_BF16)) {
+        return set_error(CKL_ERR_INVALID_ARG, "%s: bad dtype %d or %d", what, ab_dtype, c_dtype);
+    }
+    return CKL_OK;
+}
+
+int check_groups(const char* what, const int* offsets, int groups, int rows) {
+    if (groups < 1 || rows < 0 || offsets == nullptr || misaligned(offsets, 4)) {
+        return set_error(CKL_ERR_INVALID_ARG, "%s: offsets %p of %d groups, %d rows", what,
+                         static_cast<const void*>(offsets), groups, rows);
+    }
+    if (groups > kMaxGemmGroups) {
+        return set_error(CKL_ERR_TOO_LARGE, "%s: %d groups (at most %d)", what, groups, kMaxGemmGroups);
+    }
+    return CKL_OK;
+}
+
+struct Maps {
+    CUtensorMap a_box, a_row, b_box, b_row, t_row, e_box;
+};
+
+template <typename OutT>
+int launch(const Maps& maps, const GroupedParams& p, int grid, cudaStream_t stream) {
+    using Cfg = GroupedConfig;
+    static std::mutex mu;
+    static bool ready[64] = {};
+    int dev = 0;
+    GRP_TRY_CUDA(cudaGetDevice(&dev));
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        if (dev < 0 || dev >= 64 || !ready[dev]) {
+            GRP_TRY_CUDA(cudaFuncSetAttribute(grouped_gemm_kernel<OutT>,
+                                              cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                              static_cast<int>(Cfg::kSmemBytes)));
+            if (dev >= 0 && dev < 64) {
+                ready[dev] = true;
+            }
+        }
+    }
+    grouped_gemm_kernel<OutT><<<static_cast<unsigned>(grid), Cfg::kThreads, Cfg::kSmemBytes, stream>>>(
+        maps.a_box, maps.a_row, maps.b_box, maps.b_row, maps.t_row, maps.e_box, p);
+    GRP_TRY_CUDA(cudaGetLastError());
+    return CKL_OK;
+}
+
+// One product in terms of its operands; fills the descriptors and launches.
+struct Product {
+    int ab_dtype, c_dtype;  // c_dtype < 0: two-part C in the operand type
+    GroupedParams p;
+    const void *a, *b, *t, *e;
+    int lda, ldb, ldt, lde;
+    int a_cols, b_cols, b_outer;  // extents of A's rows, of B's rows, and B's row count (kFormRows)
+    int b_depth;
+    long long b_stack, e_stack;
+    int e_cols, e_outer;
+};
+
+int run(Product& q, cudaStream_t stream) {
+    GroupedParams& p = q.p;
+    DeviceView view;
+    GRP_TRY(device_view(&view));
+    p.status = view.status;
+    p.fmt = q.ab_dtype == CKL_BF16 ? 1u : 0u;
+    const bool wgrad = p.form == kFormWgrad;
+    // Upper bound of the tile rows: the groups' sizes are known on the device only.
+    const long long m_tiles = wgrad ? static_cast<long long>(p.groups) * ((p.m + 127) / 128)
+                              : p.offsets == nullptr || p.ext_groups > 0
+                                  ? (p.rows + 127) / 128
+                                  : p.rows / 128 + std::min(p.groups, p.rows);
+    // Tile width: the widest that still gives every SM a tile, so that a row of A is read the
+    // fewest times.
+    p.bn = p.n > 128 && m_tiles * ((p.n + 255) / 256) >= view.sm_count ? 256 : p.n > 64 ? 128 : 64;
+    const long long tiles = m_tiles * ((p.n + p.bn - 1) / p.bn);
+    if (tiles > 0x7fffffffll) {
+        return set_error(CKL_ERR_TOO_LARGE, "%lld output tiles", tiles);
+    }
+    if (tiles == 0) {
+        return CKL_OK;
+    }
+    Maps maps;
+    GRP_TRY(encode_operand(&maps.a_box, q.ab_dtype, q.a, q.a_cols, p.a_count, q.lda, 0, 0, 64, wgrad ? 64 : 128));
+    GRP_TRY(encode_operand(&maps.a_row, q.ab_dtype, q.a, q.a_cols, p.a_count, q.lda, 0, 0, 64, 1));
+    GRP_TRY(encode_operand(&maps.b_box, q.ab_dtype, q.b, q.b_cols, wgrad ? p.b_count : q.b_outer, q.ldb,
+                           static_cast<uint64_t>(q.b_depth), static_cast<uint64_t>(q.b_stack), 64, 64));
+    std::memset(&maps.b_row, 0, sizeof maps.b_row);
+    std::memset(&maps.t_row, 0, sizeof maps.t_row);
+    std::memset(&maps.e_box, 0, sizeof maps.e_box);
+    if (wgrad) {
+        GRP_TRY(encode_operand(&maps.b_row, q.ab_dtype, q.b, q.b_cols, p.b_count, q.ldb, 0, 0, 64, 1));
+    }
+    if (p.ext_groups > 0) {
+        GRP_TRY(encode_operand(&maps.t_row, q.ab_dtype, q.t, 2 * p.ext_cols, p.rows, q.ldt, 0, 0, 64, 1));
+        GRP_TRY(encode_operand(&maps.e_box, q.ab_dtype, q.e, q.e_cols, q.e_outer, q.lde, p.ext_groups,
+                               static_cast<uint64_t>(q.e_stack), 64, 64));
+    }
+    unsigned long long limit_ns = 0;
+    const int fault = take_wait_fault(&limit_ns);
+    p.wait_limit_ns = limit_ns;
+    p.overstate_first_stage = fault == 1 ? 1 : 0;
+    const int grid = static_cast<int>(std::min<long long>(view.sm_count, tiles));
+    if (q.c_dtype < 0) {
+        return q.ab_dtype == CKL_BF16 ? launch<TwoPart<__nv_bfloat16>>(maps, p, grid, stream)
+                                      : launch<TwoPart<__half>>(maps, p, grid, stream);
+    }
+    const int bytes = size_of(q.c_dtype);
+    p.c_vec = !misaligned(p.c, 16) && (static_cast<long long>(p.ldc) * bytes) % 16 == 0 &&
+              (p.c_stride * bytes) % 16 == 0;
+    switch (q.c_dtype) {
+        case CKL_F16: return launch<__half>(maps, p, grid, stream);
+        case CKL_BF16: return launch<__nv_bfloat16>(maps, p, grid, stream);
+        default: return launch<float>(maps, p, grid, stream);
+    }
+}
+
+Product blank(int ab_dtype, int c_dtype, int form) {
+    Product q;
+    std::memset(&q, 0, sizeof q);
+    q.ab_dtype = ab_dtype;
+    q.c_dtype = c_dtype;
+    q.p.form = form;
+    q.p.alpha = 1.0f;
+    q.p.a_parts = q.p.b_parts = 1;
+    return q;
+}
+
+int padded_rank(int rank) { return (rank + 15) / 16 * 16; }
+size_t two_part_bytes(int m, int rank) {
+    return (static_cast<size_t>(std::max(m, 0)) * 2 * padded_rank(rank) * 2 + 255) / 256 * 256;
+}
+
+// T[p] = scales[g] * A[rows[p]] * op(B_g) in two parts, for the positions of every adapter.
+Product shrink(int ab_dtype, const void* a, int lda, int k, const void* b, int ldb, long long stack,
+               bool trans, int rank, const float* scales, void* t, const int* offsets, const int* rows,
+               int adapters, int m) {
+    Product q = blank(ab_dtype, -1, kFormRows);
+    const int rp = padded_rank(rank);
+    q.p.offsets = offsets;
+    q.p.a_rows = rows;
+    q.p.c = t;
+    q.p.scales = scales;
+    q.p.groups = adapters;
+    q.p.rows = q.p.a_count = q.p.c_count = m;
+    q.p.n = rp;  // columns rank .. rp read weights outside their matrix, which are zeros
+    q.p.k = k;
+    q.p.ldc = 2 * rp;
+    q.p.c_part_cols = rp;
+    q.p.trans_b = trans ? 1 : 0;
+    q.a = a;
+    q.lda = lda;
+    q.a_cols = k;
+    q.b = b;
+    q.ldb = ldb;
+    q.b_cols = trans ? k : rank;
+    q.b_outer = trans ? rank : k;
+    q.b_depth = adapters;
+    q.b_stack = stack;
+    return q;
+}
+
+// C[rows[p]] = A[rows[p]] * op(B) + T[p] * op(E_g) + beta * C[rows[p]], C of n columns.
+Product expand(int ab_dtype, int c_dtype, const void* a, int lda, int k, const void* b, int ldb, int n,
+               bool trans, const void* t, int rank, const void* e, int lde, long long e_stack, void* c,
+               int ldc, const int* offsets, const int* rows, int adapters, int m, float beta) {
+    Product q = blank(ab_dtype, c_dtype, kFormRows);
+    const int rp = padded_rank(rank);
+    q.p.offsets = offsets;
+    q.p.a_rows = q.p.c_rows = rows;
+    q.p.c = c;
+    q.p.groups = q.p.ext_groups = adapters;
+    q.p.ext_cols = rp;
+    q.p.rows = q.p.a_count = q.p.c_count = m;
+    q.p.n = n;
+    q.p.k = k;
+    q.p.ldc = ldc;
+    q.p.beta = beta;
+    q.p.trans_b = trans ? 1 : 0;
+    q.a = a;
+    q.lda = lda;
+    q.a_cols = k;
+    q.b = b;
+    q.ldb = ldb;
+    q.b_cols = trans ? k : n;
+    q.b_outer = trans ? n : k;
+    q.b_depth = 1;
+    q.b_stack = static_cast<long long>(ldb) * q.b_outer;
+    q.t = t;
+    q.ldt = 2 * rp;
+    q.e = e;
+    q.lde = lde;
+    q.e_stack = e_stack;
+    q.e_cols = trans ? rank : n;
+    q.e_outer = trans ? n : rank;
+    return q;
+}
+
+int check_lora(const char* what, int ab_dtype, int out_dtype, const void* w, int ldw, const void* lora_a,
+               int ldla, long long stride_a, const void* lora_b, int ldlb, long long stride_b,
+               const float* scales, const int* offsets, const int* rows, int adapters, int m, int n,
+               int k, int rank, const void* workspace, size_t have, size_t need) {
+    GRP_TRY(check_types(what, ab_dtype, out_dtype));
+    GRP_TRY(check_groups(what, offsets, adapters, m));
+    if (rank < 1 || rank > kMaxLoraRank) {
+        return set_error(rank < 1 ? CKL_ERR_INVALID_ARG : CKL_ERR_TOO_LARGE, "%s: rank %d (1 to %d)", what,
+                         rank, kMaxLoraRank);
+    }
+    if (k < 1) {
+        return set_error(CKL_ERR_INVALID_ARG, "%s: k = %d", what, k);
+    }
+    GRP_TRY(check_operand(what, "w", w, ldw, n, 0));
+    GRP_TRY(check_operand(what, "lora_a", lora_a, ldla, rank, stride_a));
+    GRP_TRY(check_operand(what, "lora_b", lora_b, ldlb, n, stride_b));
+    if (misaligned(scales, 4) || misaligned(rows, 4)) {
+        return set_error(CKL_ERR_INVALID_ARG, "%s: misaligned scales or rows", what);
+    }
+    if (workspace == nullptr || misaligned(workspace, 256) || have < need) {
+        return set_error(CKL_ERR_INVALID_ARG,
+                         "%s: the workspace is %p of %zu bytes, needed are %zu on a 256-byte boundary", what,
+                         workspace, have, need);
+    }
+    return CKL_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ckl_gemm_grouped(int ab_dtype, const void* a, const int* a_rows, int a_count, const void* b, void* c,
+                     int c_dtype, const int* offsets, int groups, int rows, int n, int k, int lda, int ldb,
+                     long long stride_b, int ldc, int trans_b, float alpha, float beta,
+                     ckl_stream_t stream) {
+    const char* what = "gemm_grouped";
+    if (rows <= 0 || n <= 0) {
+        return CKL_OK;
+    }
+    GRP_TRY(check_types(what, ab_dtype, c_dtype));
+    GRP_TRY(check_groups(what, offsets, groups, rows));
+    k = std::max(k, 0);
+    if (k > 0) {
+        GRP_TRY(check_operand(what, "a", a, lda, k, 0));
+        GRP_TRY(check_operand(what, "b", b, ldb, trans_b ? k : n, stride_b));
+    }
+    if (a_rows == nullptr) {
+        a_count = rows;
+    }
+    if (a_count < 0 || misaligned(a_rows, 4) || c == nullptr || ldc < n || misaligned(c, size_of(c_dtype))) {
+        return set_error(CKL_ERR_INVALID_ARG, "%s: a_count %d, c %p, ldc %d for n %d", what, a_count, c, ldc, n);
+    }
+    Product q = blank(ab_dtype, c_dtype, kFormRows);
+    q.p.offsets = offsets;
+    q.p.a_rows = a_rows;
+    q.p.c = c;
+    q.p.groups = groups;
+    q.p.rows = q.p.c_count = rows;
+    q.p.a_count = a_count;
+    q.p.n = n;
+    q.p.k = k;
+    q.p.ldc = ldc;
+    q.p.alpha = alpha;
+    q.p.beta = beta;
+    q.p.trans_b = trans_b != 0 ? 1 : 0;
+    q.a = a;
+    q.lda = lda;
+    q.a_cols = k;
+    q.b = b;
+    q.ldb = ldb;
+    q.b_cols = trans_b ? k : n;
+    q.b_outer = trans_b ? n : k;
+    q.b_depth = groups;
+    q.b_stack = stride_b;
+    return run(q, static_cast<cudaStream_t>(stream));
+}
+
+int ckl_gemm_grouped_wgrad(int ab_dtype, const void* a, const int* a_rows, int a_count, const void* g,
+                           void* dw, int dw_dtype, const int* offsets, int groups, int rows, int m, int n,
+                           int lda, int ldg, int lddw, long long stride_dw, float alpha, float beta,
+                           ckl_stream_t stream) {
+    const char* what = "gemm_grouped_wgrad";
+    if (m <= 0 || n <= 0) {
+        return CKL_OK;
+    }
+    rows = std::max(rows, 0);
+    GRP_TRY(check_types(what, ab_dtype, dw_dtype));
+    GRP_TRY(check_groups(what, offsets, groups, rows));
+    if (rows > 0) {
+        GRP_TRY(check_operand(what, "a", a, lda, m, 0));
+        GRP_TRY(check_operand(what, "g", g, ldg, n, 0));
+    }
+    if (a_rows == nullptr) {
+        a_count = rows;
+    }
+    if (a_count < 0 || misaligned(a_rows, 4) || dw == nullptr || lddw < n || stride_dw < 0 ||
+        misaligned(dw, size_of(dw_dtype))) {
+        return set_error(CKL_ERR_INVALID_ARG, "%s: a_count %d, dw %p, lddw %d for n %d, stride %lld", what,
+                         a_count, dw, lddw, n, stride_dw);
+    }
+    Product q = blank(ab_dtype, dw_dtype, kFormWgrad);
+    q.p.offsets = offsets;
+    q.p.a_rows = a_rows;
+    q.p.c = dw;
+    q.p.c_stride = stride_dw;
+    q.p.groups = groups;
+    q.p.rows = q.p.b_count = rows;
+    q.p.a_count = a_count;
+    q.p.m = m;
+    q.p.n = n;
+    q.p.ldc = lddw;
+    q.p.alpha = alpha;
+    q.p.beta = beta;
+    q.a = a;
+    q.lda = lda;
+    q.a_cols = m;
+    q.b = g;
+    q.ldb = ldg;
+    q.b_cols = n;
+    q.b_depth = 1;
+    q.b_stack = static_cast<long long>(ldg) * std::max(rows, 1);
+    return run(q, static_cast<cudaStream_t>(stream));
+}
+
+size_t ckl_gemm_lora_workspace_bytes(int m, int rank, int backward) {
+    return rank < 1 || rank > kMaxLoraRank ? 0 : two_part_bytes(m, rank) * (backward != 0 ? 2 : 1);
+}
+
+int ckl_gemm_lora(int ab_dtype, const void* x, const void* w, const void* lora_a, const void* lora_b,
+                  const float* scales, void* y, int y_dtype, const int* offsets, const int* rows,
+                  int adapters, int m, int n, int k, int rank, int ldx, int ldw, int ldla,
+                  long long stride_a, int ldlb, long long stride_b, int ldy, float beta, void* workspace,
+                  size_t workspace_bytes, ckl_stream_t stream) {
+    const char* what = "gemm_lora";
+    if (m <= 0 || n <= 0) {
+        return CKL_OK;
+    }
+    GRP_TRY(check_lora(what, ab_dtype, y_dtype, w, ldw, lora_a, ldla, stride_a, lora_b, ldlb, stride_b, scales,
+                       offsets, rows, adapters, m, n, k, rank, workspace, workspace_bytes,
+                       ckl_gemm_lora_workspace_bytes(m, rank, 0)));
+    GRP_TRY(check_operand(what, "x", x, ldx, k, 0));
+    if (y == nullptr || ldy < n || misaligned(y, size_of(y_dtype))) {
+        return set_error(CKL_ERR_INVALID_ARG, "%s: y %p, ldy %d for n %d", what, y, ldy, n);
+    }
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    Product t = shrink(ab_dtype, x, ldx, k, lora_a, ldla, stride_a, false, rank, scales, workspace, offsets,
+                       rows, adapters, m);
+    GRP_TRY(run(t, s));
+    Product q = expand(ab_dtype, y_dtype, x, ldx, k, w, ldw, n, false, workspace, rank, lora_b, ldlb, stride_b,
+                       y, ldy, offsets, rows, adapters, m, beta);
+    return run(q, s);
+}
+
+int ckl_gemm_lora_backward(int ab_dtype, const void* dy, const void* x, const void* w, const void* lora_a,
+                           const void* lora_b, const float* scales, void* dx, int dx_dtype, void* da,
+                           void* db, int dab_dtype, const int* offsets, const int* rows, int adapters, int m,
+                           int n, int k, int rank, int lddy, int ldx, int ldw, int ldla, long long stride_a,
+                           int ldlb, long long stride_b, int lddx, int ldda, long long stride_da, int lddb,
+                           long long stride_db, float beta, void* workspace, size_t workspace_bytes,
+                           ckl_stream_t stream) {
+    const char* what = "gemm_lora_backward";
+    if (n <= 0 || k <= 0) {
+        return CKL_OK;
+    }
+    m = std::max(m, 0);
+    GRP_TRY(check_types(what, ab_dtype, dab_dtype));
+    GRP_TRY(check_lora(what, ab_dtype, dx_dtype, w, ldw, lora_a, ldla, stride_a, lora_b, ldlb, stride_b, scales,
+                       offsets, rows, adapters, m, n, k, rank, workspace, workspace_bytes,
+                       ckl_gemm_lora_workspace_bytes(m, rank, 1)));
+    if (m > 0) {
+        GRP_TRY(check_operand(what, "dy", dy, lddy, n, 0));
+        if (da != nullptr || db != nullptr) {
+            GRP_TRY(check_operand(what, "x", x, ldx, k, 0));
+        }
+    }
+    if ((dx != nullptr && (lddx < k || misaligned(dx, size_of(dx_dtype)))) ||
+        (da != nullptr && (ldda < rank || stride_da < 0 || misaligned(da, size_of(dab_dtype)))) ||
+        (db != nullptr && (lddb < n || stride_db < 0 || misaligned(db, size_of(dab_dtype))))) {
+        return set_error(CKL_ERR_INVALID_ARG, "%s: a gradient is misaligned or lddx %d, ldda %d, lddb %d is too small",
+                         what, lddx, ldda, lddb);
+    }
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    void* u = workspace;
+    void* t = static_cast<unsigned char*>(workspace) + two_part_bytes(m, rank);
+    const int rp = padded_rank(rank);
+    if (m > 0 && (dx != nullptr || da != nullptr)) {
+        Product q = shrink(ab_dtype, dy, lddy, n, lora_b, ldlb, stride_b, true, rank, scales, u, offsets, rows,
+                           adapters, m);
+        GRP_TRY(run(q, s));
+    }
+    if (m > 0 && dx != nullptr) {
+        Product q = expand(ab_dtype, dx_dtype, dy, lddy, n, w, ldw, k, true, u, rank, lora_a, ldla, stride_a, dx,
+                           lddx, offsets, rows, adapters, m, 0.0f);
+        GRP_TRY(run(q, s));
+    }
+    if (da != nullptr) {
+        Product q = blank(ab_dtype, dab_dtype, kFormWgrad);
+        q.p.offsets = offsets;
+        q.p.a_rows = rows;
+        q.p.c = da;
+        q.p.c_stride = stride_da;
+        q.p.groups = adapters;
+        q.p.rows = q.p.a_count = q.p.b_count = m;
+        q.p.m = k;
+        q.p.n = rank;
+        q.p.ldc = ldda;
+        q.p.beta = beta;
+        q.p.b_parts = 2;
+        q.p.b_part_cols = rp;
+        q.a = x;
+        q.lda = ldx;
+        q.a_cols = k;
+        q.b = u;
+        q.ldb = q.b_cols = 2 * rp;
+        q.b_depth = 1;
+        q.b_stack = static_cast<long long>(q.ldb) * std::max(m, 1);
+        GRP_TRY(run(q, s));
+    }
+    if (db != nullptr) {
+        if (m > 0) {
+            Product q = shrink(ab_dtype, x, ldx, k, lora_a, ldla, stride_a, false, rank, scales, t, offsets, rows,
+                               adapters, m);
+            GRP_TRY(run(q, s));
+        }
+        Product q = blank(ab_dtype, dab_dtype, kFormWgrad);
+        q.p.offsets = offsets;
+        q.p.b_rows = rows;
+        q.p.c = db;
+        q.p.c_stride = stride_db;
+        q.p.groups = adapters;
+        q.p.rows = q.p.a_count = q.p.b_count = m;
+        q.p.m = rank;
+        q.p.n = n;
+        q.p.ldc = lddb;
+        q.p.beta = beta;
+        q.p.a_parts = 2;
+        q.p.a_part_cols = rp;
+        q.a = t;
+        q.lda = q.a_cols = 2 * rp;
+        q.b = dy;
+        q.ldb = lddy;
+        q.b_cols = n;
+        q.b_depth = 1;
+        q.b_stack = static_cast<long long>(lddy) * std::max(m, 1);
+        GRP_TRY(run(q, s));
+    }
+    return CKL_OK;
+}
+
+}  // extern "C"

@@ -1,10 +1,34 @@
 // Shared by the translation units of the library; not part of the public ABI.
 #pragma once
 
+#include <cstdint>
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+
 namespace ckl {
 
 // Records `fmt` as the calling thread's last error (what ckl_last_error() returns) and
 // returns `code`, so a failing path can `return set_error(CKL_ERR_..., "...", ...)`.
 int set_error(int code, const char* fmt, ...);
+
+// What the entry points share of the current device's state.  device_view creates the state on
+// a device's first use (a small cudaMalloc) and fails with CKL_ERR_UNSUPPORTED off sm_100.
+struct DeviceView {
+    int device;
+    int sm_count;
+    unsigned int* status;  // 4 words on the device, read by ckl_device_status
+};
+int device_view(DeviceView* out);
+
+// Encodes a TMA descriptor of a stack of row-major 16-bit matrices: `inner` columns, `outer` rows
+// of `pitch` elements, `depth` matrices `stack` elements apart (depth 0: one matrix, a 2-D map).
+// 128-byte swizzle, zeros outside.  An empty tensor gives an unused, zeroed descriptor.
+int encode_operand(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uint64_t outer,
+                   uint64_t pitch, uint64_t depth, uint64_t stack, uint32_t box_inner,
+                   uint32_t box_outer);
+
+// The wait fault armed by ckl_test_arm_wait_fault for the calling thread (kind 0: none); disarms it.
+int take_wait_fault(unsigned long long* limit_ns);
 
 }  // namespace ckl

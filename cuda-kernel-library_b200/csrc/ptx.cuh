@@ -179,6 +179,31 @@ __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap
         : "memory");
 }
 
+// 3-D form: z selects one matrix of a stack.
+__device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap* map, uint32_t bar,
+                                            int32_t x, int32_t y, int32_t z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];"
+        :
+        : "r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+// Gather of four rows of a 2-D tensor whose map has a box one row high: the rows land one
+// behind the other at smem_dst.  A row index outside the tensor reads the fill value (0).
+__device__ __forceinline__ void tma_gather4(uint32_t smem_dst, const CUtensorMap* map, uint32_t bar,
+                                            int32_t x, int32_t r0, int32_t r1, int32_t r2,
+                                            int32_t r3) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+        :
+        : "r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(r0), "r"(r1),
+          "r"(r2), "r"(r3)
+        : "memory");
+}
+
 // L2 eviction-priority hints for TMA loads (the 64-bit policy words that
 // createpolicy.fractional.L2::evict_{first,last} with fraction 1.0 produce).
 constexpr uint64_t kL2EvictNormal = 0x1000000000000000ull;

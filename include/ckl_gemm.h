@@ -285,6 +285,120 @@ int ckl_gemm_gathered(ckl_comm* comm, int ab_dtype, const void* a, const void* b
 int ckl_scatter_column_block(void* const* dsts, int parts, const void* src, int elem_size,
                              int rows, int width, int n, int col0, ckl_stream_t stream);
 
+/* ---- products whose weight is chosen per row ------------------------------------------------
+ *
+ * (No counterpart in the reference.)  Rows that use the same weight form a group: the rows sent
+ * to one expert, or the rows of the requests that use one adapter.  ckl_group_rows orders rows by
+ * group on the device; the products read that order there, so the host never waits for group
+ * sizes and every call can be captured into a graph.
+ *
+ * All of these: pointers are device memory of the current device, work is enqueued on `stream`,
+ * nothing is allocated per call and nothing is kept between calls; the first call on a device
+ * creates its small state (make it outside stream capture).  Two calls may overlap as long as they
+ * do not share outputs or a workspace.  No result depends on the order in which threads run. */
+
+/* Stable order of `slots` ids by group.  ids[s] names the group of slot s; an id outside
+ * [0, groups) names none.  offsets[g] .. offsets[g+1] (groups + 1 values) are the positions of
+ * group g; positions[s] is the position of slot s and rows[positions[s]] = s / slots_per_row the
+ * row it came from.  Slots of one group keep their order; slots of no group come last, behind
+ * offsets[groups].  groups <= 1024. */
+int ckl_group_rows(const int* ids, int slots, int groups, int slots_per_row, int* offsets, int* rows,
+                   int* positions, ckl_stream_t stream);
+
+/* Scores of ckl_moe_route. */
+typedef enum ckl_score { CKL_SCORE_SOFTMAX = 0, CKL_SCORE_SIGMOID = 1 } ckl_score;
+
+/* Routing: for each of `tokens` rows of logits (tokens x n_experts, leading dimension ldl, any
+ * ckl_dtype) the top_k experts and their weights (both tokens x top_k, packed; best first).
+ *   score s = softmax(l) over the row, or sigmoid(l) per expert;
+ *   choice by s + bias (bias: n_experts floats or NULL; it moves the choice, never the weight),
+ *   ties to the lowest index; with groups > 1 only inside the top_groups best groups of
+ *   n_experts / groups neighbours, a group's score being the sum of its two best s + bias;
+ *   weight = scale * s, or scale * s / (sum of the chosen s) with renormalise.
+ * An expert whose logit is -inf or NaN (or whose bias is) is never chosen and scores 0; +inf
+ * counts as the largest float.  Places that cannot be filled hold expert -1 and weight 0, so a row
+ * of -inf routes nowhere.  Scores without a bias and groups are compared as logits, otherwise in
+ * 64 bits.  n_experts <= 1024, top_k <= 32, groups <= 32 and a divisor of n_experts. */
+int ckl_moe_route(int logit_dtype, const void* logits, int ldl, const float* bias, float* weights,
+                  int* experts, int tokens, int n_experts, int top_k, int score, int groups,
+                  int top_groups, int renormalise, float scale, ckl_stream_t stream);
+
+/* Gradient of the weights with respect to the logits: dlogits (tokens x n_experts in the logits'
+ * type, leading dimension ldd, every element written) from dweights and the experts that
+ * ckl_moe_route chose.  The choice itself has no gradient; an expert outside [0, n_experts) gets
+ * none. */
+int ckl_moe_route_backward(int logit_dtype, const void* logits, int ldl, const int* experts,
+                           const float* dweights, void* dlogits, int ldd, int tokens, int n_experts,
+                           int top_k, int score, int renormalise, float scale, ckl_stream_t stream);
+
+/* Grouped product.  For every position p of group g (offsets[g] <= p < offsets[g+1]):
+ *     C[p] = alpha * A[a_rows[p]] * op(B_g) + beta * C[p]
+ * A: a_count x k (a_rows NULL: row p itself, a_count is then `rows`); B_g = b + g * stride_b,
+ * k x n, or n x k with trans_b (op = transpose); C: rows x n.  A and B FP16 or BF16, C any type,
+ * FP32 accumulation.  With a layer's weights, trans_b gives the gradient of its input.  `rows`
+ * bounds the positions: rows of C behind offsets[groups] are left as they are.  An a_rows entry
+ * outside [0, a_count) reads a row of zeros.  k <= 0 scales C; C is not read when beta == 0.
+ * A and B must be 16-byte aligned with leading dimensions and stride_b multiples of 8, else
+ * CKL_ERR_UNSUPPORTED; n, k and C are free.  groups <= 1024. */
+int ckl_gemm_grouped(int ab_dtype, const void* a, const int* a_rows, int a_count, const void* b, void* c,
+                     int c_dtype, const int* offsets, int groups, int rows, int n, int k, int lda, int ldb,
+                     long long stride_b, int ldc, int trans_b, float alpha, float beta,
+                     ckl_stream_t stream);
+
+/* Gradient of the weights of ckl_gemm_grouped, for every group (an empty one gets beta * dW_g):
+ *     dW_g = alpha * sum over p in g of A[a_rows[p]]^T G[p] + beta * dW_g
+ * A: a_count x m, G: rows x n, dW_g = dw + g * stride_dw, m x n.  Same types and rules. */
+int ckl_gemm_grouped_wgrad(int ab_dtype, const void* a, const int* a_rows, int a_count, const void* g,
+                           void* dw, int dw_dtype, const int* offsets, int groups, int rows, int m, int n,
+                           int lda, int ldg, int lddw, long long stride_dw, float alpha, float beta,
+                           ckl_stream_t stream);
+
+/* Rows back to their tokens: out[t] = sum over j < top_k of weights[t][j] * y[positions[t][j]],
+ * summed in FP32 in the order of j.  y: y_rows x n, out: tokens x n, any types; a position outside
+ * [0, y_rows) adds nothing.  tokens <= 0 or n <= 0 is a no-op. */
+int ckl_moe_combine(int y_dtype, const void* y, const int* positions, const float* weights, void* out,
+                    int out_dtype, int tokens, int top_k, int n, int y_rows, int ldy, int ldo,
+                    ckl_stream_t stream);
+
+/* Its gradient: dy[positions[t][j]] = weights[t][j] * dout[t] (dy in y's type; rows that no position
+ * names are left as they are; a row named twice holds one of the two) and
+ * dweights[t][j] = <dout[t], y[positions[t][j]]>. */
+int ckl_moe_combine_backward(int y_dtype, const void* y, const int* positions, const float* weights,
+                             const void* dout, int dout_dtype, void* dy, float* dweights, int tokens,
+                             int top_k, int n, int y_rows, int ldy, int ldo, int lddy,
+                             ckl_stream_t stream);
+
+/* Low-rank adapters beside a shared projection.  Row i of x uses adapter g (or none):
+ *     y[i] = x[i] W + scales[g] * (x[i] A_g) B_g + beta * y[i]
+ * x: m x k, W: k x n, A_g = lora_a + g * stride_a (k x rank, ldla), B_g = lora_b + g * stride_b
+ * (rank x n, ldlb), y: m x n of any type.  offsets (adapters + 1) and rows (a permutation of
+ * 0 .. m-1, NULL: the identity) are what ckl_group_rows makes of the rows' adapter ids: position p
+ * is row rows[p]; positions behind offsets[adapters] use no adapter.  scales NULL: 1.  The
+ * product x A_g is held as the sum of two operand-type values (16 bits of BF16, 22 of FP16), so it
+ * has the operand type's range.  rank <= 128, adapters <= 1024; operands 16-byte aligned with
+ * leading dimensions and strides multiples of 8, else CKL_ERR_UNSUPPORTED.  The workspace holds
+ * ckl_gemm_lora_workspace_bytes(m, rank, 0) bytes on a 256-byte boundary and is free again when
+ * the call's work on the stream has run. */
+size_t ckl_gemm_lora_workspace_bytes(int m, int rank, int backward);
+int ckl_gemm_lora(int ab_dtype, const void* x, const void* w, const void* lora_a, const void* lora_b,
+                  const float* scales, void* y, int y_dtype, const int* offsets, const int* rows,
+                  int adapters, int m, int n, int k, int rank, int ldx, int ldw, int ldla,
+                  long long stride_a, int ldlb, long long stride_b, int ldy, float beta, void* workspace,
+                  size_t workspace_bytes, ckl_stream_t stream);
+
+/* Gradients of ckl_gemm_lora with a frozen W (dx, da, db: any may be NULL), U = scales[g] dy B_g^T:
+ *     dx = dy W^T + U A_g^T      (dx_dtype; written whole)
+ *     dA_g = X_g^T U + beta * dA_g      dB_g = (scales[g] X_g A_g)^T dY_g + beta * dB_g
+ * X_g and dY_g being the rows of adapter g; an adapter without rows gets beta times its old
+ * gradient.  The workspace holds ckl_gemm_lora_workspace_bytes(m, rank, 1) bytes. */
+int ckl_gemm_lora_backward(int ab_dtype, const void* dy, const void* x, const void* w, const void* lora_a,
+                           const void* lora_b, const float* scales, void* dx, int dx_dtype, void* da,
+                           void* db, int dab_dtype, const int* offsets, const int* rows, int adapters, int m,
+                           int n, int k, int rank, int lddy, int ldx, int ldw, int ldla, long long stride_a,
+                           int ldlb, long long stride_b, int lddx, int ldda, long long stride_da, int lddb,
+                           long long stride_db, float beta, void* workspace, size_t workspace_bytes,
+                           ckl_stream_t stream);
+
 /* No counterpart in the reference.  The stream-K tensor-core GEMM for callers that
  * must not allocate device memory: hosts that have given all device memory to an
  * arena of their own (a cudaMalloc inside a library would fail or break their

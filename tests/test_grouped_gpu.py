@@ -1,0 +1,363 @@
+"""Products whose weight is chosen per row (ckl_gemm_grouped, its weight gradient, low-rank
+adapters) against plain 64-bit sums on the same inputs.
+
+Tolerances, element by element.  The tensor cores add products into an FP32 accumulator that is
+truncated, so each of at most k additions is off by at most 2^-23 of the partial sum, which
+sum |a||b| bounds: ACC = k * 2^-23 * (|A| |B|).  The result is rounded once, by at most half a
+step: eps/2 of its value.  beta * C and alpha each add one FP32 rounding, covered by a further 2^-22.
+The intermediate of the adapters is kept as two operand-type values: off by 2^-16 (BF16) or 2^-22
+(FP16, plus its smallest step) of its value.
+"""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
+HALF_STEP = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8, "f32": 2.0 ** -24}
+TWO_PART = {"f16": 2.0 ** -22, "bf16": 2.0 ** -16}
+
+
+def code(ckl, name):
+    return {"f16": ckl.F16, "bf16": ckl.BF16, "f32": ckl.F32}[name]
+
+
+@pytest.fixture(autouse=True)
+def device_healthy(ckl):
+    if not torch.cuda.is_available():
+        pytest.fail("tests marked gpu need a CUDA device")
+    yield
+    ckl.device_status()
+
+
+def rand(shape, dtype, seed, std=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * std).to(dtype)
+
+
+def offsets_of(sizes, start=0):
+    o = [start]
+    for s in sizes:
+        o.append(o[-1] + s)
+    return torch.tensor(o, dtype=torch.int32, device="cuda")
+
+
+def check(got, ref, absolute, steps, out, extra=0.0):
+    """absolute = sum |a||b| of the element, steps = additions behind it."""
+    tol = steps * 2.0 ** -23 * absolute + (HALF_STEP[out] + 2.0 ** -22) * ref.abs() + extra
+    if out == "f16":
+        tol = tol + 2.0 ** -25  # half the smallest step of a subnormal result
+    err = (got.double() - ref).abs()
+    assert torch.isfinite(got).all()
+    worst = (err / tol.clamp(min=1e-300)).max().item() if err.numel() else 0.0
+    assert worst <= 1.0, f"error {worst:.3g} times the tolerance"
+
+
+SIZES = {
+    "ragged": [0, 1, 5, 127, 128, 129, 300, 0],
+    "single_rows": [1] * 9,
+    "one": [77],
+    "empty": [0, 0, 0],
+    "long": [700, 3],
+}
+
+
+@pytest.mark.parametrize("sizes", SIZES, ids=list(SIZES))
+@pytest.mark.parametrize("trans", [False, True], ids=["nn", "nt"])
+@pytest.mark.parametrize("gather", [False, True], ids=["rows", "gather"])
+def test_grouped_sizes(ckl, sizes, trans, gather):
+    sizes = SIZES[sizes]
+    n, k, tail, tokens = 200, 328, 3, 50
+    offs = offsets_of(sizes)
+    kept = int(offs[-1])
+    rows = kept + tail
+    a = rand((tokens if gather else rows, k), torch.bfloat16, 1)
+    idx = torch.randint(0, tokens, (rows,), device="cuda", dtype=torch.int32) if gather else None
+    b = rand((len(sizes), n, k) if trans else (len(sizes), k, n), torch.bfloat16, 2, k ** -0.5)
+    c = torch.full((rows, n), 7.25, dtype=torch.bfloat16, device="cuda")
+    ckl.gemm_grouped(ckl.BF16, a, b, c, ckl.BF16, offs, len(sizes), rows, n, k, a_rows=idx,
+                     a_count=tokens if gather else None, trans_b=trans)
+    torch.cuda.synchronize()
+    assert (c[kept:] == 7.25).all()  # rows behind the last group stay as they were
+    src = a[idx.long()] if gather else a
+    o = offs.tolist()
+    for g in range(len(sizes)):
+        x = src[o[g]:o[g + 1]].double()
+        w = (b[g].t() if trans else b[g]).double()
+        check(c[o[g]:o[g + 1]], x @ w, x.abs() @ w.abs(), k, "bf16")
+
+
+@pytest.mark.parametrize("ab,out", [("f16", "f16"), ("f16", "f32"), ("bf16", "f32"), ("bf16", "f16")])
+@pytest.mark.parametrize("n,k", [(1, 8), (17, 8), (64, 64), (65, 130), (257, 1), (1000, 72), (520, 1500)])
+def test_grouped_types_and_odd_sizes(ckl, ab, out, n, k):
+    sizes = [130, 0, 6]
+    offs, rows = offsets_of(sizes), 136
+    lda, ldb, ldc = (k + 7) // 8 * 8 + 8, (n + 7) // 8 * 8, n + 3
+    a = rand((rows, lda), DT[ab], 3)
+    b = rand((3, k, ldb), DT[ab], 4, k ** -0.5)
+    c = rand((rows, ldc), DT[out], 5)
+    c0 = c.clone()
+    alpha, beta = 1.25, 0.5
+    ckl.gemm_grouped(code(ckl, ab), a, b, c, code(ckl, out), offs, 3, rows, n, k, lda=lda, ldb=ldb, ldc=ldc,
+                     stride_b=k * ldb, alpha=alpha, beta=beta)
+    torch.cuda.synchronize()
+    assert torch.equal(c[:, n:], c0[:, n:])
+    o = offs.tolist()
+    for g in range(3):
+        x, w = a[o[g]:o[g + 1], :k].double(), b[g, :, :n].double()
+        old = beta * c0[o[g]:o[g + 1], :n].double()
+        check(c[o[g]:o[g + 1], :n], alpha * (x @ w) + old, alpha * (x.abs() @ w.abs()) + old.abs(), k + 2, out)
+
+
+def test_grouped_wide_tiles_and_many_groups(ckl):
+    """Enough tiles for 256 columns, and more groups than lanes in a warp."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    counts = torch.randint(0, 260, (100,), generator=g, device="cuda")
+    offs = torch.zeros(101, dtype=torch.int32, device="cuda")
+    offs[1:] = torch.cumsum(counts, 0)
+    rows, n, k = int(offs[-1]), 640, 192
+    a, b = rand((rows, k), torch.float16, 12), rand((100, k, n), torch.float16, 13, k ** -0.5)
+    c = torch.empty(rows, n, dtype=torch.float32, device="cuda")
+    ckl.gemm_grouped(ckl.F16, a, b, c, ckl.F32, offs, 100, rows, n, k)
+    torch.cuda.synchronize()
+    w = b.double()[torch.repeat_interleave(torch.arange(100, device="cuda"), counts)]
+    ref = torch.einsum("rk,rkn->rn", a.double(), w)
+    check(c, ref, torch.einsum("rk,rkn->rn", a.double().abs(), w.abs()), k, "f32")
+
+
+def test_grouped_masked_rows_and_neighbours(ckl):
+    """An index outside A reads zeros; NaN in rows of one group does not reach the others."""
+    offs = offsets_of([3, 4])
+    a = rand((6, 64), torch.bfloat16, 1)
+    a[5] = float("nan")
+    idx = torch.tensor([0, -1, 6, 5, 1, 2, 2147483647], dtype=torch.int32, device="cuda")
+    b = rand((2, 64, 64), torch.bfloat16, 2, 0.125)
+    c = torch.full((7, 64), float("nan"), device="cuda")
+    ckl.gemm_grouped(ckl.BF16, a, b, c, ckl.F32, offs, 2, 7, 64, 64, a_rows=idx, a_count=6)
+    torch.cuda.synchronize()
+    assert (c[[1, 2, 6]] == 0).all() and torch.isnan(c[3]).all()
+    for row, src, g in ((0, 0, 0), (4, 1, 1), (5, 2, 1)):
+        x, w = a[src:src + 1].double(), b[g].double()
+        check(c[row:row + 1], x @ w, x.abs() @ w.abs(), 64, "f32")
+
+
+def test_grouped_without_k_and_partial_cover(ckl):
+    """k = 0 scales C; one group that starts and ends inside the rows leaves the others alone."""
+    offs = torch.tensor([2, 5], dtype=torch.int32, device="cuda")
+    c = rand((9, 40), torch.float32, 1)
+    c0 = c.clone()
+    ckl.gemm_grouped(ckl.F16, None, None, c, ckl.F32, offs, 1, 9, 40, 0, beta=0.5)
+    assert torch.equal(c[2:5], 0.5 * c0[2:5])
+    assert torch.equal(c[:2], c0[:2]) and torch.equal(c[5:], c0[5:])
+    a, b = rand((9, 72), torch.float16, 2), rand((1, 72, 40), torch.float16, 3)
+    ckl.gemm_grouped(ckl.F16, a, b, c, ckl.F32, offs, 1, 9, 40, 72)
+    assert torch.equal(c[:2], c0[:2]) and torch.equal(c[5:], c0[5:])
+    x, w = a[2:5].double(), b[0].double()
+    check(c[2:5], x @ w, x.abs() @ w.abs(), 72, "f32")
+
+
+@pytest.mark.parametrize("sizes", SIZES, ids=list(SIZES))
+@pytest.mark.parametrize("gather", [False, True], ids=["rows", "gather"])
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+def test_weight_gradient(ckl, sizes, gather, out):
+    sizes = SIZES[sizes]
+    m, n, tokens = 136, 328, 40
+    offs = offsets_of(sizes)
+    rows = int(offs[-1]) + 2
+    a = rand((tokens if gather else rows, m), torch.bfloat16, 1)
+    idx = torch.randint(0, tokens, (rows,), device="cuda", dtype=torch.int32) if gather else None
+    d = rand((rows, n), torch.bfloat16, 2)
+    d[rows - 2:] = float("nan")  # behind the last group: never read into a sum
+    w = rand((len(sizes), m, n), DT[out], 3)
+    w0 = w.clone()
+    ckl.gemm_grouped_wgrad(ckl.BF16, a, d, w, code(ckl, out), offs, len(sizes), rows, m, n, a_rows=idx,
+                           a_count=tokens if gather else None, beta=0.25)
+    torch.cuda.synchronize()
+    src = a[idx.long()] if gather else a
+    o = offs.tolist()
+    for g in range(len(sizes)):
+        x, y = src[o[g]:o[g + 1]].double(), d[o[g]:o[g + 1]].double()
+        old = 0.25 * w0[g].double()
+        check(w[g], x.t() @ y + old, x.abs().t() @ y.abs() + old.abs(), sizes[g] + 2, out)
+
+
+def test_weight_gradient_odd_shapes(ckl):
+    sizes, m, n = [65, 64, 0, 1], 37, 9
+    offs, rows = offsets_of(sizes), 130
+    a, d = rand((rows, 40), torch.float16, 1), rand((rows, 16), torch.float16, 2)
+    w = torch.full((4, m, n + 1), 3.0, device="cuda")
+    ckl.gemm_grouped_wgrad(ckl.F16, a, d, w, ckl.F32, offs, 4, rows, m, n, lda=40, ldg=16, lddw=n + 1, alpha=0.5)
+    torch.cuda.synchronize()
+    assert (w[:, :, n] == 3.0).all()
+    o = offs.tolist()
+    for g in range(4):
+        x, y = a[o[g]:o[g + 1], :m].double(), d[o[g]:o[g + 1], :n].double()
+        check(w[g, :, :n], 0.5 * (x.t() @ y), 0.5 * (x.abs().t() @ y.abs()), sizes[g], "f32")
+
+
+def plan(ckl, ids, groups, per_row=1):
+    slots = ids.numel()
+    offs = torch.empty(groups + 1, dtype=torch.int32, device="cuda")
+    rows = torch.empty(slots, dtype=torch.int32, device="cuda")
+    pos = torch.empty(slots, dtype=torch.int32, device="cuda")
+    ckl.group_rows(ids, slots, groups, offs, rows, pos, slots_per_row=per_row)
+    return offs, rows, pos
+
+
+def lora_case(ckl, ids, g, k, n, r, dt, seed=0):
+    m = ids.numel()
+    x = rand((m, k), DT[dt], seed + 1)
+    w = rand((k, n), DT[dt], seed + 2, k ** -0.5)
+    a = rand((g, k, r), DT[dt], seed + 3, k ** -0.5)
+    b = rand((g, r, n), DT[dt], seed + 4, r ** -0.5)
+    s = 0.5 + torch.rand(g, device="cuda")
+    offs, rows, _ = plan(ckl, ids, g)
+    return m, x, w, a, b, s, offs, rows
+
+
+def adapter_ids(kind, g):
+    gen = torch.Generator().manual_seed(3)
+    if kind == "one_row":
+        ids = [0]
+    elif kind == "none":
+        ids = [-1] * 5
+    elif kind == "each_its_own":
+        ids = list(range(g))
+    elif kind == "one_adapter":
+        ids = [g - 1] * 300
+    else:
+        ids = torch.randint(-1, g, (333,), generator=gen).tolist()
+    return torch.tensor(ids, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("kind", ["one_row", "none", "each_its_own", "one_adapter", "mixed"])
+@pytest.mark.parametrize("dt,out,r", [("bf16", "bf16", 16), ("f16", "f32", 8), ("bf16", "f32", 72), ("f16", "f16", 128)])
+def test_lora(ckl, kind, dt, out, r):
+    g, k, n = 7, 264, 328
+    ids = adapter_ids(kind, g)
+    m, x, w, a, b, s, offs, rows = lora_case(ckl, ids, g, k, n, r, dt)
+    y = rand((m, n + 8), DT[out], 9)
+    y0 = y.clone()
+    size = ckl.gemm_lora_workspace_bytes(m, r)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    beta = 0.5
+    ckl.gemm_lora(code(ckl, dt), x, w, a, b, s, y, code(ckl, out), offs, rows, g, m, n, k, r, ws, size, ldy=n + 8,
+                  beta=beta)
+    torch.cuda.synchronize()
+    assert torch.equal(y[:, n:], y0[:, n:])
+    for i in range(-1, g):
+        sel = ids == i
+        xs, old = x[sel].double(), beta * y0[sel][:, :n].double()
+        ref, mag = xs @ w.double() + old, xs.abs() @ w.double().abs() + old.abs()
+        steps, extra = k + 2, 0.0
+        if i >= 0:
+            f = s[i].double()
+            t, ta = f * (xs @ a[i].double()), f * (xs.abs() @ a[i].double().abs())
+            ref, mag = ref + t @ b[i].double(), mag + ta @ b[i].double().abs()
+            floor = 2.0 ** -25 * r * b[i].double().abs().max() if dt == "f16" else 0.0
+            extra = TWO_PART[dt] * (t.abs() @ b[i].double().abs()) + floor
+            steps += k + 2 * r
+        check(y[sel][:, :n], ref, mag, steps, out, extra)
+
+
+@pytest.mark.parametrize("kind", ["one_row", "none", "each_its_own", "mixed"])
+@pytest.mark.parametrize("dt,out,r", [("bf16", "f32", 16), ("f16", "f16", 40), ("bf16", "bf16", 128)])
+def test_lora_gradients(ckl, kind, dt, out, r):
+    g, k, n = 5, 264, 200
+    ids = adapter_ids(kind, g)
+    m, x, w, a, b, s, offs, rows = lora_case(ckl, ids, g, k, n, r, dt, 20)
+    dy = rand((m, n), DT[dt], 30)
+    dx = torch.full((m, k), float("nan"), dtype=DT[out], device="cuda")
+    da, db = rand((g, k, r), DT[out], 31), rand((g, r, n), DT[out], 32)
+    da0, db0 = da.clone(), db.clone()
+    size = ckl.gemm_lora_workspace_bytes(m, r, True)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    ckl.gemm_lora_backward(code(ckl, dt), dy, x, w, a, b, s, dx, code(ckl, out), da, db, code(ckl, out), offs, rows, g,
+                           m, n, k, r, ws, size, beta=1.0)
+    torch.cuda.synchronize()
+    for i in range(-1, g):
+        sel = ids == i
+        ys, xs = dy[sel].double(), x[sel].double()
+        ref, mag, steps, extra = ys @ w.double().t(), ys.abs() @ w.double().abs().t(), n, 0.0
+        if i >= 0:
+            f, aa, bb = s[i].double(), a[i].double(), b[i].double()
+            two = TWO_PART[dt]
+            tiny = 2.0 ** -25 if dt == "f16" else 0.0
+            u, um = f * (ys @ bb.t()), f * (ys.abs() @ bb.abs().t())
+            t, tm = f * (xs @ aa), f * (xs.abs() @ aa.abs())
+            ref, mag, steps = ref + u @ aa.t(), mag + um @ aa.abs().t(), 2 * n + 2 * r
+            extra = two * (u.abs() @ aa.abs().t()) + tiny * r * aa.abs().max()
+            count = int(sel.sum())
+            check(da[i], xs.t() @ u + da0[i].double(), xs.abs().t() @ um + da0[i].double().abs(),
+                  n + 2 * count + 2, out, two * (xs.abs().t() @ u.abs()) + tiny * xs.abs().sum(0).unsqueeze(1))
+            check(db[i], t.t() @ ys + db0[i].double(), tm.t() @ ys.abs() + db0[i].double().abs(),
+                  k + 2 * count + 2, out, two * (t.abs().t() @ ys.abs()) + tiny * ys.abs().sum(0).unsqueeze(0))
+        check(dx[sel], ref, mag, steps, out, extra)
+
+
+def test_lora_gradients_against_differences(ckl):
+    """The loss <y, r> is linear in each of x, A and B: a central difference along a direction is the
+    gradient's product with it, up to the FP32 outputs' own error."""
+    g, k, n, r = 3, 64, 72, 16
+    ids = torch.tensor([0, 2, 2, -1, 0, 2], dtype=torch.int32, device="cuda")
+    m, x, w, a, b, s, offs, rows = lora_case(ckl, ids, g, k, n, r, "f16", 40)
+    dy = rand((m, n), torch.float16, 44)
+    size = ckl.gemm_lora_workspace_bytes(m, r, True)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+
+    def loss(x, a, b):
+        y = torch.empty(m, n, device="cuda")
+        ckl.gemm_lora(ckl.F16, x, w, a, b, s, y, ckl.F32, offs, rows, g, m, n, k, r, ws, size)
+        return (y.double() * dy.double()).sum().item()
+
+    dx, da, db = (torch.empty(t.shape, device="cuda") for t in (x, a, b))
+    ckl.gemm_lora_backward(ckl.F16, dy, x, w, a, b, s, dx, ckl.F32, da, db, ckl.F32, offs, rows, g, m, n, k, r, ws,
+                           size)
+    for which, grad in ((0, dx), (1, da), (2, db)):
+        args = [x, a, b]
+        step = (torch.randint(0, 2, args[which].shape, device="cuda") * 2 - 1).half() * 0.25
+        hi, lo = list(args), list(args)
+        hi[which], lo[which] = args[which] + step, args[which] - step
+        moved = (hi[which].double() - lo[which].double())  # the step after FP16 rounding
+        want = (grad.double() * moved).sum().item()
+        scale = (grad.double().abs() * moved.abs()).sum().item()
+        assert abs(loss(*hi) - loss(*lo) - want) <= 1e-4 * scale
+
+
+def test_lora_optional_outputs_and_defaults(ckl):
+    g, k, n, r, m = 2, 64, 64, 16, 4
+    ids = torch.tensor([1, 1, 0, -1], dtype=torch.int32, device="cuda")
+    m, x, w, a, b, s, offs, rows = lora_case(ckl, ids, g, k, n, r, "bf16", 50)
+    dy = rand((m, n), torch.bfloat16, 51)
+    size = ckl.gemm_lora_workspace_bytes(m, r, True)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    args = (offs, rows, g, m, n, k, r, ws, size)
+    whole = [torch.empty(t.shape, device="cuda") for t in (x, a, b)]
+    ckl.gemm_lora_backward(ckl.BF16, dy, x, w, a, b, None, whole[0], ckl.F32, whole[1], whole[2], ckl.F32, *args)
+    for i in range(3):
+        part = [None, None, None]
+        part[i] = torch.empty_like(whole[i])
+        ckl.gemm_lora_backward(ckl.BF16, dy, x, w, a, b, None, part[0], ckl.F32, part[1], part[2], ckl.F32, *args)
+        assert torch.equal(part[i], whole[i])
+    # rows in adapter order need no permutation
+    order = rows.long()
+    y = [torch.empty(m, n, device="cuda") for _ in range(2)]
+    ckl.gemm_lora(ckl.BF16, x, w, a, b, None, y[0], ckl.F32, *args)
+    ckl.gemm_lora(ckl.BF16, x[order].contiguous(), w, a, b, None, y[1], ckl.F32, offs, None, *args[2:])
+    assert torch.equal(y[0][order], y[1])
+
+
+def test_wait_that_runs_out_is_reported(ckl):
+    offs = offsets_of([5])
+    a, b = rand((5, 128), torch.bfloat16, 1), rand((1, 128, 64), torch.bfloat16, 2)
+    c = torch.zeros(5, 64, device="cuda")
+    ckl.arm_wait_fault(1, 50_000_000)
+    ckl.gemm_grouped(ckl.BF16, a, b, c, ckl.F32, offs, 1, 5, 64, 128)
+    with pytest.raises(ckl.CklError) as e:
+        ckl.device_status()
+    assert e.value.status == ckl.ERR_DEVICE
+    ckl.gemm_grouped(ckl.BF16, a, b, c, ckl.F32, offs, 1, 5, 64, 128)
+    torch.cuda.synchronize()
+    check(c, a.double() @ b[0].double(), a.double().abs() @ b[0].double().abs(), 128, "f32")
