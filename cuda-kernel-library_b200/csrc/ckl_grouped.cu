@@ -67,7 +67,7 @@ int check_groups(const char* what, const int* offsets, int groups, int rows) {
 }
 
 struct Maps {
-    CUtensorMap a_box, a_row, b_box, b_row, t_row, e_box;
+    CUtensorMap a_box, b_box, e_box;
 };
 
 template <typename OutT>
@@ -89,7 +89,7 @@ int launch(const Maps& maps, const GroupedParams& p, int grid, cudaStream_t stre
         }
     }
     grouped_gemm_kernel<OutT><<<static_cast<unsigned>(grid), Cfg::kThreads, Cfg::kSmemBytes, stream>>>(
-        maps.a_box, maps.a_row, maps.b_box, maps.b_row, maps.t_row, maps.e_box, p);
+        maps.a_box, maps.b_box, maps.e_box, p);
     GRP_TRY_CUDA(cudaGetLastError());
     return CKL_OK;
 }
@@ -128,22 +128,27 @@ int run(Product& q, cudaStream_t stream) {
     if (tiles == 0) {
         return CKL_OK;
     }
+    // Gathered operands are read by the loader warps, all others through these descriptors.
     Maps maps;
-    GRP_TRY(encode_operand(&maps.a_box, q.ab_dtype, q.a, q.a_cols, p.a_count, q.lda, 0, 0, 64, wgrad ? 64 : 128));
-    GRP_TRY(encode_operand(&maps.a_row, q.ab_dtype, q.a, q.a_cols, p.a_count, q.lda, 0, 0, 64, 1));
-    GRP_TRY(encode_operand(&maps.b_box, q.ab_dtype, q.b, q.b_cols, wgrad ? p.b_count : q.b_outer, q.ldb,
-                           static_cast<uint64_t>(q.b_depth), static_cast<uint64_t>(q.b_stack), 64, 64));
-    std::memset(&maps.b_row, 0, sizeof maps.b_row);
-    std::memset(&maps.t_row, 0, sizeof maps.t_row);
-    std::memset(&maps.e_box, 0, sizeof maps.e_box);
-    if (wgrad) {
-        GRP_TRY(encode_operand(&maps.b_row, q.ab_dtype, q.b, q.b_cols, p.b_count, q.ldb, 0, 0, 64, 1));
+    std::memset(&maps, 0, sizeof maps);
+    if (p.a_rows == nullptr) {
+        GRP_TRY(encode_operand(&maps.a_box, q.ab_dtype, q.a, q.a_cols, p.a_count, q.lda, 0, 0, 64,
+                               wgrad ? 64 : 128));
+    }
+    if (!wgrad || p.b_rows == nullptr) {
+        GRP_TRY(encode_operand(&maps.b_box, q.ab_dtype, q.b, q.b_cols, wgrad ? p.b_count : q.b_outer, q.ldb,
+                               static_cast<uint64_t>(q.b_depth), static_cast<uint64_t>(q.b_stack), 64, 64));
     }
     if (p.ext_groups > 0) {
-        GRP_TRY(encode_operand(&maps.t_row, q.ab_dtype, q.t, 2 * p.ext_cols, p.rows, q.ldt, 0, 0, 64, 1));
         GRP_TRY(encode_operand(&maps.e_box, q.ab_dtype, q.e, q.e_cols, q.e_outer, q.lde, p.ext_groups,
                                static_cast<uint64_t>(q.e_stack), 64, 64));
     }
+    p.a = q.a;
+    p.b = q.b;
+    p.t = q.t;
+    p.lda = q.lda;
+    p.ldb = q.ldb;
+    p.ldt = q.ldt;
     unsigned long long limit_ns = 0;
     const int fault = take_wait_fault(&limit_ns);
     p.wait_limit_ns = limit_ns;

@@ -13,16 +13,18 @@
 // read as zeros.  Low-rank adapters thereby cost neither a second pass over C nor tiles cut at
 // the borders of requests.
 //
-// Ragged edges and gathers are one mechanism: rows are fetched with TMA gather4 (four row
-// indices per copy, one copy per lane of the producer warp), and an index outside the tensor
-// reads zeros.  Whole tiles of consecutive rows use one boxed copy instead.
+// Consecutive rows arrive by boxed TMA copies.  Gathered rows arrive by cp.async from four loader
+// warps that write the same swizzled layout: TMA's own row gather (tile::gather4) took about 100
+// cycles per four rows, 3300 per 128 x 64 stage against the 512 the stage's MMAs need (4096^3:
+// 355 TFLOP/s gathered, 1113 boxed).  The loaders also write the zeros that masked rows need:
+// rows of other adapters, and in a weight gradient the positions behind the end of a group.
 //
 // Operand layout in shared memory is that of the dense kernel (gemm_umma.cuh): 128-byte rows of
 // 64 elements under the 128-byte swizzle.  The matrix whose reduced dimension is contiguous in
 // memory is read K-major, the other one MN-major, so nothing is ever transposed in memory.
 //
-// Warp roles as in the dense kernel: warp 0 producer, warp 1 MMA, warps 2-5 epilogue; two
-// accumulators in tensor memory; every wait bounded.
+// Warp roles: warp 0 TMA producer, warp 1 MMA, warps 2-5 epilogue as in the dense kernel, warps
+// 6-9 loaders; two accumulators in tensor memory; every wait bounded.
 #pragma once
 
 #include "gemm_umma.cuh"
@@ -50,6 +52,10 @@ struct GroupedParams {
     unsigned int* status;
     long long c_stride;  // kFormWgrad: elements from W_g to W_g+1
     int groups, rows;    // rows = positions in all
+    const void* a;       // what the loaders read: A, kFormWgrad's G, and T of the extension
+    const void* b;
+    const void* t;
+    int lda, ldb, ldt;
     int a_count, b_count, c_count;  // rows of A, G and C that exist
     int m, n, k;         // kFormWgrad: W_g is m x n; kFormRows: k columns of A, n columns of C
     int ldc;
@@ -57,7 +63,8 @@ struct GroupedParams {
     int form;
     int trans_b;         // kFormRows: B_g is stored n x k
     int bn;              // tile columns: 64, 128 or 256
-    // Two-part operands: the reduction runs over the matrix once per part, `part` columns apart.
+    // Two-part operands of kFormWgrad: the reduction runs over the rows once per part, the parts
+    // `part_cols` columns apart.
     int a_parts, a_part_cols;
     int b_parts, b_part_cols;
     int c_part_cols;     // TwoPart output: distance of lo behind hi
@@ -75,9 +82,9 @@ struct GroupedConfig {
     static constexpr uint32_t kBoxBytes = 64 * 64 * 2;
     static constexpr uint32_t kBBytes = 4 * kBoxBytes;
     static constexpr uint32_t kStageBytes = kABytes + kBBytes;
-    static constexpr int kThreads = 192;
+    static constexpr int kThreads = 192 + 32 * kStages;  // one loader warp per stage
     static constexpr uint32_t kStagingBytes = 4 * 4096;
-    static constexpr int kNumBarriers = 2 * kStages + 5;
+    static constexpr int kNumBarriers = 3 * kStages + 5;
     static constexpr uint32_t kTableBytes = 2 * (kMaxGemmGroups + 2) * 4;
     static constexpr uint32_t kSmemBytes =
         kStages * kStageBytes + kStagingBytes + kTableBytes + kNumBarriers * 8 + 16 + 1024;
@@ -155,7 +162,7 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, cons
         o.p0 = seg0 + mt * 128;
         o.valid = min(128, seg1 - o.p0);
         o.m0 = 0;
-        o.k_blocks = ((p.k + 63) / 64) * p.a_parts;
+        o.k_blocks = (p.k + 63) / 64;
         if (p.ext_groups > 0 && o.p0 < t.offs[p.ext_groups]) {
             // first adapter that ends behind p0, and the one after the last that starts in here
             o.ext_first = last_at_most(t.offs, p.ext_groups, o.p0);
@@ -181,10 +188,7 @@ struct GroupedStore<TwoPart<T>> {
 template <typename OutT>
 __global__ void __launch_bounds__(GroupedConfig::kThreads, 1)
 grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
-                    const __grid_constant__ CUtensorMap tmap_a_row,
                     const __grid_constant__ CUtensorMap tmap_b_box,
-                    const __grid_constant__ CUtensorMap tmap_b_row,
-                    const __grid_constant__ CUtensorMap tmap_t_row,
                     const __grid_constant__ CUtensorMap tmap_e_box, const GroupedParams p) {
     using Cfg = GroupedConfig;
     using Elem = typename GroupedStore<OutT>::Elem;
@@ -204,6 +208,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
     auto acc_full_bar = [&](uint32_t a) { return bars + 8u * (2 * kStages + a); };
     auto acc_empty_bar = [&](uint32_t a) { return bars + 8u * (2 * kStages + 2 + a); };
     const uint32_t drain_bar = bars + 8u * (2 * kStages + 4);
+    // a stage's rows written by the loaders (stages that need none never use it)
+    auto loaded_bar = [&](int s) { return bars + 8u * static_cast<uint32_t>(2 * kStages + 5 + s); };
     const uint32_t tmem_slot = bars + 8u * Cfg::kNumBarriers;
     volatile uint32_t* tmem_slot_ptr =
         reinterpret_cast<volatile uint32_t*>(bars_ptr + 8 * Cfg::kNumBarriers);
@@ -224,6 +230,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
         for (int s = 0; s < kStages; ++s) {
             ptx::mbar_init(full_bar(s), 1);
             ptx::mbar_init(empty_bar(s), 1);
+            ptx::mbar_init(loaded_bar(s), 1);
         }
         for (uint32_t a = 0; a < 2; ++a) {
             ptx::mbar_init(acc_full_bar(a), 1);
@@ -289,175 +296,103 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
     table.total = p.form == kFormWgrad ? p.groups * table.m_tiles * table.n_tiles
                                        : tile_count[table.segments] * table.n_tiles;
     const int ext_blocks_per_part = (p.ext_cols + 63) / 64;
-    const int base_blocks = (p.k + 63) / 64;
 
     // ---- roles ------------------------------------------------------------------------------
+    const bool gather_a = p.a_rows != nullptr;
+    const bool gather_b = p.form == kFormWgrad && p.b_rows != nullptr;
     if (warp == 0) {
-        // Producer: all 32 lanes, each issues its own copies.
-        uint32_t it = 0;
-        int stage = 0;
-        uint32_t phase = 0;
-        bool ok = true;
-        auto acquire_stage = [&]() -> bool {
-            int got = 1;
-            if (lane == 0) {
-                got = detail::wait_barrier(empty_bar(stage), phase ^ 1u, ctl, kRoleProducer, it) ? 1 : 0;
-            }
-            return __shfl_sync(0xFFFFFFFFu, got, 0) != 0;
-        };
-        auto announce = [&](uint32_t bytes) {
-            if (lane == 0) {
+        if (ptx::elect_one_sync()) {
+            // TMA producer.
+            uint32_t it = 0;
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            auto acquire_stage = [&](uint32_t bytes) -> bool {
+                if (!detail::wait_barrier(empty_bar(stage), phase ^ 1u, ctl, kRoleProducer, it)) {
+                    return false;
+                }
                 const bool wrong = p.overstate_first_stage != 0 && it == 0 && blockIdx.x == 0;
                 ptx::mbar_arrive_expect_tx(full_bar(stage), bytes + (wrong ? 16u : 0u));
-            }
-            __syncwarp();
-        };
-        auto advance = [&]() {
-            ++it;
-            if (++stage == kStages) {
-                stage = 0;
-                phase ^= 1u;
-            }
-        };
-        for (int tile = blockIdx.x; ok && tile < table.total; tile += gridDim.x) {
-            const detail::GroupedTile t = detail::grouped_tile(p, table, tile);
-            const int boxes = (t.cols + 63) / 64;
-            if (p.form == kFormRows) {
-                // Four rows of A per lane, the same for every k block.  Rows behind the tile's
-                // last one are not stored, so copies of only such rows are left out.
-                const int first = static_cast<int>(lane) * 4;
-                const bool gather = p.a_rows != nullptr || t.valid < 128;
-                int r[4] = {p.a_count, p.a_count, p.a_count, p.a_count};
-                if (gather) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (first + i < t.valid) {
-                            r[i] = p.a_rows != nullptr ? __ldg(p.a_rows + t.p0 + first + i)
-                                                       : t.p0 + first + i;
-                        }
-                    }
+                return true;
+            };
+            auto advance = [&]() {
+                ++it;
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1u;
                 }
-                const uint32_t a_bytes =
-                    gather ? static_cast<uint32_t>((t.valid + 3) / 4) * 512u : Cfg::kABytes;
-                const int group = table.whole ? 0 : t.group;
-                for (int kb = 0; kb < t.k_blocks; ++kb) {
-                    if (!acquire_stage()) {
-                        ok = false;
-                        break;
+            };
+            for (int tile = blockIdx.x; ok && tile < table.total; tile += gridDim.x) {
+                const detail::GroupedTile t = detail::grouped_tile(p, table, tile);
+                const int boxes = (t.cols + 63) / 64;
+                const uint32_t b_bytes = static_cast<uint32_t>(boxes) * Cfg::kBoxBytes;
+                // 64 k rows of matrix z of a stack, k0 on, as columns n0 .. of the tile
+                auto load_b = [&](uint32_t dst, const CUtensorMap* map, int k0, int z) {
+                    for (int b = 0; b < boxes; ++b) {
+                        const int col = t.n0 + b * 64;
+                        ptx::tma_load_3d(dst + b * Cfg::kBoxBytes, map, full_bar(stage),
+                                         p.trans_b ? k0 : col, p.trans_b ? col : k0, z);
                     }
-                    announce(a_bytes + static_cast<uint32_t>(boxes) * Cfg::kBoxBytes);
-                    const uint32_t a_dst = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
-                    const uint32_t b_dst = a_dst + Cfg::kABytes;
-                    const int part = kb >= base_blocks ? 1 : 0;
-                    const int k0 = (kb - part * base_blocks) * 64;
-                    const int ax = k0 + part * p.a_part_cols;
-                    if (gather) {
-                        if (first < t.valid) {
-                            ptx::tma_gather4(a_dst + lane * 512u, &tmap_a_row, full_bar(stage), ax,
-                                             r[0], r[1], r[2], r[3]);
-                        }
-                    } else if (lane == 0) {
-                        ptx::tma_load_2d(a_dst, &tmap_a_box, full_bar(stage), ax, t.p0);
-                    }
-                    if (static_cast<int>(lane) < boxes) {
-                        const int col = t.n0 + static_cast<int>(lane) * 64;
-                        ptx::tma_load_3d(b_dst + lane * Cfg::kBoxBytes, &tmap_b_box, full_bar(stage),
-                                         p.trans_b ? k0 : col, p.trans_b ? col : k0, group);
-                    }
-                    advance();
-                }
-                for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
-                    const int lo = max(offs[g], t.p0), hi = min(offs[g + 1], t.p0 + t.valid);
-                    if (lo >= hi) {
-                        continue;
-                    }
-                    int q[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int pos = t.p0 + first + i;
-                        q[i] = pos >= lo && pos < hi ? pos : p.rows;  // outside T: zeros
-                    }
-                    for (int eb = 0; eb < 2 * ext_blocks_per_part; ++eb) {
-                        if (!acquire_stage()) {
+                };
+                if (p.form == kFormRows) {
+                    const int group = table.whole ? 0 : t.group;
+                    for (int kb = 0; kb < t.k_blocks; ++kb) {
+                        if (!acquire_stage(b_bytes + (gather_a ? 0u : Cfg::kABytes))) {
                             ok = false;
                             break;
                         }
-                        announce(Cfg::kABytes + static_cast<uint32_t>(boxes) * Cfg::kBoxBytes);
                         const uint32_t a_dst = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
-                        const uint32_t b_dst = a_dst + Cfg::kABytes;
-                        const int part = eb >= ext_blocks_per_part ? 1 : 0;
-                        const int k0 = (eb - part * ext_blocks_per_part) * 64;
-                        ptx::tma_gather4(a_dst + lane * 512u, &tmap_t_row, full_bar(stage),
-                                         k0 + part * p.ext_cols, q[0], q[1], q[2], q[3]);
-                        if (static_cast<int>(lane) < boxes) {
-                            const int col = t.n0 + static_cast<int>(lane) * 64;
-                            ptx::tma_load_3d(b_dst + lane * Cfg::kBoxBytes, &tmap_e_box,
-                                             full_bar(stage), p.trans_b ? k0 : col,
-                                             p.trans_b ? col : k0, g);
+                        if (!gather_a) {
+                            // Rows behind the tile's last one belong to the next group (or lie
+                            // outside A): computed with and not stored.
+                            ptx::tma_load_2d(a_dst, &tmap_a_box, full_bar(stage), kb * 64, t.p0);
+                        }
+                        load_b(a_dst + Cfg::kABytes, &tmap_b_box, kb * 64, group);
+                        advance();
+                    }
+                    for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
+                        if (max(offs[g], t.p0) >= min(offs[g + 1], t.p0 + t.valid)) {
+                            continue;
+                        }
+                        for (int eb = 0; eb < 2 * ext_blocks_per_part; ++eb) {
+                            if (!acquire_stage(b_bytes)) {
+                                ok = false;
+                                break;
+                            }
+                            load_b(ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes + Cfg::kABytes,
+                                   &tmap_e_box,
+                                   (eb >= ext_blocks_per_part ? eb - ext_blocks_per_part : eb) * 64, g);
+                            advance();
+                        }
+                    }
+                } else {
+                    // Weight gradient: 64 positions per block, both operands MN-major.
+                    const int row_blocks = (t.valid + 63) / 64;
+                    const int a_boxes = (min(128, p.m - t.m0) + 63) / 64;
+                    const uint32_t bytes =
+                        (gather_b ? 0u : b_bytes) +
+                        (gather_a ? 0u : static_cast<uint32_t>(a_boxes) * Cfg::kBoxBytes);
+                    for (int kb = 0; kb < t.k_blocks; ++kb) {
+                        const int part = kb >= row_blocks ? 1 : 0;
+                        const int pos = t.p0 + (kb - part * row_blocks) * 64;
+                        if (!acquire_stage(bytes)) {
+                            ok = false;
+                            break;
+                        }
+                        const uint32_t a_dst = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
+                        for (int b = 0; !gather_a && b < a_boxes; ++b) {
+                            ptx::tma_load_2d(a_dst + b * Cfg::kBoxBytes, &tmap_a_box, full_bar(stage),
+                                             t.m0 + part * p.a_part_cols + b * 64, pos);
+                        }
+                        for (int b = 0; !gather_b && b < boxes; ++b) {
+                            ptx::tma_load_3d(a_dst + Cfg::kABytes + b * Cfg::kBoxBytes, &tmap_b_box,
+                                             full_bar(stage), t.n0 + part * p.b_part_cols + b * 64, pos, 0);
                         }
                         advance();
                     }
                 }
-            } else {
-                // Weight gradient: 64 positions per block, both operands MN-major.
-                const int row_blocks = (t.valid + 63) / 64;
-                const int a_boxes = (min(128, p.m - t.m0) + 63) / 64;
-                const int quad = static_cast<int>(lane & 15u);
-                const int half = static_cast<int>(lane >> 4);
-                for (int kb = 0; kb < t.k_blocks; ++kb) {
-                    const int part = kb >= row_blocks ? 1 : 0;
-                    const int i0 = (kb - part * row_blocks) * 64;
-                    const int left = t.valid - i0;
-                    const bool gather_a = p.a_rows != nullptr || left < 64;
-                    const bool gather_b = p.b_rows != nullptr || left < 64;
-                    int ra[4] = {p.a_count, p.a_count, p.a_count, p.a_count};
-                    int rb[4] = {p.b_count, p.b_count, p.b_count, p.b_count};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int in = quad * 4 + i;
-                        if (in < left) {
-                            const int pos = t.p0 + i0 + in;
-                            if (gather_a) {
-                                ra[i] = p.a_rows != nullptr ? __ldg(p.a_rows + pos) : pos;
-                            }
-                            if (gather_b) {
-                                rb[i] = p.b_rows != nullptr ? __ldg(p.b_rows + pos) : pos;
-                            }
-                        }
-                    }
-                    if (!acquire_stage()) {
-                        ok = false;
-                        break;
-                    }
-                    announce(static_cast<uint32_t>(a_boxes + boxes) * Cfg::kBoxBytes);
-                    const uint32_t a_dst = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
-                    const uint32_t b_dst = a_dst + Cfg::kABytes;
-                    const int ax = t.m0 + (p.a_parts > 1 ? part * p.a_part_cols : 0);
-                    const int bx = t.n0 + (p.b_parts > 1 ? part * p.b_part_cols : 0);
-                    if (gather_a) {
-                        if (half < a_boxes) {
-                            ptx::tma_gather4(a_dst + half * Cfg::kBoxBytes + quad * 512u, &tmap_a_row,
-                                             full_bar(stage), ax + half * 64, ra[0], ra[1], ra[2], ra[3]);
-                        }
-                    } else if (static_cast<int>(lane) < a_boxes) {
-                        ptx::tma_load_2d(a_dst + lane * Cfg::kBoxBytes, &tmap_a_box, full_bar(stage),
-                                         ax + static_cast<int>(lane) * 64, t.p0 + i0);
-                    }
-                    if (gather_b) {
-                        for (int b = half; b < boxes; b += 2) {
-                            ptx::tma_gather4(b_dst + b * Cfg::kBoxBytes + quad * 512u, &tmap_b_row,
-                                             full_bar(stage), bx + b * 64, rb[0], rb[1], rb[2], rb[3]);
-                        }
-                    } else if (static_cast<int>(lane) < boxes) {
-                        ptx::tma_load_3d(b_dst + lane * Cfg::kBoxBytes, &tmap_b_box, full_bar(stage),
-                                         bx + static_cast<int>(lane) * 64, t.p0 + i0, 0);
-                    }
-                    advance();
-                }
             }
-        }
-        // Tail: no copy may be in flight and no stage may still be signalled when the CTA ends.
-        if (lane == 0) {
+            // Tail: no copy may be in flight and no stage may still be signalled when the CTA ends.
             const uint32_t first = it > static_cast<uint32_t>(kStages) ? it - kStages : 0u;
             for (uint32_t i = first; i < it; ++i) {
                 const int s = static_cast<int>(i % kStages);
@@ -482,7 +417,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
             uint32_t it = 0;
             int stage = 0;
             uint32_t phase = 0;
+            uint32_t loaded_phase = 0;  // bit s: next phase of loaded_bar(s)
             uint32_t count = 0;
+            bool ready = false;  // the next stage's copies are known to have landed
             bool ok = true;
             for (int tile = blockIdx.x; ok && tile < table.total; tile += gridDim.x) {
                 const detail::GroupedTile t = detail::grouped_tile(p, table, tile);
@@ -500,9 +437,16 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                 const uint32_t idesc =
                     ptx::make_idesc_f16(p.fmt, a_mn ? 1u : 0u, b_mn ? 1u : 0u, 128, width);
                 uint32_t accumulate = 0;
-                auto block = [&](int steps) -> bool {
-                    if (!detail::wait_barrier(full_bar(stage), phase, ctl, kRoleMma, it)) {
+                auto block = [&](int steps, bool loaded) -> bool {
+                    if (!ready && !detail::wait_barrier(full_bar(stage), phase, ctl, kRoleMma, it)) {
                         return false;
+                    }
+                    if (loaded) {
+                        if (!detail::wait_barrier(loaded_bar(stage), (loaded_phase >> stage) & 1u, ctl,
+                                                  kRoleMma, 0x40000000u | it)) {
+                            return false;
+                        }
+                        loaded_phase ^= 1u << stage;
                     }
                     const uint32_t a_src = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
                     const uint32_t b_src = a_src + Cfg::kABytes;
@@ -517,6 +461,11 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                                           b_desc + static_cast<uint64_t>(j * b_step), idesc, accumulate);
                             accumulate = 1;
                         }
+                        if (j == 0) {
+                            // probed here so that its latency hides behind the MMAs
+                            ready = ptx::mbar_try_wait(full_bar(stage + 1 == kStages ? 0 : stage + 1),
+                                                       stage + 1 == kStages ? phase ^ 1u : phase);
+                        }
                     }
                     ptx::umma_commit(empty_bar(stage));
                     ++it;
@@ -526,8 +475,11 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     }
                     return true;
                 };
+                const int row_blocks = a_mn ? (t.valid + 63) / 64 : 0;
                 for (int kb = 0; kb < t.k_blocks; ++kb) {
-                    if (!block(4)) {
+                    const bool loaded = gather_a || gather_b ||
+                                        (a_mn && (t.valid & 63) != 0 && (kb + 1) % row_blocks == 0);
+                    if (!block(4, loaded)) {
                         ok = false;
                         break;
                     }
@@ -538,7 +490,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     }
                     for (int eb = 0; eb < 2 * ext_blocks_per_part; ++eb) {
                         const int in_part = eb >= ext_blocks_per_part ? eb - ext_blocks_per_part : eb;
-                        if (!block(min(4, (p.ext_cols - in_part * 64) / 16))) {
+                        if (!block(min(4, (p.ext_cols - in_part * 64) / 16), true)) {
                             ok = false;
                             break;
                         }
@@ -565,6 +517,258 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
             }
         }
         __syncwarp();
+    } else if (warp >= 6) {
+        // Loaders: warp 6 + s owns stage s, so four stages are in flight at once and each is handed
+        // over the moment its own copies have landed (one warp for all stages, or all warps for each
+        // stage, would hand over only in order and lag behind: 700 TFLOP/s at 4096^3).  Eight lanes
+        // copy the 128 bytes of one row (lane & 7 picks the 16-byte unit), four rows per instruction;
+        // the unit's place under the 128-byte swizzle depends on the row modulo 8.  The copies are
+        // generic-proxy writes: after they have landed a proxy fence orders them before the tensor
+        // core's reads, then one lane arrives.
+        const int own = warp - 6;
+        const int unit = static_cast<int>(lane & 7u);
+        const int sub = static_cast<int>(lane >> 3);
+        const uint32_t stage_base = ring + static_cast<uint32_t>(own) * Cfg::kStageBytes;
+        // rows 4 i + sub: row modulo 8 is sub for even i, sub + 4 for odd i
+        const uint32_t even = static_cast<uint32_t>(sub) * 128u +
+                              ((static_cast<uint32_t>(unit) ^ static_cast<uint32_t>(sub)) << 4);
+        const uint32_t odd = static_cast<uint32_t>(sub) * 128u + 512u +
+                             ((static_cast<uint32_t>(unit) ^ static_cast<uint32_t>(sub + 4)) << 4);
+        uint32_t it = 0;     // blocks of this CTA so far, whoever owns their stage
+        uint32_t phase = 0;  // of the own stage
+        bool ok = true;
+        auto wait_all = [&](uint32_t bar, uint32_t parity) -> bool {
+            const bool got = detail::wait_barrier(bar, parity, ctl, kRoleProducer, 0x20000000u | it);
+            return __all_sync(0xFFFFFFFFu, got) != 0;
+        };
+        auto mine = [&](uint32_t block) { return static_cast<int>(block % kStages) == own; };
+        // Every block of the own stage is waited for, even one that needs nothing from here: a
+        // barrier tells two adjacent phases apart, no more.
+        auto acquire = [&]() -> bool { return wait_all(empty_bar(own), phase ^ 1u); };
+        auto hand_over = [&]() {
+            ptx::cp_async_wait_all();
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                ptx::mbar_arrive(loaded_bar(own));
+            }
+        };
+        // The last unit of a row may hold fewer than 8 columns that exist: those are read one by
+        // one, so that nothing behind the last row is touched.
+        auto part_of_unit = [&](uint32_t dst, const void* row, int col, int have) {
+            uint32_t w[4] = {0, 0, 0, 0};
+            for (int e = 0; e < have; ++e) {
+                const uint32_t v = __ldg(static_cast<const unsigned short*>(row) + col + e);
+                w[0] |= e == 0 ? v : e == 1 ? v << 16 : 0u;
+                w[1] |= e == 2 ? v : e == 3 ? v << 16 : 0u;
+                w[2] |= e == 4 ? v : e == 5 ? v << 16 : 0u;
+                w[3] |= e == 6 ? v : 0u;
+            }
+            ptx::st_shared_16(dst, make_uint4(w[0], w[1], w[2], w[3]));
+        };
+        const bool needed = p.form == kFormWgrad || gather_a || p.ext_groups > 0;
+        for (int tile = blockIdx.x; needed && ok && tile < table.total; tile += gridDim.x) {
+            const detail::GroupedTile t = detail::grouped_tile(p, table, tile);
+            if (p.form == kFormRows) {
+                int src[4] = {-1, -1, -1, -1};  // lane l: rows l, 32 + l, 64 + l, 96 + l of A, -1: none
+                if (gather_a) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int r = q * 32 + static_cast<int>(lane);
+                        const int at = r < t.valid ? __ldg(p.a_rows + t.p0 + r) : -1;
+                        src[q] = at < p.a_count ? at : -1;
+                    }
+                }
+                for (int kb = 0; kb < t.k_blocks; ++kb, ++it) {
+                    if (!mine(it)) {
+                        continue;
+                    }
+                    if (!acquire()) {
+                        ok = false;
+                        break;
+                    }
+                    if (gather_a) {
+                        const int col = kb * 64 + unit * 8;
+                        const bool whole = col + 8 <= p.k;
+                        // (a unit that is not whole reads nothing here: any address will do)
+                        const char* base =
+                            static_cast<const char*>(p.a) + (whole ? static_cast<size_t>(col) * 2 : 0);
+                        const size_t pitch = static_cast<size_t>(p.lda) * 2;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            if (q * 32 >= t.valid) {
+                                break;
+                            }
+                            // eight shuffles, then eight copies: one after the other each pair would
+                            // cost its full latency (110 cycles)
+                            int at[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                at[i] = __shfl_sync(0xFFFFFFFFu, src[q], i * 4 + sub);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                ptx::cp_async_16(
+                                    stage_base + q * 4096u + (i >> 1) * 1024u + ((i & 1) ? odd : even),
+                                    base + max(at[i], 0) * pitch, at[i] >= 0 && whole);
+                            }
+                        }
+                        if (kb * 64 + 64 > p.k && (p.k & 7) != 0) {
+                            ptx::cp_async_wait_all();
+                            for (int r = 0; r < t.valid; r += 4) {
+                                const int at = __shfl_sync(
+                                    0xFFFFFFFFu, r < 32 ? src[0] : r < 64 ? src[1] : r < 96 ? src[2] : src[3],
+                                    (r & 31) + sub);
+                                if (!whole && col < p.k && at >= 0) {
+                                    part_of_unit(stage_base + (r >> 3) * 1024u + ((r & 4) ? odd : even),
+                                                 static_cast<const char*>(p.a) + at * pitch, col, p.k - col);
+                                }
+                            }
+                        }
+                        hand_over();
+                    }
+                    phase ^= 1u;
+                }
+                for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
+                    const int lo = max(offs[g], t.p0), hi = min(offs[g + 1], t.p0 + t.valid);
+                    if (lo >= hi) {
+                        continue;
+                    }
+                    for (int eb = 0; eb < 2 * ext_blocks_per_part; ++eb, ++it) {
+                        if (!mine(it)) {
+                            continue;
+                        }
+                        if (!acquire()) {
+                            ok = false;
+                            break;
+                        }
+                        const int part = eb >= ext_blocks_per_part ? 1 : 0;
+                        const int col = (eb - part * ext_blocks_per_part) * 64 + unit * 8;
+                        const char* base = static_cast<const char*>(p.t) +
+                                           (static_cast<size_t>(part) * p.ext_cols +
+                                            (col < p.ext_cols ? col : 0)) * 2;
+                        const size_t pitch = static_cast<size_t>(p.ldt) * 2;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            if (q * 32 >= t.valid) {
+                                break;
+                            }
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const int pos = t.p0 + q * 32 + i * 4 + sub;
+                                const bool take = pos >= lo && pos < hi && col < p.ext_cols;
+                                ptx::cp_async_16(
+                                    stage_base + q * 4096u + (i >> 1) * 1024u + ((i & 1) ? odd : even),
+                                    base + (take ? pos : 0) * pitch, take);
+                            }
+                        }
+                        hand_over();
+                        phase ^= 1u;
+                    }
+                }
+            } else {
+                const int row_blocks = (t.valid + 63) / 64;
+                const int a_boxes = (min(128, p.m - t.m0) + 63) / 64;
+                const int b_boxes = (t.cols + 63) / 64;
+                // Rows of A and G behind this lane's positions l and 32 + l of block kb.
+                int next_a[2], next_b[2];
+                auto fetch = [&](int kb) {
+                    const int i0 = (kb >= row_blocks ? kb - row_blocks : kb) * 64;
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int r = i0 + q * 32 + static_cast<int>(lane);
+                        const bool in = kb < t.k_blocks && r < t.valid;
+                        const int at_a = in && gather_a ? __ldg(p.a_rows + t.p0 + r) : -1;
+                        const int at_b = in && gather_b ? __ldg(p.b_rows + t.p0 + r) : -1;
+                        next_a[q] = at_a < p.a_count ? at_a : -1;
+                        next_b[q] = at_b < p.b_count ? at_b : -1;
+                    }
+                };
+                // 64 gathered rows of one operand: `boxes` boxes of 64 columns from column col0 on.
+                auto gather = [&](const void* from, int ld, const int (&rows)[2], uint32_t dst, int boxes,
+                                  int col0, int limit) {
+                    const size_t pitch = static_cast<size_t>(ld) * 2;
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const char* row[8];
+                        uint32_t exists = 0;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int at = __shfl_sync(0xFFFFFFFFu, rows[q], i * 4 + sub);
+                            exists |= at >= 0 ? 1u << i : 0u;
+                            row[i] = static_cast<const char*>(from) + max(at, 0) * pitch;
+                        }
+                        for (int b = 0; b < boxes; ++b) {
+                            const int col = col0 + b * 64 + unit * 8;
+                            const bool whole = col + 8 <= limit;
+                            const size_t skip = whole ? static_cast<size_t>(col) * 2 : 0;
+                            const uint32_t at = dst + b * Cfg::kBoxBytes + q * 4096u;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                ptx::cp_async_16(at + (i >> 1) * 1024u + ((i & 1) ? odd : even), row[i] + skip,
+                                                 ((exists >> i) & 1u) != 0 && whole);
+                            }
+                            if (!whole && col < limit) {
+                                ptx::cp_async_wait_all();
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) {
+                                    if ((exists >> i) & 1u) {
+                                        part_of_unit(at + (i >> 1) * 1024u + ((i & 1) ? odd : even), row[i],
+                                                     col, limit - col);
+                                    }
+                                }
+                            }
+                        }
+                    }
+                };
+                // the first block of this tile whose stage is the own one
+                const int first = (own - static_cast<int>(it % kStages) + kStages) % kStages;
+                fetch(first);
+                for (int kb = first; kb < t.k_blocks; kb += kStages) {
+                    const int part = kb >= row_blocks ? 1 : 0;
+                    const int left = t.valid - (kb - part * row_blocks) * 64;
+                    int ra[2] = {next_a[0], next_a[1]}, rb[2] = {next_b[0], next_b[1]};
+                    fetch(kb + kStages);
+                    if (!acquire()) {
+                        ok = false;
+                        break;
+                    }
+                    if (gather_a) {
+                        gather(p.a, p.lda, ra, stage_base, a_boxes, t.m0, p.m);
+                    }
+                    if (gather_b) {
+                        gather(p.b, p.ldb, rb, stage_base + Cfg::kABytes, b_boxes, t.n0, p.n);
+                    }
+                    if (left < 64 && !(gather_a && gather_b)) {
+                        // Positions behind the group's end: zeros in both operands (a zero in one
+                        // alone would leave 0 * NaN).  Gathered ones are zeros already; the boxed
+                        // ones are overwritten once the box has landed.
+                        if (!wait_all(full_bar(own), phase)) {
+                            ok = false;
+                            break;
+                        }
+                        for (int i = left / 4; i < 16; ++i) {
+                            if (i * 4 + sub < left) {
+                                continue;
+                            }
+                            const uint32_t at = stage_base + (i >> 1) * 1024u + ((i & 1) ? odd : even);
+                            for (int b = 0; !gather_a && b < a_boxes; ++b) {
+                                ptx::st_shared_zero_16(at + b * Cfg::kBoxBytes);
+                            }
+                            for (int b = 0; !gather_b && b < b_boxes; ++b) {
+                                ptx::st_shared_zero_16(at + Cfg::kABytes + b * Cfg::kBoxBytes);
+                            }
+                        }
+                    }
+                    if (gather_a || gather_b || left < 64) {
+                        hand_over();
+                    }
+                    phase ^= 1u;
+                }
+                it += static_cast<uint32_t>(t.k_blocks);
+            }
+        }
+        ptx::cp_async_wait_all();  // no copy may be in flight when the CTA ends
     } else {
         // Epilogue: 32 columns at a time through shared memory (FP32, 32 rows x 128 B per warp),
         // so that a warp writes whole 64- or 128-byte runs of a row wherever that row lies.
@@ -593,16 +797,12 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
             Elem* c_base = static_cast<Elem*>(p.c) +
                            (p.form == kFormWgrad ? static_cast<long long>(t.group) * p.c_stride : 0ll);
             const float factor = p.alpha * (p.scales != nullptr ? __ldg(p.scales + t.group) : 1.0f);
-            int ok = 1;
-            if (lane == 0) {
-                ok = detail::wait_barrier(acc_full_bar(acc), parity, ctl, kRoleEpilogue, count) ? 1 : 0;
-            }
-            ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
-            if (!ok) {
+            // All lanes wait: after a wait by one lane the warp may stay split in two, and the
+            // code behind it then runs several times slower.
+            const bool got = detail::wait_barrier(acc_full_bar(acc), parity, ctl, kRoleEpilogue, count);
+            if (!__all_sync(0xFFFFFFFFu, got)) {
                 alive = false;
                 break;
-            }
-            for (int i = 0; i < 1024 && !ptx::mbar_try_wait(acc_full_bar(acc), parity); ++i) {
             }
             ptx::tc_fence_after_sync();
             const bool nothing = t.k_blocks == 0 && t.ext_first == t.ext_last;

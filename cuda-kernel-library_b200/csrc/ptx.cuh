@@ -190,19 +190,27 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
         : "memory");
 }
 
-// Gather of four rows of a 2-D tensor whose map has a box one row high: the rows land one
-// behind the other at smem_dst.  A row index outside the tensor reads the fill value (0).
-__device__ __forceinline__ void tma_gather4(uint32_t smem_dst, const CUtensorMap* map, uint32_t bar,
-                                            int32_t x, int32_t r0, int32_t r1, int32_t r2,
-                                            int32_t r3) {
+// Asynchronous 16-byte copy by an ordinary thread (generic proxy); without `take` nothing is read
+// and the 16 bytes become zeros.  (All or nothing: a source size that is only known at run time
+// is emulated with branches, several times slower.)
+__device__ __forceinline__ void cp_async_16(uint32_t smem_dst, const void* src, bool take) {
     asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-        :
-        : "r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(r0), "r"(r1),
-          "r"(r2), "r"(r3)
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.eq.u32 p, %2, 0;\n\t"
+        "cp.async.cg.shared.global [%0], [%1], 16, p;\n\t"
+        "}" ::"r"(smem_dst), "l"(src), "r"(static_cast<uint32_t>(take))
         : "memory");
 }
+__device__ __forceinline__ void st_shared_16(uint32_t smem_dst, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(smem_dst), "r"(v.x), "r"(v.y), "r"(v.z),
+                 "r"(v.w)
+                 : "memory");
+}
+__device__ __forceinline__ void st_shared_zero_16(uint32_t smem_dst) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(smem_dst), "r"(0u) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // L2 eviction-priority hints for TMA loads (the 64-bit policy words that
 // createpolicy.fractional.L2::evict_{first,last} with fraction 1.0 produce).
