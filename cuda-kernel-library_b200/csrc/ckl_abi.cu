@@ -645,13 +645,18 @@ int encode_operand(CUtensorMap* map, int dtype, const void* base, uint64_t inner
     g_tensor_map_encodes.fetch_add(1, std::memory_order_relaxed);
     const cuuint32_t rank = depth == 0 ? 2 : 3;
     const cuuint64_t dims[3] = {inner, outer, depth};
-    const cuuint64_t strides[2] = {pitch * 2, stack * 2};
+    const uint64_t bytes = dtype_size(dtype);
+    const cuuint64_t strides[2] = {pitch * bytes, stack * bytes};
     const cuuint32_t box[3] = {box_inner, box_outer, 1};
     const cuuint32_t elem_strides[3] = {1, 1, 1};
     const CUresult r = ctx->encode(
-        map, dtype == CKL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
-        const_cast<void*>(base), dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
-        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+        map,
+        dtype == CKL_F16    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+        : dtype == CKL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT32,
+        rank, const_cast<void*>(base), dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        box_inner * bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+        CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         return fail(CKL_ERR_CUDA,

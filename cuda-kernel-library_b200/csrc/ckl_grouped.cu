@@ -67,7 +67,7 @@ int check_groups(const char* what, const int* offsets, int groups, int rows) {
 }
 
 struct Maps {
-    CUtensorMap a_box, b_box, e_box;
+    CUtensorMap a_box, b_box, e_box, c;
 };
 
 template <typename OutT>
@@ -89,7 +89,7 @@ int launch(const Maps& maps, const GroupedParams& p, int grid, cudaStream_t stre
         }
     }
     grouped_gemm_kernel<OutT><<<static_cast<unsigned>(grid), Cfg::kThreads, Cfg::kSmemBytes, stream>>>(
-        maps.a_box, maps.b_box, maps.e_box, p);
+        maps.a_box, maps.b_box, maps.e_box, maps.c, p);
     GRP_TRY_CUDA(cudaGetLastError());
     return CKL_OK;
 }
@@ -161,6 +161,12 @@ int run(Product& q, cudaStream_t stream) {
     const int bytes = size_of(q.c_dtype);
     p.c_vec = !misaligned(p.c, 16) && (static_cast<long long>(p.ldc) * bytes) % 16 == 0 &&
               (p.c_stride * bytes) % 16 == 0;
+    p.c_tma = p.c_vec && p.beta == 0.0f && p.c_rows == nullptr;
+    if (p.c_tma) {
+        GRP_TRY(encode_operand(&maps.c, q.c_dtype, p.c, p.n, wgrad ? p.m : p.rows, p.ldc, wgrad ? p.groups : 1,
+                               wgrad ? p.c_stride : static_cast<long long>(p.ldc) * p.rows,
+                               static_cast<uint32_t>(64 / bytes), 32));
+    }
     switch (q.c_dtype) {
         case CKL_F16: return launch<__half>(maps, p, grid, stream);
         case CKL_BF16: return launch<__nv_bfloat16>(maps, p, grid, stream);

@@ -21,9 +21,10 @@ struct DeviceView {
 };
 int device_view(DeviceView* out);
 
-// Encodes a TMA descriptor of a stack of row-major 16-bit matrices: `inner` columns, `outer` rows
-// of `pitch` elements, `depth` matrices `stack` elements apart (depth 0: one matrix, a 2-D map).
-// 128-byte swizzle, zeros outside.  An empty tensor gives an unused, zeroed descriptor.
+// Encodes a TMA descriptor of a stack of row-major matrices: `inner` columns, `outer` rows of
+// `pitch` elements, `depth` matrices `stack` elements apart (depth 0: one matrix, a 2-D map).
+// 64- or 128-byte swizzle, as wide as the box; zeros outside.  An empty tensor gives an unused,
+// zeroed descriptor.
 int encode_operand(CUtensorMap* map, int dtype, const void* base, uint64_t inner, uint64_t outer,
                    uint64_t pitch, uint64_t depth, uint64_t stack, uint32_t box_inner,
                    uint32_t box_outer);

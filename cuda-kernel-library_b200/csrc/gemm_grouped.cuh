@@ -72,6 +72,8 @@ struct GroupedParams {
     int ext_groups, ext_cols;  // adapters; columns of one part of T (a multiple of 16)
     uint32_t fmt;        // operand format for the instruction descriptor
     int c_vec;           // 16-byte accesses to C are legal
+    int c_tma;           // tmap_c describes C and nothing of it is read: whole 32-row runs are
+                         // written by TMA
     unsigned long long wait_limit_ns;
     int overstate_first_stage;  // test hook, see GemmParams
 };
@@ -189,7 +191,8 @@ template <typename OutT>
 __global__ void __launch_bounds__(GroupedConfig::kThreads, 1)
 grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     const __grid_constant__ CUtensorMap tmap_b_box,
-                    const __grid_constant__ CUtensorMap tmap_e_box, const GroupedParams p) {
+                    const __grid_constant__ CUtensorMap tmap_e_box,
+                    const __grid_constant__ CUtensorMap tmap_c, const GroupedParams p) {
     using Cfg = GroupedConfig;
     using Elem = typename GroupedStore<OutT>::Elem;
     constexpr bool kTwo = GroupedStore<OutT>::kTwo;
@@ -780,6 +783,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
         constexpr int kRowsPerPass = 32 / kLanesPerRow;
         const int sub = static_cast<int>(lane) % kLanesPerRow;
         uint32_t count = 0;
+        const uint32_t stg_addr = ring + kStages * Cfg::kStageBytes + quad * 4096u;
+        uint32_t buffer = 0;
         bool alive = true;
         for (int tile = blockIdx.x; alive && tile < table.total; tile += gridDim.x) {
             const detail::GroupedTile t = detail::grouped_tile(p, table, tile);
@@ -807,84 +812,145 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
             ptx::tc_fence_after_sync();
             const bool nothing = t.k_blocks == 0 && t.ext_first == t.ext_last;
             const uint32_t t_row = tmem_base + ((quad * 32u) << 16) + acc * 256u;
-            for (int c0 = 0; c0 < t.cols; c0 += 32) {
+            // All 32 rows of this warp are consecutive rows of C: 32-column chunks (64 or 128 bytes
+            // a row) go through one of two swizzled buffers and out by TMA, which clips at the edge
+            // of C.  Otherwise rows are written one by one.
+            const bool by_tma = !kTwo && p.c_tma != 0 &&
+                                (p.form == kFormWgrad ? t.m0 + static_cast<int>(quad) * 32 < p.m
+                                                      : static_cast<int>(quad) * 32 + 32 <= t.valid);
+            if (by_tma) {
+                constexpr uint32_t kRowBytes = 64;
+                constexpr int kCols = static_cast<int>(kRowBytes / sizeof(Elem));  // per buffer
+                const int row = p.form == kFormWgrad ? t.m0 + static_cast<int>(quad) * 32
+                                                     : t.p0 + static_cast<int>(quad) * 32;
+                const int z = p.form == kFormWgrad ? t.group : 0;
                 uint32_t r[32];
-                if (nothing) {
+                for (int c0 = 0; c0 < t.cols; c0 += 32) {
+                    if (nothing) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        r[i] = 0;
-                    }
-                } else {
-                    ptx::tmem_ld_32x32(t_row + static_cast<uint32_t>(c0), r);
-                    ptx::tmem_ld_wait();
-                }
-#pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    *reinterpret_cast<uint4*>(stg + lane * 128u + ((u ^ (lane & 7u)) << 4)) =
-                        make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]);
-                }
-                __syncwarp();
-                const int col = t.n0 + c0 + sub * kVec;
-                const int have = min(kVec, t.n0 + t.cols - col);
-#pragma unroll
-                for (int pass = 0; pass < 32 / kRowsPerPass; ++pass) {
-                    const int row = pass * kRowsPerPass + static_cast<int>(lane) / kLanesPerRow;
-                    const int c_row = __shfl_sync(0xFFFFFFFFu, my_row, row);
-                    float v[kVec];
-#pragma unroll
-                    for (int u = 0; u < kVec / 4; ++u) {
-                        const float4 x = *reinterpret_cast<const float4*>(
-                            stg + row * 128 + (((sub * (kVec / 4) + u) ^ (row & 7)) << 4));
-                        v[4 * u] = x.x; v[4 * u + 1] = x.y; v[4 * u + 2] = x.z; v[4 * u + 3] = x.w;
-                    }
-                    if (c_row < 0 || have <= 0) {
-                        continue;
-                    }
-                    Elem* dst = c_base + static_cast<size_t>(c_row) * p.ldc + col;
-                    const bool full = p.c_vec != 0 && have == kVec;
-#pragma unroll
-                    for (int i = 0; i < kVec; ++i) {
-                        v[i] *= factor;
-                    }
-                    if constexpr (kTwo) {
-                        float lo[kVec];
-#pragma unroll
-                        for (int i = 0; i < kVec; ++i) {
-                            Elem h;
-                            T::store(&h, v[i]);
-                            lo[i] = v[i] - T::load(&h);
+                        for (int i = 0; i < 32; ++i) {
+                            r[i] = 0;
                         }
-                        T::store_vec(dst, v);  // widths are multiples of 16 columns
-                        T::store_vec(dst + p.c_part_cols, lo);
                     } else {
-                        if (p.beta != 0.0f) {
-                            float old[kVec];
-                            if (full) {
-                                T::load_vec(dst, old);
-                            } else {
+                        ptx::tmem_ld_32x32(t_row + static_cast<uint32_t>(c0), r);
+                        ptx::tmem_ld_wait();
+                    }
 #pragma unroll
+                    for (int h = 0; h < 32 / kCols; ++h) {
+                        if (lane == 0) {
+                            ptx::bulk_wait_group_read<1>();  // the store two buffers ago has read its source
+                        }
+                        __syncwarp();
+                        uint8_t* buf = stg + buffer * 2048u;
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            float v[kVec];
+#pragma unroll
+                            for (int e = 0; e < kVec; ++e) {
+                                v[e] = factor * __uint_as_float(r[h * kCols + u * kVec + e]);
+                            }
+                            // 64-byte swizzle: the 16-byte unit is exchanged by row bits 1 and 2
+                            T::store_vec(reinterpret_cast<Elem*>(
+                                             buf + lane * kRowBytes +
+                                             ((static_cast<uint32_t>(u) ^ ((lane >> 1) & 3u)) << 4)),
+                                         v);
+                        }
+                        ptx::fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            ptx::tma_store_3d(&tmap_c, stg_addr + buffer * 2048u, t.n0 + c0 + h * kCols, row, z);
+                            ptx::bulk_commit_group();
+                        }
+                        buffer ^= 1u;
+                    }
+                }
+            } else {
+                if (p.c_tma != 0) {
+                    // the row-by-row path uses both buffers as one
+                    if (lane == 0) {
+                        ptx::bulk_wait_group_read<0>();
+                    }
+                    __syncwarp();
+                }
+                for (int c0 = 0; c0 < t.cols; c0 += 32) {
+                    uint32_t r[32];
+                    if (nothing) {
+    #pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            r[i] = 0;
+                        }
+                    } else {
+                        ptx::tmem_ld_32x32(t_row + static_cast<uint32_t>(c0), r);
+                        ptx::tmem_ld_wait();
+                    }
+    #pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        *reinterpret_cast<uint4*>(stg + lane * 128u + ((u ^ (lane & 7u)) << 4)) =
+                            make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]);
+                    }
+                    __syncwarp();
+                    const int col = t.n0 + c0 + sub * kVec;
+                    const int have = min(kVec, t.n0 + t.cols - col);
+    #pragma unroll
+                    for (int pass = 0; pass < 32 / kRowsPerPass; ++pass) {
+                        const int row = pass * kRowsPerPass + static_cast<int>(lane) / kLanesPerRow;
+                        const int c_row = __shfl_sync(0xFFFFFFFFu, my_row, row);
+                        float v[kVec];
+    #pragma unroll
+                        for (int u = 0; u < kVec / 4; ++u) {
+                            const float4 x = *reinterpret_cast<const float4*>(
+                                stg + row * 128 + (((sub * (kVec / 4) + u) ^ (row & 7)) << 4));
+                            v[4 * u] = x.x; v[4 * u + 1] = x.y; v[4 * u + 2] = x.z; v[4 * u + 3] = x.w;
+                        }
+                        if (c_row < 0 || have <= 0) {
+                            continue;
+                        }
+                        Elem* dst = c_base + static_cast<size_t>(c_row) * p.ldc + col;
+                        const bool full = p.c_vec != 0 && have == kVec;
+    #pragma unroll
+                        for (int i = 0; i < kVec; ++i) {
+                            v[i] *= factor;
+                        }
+                        if constexpr (kTwo) {
+                            float lo[kVec];
+    #pragma unroll
+                            for (int i = 0; i < kVec; ++i) {
+                                Elem h;
+                                T::store(&h, v[i]);
+                                lo[i] = v[i] - T::load(&h);
+                            }
+                            T::store_vec(dst, v);  // widths are multiples of 16 columns
+                            T::store_vec(dst + p.c_part_cols, lo);
+                        } else {
+                            if (p.beta != 0.0f) {
+                                float old[kVec];
+                                if (full) {
+                                    T::load_vec(dst, old);
+                                } else {
+    #pragma unroll
+                                    for (int i = 0; i < kVec; ++i) {
+                                        old[i] = i < have ? T::load(dst + i) : 0.0f;
+                                    }
+                                }
+    #pragma unroll
                                 for (int i = 0; i < kVec; ++i) {
-                                    old[i] = i < have ? T::load(dst + i) : 0.0f;
+                                    v[i] = fmaf(p.beta, old[i], v[i]);
                                 }
                             }
-#pragma unroll
-                            for (int i = 0; i < kVec; ++i) {
-                                v[i] = fmaf(p.beta, old[i], v[i]);
-                            }
-                        }
-                        if (full) {
-                            T::store_vec(dst, v);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < kVec; ++i) {
-                                if (i < have) {
-                                    T::store(dst + i, v[i]);
+                            if (full) {
+                                T::store_vec(dst, v);
+                            } else {
+    #pragma unroll
+                                for (int i = 0; i < kVec; ++i) {
+                                    if (i < have) {
+                                        T::store(dst + i, v[i]);
+                                    }
                                 }
                             }
                         }
                     }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
             ptx::tc_fence_before_sync();
             __syncwarp();
@@ -893,6 +959,10 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
             }
             ++count;
         }
+        if (lane == 0) {
+            ptx::bulk_wait_group_read<0>();  // no store may read shared memory when the CTA ends
+        }
+        __syncwarp();
     }
 
     ptx::tc_fence_before_sync();

@@ -262,6 +262,13 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t sm
                  : "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_src), "r"(x), "r"(y)
                  : "memory");
 }
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t smem_src, int32_t x,
+                                             int32_t y, int32_t z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+                 :
+                 : "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_src), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
 // Pulls one box of a tensor into L2 only (no shared-memory destination, no completion
 // to wait for); x obeys the 16-byte rule.
 __device__ __forceinline__ void tma_prefetch_l2_2d(const CUtensorMap* map, int32_t x, int32_t y) {
