@@ -85,7 +85,8 @@ struct GroupedConfig {
     static constexpr uint32_t kBBytes = 4 * kBoxBytes;
     static constexpr uint32_t kStageBytes = kABytes + kBBytes;
     static constexpr int kThreads = 192 + 32 * kStages;  // one loader warp per stage
-    static constexpr uint32_t kStagingBytes = 4 * 4096;
+    static constexpr int kBuffers = 3;  // of 2 KB (32 rows x 64 bytes) per epilogue warp
+    static constexpr uint32_t kStagingBytes = 4 * kBuffers * 2048;
     static constexpr int kNumBarriers = 3 * kStages + 5;
     static constexpr uint32_t kTableBytes = 2 * (kMaxGemmGroups + 2) * 4;
     static constexpr uint32_t kSmemBytes =
@@ -776,14 +777,14 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
         // Epilogue: 32 columns at a time through shared memory (FP32, 32 rows x 128 B per warp),
         // so that a warp writes whole 64- or 128-byte runs of a row wherever that row lies.
         const uint32_t quad = static_cast<uint32_t>(warp) & 3u;
-        uint8_t* stg = staging_ptr + quad * 4096;
+        uint8_t* stg = staging_ptr + quad * (Cfg::kBuffers * 2048);
         using T = detail::OutTraits<Elem>;
         constexpr int kVec = T::kVec;            // elements per 16 bytes
         constexpr int kLanesPerRow = 32 / kVec;  // 8 for FP32, 4 for 16-bit types
         constexpr int kRowsPerPass = 32 / kLanesPerRow;
         const int sub = static_cast<int>(lane) % kLanesPerRow;
         uint32_t count = 0;
-        const uint32_t stg_addr = ring + kStages * Cfg::kStageBytes + quad * 4096u;
+        const uint32_t stg_addr = ring + kStages * Cfg::kStageBytes + quad * (Cfg::kBuffers * 2048u);
         uint32_t buffer = 0;
         bool alive = true;
         for (int tile = blockIdx.x; alive && tile < table.total; tile += gridDim.x) {
@@ -812,8 +813,20 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
             ptx::tc_fence_after_sync();
             const bool nothing = t.k_blocks == 0 && t.ext_first == t.ext_last;
             const uint32_t t_row = tmem_base + ((quad * 32u) << 16) + acc * 256u;
+            // Hands the accumulator back to the MMA warp, once, when its last column is in registers.
+            bool released = false;
+            auto release = [&]() {
+                if (!released) {
+                    released = true;
+                    ptx::tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) {
+                        ptx::mbar_arrive(acc_empty_bar(acc));
+                    }
+                }
+            };
             // All 32 rows of this warp are consecutive rows of C: 32-column chunks (64 or 128 bytes
-            // a row) go through one of two swizzled buffers and out by TMA, which clips at the edge
+            // a row) go through a swizzled buffer and out by TMA, which clips at the edge
             // of C.  Otherwise rows are written one by one.
             const bool by_tma = !kTwo && p.c_tma != 0 &&
                                 (p.form == kFormWgrad ? t.m0 + static_cast<int>(quad) * 32 < p.m
@@ -825,35 +838,49 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                                                      : t.p0 + static_cast<int>(quad) * 32;
                 const int z = p.form == kFormWgrad ? t.group : 0;
                 uint32_t r[32];
-                for (int c0 = 0; c0 < t.cols; c0 += 32) {
-                    if (nothing) {
+                if (nothing) {
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            r[i] = 0;
+                    for (int i = 0; i < 32; ++i) {
+                        r[i] = 0;
+                    }
+                } else {
+                    ptx::tmem_ld_32x32(t_row, r);
+                }
+                for (int c0 = 0; c0 < t.cols; c0 += 32) {
+                    if (!nothing) {
+                        ptx::tmem_ld_wait();
+                    }
+                    uint4 out[32 / kVec];
+#pragma unroll
+                    for (int u = 0; u < 32 / kVec; ++u) {
+                        float v[kVec];
+#pragma unroll
+                        for (int e = 0; e < kVec; ++e) {
+                            v[e] = factor * __uint_as_float(r[u * kVec + e]);
+                        }
+                        T::store_vec(reinterpret_cast<Elem*>(&out[u]), v);
+                    }
+                    // the next chunk's columns travel while this one is stored
+                    if (c0 + 32 < t.cols) {
+                        if (!nothing) {
+                            ptx::tmem_ld_32x32(t_row + static_cast<uint32_t>(c0 + 32), r);
                         }
                     } else {
-                        ptx::tmem_ld_32x32(t_row + static_cast<uint32_t>(c0), r);
-                        ptx::tmem_ld_wait();
+                        release();
                     }
 #pragma unroll
                     for (int h = 0; h < 32 / kCols; ++h) {
                         if (lane == 0) {
-                            ptx::bulk_wait_group_read<1>();  // the store two buffers ago has read its source
+                            // the store that last used this buffer has read it
+                            ptx::bulk_wait_group_read<Cfg::kBuffers - 1>();
                         }
                         __syncwarp();
-                        uint8_t* buf = stg + buffer * 2048u;
+                        uint8_t* buf = stg + buffer * 2048u + lane * kRowBytes;
 #pragma unroll
                         for (int u = 0; u < 4; ++u) {
-                            float v[kVec];
-#pragma unroll
-                            for (int e = 0; e < kVec; ++e) {
-                                v[e] = factor * __uint_as_float(r[h * kCols + u * kVec + e]);
-                            }
                             // 64-byte swizzle: the 16-byte unit is exchanged by row bits 1 and 2
-                            T::store_vec(reinterpret_cast<Elem*>(
-                                             buf + lane * kRowBytes +
-                                             ((static_cast<uint32_t>(u) ^ ((lane >> 1) & 3u)) << 4)),
-                                         v);
+                            *reinterpret_cast<uint4*>(buf + ((static_cast<uint32_t>(u) ^ ((lane >> 1) & 3u))
+                                                             << 4)) = out[h * 4 + u];
                         }
                         ptx::fence_proxy_async_smem();
                         __syncwarp();
@@ -861,12 +888,12 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                             ptx::tma_store_3d(&tmap_c, stg_addr + buffer * 2048u, t.n0 + c0 + h * kCols, row, z);
                             ptx::bulk_commit_group();
                         }
-                        buffer ^= 1u;
+                        buffer = buffer + 1 == Cfg::kBuffers ? 0u : buffer + 1;
                     }
                 }
             } else {
                 if (p.c_tma != 0) {
-                    // the row-by-row path uses both buffers as one
+                    // the row-by-row path uses two of the buffers as one
                     if (lane == 0) {
                         ptx::bulk_wait_group_read<0>();
                     }
@@ -952,11 +979,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     __syncwarp();
                 }
             }
-            ptx::tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-                ptx::mbar_arrive(acc_empty_bar(acc));
-            }
+            release();
             ++count;
         }
         if (lane == 0) {
