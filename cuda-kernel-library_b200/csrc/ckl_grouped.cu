@@ -70,9 +70,9 @@ struct Maps {
     CUtensorMap a_box, b_box, e_box, c;
 };
 
-template <typename OutT>
+template <typename OutT, bool kSplit>
 int launch(const Maps& maps, const GroupedParams& p, int grid, cudaStream_t stream) {
-    using Cfg = GroupedConfig;
+    using Cfg = GroupedConfig<kSplit>;
     static std::mutex mu;
     static bool ready[64] = {};
     int dev = 0;
@@ -80,7 +80,7 @@ int launch(const Maps& maps, const GroupedParams& p, int grid, cudaStream_t stre
     {
         std::lock_guard<std::mutex> lock(mu);
         if (dev < 0 || dev >= 64 || !ready[dev]) {
-            GRP_TRY_CUDA(cudaFuncSetAttribute(grouped_gemm_kernel<OutT>,
+            GRP_TRY_CUDA(cudaFuncSetAttribute(grouped_gemm_kernel<OutT, kSplit>,
                                               cudaFuncAttributeMaxDynamicSharedMemorySize,
                                               static_cast<int>(Cfg::kSmemBytes)));
             if (dev >= 0 && dev < 64) {
@@ -88,10 +88,26 @@ int launch(const Maps& maps, const GroupedParams& p, int grid, cudaStream_t stre
             }
         }
     }
-    grouped_gemm_kernel<OutT><<<static_cast<unsigned>(grid), Cfg::kThreads, Cfg::kSmemBytes, stream>>>(
-        maps.a_box, maps.b_box, maps.e_box, maps.c, p);
-    GRP_TRY_CUDA(cudaGetLastError());
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(grid));
+    cfg.blockDim = dim3(Cfg::kThreads);
+    cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(p.split);
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = kSplit ? 1 : 0;
+    GRP_TRY_CUDA(cudaLaunchKernelEx(&cfg, grouped_gemm_kernel<OutT, kSplit>, maps.a_box, maps.b_box, maps.e_box,
+                                    maps.c, p));
     return CKL_OK;
+}
+template <typename OutT>
+int launch(const Maps& maps, const GroupedParams& p, int grid, cudaStream_t stream) {
+    return p.split > 1 ? launch<OutT, true>(maps, p, grid, stream)
+                       : launch<OutT, false>(maps, p, grid, stream);
 }
 
 // One product in terms of its operands; fills the descriptors and launches.
@@ -118,20 +134,40 @@ int run(Product& q, cudaStream_t stream) {
                               : p.offsets == nullptr || p.ext_groups > 0
                                   ? (p.rows + 127) / 128
                                   : p.rows / 128 + std::min(p.groups, p.rows);
-    // Tile width: the widest that still gives every SM a tile, so that a row of A is read the
-    // fewest times.
-    p.bn = p.n > 128 && m_tiles * ((p.n + 255) / 256) >= view.sm_count ? 256 : p.n > 64 ? 128 : 64;
-    const long long tiles = m_tiles * ((p.n + p.bn - 1) / p.bn);
-    if (tiles > 0x7fffffffll) {
+    // Tile width: with enough tiles for every SM the wider one, which reads A half as often, unless
+    // its last wave leaves more of the machine idle than the narrow one's extra loads cost (a tenth).
+    const auto tiles_of = [&](int bn) { return m_tiles * ((p.n + bn - 1) / bn); };
+    const auto cost_of = [&](int bn) {  // waves x columns
+        return static_cast<double>((tiles_of(bn) + view.sm_count - 1) / view.sm_count) * bn;
+    };
+    p.bn = p.n > 128 && cost_of(256) <= 1.1 * cost_of(128) ? 256 : p.n > 64 ? 128 : 64;
+    long long tiles = tiles_of(p.bn);
+    p.split = 1;
+    // Blocks of 64 reduced elements behind one tile, as far as the host can tell.
+    const long long blocks = wgrad ? static_cast<long long>(p.rows / p.groups + 63) / 64 * p.a_parts * p.b_parts
+                                   : (p.k + 63) / 64;
+    if (tiles_of(std::min(p.bn, 128)) * 2 <= view.sm_count) {
+        // Fewer tiles than half of the SMs: a cluster divides the blocks of each.
+        p.bn = std::min(p.bn, 128);
+        tiles = tiles_of(p.bn);
+        while (p.split < kMaxSplit && tiles * p.split * 2 <= view.sm_count && blocks >= p.split * 2 * 4) {
+            p.split *= 2;
+        }
+    }
+    if (tiles * p.split > 0x7fffffffll) {
         return set_error(CKL_ERR_TOO_LARGE, "%lld output tiles", tiles);
     }
     if (tiles == 0) {
         return CKL_OK;
     }
+    // Few rows to a tile: the loaders fetch those alone, where a boxed copy would fetch 128.
+    p.load_a = p.a_rows != nullptr ||
+               (!wgrad && p.k > 0 && p.offsets != nullptr && p.ext_groups == 0 &&
+                p.rows <= 32ll * std::min(p.groups, p.rows));
     // Gathered operands are read by the loader warps, all others through these descriptors.
     Maps maps;
     std::memset(&maps, 0, sizeof maps);
-    if (p.a_rows == nullptr) {
+    if (p.load_a == 0) {
         GRP_TRY(encode_operand(&maps.a_box, q.ab_dtype, q.a, q.a_cols, p.a_count, q.lda, 0, 0, 64,
                                wgrad ? 64 : 128));
     }
@@ -153,7 +189,7 @@ int run(Product& q, cudaStream_t stream) {
     const int fault = take_wait_fault(&limit_ns);
     p.wait_limit_ns = limit_ns;
     p.overstate_first_stage = fault == 1 ? 1 : 0;
-    const int grid = static_cast<int>(std::min<long long>(view.sm_count, tiles));
+    const int grid = static_cast<int>(p.split > 1 ? tiles * p.split : std::min<long long>(view.sm_count, tiles));
     if (q.c_dtype < 0) {
         return q.ab_dtype == CKL_BF16 ? launch<TwoPart<__nv_bfloat16>>(maps, p, grid, stream)
                                       : launch<TwoPart<__half>>(maps, p, grid, stream);
@@ -161,7 +197,7 @@ int run(Product& q, cudaStream_t stream) {
     const int bytes = size_of(q.c_dtype);
     p.c_vec = !misaligned(p.c, 16) && (static_cast<long long>(p.ldc) * bytes) % 16 == 0 &&
               (p.c_stride * bytes) % 16 == 0;
-    p.c_tma = p.c_vec && p.beta == 0.0f && p.c_rows == nullptr;
+    p.c_tma = p.c_vec && p.beta == 0.0f && p.c_rows == nullptr && p.split == 1;
     if (p.c_tma) {
         GRP_TRY(encode_operand(&maps.c, q.c_dtype, p.c, p.n, wgrad ? p.m : p.rows, p.ldc, wgrad ? p.groups : 1,
                                wgrad ? p.c_stride : static_cast<long long>(p.ldc) * p.rows,

@@ -71,6 +71,8 @@ struct GroupedParams {
     // Extension (ext_groups > 0): offsets/groups describe the adapters.
     int ext_groups, ext_cols;  // adapters; columns of one part of T (a multiple of 16)
     uint32_t fmt;        // operand format for the instruction descriptor
+    int split;           // CTAs per tile (a split launch)
+    int load_a;          // rows of A come through the loaders (gathered, or few per tile)
     int c_vec;           // 16-byte accesses to C are legal
     int c_tma;           // tmap_c describes C and nothing of it is read: whole 32-row runs are
                          // written by TMA
@@ -78,20 +80,24 @@ struct GroupedParams {
     int overstate_first_stage;  // test hook, see GemmParams
 };
 
+// kSplit: a cluster of CTAs shares one tile of at most 128 columns and divides its blocks; the
+// FP32 partial tiles meet in distributed shared memory.  For launches with fewer tiles than SMs.
+template <bool kSplit>
 struct GroupedConfig {
     static constexpr int kStages = 4;
     static constexpr uint32_t kABytes = 128 * 64 * 2;
     static constexpr uint32_t kBoxBytes = 64 * 64 * 2;
-    static constexpr uint32_t kBBytes = 4 * kBoxBytes;
+    static constexpr uint32_t kBBytes = (kSplit ? 2 : 4) * kBoxBytes;
     static constexpr uint32_t kStageBytes = kABytes + kBBytes;
     static constexpr int kThreads = 192 + 32 * kStages;  // one loader warp per stage
     static constexpr int kBuffers = 3;  // of 2 KB (32 rows x 64 bytes) per epilogue warp
-    static constexpr uint32_t kStagingBytes = 4 * kBuffers * 2048;
+    static constexpr uint32_t kStagingBytes = kSplit ? 128 * 128 * 4 : 4 * kBuffers * 2048;
     static constexpr int kNumBarriers = 3 * kStages + 5;
     static constexpr uint32_t kTableBytes = 2 * (kMaxGemmGroups + 2) * 4;
     static constexpr uint32_t kSmemBytes =
         kStages * kStageBytes + kStagingBytes + kTableBytes + kNumBarriers * 8 + 16 + 1024;
 };
+constexpr int kMaxSplit = 8;
 
 namespace detail {
 
@@ -175,6 +181,29 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, cons
     return o;
 }
 
+// Positions [lo, hi) of tile t that belong to adapter g.
+struct Span {
+    int lo, hi;
+};
+__device__ __forceinline__ Span adapter_span(const GroupedTable& table, const GroupedTile& t, int g) {
+    return {max(table.offs[g], t.p0), min(table.offs[g + 1], t.p0 + t.valid)};
+}
+
+// The share of a tile's blocks (main product, then adapters) that CTA `rank` of `size` runs.
+struct BlockRange {
+    int begin, end;
+};
+__device__ __forceinline__ BlockRange block_range(const GroupedParams& p, const GroupedTable& table,
+                                                  const GroupedTile& t, int rank, int size) {
+    int blocks = t.k_blocks;
+    for (int g = t.ext_first; g < t.ext_last; ++g) {
+        const Span s = adapter_span(table, t, g);
+        blocks += s.lo < s.hi ? 2 * ((p.ext_cols + 63) / 64) : 0;
+    }
+    return {static_cast<int>(static_cast<long long>(blocks) * rank / size),
+            static_cast<int>(static_cast<long long>(blocks) * (rank + 1) / size)};
+}
+
 }  // namespace detail
 
 template <typename OutT>
@@ -188,13 +217,82 @@ struct GroupedStore<TwoPart<T>> {
     static constexpr bool kTwo = true;
 };
 
-template <typename OutT>
-__global__ void __launch_bounds__(GroupedConfig::kThreads, 1)
+namespace detail {
+
+// One 16-byte unit of row c_row of C: `have` of its columns exist, v holds the raw sums.
+template <typename OutT, int kVec>
+__device__ __forceinline__ void store_unit(const GroupedParams& p,
+                                           typename GroupedStore<OutT>::Elem* c_base, int c_row, int col,
+                                           int have, float factor, float (&v)[kVec]) {
+    using Elem = typename GroupedStore<OutT>::Elem;
+    using T = OutTraits<Elem>;
+    Elem* dst = c_base + static_cast<size_t>(c_row) * p.ldc + col;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+        v[i] *= factor;
+    }
+    if constexpr (GroupedStore<OutT>::kTwo) {
+        float lo[kVec];
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+            Elem h;
+            T::store(&h, v[i]);
+            const float hi = T::load(&h);
+            lo[i] = isinf(hi) ? 0.0f : v[i] - hi;  // out of range stays infinite, inf - inf would not
+        }
+        T::store_vec(dst, v);  // widths are multiples of 16 columns
+        T::store_vec(dst + p.c_part_cols, lo);
+    } else {
+        const bool full = p.c_vec != 0 && have == kVec;
+        if (p.beta != 0.0f) {
+            float old[kVec];
+            if (full) {
+                T::load_vec(dst, old);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kVec; ++i) {
+                    old[i] = i < have ? T::load(dst + i) : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                v[i] = fmaf(p.beta, old[i], v[i]);
+            }
+        }
+        if (full) {
+            T::store_vec(dst, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                if (i < have) {
+                    T::store(dst + i, v[i]);
+                }
+            }
+        }
+    }
+}
+
+// Row of C behind row `in_tile` of a tile, -1 for none.
+__device__ __forceinline__ int row_of_c(const GroupedParams& p, const GroupedTile& t, int in_tile) {
+    if (p.form == kFormWgrad) {
+        return t.m0 + in_tile < p.m ? t.m0 + in_tile : -1;
+    }
+    if (in_tile >= t.valid) {
+        return -1;
+    }
+    const int row = p.c_rows != nullptr ? __ldg(p.c_rows + t.p0 + in_tile) : t.p0 + in_tile;
+    return row >= 0 && row < p.c_count ? row : -1;
+}
+
+}  // namespace detail
+
+template <typename OutT, bool kSplit>
+__global__ void __launch_bounds__(GroupedConfig<kSplit>::kThreads, 1)
 grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     const __grid_constant__ CUtensorMap tmap_b_box,
                     const __grid_constant__ CUtensorMap tmap_e_box,
                     const __grid_constant__ CUtensorMap tmap_c, const GroupedParams p) {
-    using Cfg = GroupedConfig;
+    using Cfg = GroupedConfig<kSplit>;
     using Elem = typename GroupedStore<OutT>::Elem;
     constexpr bool kTwo = GroupedStore<OutT>::kTwo;
     constexpr int kStages = Cfg::kStages;
@@ -299,10 +397,15 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
     const uint32_t tmem_base = *tmem_slot_ptr;
     table.total = p.form == kFormWgrad ? p.groups * table.m_tiles * table.n_tiles
                                        : tile_count[table.segments] * table.n_tiles;
-    const int ext_blocks_per_part = (p.ext_cols + 63) / 64;
+    const int ext_blocks = 2 * ((p.ext_cols + 63) / 64);  // of one adapter: both parts of T
+    // A split launch has one tile per cluster.
+    const int rank = kSplit ? static_cast<int>(ptx::cluster_cta_rank()) : 0;
+    const int size = kSplit ? p.split : 1;
+    const int first_tile = static_cast<int>(blockIdx.x) / size;
+    const int tile_step = kSplit ? 0x7fffffff - first_tile : static_cast<int>(gridDim.x);
 
     // ---- roles ------------------------------------------------------------------------------
-    const bool gather_a = p.a_rows != nullptr;
+    const bool gather_a = p.load_a != 0;
     const bool gather_b = p.form == kFormWgrad && p.b_rows != nullptr;
     if (warp == 0) {
         if (ptx::elect_one_sync()) {
@@ -326,8 +429,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     phase ^= 1u;
                 }
             };
-            for (int tile = blockIdx.x; ok && tile < table.total; tile += gridDim.x) {
+            for (int tile = first_tile; ok && tile < table.total; tile += tile_step) {
                 const detail::GroupedTile t = detail::grouped_tile(p, table, tile);
+                const detail::BlockRange mine = detail::block_range(p, table, t, rank, size);
                 const int boxes = (t.cols + 63) / 64;
                 const uint32_t b_bytes = static_cast<uint32_t>(boxes) * Cfg::kBoxBytes;
                 // 64 k rows of matrix z of a stack, k0 on, as columns n0 .. of the tile
@@ -340,7 +444,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                 };
                 if (p.form == kFormRows) {
                     const int group = table.whole ? 0 : t.group;
-                    for (int kb = 0; kb < t.k_blocks; ++kb) {
+                    for (int kb = mine.begin; kb < min(mine.end, t.k_blocks); ++kb) {
                         if (!acquire_stage(b_bytes + (gather_a ? 0u : Cfg::kABytes))) {
                             ok = false;
                             break;
@@ -354,20 +458,22 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                         load_b(a_dst + Cfg::kABytes, &tmap_b_box, kb * 64, group);
                         advance();
                     }
+                    int at = t.k_blocks;  // index of the adapter's first block in the tile
                     for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
-                        if (max(offs[g], t.p0) >= min(offs[g + 1], t.p0 + t.valid)) {
+                        const detail::Span span = detail::adapter_span(table, t, g);
+                        if (span.lo >= span.hi) {
                             continue;
                         }
-                        for (int eb = 0; eb < 2 * ext_blocks_per_part; ++eb) {
+                        for (int eb = max(0, mine.begin - at); eb < min(ext_blocks, mine.end - at); ++eb) {
                             if (!acquire_stage(b_bytes)) {
                                 ok = false;
                                 break;
                             }
                             load_b(ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes + Cfg::kABytes,
-                                   &tmap_e_box,
-                                   (eb >= ext_blocks_per_part ? eb - ext_blocks_per_part : eb) * 64, g);
+                                   &tmap_e_box, (eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb) * 64, g);
                             advance();
                         }
+                        at += ext_blocks;
                     }
                 } else {
                     // Weight gradient: 64 positions per block, both operands MN-major.
@@ -376,7 +482,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     const uint32_t bytes =
                         (gather_b ? 0u : b_bytes) +
                         (gather_a ? 0u : static_cast<uint32_t>(a_boxes) * Cfg::kBoxBytes);
-                    for (int kb = 0; kb < t.k_blocks; ++kb) {
+                    for (int kb = mine.begin; kb < mine.end; ++kb) {
                         const int part = kb >= row_blocks ? 1 : 0;
                         const int pos = t.p0 + (kb - part * row_blocks) * 64;
                         if (!acquire_stage(bytes)) {
@@ -425,7 +531,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
             uint32_t count = 0;
             bool ready = false;  // the next stage's copies are known to have landed
             bool ok = true;
-            for (int tile = blockIdx.x; ok && tile < table.total; tile += gridDim.x) {
+            for (int tile = first_tile; ok && tile < table.total; tile += tile_step) {
                 const detail::GroupedTile t = detail::grouped_tile(p, table, tile);
                 const uint32_t acc = count & 1u;
                 if (!detail::wait_barrier(acc_empty_bar(acc), ((count >> 1) & 1u) ^ 1u, ctl, kRoleMma,
@@ -479,8 +585,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     }
                     return true;
                 };
+                const detail::BlockRange mine = detail::block_range(p, table, t, rank, size);
                 const int row_blocks = a_mn ? (t.valid + 63) / 64 : 0;
-                for (int kb = 0; kb < t.k_blocks; ++kb) {
+                for (int kb = mine.begin; kb < min(mine.end, t.k_blocks); ++kb) {
                     const bool loaded = gather_a || gather_b ||
                                         (a_mn && (t.valid & 63) != 0 && (kb + 1) % row_blocks == 0);
                     if (!block(4, loaded)) {
@@ -488,17 +595,20 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                         break;
                     }
                 }
+                int at = t.k_blocks;
                 for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
-                    if (max(offs[g], t.p0) >= min(offs[g + 1], t.p0 + t.valid)) {
+                    const detail::Span span = detail::adapter_span(table, t, g);
+                    if (span.lo >= span.hi) {
                         continue;
                     }
-                    for (int eb = 0; eb < 2 * ext_blocks_per_part; ++eb) {
-                        const int in_part = eb >= ext_blocks_per_part ? eb - ext_blocks_per_part : eb;
+                    for (int eb = max(0, mine.begin - at); eb < min(ext_blocks, mine.end - at); ++eb) {
+                        const int in_part = eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb;
                         if (!block(min(4, (p.ext_cols - in_part * 64) / 16), true)) {
                             ok = false;
                             break;
                         }
                     }
+                    at += ext_blocks;
                 }
                 if (ok) {
                     if (accumulate != 0) {
@@ -571,19 +681,22 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
             ptx::st_shared_16(dst, make_uint4(w[0], w[1], w[2], w[3]));
         };
         const bool needed = p.form == kFormWgrad || gather_a || p.ext_groups > 0;
-        for (int tile = blockIdx.x; needed && ok && tile < table.total; tile += gridDim.x) {
+        for (int tile = first_tile; needed && ok && tile < table.total; tile += tile_step) {
             const detail::GroupedTile t = detail::grouped_tile(p, table, tile);
+            const detail::BlockRange range = detail::block_range(p, table, t, rank, size);
             if (p.form == kFormRows) {
                 int src[4] = {-1, -1, -1, -1};  // lane l: rows l, 32 + l, 64 + l, 96 + l of A, -1: none
                 if (gather_a) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const int r = q * 32 + static_cast<int>(lane);
-                        const int at = r < t.valid ? __ldg(p.a_rows + t.p0 + r) : -1;
+                        const int at = r >= t.valid          ? -1
+                                       : p.a_rows != nullptr ? __ldg(p.a_rows + t.p0 + r)
+                                                             : t.p0 + r;
                         src[q] = at < p.a_count ? at : -1;
                     }
                 }
-                for (int kb = 0; kb < t.k_blocks; ++kb, ++it) {
+                for (int kb = range.begin; kb < min(range.end, t.k_blocks); ++kb, ++it) {
                     if (!mine(it)) {
                         continue;
                     }
@@ -633,12 +746,14 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     }
                     phase ^= 1u;
                 }
+                int first_block = t.k_blocks;
                 for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
-                    const int lo = max(offs[g], t.p0), hi = min(offs[g + 1], t.p0 + t.valid);
-                    if (lo >= hi) {
+                    const detail::Span span = detail::adapter_span(table, t, g);
+                    if (span.lo >= span.hi) {
                         continue;
                     }
-                    for (int eb = 0; eb < 2 * ext_blocks_per_part; ++eb, ++it) {
+                    const int eb_end = min(ext_blocks, range.end - first_block);
+                    for (int eb = max(0, range.begin - first_block); eb < eb_end; ++eb, ++it) {
                         if (!mine(it)) {
                             continue;
                         }
@@ -646,8 +761,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                             ok = false;
                             break;
                         }
-                        const int part = eb >= ext_blocks_per_part ? 1 : 0;
-                        const int col = (eb - part * ext_blocks_per_part) * 64 + unit * 8;
+                        const int part = eb >= ext_blocks / 2 ? 1 : 0;
+                        const int col = (eb - part * (ext_blocks / 2)) * 64 + unit * 8;
                         const char* base = static_cast<const char*>(p.t) +
                                            (static_cast<size_t>(part) * p.ext_cols +
                                             (col < p.ext_cols ? col : 0)) * 2;
@@ -660,7 +775,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
                                 const int pos = t.p0 + q * 32 + i * 4 + sub;
-                                const bool take = pos >= lo && pos < hi && col < p.ext_cols;
+                                const bool take = pos >= span.lo && pos < span.hi && col < p.ext_cols;
                                 ptx::cp_async_16(
                                     stage_base + q * 4096u + (i >> 1) * 1024u + ((i & 1) ? odd : even),
                                     base + (take ? pos : 0) * pitch, take);
@@ -669,6 +784,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                         hand_over();
                         phase ^= 1u;
                     }
+                    first_block += ext_blocks;
                 }
             } else {
                 const int row_blocks = (t.valid + 63) / 64;
@@ -681,7 +797,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         const int r = i0 + q * 32 + static_cast<int>(lane);
-                        const bool in = kb < t.k_blocks && r < t.valid;
+                        const bool in = kb < range.end && r < t.valid;
                         const int at_a = in && gather_a ? __ldg(p.a_rows + t.p0 + r) : -1;
                         const int at_b = in && gather_b ? __ldg(p.b_rows + t.p0 + r) : -1;
                         next_a[q] = at_a < p.a_count ? at_a : -1;
@@ -726,9 +842,10 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     }
                 };
                 // the first block of this tile whose stage is the own one
-                const int first = (own - static_cast<int>(it % kStages) + kStages) % kStages;
+                const int first =
+                    range.begin + (own - static_cast<int>(it % kStages) + kStages) % kStages;
                 fetch(first);
-                for (int kb = first; kb < t.k_blocks; kb += kStages) {
+                for (int kb = first; kb < range.end; kb += kStages) {
                     const int part = kb >= row_blocks ? 1 : 0;
                     const int left = t.valid - (kb - part * row_blocks) * 64;
                     int ra[2] = {next_a[0], next_a[1]}, rb[2] = {next_b[0], next_b[1]};
@@ -769,7 +886,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     }
                     phase ^= 1u;
                 }
-                it += static_cast<uint32_t>(t.k_blocks);
+                it += static_cast<uint32_t>(range.end - range.begin);
             }
         }
         ptx::cp_async_wait_all();  // no copy may be in flight when the CTA ends
@@ -785,21 +902,16 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
         const int sub = static_cast<int>(lane) % kLanesPerRow;
         uint32_t count = 0;
         const uint32_t stg_addr = ring + kStages * Cfg::kStageBytes + quad * (Cfg::kBuffers * 2048u);
+        const uint32_t stg_all = ring + kStages * Cfg::kStageBytes;
         uint32_t buffer = 0;
         bool alive = true;
-        for (int tile = blockIdx.x; alive && tile < table.total; tile += gridDim.x) {
+        for (int tile = first_tile; alive && tile < table.total; tile += tile_step) {
             const detail::GroupedTile t = detail::grouped_tile(p, table, tile);
             const uint32_t acc = count & 1u;
             const uint32_t parity = (count >> 1) & 1u;
             // Row of C that lane `lane` of this warp stands for, -1 for none.
             const int in_tile = static_cast<int>(quad) * 32 + static_cast<int>(lane);
-            int my_row = -1;
-            if (p.form == kFormWgrad) {
-                my_row = t.m0 + in_tile < p.m ? t.m0 + in_tile : -1;
-            } else if (in_tile < t.valid) {
-                my_row = p.c_rows != nullptr ? __ldg(p.c_rows + t.p0 + in_tile) : t.p0 + in_tile;
-                my_row = my_row >= 0 && my_row < p.c_count ? my_row : -1;
-            }
+            const int my_row = detail::row_of_c(p, t, in_tile);
             Elem* c_base = static_cast<Elem*>(p.c) +
                            (p.form == kFormWgrad ? static_cast<long long>(t.group) * p.c_stride : 0ll);
             const float factor = p.alpha * (p.scales != nullptr ? __ldg(p.scales + t.group) : 1.0f);
@@ -811,7 +923,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                 break;
             }
             ptx::tc_fence_after_sync();
-            const bool nothing = t.k_blocks == 0 && t.ext_first == t.ext_last;
+            const detail::BlockRange mine = detail::block_range(p, table, t, rank, size);
+            const bool nothing = mine.begin == mine.end;
             const uint32_t t_row = tmem_base + ((quad * 32u) << 16) + acc * 256u;
             // Hands the accumulator back to the MMA warp, once, when its last column is in registers.
             bool released = false;
@@ -825,6 +938,31 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     }
                 }
             };
+            if constexpr (kSplit) {
+                // Park the partial tile: 512 bytes a row, the 16-byte units exchanged by the row
+                // so that the 32 rows of a store hit all banks.
+                const uint32_t row_addr = stg_all + static_cast<uint32_t>(in_tile) * 512u;
+                for (int c0 = 0; c0 < t.cols; c0 += 32) {
+                    uint32_t r[32];
+                    if (nothing) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            r[i] = 0;
+                        }
+                    } else {
+                        ptx::tmem_ld_32x32(t_row + static_cast<uint32_t>(c0), r);
+                        ptx::tmem_ld_wait();
+                    }
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        ptx::st_shared_16(row_addr + (((c0 / 4 + u) ^ lane) << 4),
+                                          make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]));
+                    }
+                }
+                release();
+                ++count;
+                continue;
+            }
             // All 32 rows of this warp are consecutive rows of C: 32-column chunks (64 or 128 bytes
             // a row) go through a swizzled buffer and out by TMA, which clips at the edge
             // of C.  Otherwise rows are written one by one.
@@ -902,7 +1040,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                 for (int c0 = 0; c0 < t.cols; c0 += 32) {
                     uint32_t r[32];
                     if (nothing) {
-    #pragma unroll
+#pragma unroll
                         for (int i = 0; i < 32; ++i) {
                             r[i] = 0;
                         }
@@ -910,7 +1048,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                         ptx::tmem_ld_32x32(t_row + static_cast<uint32_t>(c0), r);
                         ptx::tmem_ld_wait();
                     }
-    #pragma unroll
+#pragma unroll
                     for (int u = 0; u < 8; ++u) {
                         *reinterpret_cast<uint4*>(stg + lane * 128u + ((u ^ (lane & 7u)) << 4)) =
                             make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]);
@@ -918,62 +1056,19 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     __syncwarp();
                     const int col = t.n0 + c0 + sub * kVec;
                     const int have = min(kVec, t.n0 + t.cols - col);
-    #pragma unroll
+#pragma unroll
                     for (int pass = 0; pass < 32 / kRowsPerPass; ++pass) {
                         const int row = pass * kRowsPerPass + static_cast<int>(lane) / kLanesPerRow;
                         const int c_row = __shfl_sync(0xFFFFFFFFu, my_row, row);
                         float v[kVec];
-    #pragma unroll
+#pragma unroll
                         for (int u = 0; u < kVec / 4; ++u) {
                             const float4 x = *reinterpret_cast<const float4*>(
                                 stg + row * 128 + (((sub * (kVec / 4) + u) ^ (row & 7)) << 4));
                             v[4 * u] = x.x; v[4 * u + 1] = x.y; v[4 * u + 2] = x.z; v[4 * u + 3] = x.w;
                         }
-                        if (c_row < 0 || have <= 0) {
-                            continue;
-                        }
-                        Elem* dst = c_base + static_cast<size_t>(c_row) * p.ldc + col;
-                        const bool full = p.c_vec != 0 && have == kVec;
-    #pragma unroll
-                        for (int i = 0; i < kVec; ++i) {
-                            v[i] *= factor;
-                        }
-                        if constexpr (kTwo) {
-                            float lo[kVec];
-    #pragma unroll
-                            for (int i = 0; i < kVec; ++i) {
-                                Elem h;
-                                T::store(&h, v[i]);
-                                lo[i] = v[i] - T::load(&h);
-                            }
-                            T::store_vec(dst, v);  // widths are multiples of 16 columns
-                            T::store_vec(dst + p.c_part_cols, lo);
-                        } else {
-                            if (p.beta != 0.0f) {
-                                float old[kVec];
-                                if (full) {
-                                    T::load_vec(dst, old);
-                                } else {
-    #pragma unroll
-                                    for (int i = 0; i < kVec; ++i) {
-                                        old[i] = i < have ? T::load(dst + i) : 0.0f;
-                                    }
-                                }
-    #pragma unroll
-                                for (int i = 0; i < kVec; ++i) {
-                                    v[i] = fmaf(p.beta, old[i], v[i]);
-                                }
-                            }
-                            if (full) {
-                                T::store_vec(dst, v);
-                            } else {
-    #pragma unroll
-                                for (int i = 0; i < kVec; ++i) {
-                                    if (i < have) {
-                                        T::store(dst + i, v[i]);
-                                    }
-                                }
-                            }
+                        if (c_row >= 0 && have > 0) {
+                            detail::store_unit<OutT, kVec>(p, c_base, c_row, col, have, factor, v);
                         }
                     }
                     __syncwarp();
@@ -988,6 +1083,53 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
         __syncwarp();
     }
 
+    if constexpr (kSplit) {
+        // The parts of the tile meet: row i of the tile is summed by CTA i mod size, part 0 first.
+        ptx::cluster_arrive_release();
+        ptx::cluster_wait_acquire();
+        if (first_tile < table.total) {
+            constexpr int kVec = detail::OutTraits<Elem>::kVec;
+            constexpr int kLanesPerRow = 128 / kVec;
+            constexpr int kRowsPerWarp = 32 / kLanesPerRow;
+            constexpr int kWarps = Cfg::kThreads / 32;
+            const detail::GroupedTile t = detail::grouped_tile(p, table, first_tile);
+            const int rows = p.form == kFormWgrad ? min(128, p.m - t.m0) : t.valid;
+            const int sub = static_cast<int>(lane) % kLanesPerRow;
+            const int col = t.n0 + sub * kVec;
+            const int have = min(kVec, t.n0 + t.cols - col);
+            const float factor = p.alpha * (p.scales != nullptr ? __ldg(p.scales + t.group) : 1.0f);
+            Elem* c_base = static_cast<Elem*>(p.c) +
+                           (p.form == kFormWgrad ? static_cast<long long>(t.group) * p.c_stride : 0ll);
+            const uint32_t parts = ring + kStages * Cfg::kStageBytes;
+            for (int i = warp * kRowsPerWarp + static_cast<int>(lane) / kLanesPerRow; i * size + rank < rows;
+                 i += kWarps * kRowsPerWarp) {
+                const int row = i * size + rank;
+                const int c_row = detail::row_of_c(p, t, row);
+                if (c_row < 0 || have <= 0) {
+                    continue;
+                }
+                float v[kVec] = {};
+                for (int q = 0; q < size; ++q) {
+                    const uint32_t from =
+                        ptx::map_to_cta(parts + static_cast<uint32_t>(row) * 512u, static_cast<uint32_t>(q));
+#pragma unroll
+                    for (int u = 0; u < kVec / 4; ++u) {
+                        const float4 x = ptx::ld_cluster_16(
+                            from + (((sub * (kVec / 4) + u) ^ (row & 31)) << 4));
+                        v[4 * u] += x.x;
+                        v[4 * u + 1] += x.y;
+                        v[4 * u + 2] += x.z;
+                        v[4 * u + 3] += x.w;
+                    }
+                }
+                detail::store_unit<OutT, kVec>(p, c_base, c_row, col, have, factor, v);
+            }
+        }
+        // No CTA leaves while another still reads its part.
+        __syncwarp();
+        ptx::cluster_arrive_release();
+        ptx::cluster_wait_acquire();
+    }
     ptx::tc_fence_before_sync();
     __syncthreads();
     if (warp == 1) {

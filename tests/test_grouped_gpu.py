@@ -361,3 +361,68 @@ def test_wait_that_runs_out_is_reported(ckl):
     ckl.gemm_grouped(ckl.BF16, a, b, c, ckl.F32, offs, 1, 5, 64, 128)
     torch.cuda.synchronize()
     check(c, a.double() @ b[0].double(), a.double().abs() @ b[0].double().abs(), 128, "f32")
+
+
+@pytest.mark.parametrize("n,k", [(200, 1000), (64, 4096), (24, 2056)])
+@pytest.mark.parametrize("trans", [False, True], ids=["nn", "nt"])
+@pytest.mark.parametrize("gather", [False, True], ids=["rows", "gather"])
+def test_grouped_few_tiles_share_the_sum(ckl, n, k, trans, gather):
+    """Few tiles and a long sum: clusters of CTAs divide the sum, and the parts meet."""
+    for sizes in ([1, 0, 3, 40], [140], [2]):
+        offs = offsets_of(sizes)
+        rows = int(offs[-1])
+        a = rand((rows, k), DT["f16"], 1)
+        idx = torch.randperm(rows, device="cuda").int() if gather else None
+        b = rand((len(sizes), n, k) if trans else (len(sizes), k, n), DT["f16"], 2, k ** -0.5)
+        c = rand((rows + 1, n), torch.float32, 3)
+        c0 = c.clone()
+        ckl.gemm_grouped(ckl.F16, a, b, c, ckl.F32, offs, len(sizes), rows, n, k, a_rows=idx,
+                         a_count=rows if gather else None, trans_b=trans, alpha=0.5, beta=2.0)
+        torch.cuda.synchronize()
+        assert torch.equal(c[rows:], c0[rows:])
+        src = a[idx.long()] if gather else a
+        o = offs.tolist()
+        for g in range(len(sizes)):
+            x, w = src[o[g]:o[g + 1]].double(), (b[g].t() if trans else b[g]).double()
+            old = 2.0 * c0[o[g]:o[g + 1]].double()
+            check(c[o[g]:o[g + 1]], 0.5 * (x @ w) + old, 0.5 * (x.abs() @ w.abs()) + old.abs(), k + 10, "f32")
+
+
+@pytest.mark.parametrize("m,n", [(37, 9), (128, 200)])
+def test_weight_gradient_few_tiles_share_the_sum(ckl, m, n):
+    sizes = [1500, 0, 701]
+    offs, rows = offsets_of(sizes), 2201
+    lda, ldd = (m + 7) // 8 * 8, (n + 7) // 8 * 8
+    a, d = rand((rows, lda), torch.bfloat16, 1), rand((rows, ldd), torch.bfloat16, 2)
+    w = rand((3, m, n), torch.float32, 3)
+    w0 = w.clone()
+    ckl.gemm_grouped_wgrad(ckl.BF16, a, d, w, ckl.F32, offs, 3, rows, m, n, lda=lda, ldg=ldd, beta=1.0)
+    torch.cuda.synchronize()
+    o = offs.tolist()
+    for g in range(3):
+        x, y = a[o[g]:o[g + 1], :m].double(), d[o[g]:o[g + 1], :n].double()
+        check(w[g], x.t() @ y + w0[g].double(), x.abs().t() @ y.abs() + w0[g].double().abs(), sizes[g] + 10, "f32")
+
+
+@pytest.mark.parametrize("m,g", [(1, 1), (48, 24), (200, 3)])
+def test_lora_few_rows(ckl, m, g):
+    """Serving sizes: a long k, so that both products are divided over clusters."""
+    k, n, r = 2048, 520, 16
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    ids = torch.randint(-1, g, (m,), generator=gen, device="cuda", dtype=torch.int32)
+    ids[0] = 0
+    m, x, w, a, b, s, offs, rows = lora_case(ckl, ids, g, k, n, r, "bf16", 60)
+    size = ckl.gemm_lora_workspace_bytes(m, r)
+    ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")  # NaN in every 16-bit type
+    y = torch.full((m, n), float("nan"), dtype=torch.bfloat16, device="cuda")
+    ckl.gemm_lora(ckl.BF16, x, w, a, b, s, y, ckl.BF16, offs, rows, g, m, n, k, r, ws, size)
+    torch.cuda.synchronize()
+    for i in range(-1, g):
+        sel = ids == i
+        xs = x[sel].double()
+        ref, mag, extra = xs @ w.double(), xs.abs() @ w.double().abs(), 0.0
+        if i >= 0:
+            t, ta = s[i].double() * (xs @ a[i].double()), s[i].double() * (xs.abs() @ a[i].double().abs())
+            ref, mag = ref + t @ b[i].double(), mag + ta @ b[i].double().abs()
+            extra = TWO_PART["bf16"] * (t.abs() @ b[i].double().abs())
+        check(y[sel], ref, mag, 2 * k + 2 * r + 10, "bf16", extra)
