@@ -627,6 +627,7 @@ int device_view(DeviceView* out) {
     }
     out->device = ctx->device;
     out->sm_count = ctx->sm_count;
+    out->max_pairs = ctx->max_pairs;
     out->status = ctx->status;
     return CKL_OK;
 }

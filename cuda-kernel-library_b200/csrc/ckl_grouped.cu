@@ -8,6 +8,7 @@
 #include "ckl_gemm.h"
 #include "ckl_internal.h"
 #include "gemm_grouped.cuh"
+#include "gemm_grouped_pair.cuh"
 
 namespace {
 
@@ -70,44 +71,56 @@ struct Maps {
     CUtensorMap a_box, b_box, e_box, c;
 };
 
-template <typename OutT, bool kSplit>
-int launch(const Maps& maps, const GroupedParams& p, int grid, cudaStream_t stream) {
-    using Cfg = GroupedConfig<kSplit>;
+// A kernel that needs `bytes` of dynamic shared memory is told so once per device.
+template <auto kKernel>
+int allow_smem(int device, size_t bytes) {
     static std::mutex mu;
     static bool ready[64] = {};
-    int dev = 0;
-    GRP_TRY_CUDA(cudaGetDevice(&dev));
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        if (dev < 0 || dev >= 64 || !ready[dev]) {
-            GRP_TRY_CUDA(cudaFuncSetAttribute(grouped_gemm_kernel<OutT, kSplit>,
-                                              cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                              static_cast<int>(Cfg::kSmemBytes)));
-            if (dev >= 0 && dev < 64) {
-                ready[dev] = true;
-            }
+    std::lock_guard<std::mutex> lock(mu);
+    if (device < 0 || device >= 64 || !ready[device]) {
+        GRP_TRY_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                          static_cast<int>(bytes)));
+        if (device >= 0 && device < 64) {
+            ready[device] = true;
         }
     }
+    return CKL_OK;
+}
+
+template <auto kKernel>
+int launch_kernel(int device, int threads, size_t smem, int cluster, const Maps& maps, const GroupedParams& p,
+                  int grid, cudaStream_t stream) {
+    GRP_TRY(allow_smem<kKernel>(device, smem));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(grid));
-    cfg.blockDim = dim3(Cfg::kThreads);
-    cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = static_cast<unsigned>(p.split);
+    attr.val.clusterDim.x = static_cast<unsigned>(cluster);
     attr.val.clusterDim.y = 1;
     attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
-    cfg.numAttrs = kSplit ? 1 : 0;
-    GRP_TRY_CUDA(cudaLaunchKernelEx(&cfg, grouped_gemm_kernel<OutT, kSplit>, maps.a_box, maps.b_box, maps.e_box,
-                                    maps.c, p));
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    GRP_TRY_CUDA(cudaLaunchKernelEx(&cfg, kKernel, maps.a_box, maps.b_box, maps.e_box, maps.c, p));
     return CKL_OK;
 }
+
 template <typename OutT>
-int launch(const Maps& maps, const GroupedParams& p, int grid, cudaStream_t stream) {
-    return p.split > 1 ? launch<OutT, true>(maps, p, grid, stream)
-                       : launch<OutT, false>(maps, p, grid, stream);
+int launch(bool pair, int device, const Maps& maps, const GroupedParams& p, int grid, cudaStream_t stream) {
+    if constexpr (!GroupedStore<OutT>::kTwo) {
+        if (pair) {
+            return launch_kernel<grouped_pair_kernel<OutT>>(device, GroupedPairConfig::kThreads,
+                                                            GroupedPairConfig::kSmemBytes, 2, maps, p, grid, stream);
+        }
+    }
+    if (p.split > 1) {
+        return launch_kernel<grouped_gemm_kernel<OutT, true>>(
+            device, GroupedConfig<true>::kThreads, GroupedConfig<true>::kSmemBytes, p.split, maps, p, grid, stream);
+    }
+    return launch_kernel<grouped_gemm_kernel<OutT, false>>(
+        device, GroupedConfig<false>::kThreads, GroupedConfig<false>::kSmemBytes, 1, maps, p, grid, stream);
 }
 
 // One product in terms of its operands; fills the descriptors and launches.
@@ -129,24 +142,32 @@ int run(Product& q, cudaStream_t stream) {
     p.status = view.status;
     p.fmt = q.ab_dtype == CKL_BF16 ? 1u : 0u;
     const bool wgrad = p.form == kFormWgrad;
-    // Upper bound of the tile rows: the groups' sizes are known on the device only.
-    const long long m_tiles = wgrad ? static_cast<long long>(p.groups) * ((p.m + 127) / 128)
-                              : p.offsets == nullptr || p.ext_groups > 0
-                                  ? (p.rows + 127) / 128
-                                  : p.rows / 128 + std::min(p.groups, p.rows);
-    // Tile width: with enough tiles for every SM the wider one, which reads A half as often, unless
-    // its last wave leaves more of the machine idle than the narrow one's extra loads cost (a tenth).
-    const auto tiles_of = [&](int bn) { return m_tiles * ((p.n + bn - 1) / bn); };
+    // Upper bound of the row tiles: the groups' sizes are known on the device only.
+    const bool whole = !wgrad && (p.offsets == nullptr || p.ext_groups > 0);
+    const auto row_tiles = [&](int height) -> long long {
+        return wgrad   ? static_cast<long long>(p.groups) * ((p.m + height - 1) / height)
+               : whole ? (p.rows + height - 1) / height
+                       : p.rows / height + std::min(p.groups, p.rows);
+    };
+    // CTA pairs on 256 x 256 tiles where there are enough of them; operands in two parts and a
+    // gathered G have only a few columns or rows of output and stay with the single-CTA kernel.
+    const long long pair_tiles = row_tiles(256) * ((p.n + 255) / 256);
+    const bool pair = q.c_dtype >= 0 && p.a_parts == 1 && p.b_parts == 1 && p.b_rows == nullptr && p.n > 128 &&
+                      (!wgrad || p.m > 128) && pair_tiles * 2 > view.max_pairs;
+    // Tile width of the single-CTA kernel: with enough tiles for every SM the wider one, which
+    // reads A half as often, unless its last wave leaves more of the machine idle than the narrow
+    // one's extra loads cost (a tenth).
+    const auto tiles_of = [&](int bn) { return row_tiles(128) * ((p.n + bn - 1) / bn); };
     const auto cost_of = [&](int bn) {  // waves x columns
         return static_cast<double>((tiles_of(bn) + view.sm_count - 1) / view.sm_count) * bn;
     };
     p.bn = p.n > 128 && cost_of(256) <= 1.1 * cost_of(128) ? 256 : p.n > 64 ? 128 : 64;
-    long long tiles = tiles_of(p.bn);
+    long long tiles = pair ? pair_tiles : tiles_of(p.bn);
     p.split = 1;
     // Blocks of 64 reduced elements behind one tile, as far as the host can tell.
     const long long blocks = wgrad ? static_cast<long long>(p.rows / p.groups + 63) / 64 * p.a_parts * p.b_parts
                                    : (p.k + 63) / 64;
-    if (tiles_of(std::min(p.bn, 128)) * 2 <= view.sm_count) {
+    if (!pair && tiles_of(std::min(p.bn, 128)) * 2 <= view.sm_count) {
         // Fewer tiles than half of the SMs: a cluster divides the blocks of each.
         p.bn = std::min(p.bn, 128);
         tiles = tiles_of(p.bn);
@@ -154,7 +175,7 @@ int run(Product& q, cudaStream_t stream) {
             p.split *= 2;
         }
     }
-    if (tiles * p.split > 0x7fffffffll) {
+    if (tiles * std::max(p.split, 2) > 0x7fffffffll) {
         return set_error(CKL_ERR_TOO_LARGE, "%lld output tiles", tiles);
     }
     if (tiles == 0) {
@@ -162,14 +183,13 @@ int run(Product& q, cudaStream_t stream) {
     }
     // Few rows to a tile: the loaders fetch those alone, where a boxed copy would fetch 128.
     p.load_a = p.a_rows != nullptr ||
-               (!wgrad && p.k > 0 && p.offsets != nullptr && p.ext_groups == 0 &&
-                p.rows <= 32ll * std::min(p.groups, p.rows));
+               (!wgrad && !pair && p.k > 0 && !whole && p.rows <= 32ll * std::min(p.groups, p.rows));
     // Gathered operands are read by the loader warps, all others through these descriptors.
     Maps maps;
     std::memset(&maps, 0, sizeof maps);
     if (p.load_a == 0) {
         GRP_TRY(encode_operand(&maps.a_box, q.ab_dtype, q.a, q.a_cols, p.a_count, q.lda, 0, 0, 64,
-                               wgrad ? 64 : 128));
+                               wgrad ? 64 : pair ? 32 : 128));
     }
     if (!wgrad || p.b_rows == nullptr) {
         GRP_TRY(encode_operand(&maps.b_box, q.ab_dtype, q.b, q.b_cols, wgrad ? p.b_count : q.b_outer, q.ldb,
@@ -189,10 +209,12 @@ int run(Product& q, cudaStream_t stream) {
     const int fault = take_wait_fault(&limit_ns);
     p.wait_limit_ns = limit_ns;
     p.overstate_first_stage = fault == 1 ? 1 : 0;
-    const int grid = static_cast<int>(p.split > 1 ? tiles * p.split : std::min<long long>(view.sm_count, tiles));
+    const int grid = static_cast<int>(pair          ? 2 * std::min<long long>(view.max_pairs, tiles)
+                                      : p.split > 1 ? tiles * p.split
+                                                    : std::min<long long>(view.sm_count, tiles));
     if (q.c_dtype < 0) {
-        return q.ab_dtype == CKL_BF16 ? launch<TwoPart<__nv_bfloat16>>(maps, p, grid, stream)
-                                      : launch<TwoPart<__half>>(maps, p, grid, stream);
+        return q.ab_dtype == CKL_BF16 ? launch<TwoPart<__nv_bfloat16>>(false, view.device, maps, p, grid, stream)
+                                      : launch<TwoPart<__half>>(false, view.device, maps, p, grid, stream);
     }
     const int bytes = size_of(q.c_dtype);
     p.c_vec = !misaligned(p.c, 16) && (static_cast<long long>(p.ldc) * bytes) % 16 == 0 &&
@@ -201,12 +223,12 @@ int run(Product& q, cudaStream_t stream) {
     if (p.c_tma) {
         GRP_TRY(encode_operand(&maps.c, q.c_dtype, p.c, p.n, wgrad ? p.m : p.rows, p.ldc, wgrad ? p.groups : 1,
                                wgrad ? p.c_stride : static_cast<long long>(p.ldc) * p.rows,
-                               static_cast<uint32_t>(64 / bytes), 32));
+                               static_cast<uint32_t>(pair ? 32 : 64 / bytes), 32));
     }
     switch (q.c_dtype) {
-        case CKL_F16: return launch<__half>(maps, p, grid, stream);
-        case CKL_BF16: return launch<__nv_bfloat16>(maps, p, grid, stream);
-        default: return launch<float>(maps, p, grid, stream);
+        case CKL_F16: return launch<__half>(pair, view.device, maps, p, grid, stream);
+        case CKL_BF16: return launch<__nv_bfloat16>(pair, view.device, maps, p, grid, stream);
+        default: return launch<float>(pair, view.device, maps, p, grid, stream);
     }
 }
 

@@ -17,6 +17,7 @@ int set_error(int code, const char* fmt, ...);
 struct DeviceView {
     int device;
     int sm_count;
+    int max_pairs;         // CTA pairs that can be resident at once
     unsigned int* status;  // 4 words on the device, read by ckl_device_status
 };
 int device_view(DeviceView* out);

@@ -114,11 +114,10 @@ struct GroupedTile {
 
 struct GroupedTable {
     const int* offs;   // [groups + 1], clamped to [0, rows]
-    const int* tiles;  // [groups + 1] running count of 128-row tiles (kFormRows)
+    const int* tiles;  // [groups + 1] running count of row tiles (kFormRows)
     int segments;      // groups that are cut into tiles
     bool whole;        // one segment of all positions (extended, or no offsets)
     int n_tiles, m_tiles;
-    int total;
 };
 
 // Last index i in [0, count) with table[i] <= v (table ascending, table[0] <= v).
@@ -133,6 +132,62 @@ __device__ __forceinline__ int last_at_most(const int* table, int count, int v) 
         }
     }
     return lo;
+}
+
+// Builds the table in shared memory; all threads of the CTA, warp 0 writes the running counts,
+// which are complete after the caller's next __syncthreads().
+__device__ __forceinline__ GroupedTable make_table(const GroupedParams& p, int* offs, int* tiles,
+                                                   int tile_rows, int tile_cols, int warp, uint32_t lane,
+                                                   int threads) {
+    if (p.offsets != nullptr) {
+        for (int g = static_cast<int>(threadIdx.x); g <= p.groups; g += threads) {
+            offs[g] = min(max(p.offsets[g], 0), p.rows);
+        }
+    } else if (threadIdx.x == 0) {
+        offs[0] = 0;
+        offs[1] = p.rows;
+    }
+    __syncthreads();
+    GroupedTable t;
+    t.offs = offs;
+    t.tiles = tiles;
+    t.whole = p.offsets == nullptr || p.ext_groups > 0;
+    t.segments = t.whole ? 1 : p.groups;
+    t.n_tiles = (p.n + tile_cols - 1) / tile_cols;
+    t.m_tiles = (p.m + tile_rows - 1) / tile_rows;
+    if (warp == 0) {
+        if (t.whole) {
+            if (lane == 0) {
+                tiles[0] = 0;
+                tiles[1] = (p.rows + tile_rows - 1) / tile_rows;
+            }
+        } else {
+            int run = 0;
+            for (int g0 = 0; g0 < p.groups; g0 += 32) {
+                const int g = g0 + static_cast<int>(lane);
+                const int count =
+                    g < p.groups ? (max(0, offs[g + 1] - offs[g]) + tile_rows - 1) / tile_rows : 0;
+                int v = count;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
+                    v += static_cast<int>(lane) >= d ? u : 0;
+                }
+                if (g < p.groups) {
+                    tiles[g] = run + v - count;
+                }
+                run += __shfl_sync(0xFFFFFFFFu, v, 31);
+            }
+            if (lane == 0) {
+                tiles[p.groups] = run;
+            }
+        }
+    }
+    return t;
+}
+
+__device__ __forceinline__ int total_tiles(const GroupedParams& p, const GroupedTable& t) {
+    return p.form == kFormWgrad ? p.groups * t.m_tiles * t.n_tiles : t.tiles[t.segments] * t.n_tiles;
 }
 
 __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, const GroupedTable& t,
@@ -272,6 +327,146 @@ __device__ __forceinline__ void store_unit(const GroupedParams& p,
     }
 }
 
+// Writes one stage for a loader warp.  Eight lanes copy the 128 bytes of one row (lane & 7 picks the
+// 16-byte unit), four rows per instruction; a unit's place under the 128-byte swizzle depends on
+// the row modulo 8.  Shuffles and copies go in batches of eight: one after the other each pair
+// would cost its full latency (110 cycles).
+struct Loader {
+    uint32_t stage;      // shared address
+    int unit, sub;       // lane & 7, lane >> 3
+    uint32_t even, odd;  // offset of rows 4 i + sub inside the 1024-byte group of 8 rows, by i & 1
+
+    __device__ __forceinline__ Loader(uint32_t stage_addr, uint32_t lane) {
+        stage = stage_addr;
+        unit = static_cast<int>(lane & 7u);
+        sub = static_cast<int>(lane >> 3);
+        even = static_cast<uint32_t>(sub) * 128u + (static_cast<uint32_t>(unit ^ sub) << 4);
+        odd = static_cast<uint32_t>(sub) * 128u + 512u + (static_cast<uint32_t>(unit ^ (sub + 4)) << 4);
+    }
+
+    // The last unit of a row may hold fewer than 8 columns that exist: those are read one by one, so
+    // that nothing behind the last row is touched.
+    __device__ __forceinline__ void part_of_unit(uint32_t dst, const void* row, int col, int have) const {
+        uint32_t w[4] = {0, 0, 0, 0};
+        for (int e = 0; e < have; ++e) {
+            const uint32_t v = __ldg(static_cast<const unsigned short*>(row) + col + e);
+            w[0] |= e == 0 ? v : e == 1 ? v << 16 : 0u;
+            w[1] |= e == 2 ? v : e == 3 ? v << 16 : 0u;
+            w[2] |= e == 4 ? v : e == 5 ? v << 16 : 0u;
+            w[3] |= e == 6 ? v : 0u;
+        }
+        ptx::st_shared_16(dst, make_uint4(w[0], w[1], w[2], w[3]));
+    }
+
+    // Columns [k0, k0 + 64) of up to 128 rows, K-major; lane l holds the indices of rows l, 32 + l,
+    // 64 + l, 96 + l (-1: zeros).  Columns behind `limit` are zeros; rows behind `rows` are skipped.
+    __device__ __forceinline__ void rows128(uint32_t offset, const void* from, int ld, const int (&src)[4],
+                                            int rows, int k0, int limit) const {
+        const int col = k0 + unit * 8;
+        const bool whole = col + 8 <= limit;
+        // (a unit that is not whole reads nothing here: any address will do)
+        const char* base = static_cast<const char*>(from) + (whole ? static_cast<size_t>(col) * 2 : 0);
+        const size_t pitch = static_cast<size_t>(ld) * 2;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (q * 32 >= rows) {
+                break;
+            }
+            int at[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                at[i] = __shfl_sync(0xFFFFFFFFu, src[q], i * 4 + sub);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                ptx::cp_async_16(stage + offset + q * 4096u + (i >> 1) * 1024u + ((i & 1) ? odd : even),
+                                 base + max(at[i], 0) * pitch, at[i] >= 0 && whole);
+            }
+        }
+        if (k0 + 64 > limit && (limit & 7) != 0) {
+            ptx::cp_async_wait_all();
+            for (int r = 0; r < rows; r += 4) {
+                const int at = __shfl_sync(
+                    0xFFFFFFFFu, r < 32 ? src[0] : r < 64 ? src[1] : r < 96 ? src[2] : src[3], (r & 31) + sub);
+                if (!whole && col < limit && at >= 0) {
+                    part_of_unit(stage + offset + (r >> 3) * 1024u + ((r & 4) ? odd : even),
+                                 static_cast<const char*>(from) + at * pitch, col, limit - col);
+                }
+            }
+        }
+    }
+
+    // Columns [k0, k0 + 64) of one part of T behind positions pos0 ..; positions outside [lo, hi) and
+    // columns behind the part are zeros.
+    __device__ __forceinline__ void adapter_rows(uint32_t offset, const GroupedParams& p, int pos0, int rows,
+                                                 int lo, int hi, int part, int k0) const {
+        const int col = k0 + unit * 8;
+        const bool exists = col < p.ext_cols;
+        const char* base = static_cast<const char*>(p.t) +
+                           (static_cast<size_t>(part) * p.ext_cols + (exists ? col : 0)) * 2;
+        const size_t pitch = static_cast<size_t>(p.ldt) * 2;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (q * 32 >= rows) {
+                break;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int pos = pos0 + q * 32 + i * 4 + sub;
+                const bool take = pos >= lo && pos < hi && exists;
+                ptx::cp_async_16(stage + offset + q * 4096u + (i >> 1) * 1024u + ((i & 1) ? odd : even),
+                                 base + (take ? pos : 0) * pitch, take);
+            }
+        }
+    }
+
+    // 64 rows, MN-major: `boxes` boxes of 64 columns from col0 on; lane l holds the indices of rows l
+    // and 32 + l (-1: zeros).  Columns behind `limit` are zeros.
+    __device__ __forceinline__ void rows64(uint32_t offset, const void* from, int ld, const int (&src)[2],
+                                           int boxes, int col0, int limit) const {
+        const size_t pitch = static_cast<size_t>(ld) * 2;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const char* row[8];
+            uint32_t exists = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int at = __shfl_sync(0xFFFFFFFFu, src[q], i * 4 + sub);
+                exists |= at >= 0 ? 1u << i : 0u;
+                row[i] = static_cast<const char*>(from) + max(at, 0) * pitch;
+            }
+            for (int b = 0; b < boxes; ++b) {
+                const int col = col0 + b * 64 + unit * 8;
+                const bool whole = col + 8 <= limit;
+                const size_t skip = whole ? static_cast<size_t>(col) * 2 : 0;
+                const uint32_t at = stage + offset + b * 8192u + q * 4096u;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    ptx::cp_async_16(at + (i >> 1) * 1024u + ((i & 1) ? odd : even), row[i] + skip,
+                                     ((exists >> i) & 1u) != 0 && whole);
+                }
+                if (!whole && col < limit) {
+                    ptx::cp_async_wait_all();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if ((exists >> i) & 1u) {
+                            part_of_unit(at + (i >> 1) * 1024u + ((i & 1) ? odd : even), row[i], col, limit - col);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+        }
+    }
+
+    // The copies have landed and are ordered before the tensor core's reads; one lane may arrive.
+    __device__ __forceinline__ void finish() const {
+        ptx::cp_async_wait_all();
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+    }
+};
+
 // Row of C behind row `in_tile` of a tile, -1 for none.
 __device__ __forceinline__ int row_of_c(const GroupedParams& p, const GroupedTile& t, int in_tile) {
     if (p.form == kFormWgrad) {
@@ -347,56 +542,13 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
         ptx::tmem_relinquish();
     }
     int* offs = reinterpret_cast<int*>(table_ptr);
-    int* tile_count = offs + kMaxGemmGroups + 2;
-    if (p.offsets != nullptr) {
-        for (int g = static_cast<int>(threadIdx.x); g <= p.groups; g += Cfg::kThreads) {
-            offs[g] = min(max(p.offsets[g], 0), p.rows);
-        }
-    } else if (threadIdx.x == 0) {
-        offs[0] = 0;
-        offs[1] = p.rows;
-    }
-    __syncthreads();
-    detail::GroupedTable table;
-    table.offs = offs;
-    table.tiles = tile_count;
-    table.whole = p.offsets == nullptr || p.ext_groups > 0;
-    table.segments = table.whole ? 1 : p.groups;
-    table.n_tiles = (p.n + p.bn - 1) / p.bn;
-    table.m_tiles = (p.m + 127) / 128;
-    if (warp == 0) {
-        if (table.whole) {
-            if (lane == 0) {
-                tile_count[0] = 0;
-                tile_count[1] = (p.rows + 127) / 128;
-            }
-        } else {
-            int run = 0;
-            for (int g0 = 0; g0 < p.groups; g0 += 32) {
-                const int g = g0 + static_cast<int>(lane);
-                int v = g < p.groups ? (max(0, offs[g + 1] - offs[g]) + 127) / 128 : 0;
-                const int own_tiles = v;
-#pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
-                    v += static_cast<int>(lane) >= d ? u : 0;
-                }
-                if (g < p.groups) {
-                    tile_count[g] = run + v - own_tiles;
-                }
-                run += __shfl_sync(0xFFFFFFFFu, v, 31);
-            }
-            if (lane == 0) {
-                tile_count[p.groups] = run;
-            }
-        }
-    }
+    const detail::GroupedTable table = detail::make_table(p, offs, offs + kMaxGemmGroups + 2, 128, p.bn, warp,
+                                                          lane, Cfg::kThreads);
     ptx::tc_fence_before_sync();
     __syncthreads();
     ptx::tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot_ptr;
-    table.total = p.form == kFormWgrad ? p.groups * table.m_tiles * table.n_tiles
-                                       : tile_count[table.segments] * table.n_tiles;
+    const int total = detail::total_tiles(p, table);
     const int ext_blocks = 2 * ((p.ext_cols + 63) / 64);  // of one adapter: both parts of T
     // A split launch has one tile per cluster.
     const int rank = kSplit ? static_cast<int>(ptx::cluster_cta_rank()) : 0;
@@ -429,7 +581,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     phase ^= 1u;
                 }
             };
-            for (int tile = first_tile; ok && tile < table.total; tile += tile_step) {
+            for (int tile = first_tile; ok && tile < total; tile += tile_step) {
                 const detail::GroupedTile t = detail::grouped_tile(p, table, tile);
                 const detail::BlockRange mine = detail::block_range(p, table, t, rank, size);
                 const int boxes = (t.cols + 63) / 64;
@@ -484,19 +636,22 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                         (gather_a ? 0u : static_cast<uint32_t>(a_boxes) * Cfg::kBoxBytes);
                     for (int kb = mine.begin; kb < mine.end; ++kb) {
                         const int part = kb >= row_blocks ? 1 : 0;
-                        const int pos = t.p0 + (kb - part * row_blocks) * 64;
-                        if (!acquire_stage(bytes)) {
+                        const int at = (kb - part * row_blocks) * 64;
+                        // A last block that is not whole comes through the loaders in both operands,
+                        // with zeros behind the group's end (a zero in one alone would leave 0 * NaN).
+                        const bool whole = t.valid - at >= 64;
+                        if (!acquire_stage(whole ? bytes : 0u)) {
                             ok = false;
                             break;
                         }
                         const uint32_t a_dst = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
-                        for (int b = 0; !gather_a && b < a_boxes; ++b) {
+                        for (int b = 0; whole && !gather_a && b < a_boxes; ++b) {
                             ptx::tma_load_2d(a_dst + b * Cfg::kBoxBytes, &tmap_a_box, full_bar(stage),
-                                             t.m0 + part * p.a_part_cols + b * 64, pos);
+                                             t.m0 + part * p.a_part_cols + b * 64, t.p0 + at);
                         }
-                        for (int b = 0; !gather_b && b < boxes; ++b) {
+                        for (int b = 0; whole && !gather_b && b < boxes; ++b) {
                             ptx::tma_load_3d(a_dst + Cfg::kABytes + b * Cfg::kBoxBytes, &tmap_b_box,
-                                             full_bar(stage), t.n0 + part * p.b_part_cols + b * 64, pos, 0);
+                                             full_bar(stage), t.n0 + part * p.b_part_cols + b * 64, t.p0 + at, 0);
                         }
                         advance();
                     }
@@ -531,7 +686,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
             uint32_t count = 0;
             bool ready = false;  // the next stage's copies are known to have landed
             bool ok = true;
-            for (int tile = first_tile; ok && tile < table.total; tile += tile_step) {
+            for (int tile = first_tile; ok && tile < total; tile += tile_step) {
                 const detail::GroupedTile t = detail::grouped_tile(p, table, tile);
                 const uint32_t acc = count & 1u;
                 if (!detail::wait_barrier(acc_empty_bar(acc), ((count >> 1) & 1u) ^ 1u, ctl, kRoleMma,
@@ -640,48 +795,26 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
         // generic-proxy writes: after they have landed a proxy fence orders them before the tensor
         // core's reads, then one lane arrives.
         const int own = warp - 6;
-        const int unit = static_cast<int>(lane & 7u);
-        const int sub = static_cast<int>(lane >> 3);
-        const uint32_t stage_base = ring + static_cast<uint32_t>(own) * Cfg::kStageBytes;
-        // rows 4 i + sub: row modulo 8 is sub for even i, sub + 4 for odd i
-        const uint32_t even = static_cast<uint32_t>(sub) * 128u +
-                              ((static_cast<uint32_t>(unit) ^ static_cast<uint32_t>(sub)) << 4);
-        const uint32_t odd = static_cast<uint32_t>(sub) * 128u + 512u +
-                             ((static_cast<uint32_t>(unit) ^ static_cast<uint32_t>(sub + 4)) << 4);
+        const detail::Loader load(ring + static_cast<uint32_t>(own) * Cfg::kStageBytes, lane);
         uint32_t it = 0;     // blocks of this CTA so far, whoever owns their stage
         uint32_t phase = 0;  // of the own stage
         bool ok = true;
-        auto wait_all = [&](uint32_t bar, uint32_t parity) -> bool {
-            const bool got = detail::wait_barrier(bar, parity, ctl, kRoleProducer, 0x20000000u | it);
-            return __all_sync(0xFFFFFFFFu, got) != 0;
-        };
-        auto mine = [&](uint32_t block) { return static_cast<int>(block % kStages) == own; };
         // Every block of the own stage is waited for, even one that needs nothing from here: a
         // barrier tells two adjacent phases apart, no more.
-        auto acquire = [&]() -> bool { return wait_all(empty_bar(own), phase ^ 1u); };
+        auto acquire = [&]() -> bool {
+            const bool got =
+                detail::wait_barrier(empty_bar(own), phase ^ 1u, ctl, kRoleProducer, 0x20000000u | it);
+            phase ^= 1u;
+            return __all_sync(0xFFFFFFFFu, got) != 0;
+        };
         auto hand_over = [&]() {
-            ptx::cp_async_wait_all();
-            ptx::fence_proxy_async_smem();
-            __syncwarp();
+            load.finish();
             if (lane == 0) {
                 ptx::mbar_arrive(loaded_bar(own));
             }
         };
-        // The last unit of a row may hold fewer than 8 columns that exist: those are read one by
-        // one, so that nothing behind the last row is touched.
-        auto part_of_unit = [&](uint32_t dst, const void* row, int col, int have) {
-            uint32_t w[4] = {0, 0, 0, 0};
-            for (int e = 0; e < have; ++e) {
-                const uint32_t v = __ldg(static_cast<const unsigned short*>(row) + col + e);
-                w[0] |= e == 0 ? v : e == 1 ? v << 16 : 0u;
-                w[1] |= e == 2 ? v : e == 3 ? v << 16 : 0u;
-                w[2] |= e == 4 ? v : e == 5 ? v << 16 : 0u;
-                w[3] |= e == 6 ? v : 0u;
-            }
-            ptx::st_shared_16(dst, make_uint4(w[0], w[1], w[2], w[3]));
-        };
         const bool needed = p.form == kFormWgrad || gather_a || p.ext_groups > 0;
-        for (int tile = first_tile; needed && ok && tile < table.total; tile += tile_step) {
+        for (int tile = first_tile; needed && ok && tile < total; tile += tile_step) {
             const detail::GroupedTile t = detail::grouped_tile(p, table, tile);
             const detail::BlockRange range = detail::block_range(p, table, t, rank, size);
             if (p.form == kFormRows) {
@@ -697,7 +830,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     }
                 }
                 for (int kb = range.begin; kb < min(range.end, t.k_blocks); ++kb, ++it) {
-                    if (!mine(it)) {
+                    if (static_cast<int>(it % kStages) != own) {
                         continue;
                     }
                     if (!acquire()) {
@@ -705,46 +838,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                         break;
                     }
                     if (gather_a) {
-                        const int col = kb * 64 + unit * 8;
-                        const bool whole = col + 8 <= p.k;
-                        // (a unit that is not whole reads nothing here: any address will do)
-                        const char* base =
-                            static_cast<const char*>(p.a) + (whole ? static_cast<size_t>(col) * 2 : 0);
-                        const size_t pitch = static_cast<size_t>(p.lda) * 2;
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            if (q * 32 >= t.valid) {
-                                break;
-                            }
-                            // eight shuffles, then eight copies: one after the other each pair would
-                            // cost its full latency (110 cycles)
-                            int at[8];
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                at[i] = __shfl_sync(0xFFFFFFFFu, src[q], i * 4 + sub);
-                            }
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                ptx::cp_async_16(
-                                    stage_base + q * 4096u + (i >> 1) * 1024u + ((i & 1) ? odd : even),
-                                    base + max(at[i], 0) * pitch, at[i] >= 0 && whole);
-                            }
-                        }
-                        if (kb * 64 + 64 > p.k && (p.k & 7) != 0) {
-                            ptx::cp_async_wait_all();
-                            for (int r = 0; r < t.valid; r += 4) {
-                                const int at = __shfl_sync(
-                                    0xFFFFFFFFu, r < 32 ? src[0] : r < 64 ? src[1] : r < 96 ? src[2] : src[3],
-                                    (r & 31) + sub);
-                                if (!whole && col < p.k && at >= 0) {
-                                    part_of_unit(stage_base + (r >> 3) * 1024u + ((r & 4) ? odd : even),
-                                                 static_cast<const char*>(p.a) + at * pitch, col, p.k - col);
-                                }
-                            }
-                        }
+                        load.rows128(0, p.a, p.lda, src, t.valid, kb * 64, p.k);
                         hand_over();
                     }
-                    phase ^= 1u;
                 }
                 int first_block = t.k_blocks;
                 for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
@@ -754,7 +850,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     }
                     const int eb_end = min(ext_blocks, range.end - first_block);
                     for (int eb = max(0, range.begin - first_block); eb < eb_end; ++eb, ++it) {
-                        if (!mine(it)) {
+                        if (static_cast<int>(it % kStages) != own) {
                             continue;
                         }
                         if (!acquire()) {
@@ -762,27 +858,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                             break;
                         }
                         const int part = eb >= ext_blocks / 2 ? 1 : 0;
-                        const int col = (eb - part * (ext_blocks / 2)) * 64 + unit * 8;
-                        const char* base = static_cast<const char*>(p.t) +
-                                           (static_cast<size_t>(part) * p.ext_cols +
-                                            (col < p.ext_cols ? col : 0)) * 2;
-                        const size_t pitch = static_cast<size_t>(p.ldt) * 2;
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            if (q * 32 >= t.valid) {
-                                break;
-                            }
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const int pos = t.p0 + q * 32 + i * 4 + sub;
-                                const bool take = pos >= span.lo && pos < span.hi && col < p.ext_cols;
-                                ptx::cp_async_16(
-                                    stage_base + q * 4096u + (i >> 1) * 1024u + ((i & 1) ? odd : even),
-                                    base + (take ? pos : 0) * pitch, take);
-                            }
-                        }
+                        load.adapter_rows(0, p, t.p0, t.valid, span.lo, span.hi, part,
+                                          (eb - part * (ext_blocks / 2)) * 64);
                         hand_over();
-                        phase ^= 1u;
                     }
                     first_block += ext_blocks;
                 }
@@ -790,7 +868,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                 const int row_blocks = (t.valid + 63) / 64;
                 const int a_boxes = (min(128, p.m - t.m0) + 63) / 64;
                 const int b_boxes = (t.cols + 63) / 64;
-                // Rows of A and G behind this lane's positions l and 32 + l of block kb.
+                // Rows of A and G behind this lane's positions l and 32 + l of block kb, -1 behind the
+                // end of the group.
                 int next_a[2], next_b[2];
                 auto fetch = [&](int kb) {
                     const int i0 = (kb >= row_blocks ? kb - row_blocks : kb) * 64;
@@ -798,47 +877,10 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     for (int q = 0; q < 2; ++q) {
                         const int r = i0 + q * 32 + static_cast<int>(lane);
                         const bool in = kb < range.end && r < t.valid;
-                        const int at_a = in && gather_a ? __ldg(p.a_rows + t.p0 + r) : -1;
-                        const int at_b = in && gather_b ? __ldg(p.b_rows + t.p0 + r) : -1;
+                        const int at_a = !in ? -1 : p.a_rows != nullptr ? __ldg(p.a_rows + t.p0 + r) : t.p0 + r;
+                        const int at_b = !in ? -1 : p.b_rows != nullptr ? __ldg(p.b_rows + t.p0 + r) : t.p0 + r;
                         next_a[q] = at_a < p.a_count ? at_a : -1;
                         next_b[q] = at_b < p.b_count ? at_b : -1;
-                    }
-                };
-                // 64 gathered rows of one operand: `boxes` boxes of 64 columns from column col0 on.
-                auto gather = [&](const void* from, int ld, const int (&rows)[2], uint32_t dst, int boxes,
-                                  int col0, int limit) {
-                    const size_t pitch = static_cast<size_t>(ld) * 2;
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const char* row[8];
-                        uint32_t exists = 0;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int at = __shfl_sync(0xFFFFFFFFu, rows[q], i * 4 + sub);
-                            exists |= at >= 0 ? 1u << i : 0u;
-                            row[i] = static_cast<const char*>(from) + max(at, 0) * pitch;
-                        }
-                        for (int b = 0; b < boxes; ++b) {
-                            const int col = col0 + b * 64 + unit * 8;
-                            const bool whole = col + 8 <= limit;
-                            const size_t skip = whole ? static_cast<size_t>(col) * 2 : 0;
-                            const uint32_t at = dst + b * Cfg::kBoxBytes + q * 4096u;
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                ptx::cp_async_16(at + (i >> 1) * 1024u + ((i & 1) ? odd : even), row[i] + skip,
-                                                 ((exists >> i) & 1u) != 0 && whole);
-                            }
-                            if (!whole && col < limit) {
-                                ptx::cp_async_wait_all();
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) {
-                                    if ((exists >> i) & 1u) {
-                                        part_of_unit(at + (i >> 1) * 1024u + ((i & 1) ? odd : even), row[i],
-                                                     col, limit - col);
-                                    }
-                                }
-                            }
-                        }
                     }
                 };
                 // the first block of this tile whose stage is the own one
@@ -847,44 +889,24 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                 fetch(first);
                 for (int kb = first; kb < range.end; kb += kStages) {
                     const int part = kb >= row_blocks ? 1 : 0;
-                    const int left = t.valid - (kb - part * row_blocks) * 64;
-                    int ra[2] = {next_a[0], next_a[1]}, rb[2] = {next_b[0], next_b[1]};
+                    const bool tail = t.valid - (kb - part * row_blocks) * 64 < 64;
+                    const int ra[2] = {next_a[0], next_a[1]}, rb[2] = {next_b[0], next_b[1]};
                     fetch(kb + kStages);
                     if (!acquire()) {
                         ok = false;
                         break;
                     }
-                    if (gather_a) {
-                        gather(p.a, p.lda, ra, stage_base, a_boxes, t.m0, p.m);
+                    if (gather_a || tail) {
+                        load.rows64(0, p.a, p.lda, ra, a_boxes, t.m0 + part * p.a_part_cols,
+                                    p.m + part * p.a_part_cols);
                     }
-                    if (gather_b) {
-                        gather(p.b, p.ldb, rb, stage_base + Cfg::kABytes, b_boxes, t.n0, p.n);
+                    if (gather_b || tail) {
+                        load.rows64(Cfg::kABytes, p.b, p.ldb, rb, b_boxes, t.n0 + part * p.b_part_cols,
+                                    p.n + part * p.b_part_cols);
                     }
-                    if (left < 64 && !(gather_a && gather_b)) {
-                        // Positions behind the group's end: zeros in both operands (a zero in one
-                        // alone would leave 0 * NaN).  Gathered ones are zeros already; the boxed
-                        // ones are overwritten once the box has landed.
-                        if (!wait_all(full_bar(own), phase)) {
-                            ok = false;
-                            break;
-                        }
-                        for (int i = left / 4; i < 16; ++i) {
-                            if (i * 4 + sub < left) {
-                                continue;
-                            }
-                            const uint32_t at = stage_base + (i >> 1) * 1024u + ((i & 1) ? odd : even);
-                            for (int b = 0; !gather_a && b < a_boxes; ++b) {
-                                ptx::st_shared_zero_16(at + b * Cfg::kBoxBytes);
-                            }
-                            for (int b = 0; !gather_b && b < b_boxes; ++b) {
-                                ptx::st_shared_zero_16(at + Cfg::kABytes + b * Cfg::kBoxBytes);
-                            }
-                        }
-                    }
-                    if (gather_a || gather_b || left < 64) {
+                    if (gather_a || gather_b || tail) {
                         hand_over();
                     }
-                    phase ^= 1u;
                 }
                 it += static_cast<uint32_t>(range.end - range.begin);
             }
@@ -905,7 +927,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
         const uint32_t stg_all = ring + kStages * Cfg::kStageBytes;
         uint32_t buffer = 0;
         bool alive = true;
-        for (int tile = first_tile; alive && tile < table.total; tile += tile_step) {
+        for (int tile = first_tile; alive && tile < total; tile += tile_step) {
             const detail::GroupedTile t = detail::grouped_tile(p, table, tile);
             const uint32_t acc = count & 1u;
             const uint32_t parity = (count >> 1) & 1u;
@@ -1087,7 +1109,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
         // The parts of the tile meet: row i of the tile is summed by CTA i mod size, part 0 first.
         ptx::cluster_arrive_release();
         ptx::cluster_wait_acquire();
-        if (first_tile < table.total) {
+        if (first_tile < total) {
             constexpr int kVec = detail::OutTraits<Elem>::kVec;
             constexpr int kLanesPerRow = 128 / kVec;
             constexpr int kRowsPerWarp = 32 / kLanesPerRow;

@@ -1,0 +1,693 @@
+// The CTA-pair form of the grouped products, for launches with tiles enough for every pair.
+//
+// A pair computes a transposed tile: the COLUMNS of C are the 256 rows of the tensor core's
+// product (128 per CTA: the weights, or G of a weight gradient) and the ROWS of C (positions, or
+// the rows of W_g) are its N, up to 256 in steps of 32.  So the ragged dimension is the one the
+// instruction takes in fine steps: a group of 300 rows runs as two tiles of 160 and 140 (N = 160
+// each), where 128-row tiles would compute 384 and 256-row ones 512; and each CTA reads half of
+// the rows and its own columns only, 32 KB per 64 k for 256 x 256 outputs, where the single-CTA
+// tile reads 48 KB for half as many.
+//
+//   columns operand (A of the instruction): W_g, MN-major (or K-major when op is the transpose);
+//       G of a weight gradient, MN-major.  Always boxed TMA copies, 64 x 64 boxes.
+//   rows operand (B of the instruction, half of the rows per CTA): positions of A, K-major; columns
+//       of A in a weight gradient, MN-major.  Boxed, or gathered by the loader warps.
+// The last block of a group's sum in a weight gradient, when it is not whole, comes through the
+// loaders in both operands, which put zeros behind the group's end.
+//
+// Epilogue: a lane holds one column of C and 32 rows at a time, so the staging buffer is
+// written row by row across the lanes; from there rows leave as in the single-CTA kernel.
+#pragma once
+
+#include "gemm_grouped.cuh"
+
+namespace ckl {
+
+struct GroupedPairConfig {
+    static constexpr int kStages = 6;
+    static constexpr uint32_t kBoxBytes = 64 * 64 * 2;
+    static constexpr uint32_t kColsBytes = 2 * kBoxBytes;
+    static constexpr uint32_t kRowsBytes = 2 * kBoxBytes;
+    static constexpr uint32_t kStageBytes = kColsBytes + kRowsBytes;
+    static constexpr int kFirstLoader = 6;
+    static constexpr int kThreads = 32 * (kFirstLoader + kStages);  // one loader warp per stage
+    static constexpr uint32_t kWarpStaging = 3 * 2048;  // per epilogue warp
+    static constexpr uint32_t kStagingBytes = 4 * kWarpStaging;
+    static constexpr int kNumBarriers = 3 * kStages + 5;
+    static constexpr uint32_t kTableBytes = 2 * (kMaxGemmGroups + 2) * 4;
+    static constexpr uint32_t kSmemBytes =
+        kStages * kStageBytes + kStagingBytes + kTableBytes + kNumBarriers * 8 + 16 + 1024;
+};
+
+namespace detail {
+
+struct PairTile {
+    int group;
+    int p0, valid;  // kFormRows: positions of the tile; kFormWgrad: of the group (the sum)
+    int r0, rows;   // first row of C and rows of the tile (kFormRows: r0 = p0, rows = valid)
+    int c0;         // first column
+    int half;       // rows per CTA: 16, 32, ... 128 (kFormWgrad: 64 or 128)
+    int k_blocks;
+    int ext_first, ext_last;
+};
+
+__device__ __forceinline__ PairTile pair_tile(const GroupedParams& p, const GroupedTable& t, int tile) {
+    PairTile o;
+    int local, row_tiles, total_rows, seg0;
+    if (p.form == kFormWgrad) {
+        const int per = t.m_tiles * t.n_tiles;
+        o.group = tile / per;
+        local = tile - o.group * per;
+        row_tiles = t.m_tiles;
+        total_rows = p.m;
+        seg0 = 0;
+    } else {
+        o.group = t.segments == 1 ? 0 : last_at_most(t.tiles, t.segments, tile / t.n_tiles);
+        local = tile - t.tiles[o.group] * t.n_tiles;
+        row_tiles = t.tiles[o.group + 1] - t.tiles[o.group];
+        seg0 = t.whole ? 0 : t.offs[o.group];
+        total_rows = (t.whole ? p.rows : t.offs[o.group + 1]) - seg0;
+    }
+    constexpr int kBand = 8;
+    const int band = local / (kBand * t.n_tiles);
+    const int height = min(kBand, row_tiles - band * kBand);
+    const int in_band = local - band * kBand * t.n_tiles;
+    const int ct = in_band / height;
+    const int rt = band * kBand + in_band - ct * height;
+    o.c0 = ct * 256;
+    // Tiles of one group are equally high.
+    const int unit = p.form == kFormWgrad ? 128 : 32;
+    const int step = ((total_rows + row_tiles - 1) / row_tiles + unit - 1) / unit * unit;
+    o.r0 = seg0 + rt * step;
+    o.rows = max(0, min(step, total_rows - rt * step));
+    o.half = max(unit, (o.rows + unit - 1) / unit * unit) / 2;
+    o.ext_first = o.ext_last = 0;
+    if (p.form == kFormWgrad) {
+        o.p0 = t.offs[o.group];
+        o.valid = max(0, t.offs[o.group + 1] - o.p0);
+        o.k_blocks = o.rows > 0 ? (o.valid + 63) / 64 : 0;
+    } else {
+        o.p0 = o.r0;
+        o.valid = o.rows;
+        o.k_blocks = o.rows > 0 ? (p.k + 63) / 64 : 0;
+        if (p.ext_groups > 0 && o.rows > 0 && o.p0 < t.offs[p.ext_groups]) {
+            o.ext_first = last_at_most(t.offs, p.ext_groups, o.p0);
+            o.ext_last = last_at_most(t.offs, p.ext_groups, o.p0 + o.valid - 1) + 1;
+        }
+    }
+    return o;
+}
+
+__device__ __forceinline__ Span adapter_span(const GroupedTable& table, const PairTile& t, int g) {
+    return {max(table.offs[g], t.p0), min(table.offs[g + 1], t.p0 + t.valid)};
+}
+
+// As wait_barrier, ordered after writes that the other CTA of the cluster released.
+__device__ __forceinline__ bool wait_cluster_barrier(uint32_t bar, uint32_t parity, const Control& ctl,
+                                                     unsigned int role, unsigned int detail_word) {
+    if (!wait_barrier(bar, parity, ctl, role, detail_word)) {
+        return false;
+    }
+    for (int i = 0; i < 1024 && !ptx::mbar_try_wait_cluster(bar, parity); ++i) {
+    }
+    return true;
+}
+
+}  // namespace detail
+
+template <typename OutT>
+__global__ void __launch_bounds__(GroupedPairConfig::kThreads, 1)
+grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
+                    const __grid_constant__ CUtensorMap tmap_cols,
+                    const __grid_constant__ CUtensorMap tmap_ext,
+                    const __grid_constant__ CUtensorMap tmap_c, const GroupedParams p) {
+    using Cfg = GroupedPairConfig;
+    using Elem = typename GroupedStore<OutT>::Elem;
+    constexpr int kStages = Cfg::kStages;
+
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_addr = ptx::smem_u32(smem_raw);
+    const uint32_t ring = (raw_addr + 1023u) & ~1023u;
+    uint8_t* ring_ptr = smem_raw + (ring - raw_addr);
+    uint8_t* staging_ptr = ring_ptr + kStages * Cfg::kStageBytes;
+    uint8_t* table_ptr = staging_ptr + Cfg::kStagingBytes;
+    uint8_t* bars_ptr = table_ptr + Cfg::kTableBytes;
+    const uint32_t bars = ring + (kStages * Cfg::kStageBytes + Cfg::kStagingBytes + Cfg::kTableBytes);
+    auto full_bar = [&](int s) { return bars + 8u * static_cast<uint32_t>(s); };
+    auto empty_bar = [&](int s) { return bars + 8u * static_cast<uint32_t>(kStages + s); };
+    auto loaded_bar = [&](int s) { return bars + 8u * static_cast<uint32_t>(2 * kStages + s); };
+    auto acc_full_bar = [&](uint32_t a) { return bars + 8u * (3 * kStages + a); };
+    auto acc_empty_bar = [&](uint32_t a) { return bars + 8u * (3 * kStages + 2 + a); };
+    const uint32_t drain_bar = bars + 8u * (3 * kStages + 4);
+    const uint32_t tmem_slot = bars + 8u * Cfg::kNumBarriers;
+    volatile uint32_t* tmem_slot_ptr =
+        reinterpret_cast<volatile uint32_t*>(bars_ptr + 8 * Cfg::kNumBarriers);
+
+    const int warp = static_cast<int>(threadIdx.x >> 5);
+    const uint32_t lane = ptx::lane_id();
+    const uint32_t rank = ptx::cluster_cta_rank();
+    const bool leader = rank == 0;
+
+    detail::Control ctl;
+    ctl.abort_flag = reinterpret_cast<volatile int*>(bars_ptr + 8 * Cfg::kNumBarriers + 4);
+    ctl.abort_flag_smem = tmem_slot + 4u;
+    ctl.status = p.status;
+    ctl.pair = true;
+    ctl.peer_rank = rank ^ 1u;
+    ctl.limit_ns = p.wait_limit_ns != 0 ? p.wait_limit_ns : kWaitLimitNs;
+
+    // ---- set-up -------------------------------------------------------------------------------
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            ptx::mbar_init(full_bar(s), 1);
+            ptx::mbar_init(empty_bar(s), 1);
+            ptx::mbar_init(loaded_bar(s), 2);  // the loaders of both CTAs, at the leader
+        }
+        for (uint32_t a = 0; a < 2; ++a) {
+            ptx::mbar_init(acc_full_bar(a), 1);
+            ptx::mbar_init(acc_empty_bar(a), 8);  // four warps of either CTA, at the leader
+        }
+        ptx::mbar_init(drain_bar, 1);
+        *ctl.abort_flag = 0;
+        ptx::fence_barrier_init();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc_pair(tmem_slot, 512);
+        ptx::tmem_relinquish_pair();
+    }
+    int* offs = reinterpret_cast<int*>(table_ptr);
+    const detail::GroupedTable table =
+        detail::make_table(p, offs, offs + kMaxGemmGroups + 2, 256, 256, warp, lane, Cfg::kThreads);
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::cluster_arrive_release();
+    ptx::cluster_wait_acquire();
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot_ptr;
+    const int total = detail::total_tiles(p, table);
+    const int ext_blocks = 2 * ((p.ext_cols + 63) / 64);
+    const int unit = static_cast<int>(blockIdx.x >> 1);
+    const int units = static_cast<int>(gridDim.x >> 1);
+    const bool wgrad = p.form == kFormWgrad;
+    const bool gather = p.load_a != 0;
+
+    // ---- roles --------------------------------------------------------------------------------
+    if (warp == 0) {
+        if (ptx::elect_one_sync()) {
+            // TMA producer: this CTA's columns and, unless gathered, its half of the rows.  All bytes
+            // of a stage are credited to the leader's barrier.
+            uint32_t it = 0;
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            uint32_t bar = 0;
+            auto acquire_stage = [&](uint32_t bytes_of_both) -> bool {
+                if (!detail::wait_barrier(empty_bar(stage), phase ^ 1u, ctl, kRoleProducer, it)) {
+                    return false;
+                }
+                if (leader) {
+                    const bool wrong = p.overstate_first_stage != 0 && it == 0 && blockIdx.x == 0;
+                    ptx::mbar_arrive_expect_tx(full_bar(stage), bytes_of_both + (wrong ? 16u : 0u));
+                }
+                bar = ptx::map_to_cta(full_bar(stage), 0);
+                return true;
+            };
+            auto advance = [&]() {
+                ++it;
+                if (++stage == kStages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+            };
+            for (int tile = unit; ok && tile < total; tile += units) {
+                const detail::PairTile t = detail::pair_tile(p, table, tile);
+                const int col0 = t.c0 + static_cast<int>(rank) * 128;
+                // 64-column boxes that exist, of this CTA and of both
+                const int boxes = min(2, max(0, (p.n - col0 + 63) / 64));
+                const uint32_t cols_bytes =
+                    static_cast<uint32_t>(min(4, (p.n - t.c0 + 63) / 64)) * Cfg::kBoxBytes;
+                auto load_cols = [&](uint32_t dst, const CUtensorMap* map, int k0, int z) {
+                    for (int b = 0; b < boxes; ++b) {
+                        const int col = col0 + b * 64;
+                        ptx::tma_load_3d_pair(dst + b * Cfg::kBoxBytes, map, bar, p.trans_b ? k0 : col,
+                                              p.trans_b ? col : k0, z);
+                    }
+                };
+                if (!wgrad) {
+                    const int group = table.whole ? 0 : t.group;
+                    const int row0 = t.p0 + static_cast<int>(rank) * t.half;
+                    const int row_boxes = (t.half + 31) / 32;  // 32 rows each
+                    const uint32_t rows_bytes = gather ? 0u : 2u * static_cast<uint32_t>(row_boxes) * 4096u;
+                    for (int kb = 0; kb < t.k_blocks; ++kb) {
+                        if (!acquire_stage(cols_bytes + rows_bytes)) {
+                            ok = false;
+                            break;
+                        }
+                        const uint32_t dst = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
+                        load_cols(dst, &tmap_cols, kb * 64, group);
+                        for (int b = 0; !gather && b < row_boxes; ++b) {
+                            // rows behind the tile's last are another tile's, or zeros: not stored
+                            ptx::tma_load_2d_pair(dst + Cfg::kColsBytes + b * 4096u, &tmap_rows, bar, kb * 64,
+                                                  row0 + b * 32);
+                        }
+                        advance();
+                    }
+                    for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
+                        const detail::Span span = detail::adapter_span(table, t, g);
+                        if (span.lo >= span.hi) {
+                            continue;
+                        }
+                        for (int eb = 0; eb < ext_blocks; ++eb) {
+                            if (!acquire_stage(cols_bytes)) {
+                                ok = false;
+                                break;
+                            }
+                            load_cols(ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes, &tmap_ext,
+                                      (eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb) * 64, g);
+                            advance();
+                        }
+                    }
+                } else {
+                    const int row0 = t.r0 + static_cast<int>(rank) * t.half;
+                    // boxes of 64 rows of W_g (columns of A) that exist, of this CTA and of both
+                    auto existing = [&](int from) { return min(t.half / 64, max(0, (p.m - from + 63) / 64)); };
+                    const int row_boxes = existing(row0);
+                    const uint32_t rows_bytes =
+                        gather ? 0u
+                               : static_cast<uint32_t>(existing(t.r0) + existing(t.r0 + t.half)) * Cfg::kBoxBytes;
+                    for (int kb = 0; kb < t.k_blocks; ++kb) {
+                        // a last block that is not whole comes through the loaders
+                        const bool whole = t.valid - kb * 64 >= 64;
+                        if (!acquire_stage(whole ? cols_bytes + rows_bytes : 0u)) {
+                            ok = false;
+                            break;
+                        }
+                        const uint32_t dst = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
+                        const int pos = t.p0 + kb * 64;
+                        for (int b = 0; whole && b < boxes; ++b) {
+                            ptx::tma_load_3d_pair(dst + b * Cfg::kBoxBytes, &tmap_cols, bar, col0 + b * 64, pos, 0);
+                        }
+                        for (int b = 0; whole && !gather && b < row_boxes; ++b) {
+                            ptx::tma_load_2d_pair(dst + Cfg::kColsBytes + b * Cfg::kBoxBytes, &tmap_rows, bar,
+                                                  row0 + b * 64, pos);
+                        }
+                        advance();
+                    }
+                }
+            }
+            // Tail: no copy into this CTA may be in flight and no stage may still be signalled when
+            // it ends.
+            const uint32_t first = it > static_cast<uint32_t>(kStages) ? it - kStages : 0u;
+            for (uint32_t i = first; i < it; ++i) {
+                const int s = static_cast<int>(i % kStages);
+                const uint32_t use = i / kStages;
+                if (ok && !detail::wait_barrier(empty_bar(s), use & 1u, ctl, kRoleDrain, i)) {
+                    ok = false;
+                }
+                if (!ok) {
+                    if (leader) {
+                        detail::drain_wait(full_bar(s), use & 1u);
+                    } else {
+                        __nanosleep(20000);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (leader && ptx::elect_one_sync()) {
+            // MMA issuer, for both CTAs.  Offsets per 16 reduced elements: 32 B along a K-major row,
+            // 2048 B (16 rows) in an MN-major box.
+            const bool cols_mn = wgrad || !p.trans_b;
+            const bool rows_mn = wgrad;
+            const uint32_t cols_step = cols_mn ? 2048u >> 4 : 32u >> 4;
+            const uint32_t rows_step = rows_mn ? 2048u >> 4 : 32u >> 4;
+            uint32_t it = 0;
+            int stage = 0;
+            uint32_t phase = 0;
+            uint32_t loaded_phase = 0;
+            uint32_t count = 0;
+            bool ready = false;
+            bool ok = true;
+            for (int tile = unit; ok && tile < total; tile += units) {
+                const detail::PairTile t = detail::pair_tile(p, table, tile);
+                const uint32_t acc = count & 1u;
+                if (!detail::wait_barrier(acc_empty_bar(acc), ((count >> 1) & 1u) ^ 1u, ctl, kRoleMma,
+                                          0x80000000u | count)) {
+                    ok = false;
+                    break;
+                }
+                ptx::tc_fence_after_sync();
+                const uint32_t d_tmem = tmem_base + acc * 256u;
+                const uint32_t idesc = ptx::make_idesc_f16(p.fmt, cols_mn ? 1u : 0u, rows_mn ? 1u : 0u, 256,
+                                                           static_cast<uint32_t>(2 * t.half));
+                uint32_t accumulate = 0;
+                auto block = [&](int steps, bool loaded) -> bool {
+                    if (!ready && !detail::wait_barrier(full_bar(stage), phase, ctl, kRoleMma, it)) {
+                        return false;
+                    }
+                    if (loaded) {
+                        if (!detail::wait_cluster_barrier(loaded_bar(stage), (loaded_phase >> stage) & 1u, ctl,
+                                                          kRoleMma, 0x40000000u | it)) {
+                            return false;
+                        }
+                        loaded_phase ^= 1u << stage;
+                    }
+                    const uint32_t cols_src = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
+                    const uint64_t cols_desc =
+                        ptx::make_smem_desc_sw128(cols_src, cols_mn ? Cfg::kBoxBytes : 16u, 1024);
+                    const uint64_t rows_desc = ptx::make_smem_desc_sw128(
+                        cols_src + Cfg::kColsBytes, rows_mn ? Cfg::kBoxBytes : 16u, 1024);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (j < steps) {
+                            ptx::umma_f16_pair(d_tmem, cols_desc + static_cast<uint64_t>(j * cols_step),
+                                               rows_desc + static_cast<uint64_t>(j * rows_step), idesc, accumulate);
+                            accumulate = 1;
+                        }
+                        if (j == 0) {
+                            ready = ptx::mbar_try_wait(full_bar(stage + 1 == kStages ? 0 : stage + 1),
+                                                       stage + 1 == kStages ? phase ^ 1u : phase);
+                        }
+                    }
+                    ptx::umma_commit_pair(empty_bar(stage));
+                    ptx::umma_commit_pair(ptx::map_to_cta(empty_bar(stage), 1));
+                    ++it;
+                    if (++stage == kStages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                    return true;
+                };
+                for (int kb = 0; kb < t.k_blocks; ++kb) {
+                    if (!block(4, gather || (wgrad && t.valid - kb * 64 < 64))) {
+                        ok = false;
+                        break;
+                    }
+                }
+                for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
+                    const detail::Span span = detail::adapter_span(table, t, g);
+                    if (span.lo >= span.hi) {
+                        continue;
+                    }
+                    for (int eb = 0; eb < ext_blocks; ++eb) {
+                        const int in_part = eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb;
+                        if (!block(min(4, (p.ext_cols - in_part * 64) / 16), true)) {
+                            ok = false;
+                            break;
+                        }
+                    }
+                }
+                if (ok) {
+                    if (accumulate != 0) {
+                        ptx::umma_commit_pair(acc_full_bar(acc));
+                        ptx::umma_commit_pair(ptx::map_to_cta(acc_full_bar(acc), 1));
+                    } else {  // nothing to sum: the epilogue uses zeros
+                        ptx::mbar_arrive(acc_full_bar(acc));
+                        ptx::mbar_arrive_cluster(ptx::map_to_cta(acc_full_bar(acc), 1));
+                    }
+                    ++count;
+                }
+            }
+            if (ok) {
+                const uint32_t first = count > 2u ? count - 2u : 0u;
+                for (uint32_t i = first; i < count && ok; ++i) {
+                    ok = detail::wait_barrier(acc_empty_bar(i & 1u), (i >> 1) & 1u, ctl, kRoleDrain,
+                                              0x80000000u | i);
+                }
+            } else {
+                ptx::umma_commit_pair(drain_bar);
+                detail::drain_wait(drain_bar, 0);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= Cfg::kFirstLoader) {
+        // Loaders, one warp per stage as in the single-CTA kernel; a stage is handed to the leader.
+        const detail::Loader load(ring + static_cast<uint32_t>(warp - Cfg::kFirstLoader) * Cfg::kStageBytes, lane);
+        const int own = warp - Cfg::kFirstLoader;
+        uint32_t it = 0;     // blocks so far, whoever owns their stage
+        uint32_t phase = 0;  // of the own stage
+        bool ok = true;
+        auto acquire = [&]() -> bool {
+            const bool got =
+                detail::wait_barrier(empty_bar(own), phase ^ 1u, ctl, kRoleProducer, 0x20000000u | it);
+            phase ^= 1u;
+            return __all_sync(0xFFFFFFFFu, got) != 0;
+        };
+        auto hand_over = [&]() {
+            load.finish();
+            if (lane == 0) {
+                ptx::mbar_arrive_cluster_release(ptx::map_to_cta(loaded_bar(own), 0));
+            }
+        };
+        for (int tile = unit; (wgrad || gather || p.ext_groups > 0) && ok && tile < total; tile += units) {
+            const detail::PairTile t = detail::pair_tile(p, table, tile);
+            const int first_row = static_cast<int>(rank) * t.half;  // of this CTA, in the tile
+            if (!wgrad) {
+                const int rows = max(0, min(t.half, t.valid - first_row));  // of this CTA that exist
+                int src[4] = {-1, -1, -1, -1};  // lane l: rows l, 32 + l, 64 + l, 96 + l of A, -1: none
+                if (gather) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int r = q * 32 + static_cast<int>(lane);
+                        const int at = r >= rows             ? -1
+                                       : p.a_rows != nullptr ? __ldg(p.a_rows + t.p0 + first_row + r)
+                                                             : t.p0 + first_row + r;
+                        src[q] = at < p.a_count ? at : -1;
+                    }
+                }
+                for (int kb = 0; kb < t.k_blocks; ++kb, ++it) {
+                    if (static_cast<int>(it % kStages) != own) {
+                        continue;
+                    }
+                    if (!acquire()) {
+                        ok = false;
+                        break;
+                    }
+                    if (gather) {
+                        load.rows128(Cfg::kColsBytes, p.a, p.lda, src, rows, kb * 64, p.k);
+                        hand_over();
+                    }
+                }
+                for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
+                    const detail::Span span = detail::adapter_span(table, t, g);
+                    if (span.lo >= span.hi) {
+                        continue;
+                    }
+                    for (int eb = 0; eb < ext_blocks; ++eb, ++it) {
+                        if (static_cast<int>(it % kStages) != own) {
+                            continue;
+                        }
+                        if (!acquire()) {
+                            ok = false;
+                            break;
+                        }
+                        const int part = eb >= ext_blocks / 2 ? 1 : 0;
+                        load.adapter_rows(Cfg::kColsBytes, p, t.p0 + first_row, rows, span.lo, span.hi, part,
+                                          (eb - part * (ext_blocks / 2)) * 64);
+                        hand_over();
+                    }
+                }
+            } else {
+                const int first = (own - static_cast<int>(it % kStages) + kStages) % kStages;
+                int next[2];
+                auto fetch = [&](int kb) {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int r = kb * 64 + q * 32 + static_cast<int>(lane);
+                        const int at = r >= t.valid          ? -1
+                                       : p.a_rows != nullptr ? __ldg(p.a_rows + t.p0 + r)
+                                                             : t.p0 + r;
+                        next[q] = at < p.a_count ? at : -1;
+                    }
+                };
+                fetch(first);
+                for (int kb = first; kb < t.k_blocks; kb += kStages) {
+                    const int left = t.valid - kb * 64;
+                    const int rows[2] = {next[0], next[1]};
+                    fetch(kb + kStages);
+                    if (!acquire()) {
+                        ok = false;
+                        break;
+                    }
+                    if (gather || left < 64) {
+                        load.rows64(Cfg::kColsBytes, p.a, p.lda, rows, t.half / 64, t.r0 + first_row, p.m);
+                        if (left < 64) {
+                            int at[2];
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                const int r = q * 32 + static_cast<int>(lane);
+                                at[q] = r < left ? t.p0 + kb * 64 + r : -1;
+                            }
+                            load.rows64(0, p.b, p.ldb, at, 2, t.c0 + static_cast<int>(rank) * 128, p.n);
+                        }
+                        hand_over();
+                    }
+                }
+                it += static_cast<uint32_t>(t.k_blocks);
+            }
+        }
+        ptx::cp_async_wait_all();  // no copy may be in flight when the CTA ends
+    } else {
+        // Epilogue warps 2-5: TMEM lane quarter = warp id mod 4 = 32 columns of C.
+        using T = detail::OutTraits<Elem>;
+        constexpr int kVec = T::kVec;
+        constexpr int kLanesPerRow = 32 / kVec;
+        constexpr int kRowsPerPass = 32 / kLanesPerRow;
+        // one buffer of 32 rows x 32 columns: 64-byte rows for 16-bit types (three buffers), 128-byte
+        // rows for FP32 (one; the third 2 KB stay unused)
+        constexpr uint32_t kRowBytes = 32 * sizeof(Elem);
+        constexpr uint32_t kBuffers = kRowBytes == 64 ? 3 : 1;
+        const uint32_t quad = static_cast<uint32_t>(warp) & 3u;
+        uint8_t* stg = staging_ptr + quad * Cfg::kWarpStaging;
+        const uint32_t stg_addr = ring + kStages * Cfg::kStageBytes + quad * Cfg::kWarpStaging;
+        const int sub = static_cast<int>(lane) % kLanesPerRow;
+        uint32_t buffer = 0;
+        uint32_t count = 0;
+        bool alive = true;
+        for (int tile = unit; alive && tile < total; tile += units) {
+            const detail::PairTile t = detail::pair_tile(p, table, tile);
+            const uint32_t acc = count & 1u;
+            const bool got =
+                detail::wait_barrier(acc_full_bar(acc), (count >> 1) & 1u, ctl, kRoleEpilogue, count);
+            if (!__all_sync(0xFFFFFFFFu, got)) {
+                alive = false;
+                break;
+            }
+            ptx::tc_fence_after_sync();
+            const bool nothing = t.k_blocks == 0;
+            const int col0 = t.c0 + static_cast<int>(rank) * 128 + static_cast<int>(quad) * 32;
+            const uint32_t t_row = tmem_base + ((quad * 32u) << 16) + acc * 256u;
+            const int rows = col0 < p.n ? t.rows : 0;  // rows this warp stores
+            Elem* c_base =
+                static_cast<Elem*>(p.c) + (wgrad ? static_cast<long long>(t.group) * p.c_stride : 0ll);
+            const float factor = p.alpha * (p.scales != nullptr ? __ldg(p.scales + t.group) : 1.0f);
+            const int z = wgrad ? t.group : 0;
+            uint32_t r[32];
+            auto fetch = [&](int j0) {
+                if (nothing) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        r[i] = 0;
+                    }
+                } else {
+                    ptx::tmem_ld_32x32(t_row + static_cast<uint32_t>(j0), r);
+                }
+            };
+            if (rows > 0) {
+                fetch(0);
+            }
+            bool released = false;
+            auto release = [&]() {  // once, when the last accumulator column is in registers
+                if (!released) {
+                    released = true;
+                    ptx::tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) {
+                        ptx::mbar_arrive_cluster(ptx::map_to_cta(acc_empty_bar(acc), 0));
+                    }
+                }
+            };
+            for (int j0 = 0; j0 < rows; j0 += 32) {
+                ptx::tmem_ld_wait();
+                if (j0 + 32 >= rows) {
+                    release();
+                }
+                // Whole runs of 32 consecutive rows leave by TMA, which clips at the edge of C; in a
+                // weight gradient it clips rows as well.
+                const bool by_tma = p.c_tma != 0 && (wgrad || j0 + 32 <= rows);
+                if (lane == 0) {
+                    // the stores that last used the buffer have read it
+                    if (by_tma) {
+                        ptx::bulk_wait_group_read<kBuffers - 1>();
+                    } else {
+                        ptx::bulk_wait_group_read<0>();
+                    }
+                }
+                __syncwarp();
+                if (by_tma) {
+                    uint8_t* buf = stg + buffer * 2048u;
+                    if constexpr (kRowBytes == 64) {
+                        // 64-byte swizzle: the 16-byte unit is exchanged by row bits 1 and 2
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            T::store(reinterpret_cast<Elem*>(buf + j * 64 +
+                                                             (((lane >> 3) ^ ((j >> 1) & 3u)) << 4) +
+                                                             (lane & 7u) * 2u),
+                                     factor * __uint_as_float(r[j]));
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            *reinterpret_cast<float*>(buf + j * 128 + (((lane >> 2) ^ (j & 7u)) << 4) +
+                                                      (lane & 3u) * 4u) = factor * __uint_as_float(r[j]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        *reinterpret_cast<uint32_t*>(stg + j * 128 + (((lane >> 2) ^ (j & 7u)) << 4) +
+                                                     (lane & 3u) * 4u) = r[j];
+                    }
+                }
+                if (j0 + 32 < rows) {
+                    fetch(j0 + 32);
+                }
+                if (by_tma) {
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        ptx::tma_store_3d(&tmap_c, stg_addr + buffer * 2048u, col0, t.r0 + j0, z);
+                        ptx::bulk_commit_group();
+                    }
+                    buffer = buffer + 1 == kBuffers ? 0u : buffer + 1;
+                } else {
+                    __syncwarp();
+                    const int col = col0 + sub * kVec;
+                    const int have = min(kVec, p.n - col);
+#pragma unroll
+                    for (int pass = 0; pass < 32 / kRowsPerPass; ++pass) {
+                        const int j = pass * kRowsPerPass + static_cast<int>(lane) / kLanesPerRow;
+                        int c_row = -1;
+                        if (j0 + j < rows) {
+                            c_row = wgrad || p.c_rows == nullptr ? t.r0 + j0 + j
+                                                                 : __ldg(p.c_rows + t.p0 + j0 + j);
+                            c_row = wgrad || (c_row >= 0 && c_row < p.c_count) ? c_row : -1;
+                        }
+                        float v[kVec];
+#pragma unroll
+                        for (int u = 0; u < kVec / 4; ++u) {
+                            const float4 x = *reinterpret_cast<const float4*>(
+                                stg + j * 128 + (((sub * (kVec / 4) + u) ^ (j & 7)) << 4));
+                            v[4 * u] = x.x;
+                            v[4 * u + 1] = x.y;
+                            v[4 * u + 2] = x.z;
+                            v[4 * u + 3] = x.w;
+                        }
+                        if (c_row >= 0 && have > 0) {
+                            detail::store_unit<OutT, kVec>(p, c_base, c_row, col, have, factor, v);
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            release();
+            ++count;
+        }
+        if (lane == 0) {
+            ptx::bulk_wait_group_read<0>();  // no store may read shared memory when the CTA ends
+        }
+        __syncwarp();
+    }
+
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::cluster_arrive_release();
+    ptx::cluster_wait_acquire();
+    if (warp == 1) {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+}  // namespace ckl

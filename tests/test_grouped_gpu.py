@@ -426,3 +426,104 @@ def test_lora_few_rows(ckl, m, g):
             ref, mag = ref + t @ b[i].double(), mag + ta @ b[i].double().abs()
             extra = TWO_PART["bf16"] * (t.abs() @ b[i].double().abs())
         check(y[sel], ref, mag, 2 * k + 2 * r + 10, "bf16", extra)
+
+
+def many_groups(seed, count, most):
+    g = torch.Generator().manual_seed(seed)
+    sizes = torch.randint(0, most, (count,), generator=g)
+    sizes[::7] = 0
+    sizes[1], sizes[2], sizes[3] = 1, 256, 257
+    return sizes.tolist()
+
+
+@pytest.mark.parametrize("trans", [False, True], ids=["nn", "nt"])
+@pytest.mark.parametrize("gather", [False, True], ids=["rows", "gather"])
+@pytest.mark.parametrize("out,beta,ldc,k", [("bf16", 0.0, 264, 136), ("f32", 0.0, 264, 72), ("f32", 0.5, 265, 72),
+                                            ("f16", 0.0, 267, 13)])
+def test_grouped_pairs(ckl, trans, gather, out, beta, ldc, k):
+    """Tiles enough for CTA pairs: ragged groups from none to two tiles, edges in every direction."""
+    sizes, n = many_groups(5, 60, 600), 264
+    offs = offsets_of(sizes)
+    kept, tokens = int(offs[-1]), 333
+    rows, lda, ldb = kept + 5, (k + 7) // 8 * 8, (k + 7) // 8 * 8 if trans else n
+    a = rand((tokens if gather else rows, lda), torch.bfloat16, 1)
+    if not gather:
+        a[kept:] = float("nan")
+    idx = torch.randint(-1, tokens, (rows,), device="cuda", dtype=torch.int32) if gather else None
+    b = rand((60, n, ldb) if trans else (60, k, ldb), torch.bfloat16, 2, k ** -0.5)
+    c = rand((rows, ldc), DT[out], 3)
+    c0 = c.clone()
+    ckl.gemm_grouped(ckl.BF16, a, b, c, code(ckl, out), offs, 60, rows, n, k, lda=lda, ldb=ldb, ldc=ldc,
+                     stride_b=b.stride(0), a_rows=idx, a_count=tokens if gather else None, trans_b=trans, alpha=1.5,
+                     beta=beta)
+    torch.cuda.synchronize()
+    assert torch.equal(c[kept:], c0[kept:]) and torch.equal(c[:, n:], c0[:, n:])
+    src = a[:, :k].double()
+    if gather:
+        src = torch.where((idx >= 0).unsqueeze(1), src[idx.long().clamp(min=0)], 0.0)
+    o = offs.tolist()
+    for g in range(60):
+        x, w = src[o[g]:o[g + 1]], (b[g, :, :k].t() if trans else b[g]).double()
+        old = beta * c0[o[g]:o[g + 1], :n].double()
+        check(c[o[g]:o[g + 1], :n], 1.5 * (x @ w) + old, 1.5 * (x.abs() @ w.abs()) + old.abs(), k + 2, out)
+
+
+@pytest.mark.parametrize("gather", [False, True], ids=["rows", "gather"])
+@pytest.mark.parametrize("out,beta,m,n", [("bf16", 0.0, 264, 264), ("f32", 0.0, 133, 520), ("f32", 1.0, 392, 131),
+                                          ("f16", 0.0, 600, 200)])
+def test_weight_gradient_pairs(ckl, gather, out, beta, m, n):
+    sizes = many_groups(6, 50, 200)
+    offs = offsets_of(sizes)
+    kept, tokens = int(offs[-1]), 300
+    rows, lda, ldg = kept + 3, (m + 7) // 8 * 8, (n + 7) // 8 * 8
+    a = rand((tokens if gather else rows, lda), torch.float16, 1)
+    idx = torch.randint(-1, tokens, (rows,), device="cuda", dtype=torch.int32) if gather else None
+    d = rand((rows, ldg), torch.float16, 2)
+    d[kept:] = float("nan")
+    w = rand((50, m, n), DT[out], 3)
+    w0 = w.clone()
+    ckl.gemm_grouped_wgrad(ckl.F16, a, d, w, code(ckl, out), offs, 50, rows, m, n, lda=lda, ldg=ldg, a_rows=idx,
+                           a_count=tokens if gather else None, alpha=0.5, beta=beta)
+    torch.cuda.synchronize()
+    src = a[:, :m].double()
+    if gather:
+        src = torch.where((idx >= 0).unsqueeze(1), src[idx.long().clamp(min=0)], 0.0)
+    o = offs.tolist()
+    for g in range(50):
+        x, y, old = src[o[g]:o[g + 1]], d[o[g]:o[g + 1], :n].double(), beta * w0[g].double()
+        check(w[g], 0.5 * (x.t() @ y) + old, 0.5 * (x.abs().t() @ y.abs()) + old.abs(), sizes[g] + 2, out)
+
+
+@pytest.mark.parametrize("trans", [False, True], ids=["forward", "dx"])
+@pytest.mark.parametrize("r", [8, 72])
+def test_lora_pairs(ckl, trans, r):
+    """A prefill batch: adapters begin and end inside the tiles, and one tile holds many of them."""
+    m, g, k, n = 2701, 90, 200, 1032
+    if trans:
+        k, n = n, k
+    gen = torch.Generator(device="cuda").manual_seed(r)
+    ids = torch.randint(-1, g, (m,), generator=gen, device="cuda", dtype=torch.int32)
+    ids[:900] = 3
+    m, x, w, a, b, s, offs, rows = lora_case(ckl, ids, g, k, n, r, "f16", 70)
+    size = ckl.gemm_lora_workspace_bytes(m, r, True)
+    ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    dy = rand((m, n), torch.float16, 80)
+    out = torch.full((m, k if trans else n), float("nan"), device="cuda")
+    if trans:
+        ckl.gemm_lora_backward(ckl.F16, dy, x, w, a, b, s, out, ckl.F32, None, None, ckl.F32, offs, rows, g, m, n, k, r,
+                               ws, size)
+    else:
+        ckl.gemm_lora(ckl.F16, x, w, a, b, s, out, ckl.F32, offs, rows, g, m, n, k, r, ws, size)
+    torch.cuda.synchronize()
+    for i in range(-1, g):
+        sel = ids == i
+        v, ww = (dy[sel], w.t()) if trans else (x[sel], w)
+        v, ww = v.double(), ww.double()
+        ref, mag, extra = v @ ww, v.abs() @ ww.abs(), 0.0
+        if i >= 0:
+            p1, p2 = (b[i].t(), a[i].t()) if trans else (a[i], b[i])
+            t = s[i].double() * (v @ p1.double())
+            ta = s[i].double() * (v.abs() @ p1.double().abs())
+            ref, mag = ref + t @ p2.double(), mag + ta @ p2.double().abs()
+            extra = TWO_PART["f16"] * (t.abs() @ p2.double().abs()) + 2.0 ** -25 * r * p2.double().abs().max()
+        check(out[sel], ref, mag, 2 * max(k, n) + 2 * r, "f32", extra)
