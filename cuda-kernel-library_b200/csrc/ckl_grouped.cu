@@ -189,7 +189,7 @@ int run(Product& q, cudaStream_t stream) {
     std::memset(&maps, 0, sizeof maps);
     if (p.load_a == 0) {
         GRP_TRY(encode_operand(&maps.a_box, q.ab_dtype, q.a, q.a_cols, p.a_count, q.lda, 0, 0, 64,
-                               wgrad ? 64 : pair ? 32 : 128));
+                               wgrad || pair ? 64 : 128));
     }
     if (!wgrad || p.b_rows == nullptr) {
         GRP_TRY(encode_operand(&maps.b_box, q.ab_dtype, q.b, q.b_cols, wgrad ? p.b_count : q.b_outer, q.ldb,

@@ -587,11 +587,16 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                 const int boxes = (t.cols + 63) / 64;
                 const uint32_t b_bytes = static_cast<uint32_t>(boxes) * Cfg::kBoxBytes;
                 // 64 k rows of matrix z of a stack, k0 on, as columns n0 .. of the tile
+                // (all box loops are unrolled: one thread issues them, and a rolled loop spends about
+                // 100 cycles on each)
                 auto load_b = [&](uint32_t dst, const CUtensorMap* map, int k0, int z) {
-                    for (int b = 0; b < boxes; ++b) {
-                        const int col = t.n0 + b * 64;
-                        ptx::tma_load_3d(dst + b * Cfg::kBoxBytes, map, full_bar(stage),
-                                         p.trans_b ? k0 : col, p.trans_b ? col : k0, z);
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        if (b < boxes) {
+                            const int col = t.n0 + b * 64;
+                            ptx::tma_load_3d(dst + b * Cfg::kBoxBytes, map, full_bar(stage),
+                                             p.trans_b ? k0 : col, p.trans_b ? col : k0, z);
+                        }
                     }
                 };
                 if (p.form == kFormRows) {
@@ -645,13 +650,20 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                             break;
                         }
                         const uint32_t a_dst = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
-                        for (int b = 0; whole && !gather_a && b < a_boxes; ++b) {
-                            ptx::tma_load_2d(a_dst + b * Cfg::kBoxBytes, &tmap_a_box, full_bar(stage),
-                                             t.m0 + part * p.a_part_cols + b * 64, t.p0 + at);
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            if (whole && !gather_a && b < a_boxes) {
+                                ptx::tma_load_2d(a_dst + b * Cfg::kBoxBytes, &tmap_a_box, full_bar(stage),
+                                                 t.m0 + part * p.a_part_cols + b * 64, t.p0 + at);
+                            }
                         }
-                        for (int b = 0; whole && !gather_b && b < boxes; ++b) {
-                            ptx::tma_load_3d(a_dst + Cfg::kABytes + b * Cfg::kBoxBytes, &tmap_b_box,
-                                             full_bar(stage), t.n0 + part * p.b_part_cols + b * 64, t.p0 + at, 0);
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            if (whole && !gather_b && b < boxes) {
+                                ptx::tma_load_3d(a_dst + Cfg::kABytes + b * Cfg::kBoxBytes, &tmap_b_box,
+                                                 full_bar(stage), t.n0 + part * p.b_part_cols + b * 64, t.p0 + at,
+                                                 0);
+                            }
                         }
                         advance();
                     }

@@ -102,17 +102,6 @@ __device__ __forceinline__ Span adapter_span(const GroupedTable& table, const Pa
     return {max(table.offs[g], t.p0), min(table.offs[g + 1], t.p0 + t.valid)};
 }
 
-// As wait_barrier, ordered after writes that the other CTA of the cluster released.
-__device__ __forceinline__ bool wait_cluster_barrier(uint32_t bar, uint32_t parity, const Control& ctl,
-                                                     unsigned int role, unsigned int detail_word) {
-    if (!wait_barrier(bar, parity, ctl, role, detail_word)) {
-        return false;
-    }
-    for (int i = 0; i < 1024 && !ptx::mbar_try_wait_cluster(bar, parity); ++i) {
-    }
-    return true;
-}
-
 }  // namespace detail
 
 template <typename OutT>
@@ -226,18 +215,23 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                 const int boxes = min(2, max(0, (p.n - col0 + 63) / 64));
                 const uint32_t cols_bytes =
                     static_cast<uint32_t>(min(4, (p.n - t.c0 + 63) / 64)) * Cfg::kBoxBytes;
+                // (all box loops are unrolled: one thread issues them, and a rolled loop spends about
+                // 100 cycles on each)
                 auto load_cols = [&](uint32_t dst, const CUtensorMap* map, int k0, int z) {
-                    for (int b = 0; b < boxes; ++b) {
-                        const int col = col0 + b * 64;
-                        ptx::tma_load_3d_pair(dst + b * Cfg::kBoxBytes, map, bar, p.trans_b ? k0 : col,
-                                              p.trans_b ? col : k0, z);
+#pragma unroll
+                    for (int b = 0; b < 2; ++b) {
+                        if (b < boxes) {
+                            const int col = col0 + b * 64;
+                            ptx::tma_load_3d_pair(dst + b * Cfg::kBoxBytes, map, bar, p.trans_b ? k0 : col,
+                                                  p.trans_b ? col : k0, z);
+                        }
                     }
                 };
                 if (!wgrad) {
                     const int group = table.whole ? 0 : t.group;
                     const int row0 = t.p0 + static_cast<int>(rank) * t.half;
-                    const int row_boxes = (t.half + 31) / 32;  // 32 rows each
-                    const uint32_t rows_bytes = gather ? 0u : 2u * static_cast<uint32_t>(row_boxes) * 4096u;
+                    const int row_boxes = gather ? 0 : (t.half + 63) / 64;
+                    const uint32_t rows_bytes = 2u * static_cast<uint32_t>(row_boxes) * Cfg::kBoxBytes;
                     for (int kb = 0; kb < t.k_blocks; ++kb) {
                         if (!acquire_stage(cols_bytes + rows_bytes)) {
                             ok = false;
@@ -245,10 +239,13 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                         }
                         const uint32_t dst = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
                         load_cols(dst, &tmap_cols, kb * 64, group);
-                        for (int b = 0; !gather && b < row_boxes; ++b) {
-                            // rows behind the tile's last are another tile's, or zeros: not stored
-                            ptx::tma_load_2d_pair(dst + Cfg::kColsBytes + b * 4096u, &tmap_rows, bar, kb * 64,
-                                                  row0 + b * 32);
+                        // rows behind the tile's last are another tile's, or zeros: not stored
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            if (b < row_boxes) {
+                                ptx::tma_load_2d_pair(dst + Cfg::kColsBytes + b * Cfg::kBoxBytes, &tmap_rows, bar,
+                                                      kb * 64, row0 + b * 64);
+                            }
                         }
                         advance();
                     }
@@ -284,12 +281,19 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                         }
                         const uint32_t dst = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
                         const int pos = t.p0 + kb * 64;
-                        for (int b = 0; whole && b < boxes; ++b) {
-                            ptx::tma_load_3d_pair(dst + b * Cfg::kBoxBytes, &tmap_cols, bar, col0 + b * 64, pos, 0);
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            if (whole && b < boxes) {
+                                ptx::tma_load_3d_pair(dst + b * Cfg::kBoxBytes, &tmap_cols, bar, col0 + b * 64, pos,
+                                                      0);
+                            }
                         }
-                        for (int b = 0; whole && !gather && b < row_boxes; ++b) {
-                            ptx::tma_load_2d_pair(dst + Cfg::kColsBytes + b * Cfg::kBoxBytes, &tmap_rows, bar,
-                                                  row0 + b * 64, pos);
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            if (whole && !gather && b < row_boxes) {
+                                ptx::tma_load_2d_pair(dst + Cfg::kColsBytes + b * Cfg::kBoxBytes, &tmap_rows, bar,
+                                                      row0 + b * 64, pos);
+                            }
                         }
                         advance();
                     }
@@ -347,8 +351,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                         return false;
                     }
                     if (loaded) {
-                        if (!detail::wait_cluster_barrier(loaded_bar(stage), (loaded_phase >> stage) & 1u, ctl,
-                                                          kRoleMma, 0x40000000u | it)) {
+                        if (!detail::wait_barrier(loaded_bar(stage), (loaded_phase >> stage) & 1u, ctl, kRoleMma,
+                                                  0x40000000u | it)) {
                             return false;
                         }
                         loaded_phase ^= 1u << stage;
@@ -370,8 +374,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                                                        stage + 1 == kStages ? phase ^ 1u : phase);
                         }
                     }
-                    ptx::umma_commit_pair(empty_bar(stage));
-                    ptx::umma_commit_pair(ptx::map_to_cta(empty_bar(stage), 1));
+                    ptx::umma_commit_pair_both(empty_bar(stage));
                     ++it;
                     if (++stage == kStages) {
                         stage = 0;
@@ -400,8 +403,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                 }
                 if (ok) {
                     if (accumulate != 0) {
-                        ptx::umma_commit_pair(acc_full_bar(acc));
-                        ptx::umma_commit_pair(ptx::map_to_cta(acc_full_bar(acc), 1));
+                        ptx::umma_commit_pair_both(acc_full_bar(acc));
                     } else {  // nothing to sum: the epilogue uses zeros
                         ptx::mbar_arrive(acc_full_bar(acc));
                         ptx::mbar_arrive_cluster(ptx::map_to_cta(acc_full_bar(acc), 1));
@@ -437,7 +439,10 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
         auto hand_over = [&]() {
             load.finish();
             if (lane == 0) {
-                ptx::mbar_arrive_cluster_release(ptx::map_to_cta(loaded_bar(own), 0));
+                // The stage lies in this CTA's shared memory and this SM's tensor core reads it: the
+                // proxy fence in finish() has made the writes visible to it, the arrival only tells
+                // the issuing thread.  (The cluster-scope release form waits about 2500 cycles.)
+                ptx::mbar_arrive_cluster(ptx::map_to_cta(loaded_bar(own), 0));
             }
         };
         for (int tile = unit; (wgrad || gather || p.ext_groups > 0) && ok && tile < total; tile += units) {

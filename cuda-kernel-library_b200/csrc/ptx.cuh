@@ -109,25 +109,6 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
     return done != 0;
 }
 
-// The same, ordered after what the other CTAs of the cluster released with their arrivals.
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t"
-        "}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-// Arrival (possibly at another CTA's barrier) that publishes this thread's writes to the cluster.
-__device__ __forceinline__ void mbar_arrive_cluster_release(uint32_t cluster_bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
-}
-
 // Same probe, but the hardware may park the thread for up to `hint_ns` while
 // the phase is incomplete (it resumes at once when the phase completes), so a
 // long wait costs a handful of instructions instead of a busy spin.
@@ -404,7 +385,14 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t cluster_bar) {
                      cluster_bar)
                  : "memory");
 }
-
+// The same arrival at the barriers of both CTAs of the pair (same offset in either), one instruction.
+__device__ __forceinline__ void umma_commit_pair_both(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(bar),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
 
 // ---- tcgen05.ld -------------------------------------------------------------
 
