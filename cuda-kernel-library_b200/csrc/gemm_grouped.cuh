@@ -89,13 +89,14 @@ struct GroupedConfig {
     static constexpr uint32_t kBoxBytes = 64 * 64 * 2;
     static constexpr uint32_t kBBytes = (kSplit ? 2 : 4) * kBoxBytes;
     static constexpr uint32_t kStageBytes = kABytes + kBBytes;
-    static constexpr int kThreads = 192 + 32 * kStages;  // one loader warp per stage
+    static constexpr int kThreads = 192 + 32 * kStages + 32;  // one loader warp per stage, a scheduler
     static constexpr int kBuffers = 3;  // of 2 KB (32 rows x 64 bytes) per epilogue warp
     static constexpr uint32_t kStagingBytes = kSplit ? 128 * 128 * 4 : 4 * kBuffers * 2048;
-    static constexpr int kNumBarriers = 3 * kStages + 5;
+    static constexpr int kNumBarriers = 3 * kStages + 5 + 8;
     static constexpr uint32_t kTableBytes = 2 * (kMaxGemmGroups + 2) * 4;
+    static constexpr uint32_t kQueueBytes = 4 * 64;
     static constexpr uint32_t kSmemBytes =
-        kStages * kStageBytes + kStagingBytes + kTableBytes + kNumBarriers * 8 + 16 + 1024;
+        kStages * kStageBytes + kStagingBytes + kTableBytes + kQueueBytes + kNumBarriers * 8 + 16 + 1024;
 };
 constexpr int kMaxSplit = 8;
 
@@ -110,6 +111,7 @@ struct GroupedTile {
     int cols;       // columns of the tile that exist
     int k_blocks;   // 64-wide blocks of the main product
     int ext_first, ext_last;  // adapters [first, last) that may have rows in the tile
+    int begin, end;  // this CTA's share of the tile's blocks (main product, then adapters)
 };
 
 struct GroupedTable {
@@ -236,6 +238,73 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, cons
     return o;
 }
 
+// Tiles travel from a scheduler thread to the CTA's roles through a short queue in shared memory:
+// working out a tile takes some 2000 cycles of dependent integer work, which the roles would each
+// spend between two tiles (24576 rows, 64 groups, weight gradient 2048 x 1408: 6 blocks of MMAs a
+// tile).  A slot's full barrier has one arrival, its empty barrier one per role.
+constexpr int kTileSlots = 4;
+template <typename Tile>
+struct TileQueue {
+    static constexpr int kWords = (sizeof(Tile) + 15) / 16 * 4;
+    static constexpr uint32_t kBytes = kTileSlots * kWords * 4;
+    int4* slots;
+    uint32_t bars;  // kTileSlots full barriers, then as many empty ones
+
+    __device__ __forceinline__ uint32_t full(int s) const { return bars + 8u * static_cast<uint32_t>(s); }
+    __device__ __forceinline__ uint32_t empty(int s) const {
+        return bars + 8u * static_cast<uint32_t>(kTileSlots + s);
+    }
+    __device__ __forceinline__ void init(uint32_t roles) const {
+        for (int s = 0; s < kTileSlots; ++s) {
+            ptx::mbar_init(full(s), 1);
+            ptx::mbar_init(empty(s), roles);
+        }
+    }
+    // Scheduler thread: the i-th tile of this CTA.
+    __device__ __forceinline__ bool push(uint32_t i, const Tile& t, const Control& ctl) const {
+        const int s = static_cast<int>(i % kTileSlots);
+        if (!wait_barrier(empty(s), ((i / kTileSlots) & 1u) ^ 1u, ctl, kRoleProducer, 0x60000000u | i)) {
+            return false;
+        }
+        union {
+            Tile tile;
+            int4 words[kWords / 4];
+        } u;
+        u.tile = t;
+#pragma unroll
+        for (int w = 0; w < kWords / 4; ++w) {
+            slots[s * (kWords / 4) + w] = u.words[w];
+        }
+        ptx::mbar_arrive(full(s));
+        return true;
+    }
+    // A role (a thread, or all lanes of a warp with `lane` 0 arriving for it).
+    __device__ __forceinline__ bool pop(uint32_t i, Tile* t, const Control& ctl, bool whole_warp,
+                                        uint32_t lane) const {
+        const int s = static_cast<int>(i % kTileSlots);
+        const bool got = wait_barrier(full(s), (i / kTileSlots) & 1u, ctl, kRoleProducer, 0x61000000u | i);
+        if (whole_warp ? !__all_sync(0xFFFFFFFFu, got) : !got) {
+            return false;
+        }
+        union {
+            Tile tile;
+            int4 words[kWords / 4];
+        } u;
+#pragma unroll
+        for (int w = 0; w < kWords / 4; ++w) {
+            u.words[w] = slots[s * (kWords / 4) + w];
+        }
+        *t = u.tile;
+        if (whole_warp) {
+            __syncwarp();
+        }
+        if (!whole_warp || lane == 0) {
+            ptx::mbar_arrive(empty(s));
+        }
+        return t->group >= 0;
+    }
+};
+
 // Positions [lo, hi) of tile t that belong to adapter g.
 struct Span {
     int lo, hi;
@@ -244,19 +313,16 @@ __device__ __forceinline__ Span adapter_span(const GroupedTable& table, const Gr
     return {max(table.offs[g], t.p0), min(table.offs[g + 1], t.p0 + t.valid)};
 }
 
-// The share of a tile's blocks (main product, then adapters) that CTA `rank` of `size` runs.
-struct BlockRange {
-    int begin, end;
-};
-__device__ __forceinline__ BlockRange block_range(const GroupedParams& p, const GroupedTable& table,
-                                                  const GroupedTile& t, int rank, int size) {
-    int blocks = t.k_blocks;
-    for (int g = t.ext_first; g < t.ext_last; ++g) {
-        const Span s = adapter_span(table, t, g);
+// Fills in the share of a tile's blocks that CTA `rank` of `size` runs.
+__device__ __forceinline__ void take_share(const GroupedParams& p, const GroupedTable& table, GroupedTile* t,
+                                           int rank, int size) {
+    int blocks = t->k_blocks;
+    for (int g = t->ext_first; g < t->ext_last; ++g) {
+        const Span s = adapter_span(table, *t, g);
         blocks += s.lo < s.hi ? 2 * ((p.ext_cols + 63) / 64) : 0;
     }
-    return {static_cast<int>(static_cast<long long>(blocks) * rank / size),
-            static_cast<int>(static_cast<long long>(blocks) * (rank + 1) / size)};
+    t->begin = static_cast<int>(static_cast<long long>(blocks) * rank / size);
+    t->end = static_cast<int>(static_cast<long long>(blocks) * (rank + 1) / size);
 }
 
 }  // namespace detail
@@ -498,8 +564,10 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
     uint8_t* ring_ptr = smem_raw + (ring - raw_addr);
     uint8_t* staging_ptr = ring_ptr + kStages * Cfg::kStageBytes;
     uint8_t* table_ptr = staging_ptr + Cfg::kStagingBytes;
-    uint8_t* bars_ptr = table_ptr + Cfg::kTableBytes;
-    const uint32_t bars = ring + (kStages * Cfg::kStageBytes + Cfg::kStagingBytes + Cfg::kTableBytes);
+    uint8_t* queue_ptr = table_ptr + Cfg::kTableBytes;
+    uint8_t* bars_ptr = queue_ptr + Cfg::kQueueBytes;
+    const uint32_t bars =
+        ring + (kStages * Cfg::kStageBytes + Cfg::kStagingBytes + Cfg::kTableBytes + Cfg::kQueueBytes);
     auto full_bar = [&](int s) { return bars + 8u * static_cast<uint32_t>(s); };
     auto empty_bar = [&](int s) { return bars + 8u * static_cast<uint32_t>(kStages + s); };
     auto acc_full_bar = [&](uint32_t a) { return bars + 8u * (2 * kStages + a); };
@@ -507,9 +575,13 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
     const uint32_t drain_bar = bars + 8u * (2 * kStages + 4);
     // a stage's rows written by the loaders (stages that need none never use it)
     auto loaded_bar = [&](int s) { return bars + 8u * static_cast<uint32_t>(2 * kStages + 5 + s); };
+    using Queue = detail::TileQueue<detail::GroupedTile>;
+    static_assert(Queue::kBytes <= Cfg::kQueueBytes && 2 * detail::kTileSlots == 8, "queue layout");
+    const Queue queue = {reinterpret_cast<int4*>(queue_ptr), bars + 8u * (3 * kStages + 5)};
     const uint32_t tmem_slot = bars + 8u * Cfg::kNumBarriers;
     volatile uint32_t* tmem_slot_ptr =
         reinterpret_cast<volatile uint32_t*>(bars_ptr + 8 * Cfg::kNumBarriers);
+    const bool loads = p.form == kFormWgrad || p.load_a != 0 || p.ext_groups > 0;  // the loaders work
 
     detail::Control ctl;
     ctl.abort_flag = reinterpret_cast<volatile int*>(bars_ptr + 8 * Cfg::kNumBarriers + 4);
@@ -534,6 +606,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
             ptx::mbar_init(acc_empty_bar(a), 4);
         }
         ptx::mbar_init(drain_bar, 1);
+        queue.init(6u + (loads ? kStages : 0u));  // producer, MMA, four epilogue warps, loaders
         *ctl.abort_flag = 0;
         ptx::fence_barrier_init();
     }
@@ -581,9 +654,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     phase ^= 1u;
                 }
             };
-            for (int tile = first_tile; ok && tile < total; tile += tile_step) {
-                const detail::GroupedTile t = detail::grouped_tile(p, table, tile);
-                const detail::BlockRange mine = detail::block_range(p, table, t, rank, size);
+            detail::GroupedTile t;
+            for (uint32_t i = 0; ok && queue.pop(i, &t, ctl, false, lane); ++i) {
                 const int boxes = (t.cols + 63) / 64;
                 const uint32_t b_bytes = static_cast<uint32_t>(boxes) * Cfg::kBoxBytes;
                 // 64 k rows of matrix z of a stack, k0 on, as columns n0 .. of the tile
@@ -601,7 +673,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                 };
                 if (p.form == kFormRows) {
                     const int group = table.whole ? 0 : t.group;
-                    for (int kb = mine.begin; kb < min(mine.end, t.k_blocks); ++kb) {
+                    for (int kb = t.begin; kb < min(t.end, t.k_blocks); ++kb) {
                         if (!acquire_stage(b_bytes + (gather_a ? 0u : Cfg::kABytes))) {
                             ok = false;
                             break;
@@ -621,7 +693,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                         if (span.lo >= span.hi) {
                             continue;
                         }
-                        for (int eb = max(0, mine.begin - at); eb < min(ext_blocks, mine.end - at); ++eb) {
+                        for (int eb = max(0, t.begin - at); eb < min(ext_blocks, t.end - at); ++eb) {
                             if (!acquire_stage(b_bytes)) {
                                 ok = false;
                                 break;
@@ -639,7 +711,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     const uint32_t bytes =
                         (gather_b ? 0u : b_bytes) +
                         (gather_a ? 0u : static_cast<uint32_t>(a_boxes) * Cfg::kBoxBytes);
-                    for (int kb = mine.begin; kb < mine.end; ++kb) {
+                    for (int kb = t.begin; kb < t.end; ++kb) {
                         const int part = kb >= row_blocks ? 1 : 0;
                         const int at = (kb - part * row_blocks) * 64;
                         // A last block that is not whole comes through the loaders in both operands,
@@ -698,8 +770,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
             uint32_t count = 0;
             bool ready = false;  // the next stage's copies are known to have landed
             bool ok = true;
-            for (int tile = first_tile; ok && tile < total; tile += tile_step) {
-                const detail::GroupedTile t = detail::grouped_tile(p, table, tile);
+            detail::GroupedTile t;
+            for (uint32_t i = 0; ok && queue.pop(i, &t, ctl, false, lane); ++i) {
                 const uint32_t acc = count & 1u;
                 if (!detail::wait_barrier(acc_empty_bar(acc), ((count >> 1) & 1u) ^ 1u, ctl, kRoleMma,
                                           0x80000000u | count)) {
@@ -752,9 +824,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     }
                     return true;
                 };
-                const detail::BlockRange mine = detail::block_range(p, table, t, rank, size);
                 const int row_blocks = a_mn ? (t.valid + 63) / 64 : 0;
-                for (int kb = mine.begin; kb < min(mine.end, t.k_blocks); ++kb) {
+                for (int kb = t.begin; kb < min(t.end, t.k_blocks); ++kb) {
                     const bool loaded = gather_a || gather_b ||
                                         (a_mn && (t.valid & 63) != 0 && (kb + 1) % row_blocks == 0);
                     if (!block(4, loaded)) {
@@ -768,7 +839,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     if (span.lo >= span.hi) {
                         continue;
                     }
-                    for (int eb = max(0, mine.begin - at); eb < min(ext_blocks, mine.end - at); ++eb) {
+                    for (int eb = max(0, t.begin - at); eb < min(ext_blocks, t.end - at); ++eb) {
                         const int in_part = eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb;
                         if (!block(min(4, (p.ext_cols - in_part * 64) / 16), true)) {
                             ok = false;
@@ -795,6 +866,23 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
             } else {
                 ptx::umma_commit(drain_bar);
                 detail::drain_wait(drain_bar, 0);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 6 + kStages) {
+        // Scheduler.
+        if (ptx::elect_one_sync()) {
+            uint32_t i = 0;
+            detail::GroupedTile t;
+            bool ok = true;
+            for (int tile = first_tile; ok && tile < total; tile += tile_step, ++i) {
+                t = detail::grouped_tile(p, table, tile);
+                detail::take_share(p, table, &t, rank, size);
+                ok = queue.push(i, t, ctl);
+            }
+            t.group = -1;  // no more
+            if (ok) {
+                queue.push(i, t, ctl);
             }
         }
         __syncwarp();
@@ -825,10 +913,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                 ptx::mbar_arrive(loaded_bar(own));
             }
         };
-        const bool needed = p.form == kFormWgrad || gather_a || p.ext_groups > 0;
-        for (int tile = first_tile; needed && ok && tile < total; tile += tile_step) {
-            const detail::GroupedTile t = detail::grouped_tile(p, table, tile);
-            const detail::BlockRange range = detail::block_range(p, table, t, rank, size);
+        detail::GroupedTile t;
+        for (uint32_t i = 0; loads && ok && queue.pop(i, &t, ctl, true, lane); ++i) {
             if (p.form == kFormRows) {
                 int src[4] = {-1, -1, -1, -1};  // lane l: rows l, 32 + l, 64 + l, 96 + l of A, -1: none
                 if (gather_a) {
@@ -841,7 +927,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                         src[q] = at < p.a_count ? at : -1;
                     }
                 }
-                for (int kb = range.begin; kb < min(range.end, t.k_blocks); ++kb, ++it) {
+                for (int kb = t.begin; kb < min(t.end, t.k_blocks); ++kb, ++it) {
                     if (static_cast<int>(it % kStages) != own) {
                         continue;
                     }
@@ -860,8 +946,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                     if (span.lo >= span.hi) {
                         continue;
                     }
-                    const int eb_end = min(ext_blocks, range.end - first_block);
-                    for (int eb = max(0, range.begin - first_block); eb < eb_end; ++eb, ++it) {
+                    const int eb_end = min(ext_blocks, t.end - first_block);
+                    for (int eb = max(0, t.begin - first_block); eb < eb_end; ++eb, ++it) {
                         if (static_cast<int>(it % kStages) != own) {
                             continue;
                         }
@@ -888,7 +974,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         const int r = i0 + q * 32 + static_cast<int>(lane);
-                        const bool in = kb < range.end && r < t.valid;
+                        const bool in = kb < t.end && r < t.valid;
                         const int at_a = !in ? -1 : p.a_rows != nullptr ? __ldg(p.a_rows + t.p0 + r) : t.p0 + r;
                         const int at_b = !in ? -1 : p.b_rows != nullptr ? __ldg(p.b_rows + t.p0 + r) : t.p0 + r;
                         next_a[q] = at_a < p.a_count ? at_a : -1;
@@ -897,9 +983,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                 };
                 // the first block of this tile whose stage is the own one
                 const int first =
-                    range.begin + (own - static_cast<int>(it % kStages) + kStages) % kStages;
+                    t.begin + (own - static_cast<int>(it % kStages) + kStages) % kStages;
                 fetch(first);
-                for (int kb = first; kb < range.end; kb += kStages) {
+                for (int kb = first; kb < t.end; kb += kStages) {
                     const int part = kb >= row_blocks ? 1 : 0;
                     const bool tail = t.valid - (kb - part * row_blocks) * 64 < 64;
                     const int ra[2] = {next_a[0], next_a[1]}, rb[2] = {next_b[0], next_b[1]};
@@ -920,7 +1006,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                         hand_over();
                     }
                 }
-                it += static_cast<uint32_t>(range.end - range.begin);
+                it += static_cast<uint32_t>(t.end - t.begin);
             }
         }
         ptx::cp_async_wait_all();  // no copy may be in flight when the CTA ends
@@ -939,8 +1025,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
         const uint32_t stg_all = ring + kStages * Cfg::kStageBytes;
         uint32_t buffer = 0;
         bool alive = true;
-        for (int tile = first_tile; alive && tile < total; tile += tile_step) {
-            const detail::GroupedTile t = detail::grouped_tile(p, table, tile);
+        detail::GroupedTile t;
+        for (uint32_t i = 0; alive && queue.pop(i, &t, ctl, true, lane); ++i) {
             const uint32_t acc = count & 1u;
             const uint32_t parity = (count >> 1) & 1u;
             // Row of C that lane `lane` of this warp stands for, -1 for none.
@@ -957,8 +1043,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                 break;
             }
             ptx::tc_fence_after_sync();
-            const detail::BlockRange mine = detail::block_range(p, table, t, rank, size);
-            const bool nothing = mine.begin == mine.end;
+            const bool nothing = t.begin == t.end;
             const uint32_t t_row = tmem_base + ((quad * 32u) << 16) + acc * 256u;
             // Hands the accumulator back to the MMA warp, once, when its last column is in registers.
             bool released = false;

@@ -19,6 +19,8 @@
 // written row by row across the lanes; from there rows leave as in the single-CTA kernel.
 #pragma once
 
+#include <type_traits>
+
 #include "gemm_grouped.cuh"
 
 namespace ckl {
@@ -30,13 +32,15 @@ struct GroupedPairConfig {
     static constexpr uint32_t kRowsBytes = 2 * kBoxBytes;
     static constexpr uint32_t kStageBytes = kColsBytes + kRowsBytes;
     static constexpr int kFirstLoader = 6;
-    static constexpr int kThreads = 32 * (kFirstLoader + kStages);  // one loader warp per stage
+    static constexpr int kScheduler = kFirstLoader + kStages;  // one loader warp per stage
+    static constexpr int kThreads = 32 * (kScheduler + 1);
     static constexpr uint32_t kWarpStaging = 3 * 2048;  // per epilogue warp
     static constexpr uint32_t kStagingBytes = 4 * kWarpStaging;
-    static constexpr int kNumBarriers = 3 * kStages + 5;
+    static constexpr int kNumBarriers = 3 * kStages + 5 + 8;
     static constexpr uint32_t kTableBytes = 2 * (kMaxGemmGroups + 2) * 4;
+    static constexpr uint32_t kQueueBytes = 4 * 64;
     static constexpr uint32_t kSmemBytes =
-        kStages * kStageBytes + kStagingBytes + kTableBytes + kNumBarriers * 8 + 16 + 1024;
+        kStages * kStageBytes + kStagingBytes + kTableBytes + kQueueBytes + kNumBarriers * 8 + 16 + 1024;
 };
 
 namespace detail {
@@ -102,6 +106,21 @@ __device__ __forceinline__ Span adapter_span(const GroupedTable& table, const Pa
     return {max(table.offs[g], t.p0), min(table.offs[g + 1], t.p0 + t.valid)};
 }
 
+// factor * a and factor * b (FP32 bits), rounded and packed with a in the low half.
+template <typename Elem>
+__device__ __forceinline__ uint32_t pack16(float factor, uint32_t a, uint32_t b) {
+    const float x = factor * __uint_as_float(a), y = factor * __uint_as_float(b);
+    uint32_t w;
+    if constexpr (std::is_same<Elem, __half>::value) {
+        const __half2 h = __floats2half2_rn(x, y);
+        w = *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        w = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return w;
+}
+
 }  // namespace detail
 
 template <typename OutT>
@@ -120,14 +139,19 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
     uint8_t* ring_ptr = smem_raw + (ring - raw_addr);
     uint8_t* staging_ptr = ring_ptr + kStages * Cfg::kStageBytes;
     uint8_t* table_ptr = staging_ptr + Cfg::kStagingBytes;
-    uint8_t* bars_ptr = table_ptr + Cfg::kTableBytes;
-    const uint32_t bars = ring + (kStages * Cfg::kStageBytes + Cfg::kStagingBytes + Cfg::kTableBytes);
+    uint8_t* queue_ptr = table_ptr + Cfg::kTableBytes;
+    uint8_t* bars_ptr = queue_ptr + Cfg::kQueueBytes;
+    const uint32_t bars =
+        ring + (kStages * Cfg::kStageBytes + Cfg::kStagingBytes + Cfg::kTableBytes + Cfg::kQueueBytes);
     auto full_bar = [&](int s) { return bars + 8u * static_cast<uint32_t>(s); };
     auto empty_bar = [&](int s) { return bars + 8u * static_cast<uint32_t>(kStages + s); };
     auto loaded_bar = [&](int s) { return bars + 8u * static_cast<uint32_t>(2 * kStages + s); };
     auto acc_full_bar = [&](uint32_t a) { return bars + 8u * (3 * kStages + a); };
     auto acc_empty_bar = [&](uint32_t a) { return bars + 8u * (3 * kStages + 2 + a); };
     const uint32_t drain_bar = bars + 8u * (3 * kStages + 4);
+    using Queue = detail::TileQueue<detail::PairTile>;
+    static_assert(Queue::kBytes <= Cfg::kQueueBytes && 2 * detail::kTileSlots == 8, "queue layout");
+    const Queue queue = {reinterpret_cast<int4*>(queue_ptr), bars + 8u * (3 * kStages + 5)};
     const uint32_t tmem_slot = bars + 8u * Cfg::kNumBarriers;
     volatile uint32_t* tmem_slot_ptr =
         reinterpret_cast<volatile uint32_t*>(bars_ptr + 8 * Cfg::kNumBarriers);
@@ -136,6 +160,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
     const uint32_t lane = ptx::lane_id();
     const uint32_t rank = ptx::cluster_cta_rank();
     const bool leader = rank == 0;
+    const bool wgrad = p.form == kFormWgrad;
+    const bool gather = p.load_a != 0;
+    const bool loads = wgrad || gather || p.ext_groups > 0;  // the loaders work
 
     detail::Control ctl;
     ctl.abort_flag = reinterpret_cast<volatile int*>(bars_ptr + 8 * Cfg::kNumBarriers + 4);
@@ -157,6 +184,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
             ptx::mbar_init(acc_empty_bar(a), 8);  // four warps of either CTA, at the leader
         }
         ptx::mbar_init(drain_bar, 1);
+        // producer, the leader's MMA thread, four epilogue warps, loaders
+        queue.init(5u + (leader ? 1u : 0u) + (loads ? kStages : 0u));
         *ctl.abort_flag = 0;
         ptx::fence_barrier_init();
     }
@@ -177,8 +206,6 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
     const int ext_blocks = 2 * ((p.ext_cols + 63) / 64);
     const int unit = static_cast<int>(blockIdx.x >> 1);
     const int units = static_cast<int>(gridDim.x >> 1);
-    const bool wgrad = p.form == kFormWgrad;
-    const bool gather = p.load_a != 0;
 
     // ---- roles --------------------------------------------------------------------------------
     if (warp == 0) {
@@ -208,8 +235,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                     phase ^= 1u;
                 }
             };
-            for (int tile = unit; ok && tile < total; tile += units) {
-                const detail::PairTile t = detail::pair_tile(p, table, tile);
+            detail::PairTile t;
+            for (uint32_t i = 0; ok && queue.pop(i, &t, ctl, false, lane); ++i) {
                 const int col0 = t.c0 + static_cast<int>(rank) * 128;
                 // 64-column boxes that exist, of this CTA and of both
                 const int boxes = min(2, max(0, (p.n - col0 + 63) / 64));
@@ -333,8 +360,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
             uint32_t count = 0;
             bool ready = false;
             bool ok = true;
-            for (int tile = unit; ok && tile < total; tile += units) {
-                const detail::PairTile t = detail::pair_tile(p, table, tile);
+            detail::PairTile t;
+            for (uint32_t i = 0; ok && queue.pop(i, &t, ctl, false, lane); ++i) {
                 const uint32_t acc = count & 1u;
                 if (!detail::wait_barrier(acc_empty_bar(acc), ((count >> 1) & 1u) ^ 1u, ctl, kRoleMma,
                                           0x80000000u | count)) {
@@ -423,6 +450,21 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
             }
         }
         __syncwarp();
+    } else if (warp == Cfg::kScheduler) {
+        if (ptx::elect_one_sync()) {
+            uint32_t i = 0;
+            detail::PairTile t;
+            bool ok = true;
+            for (int tile = unit; ok && tile < total; tile += units, ++i) {
+                t = detail::pair_tile(p, table, tile);
+                ok = queue.push(i, t, ctl);
+            }
+            t.group = -1;  // no more
+            if (ok) {
+                queue.push(i, t, ctl);
+            }
+        }
+        __syncwarp();
     } else if (warp >= Cfg::kFirstLoader) {
         // Loaders, one warp per stage as in the single-CTA kernel; a stage is handed to the leader.
         const detail::Loader load(ring + static_cast<uint32_t>(warp - Cfg::kFirstLoader) * Cfg::kStageBytes, lane);
@@ -445,8 +487,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                 ptx::mbar_arrive_cluster(ptx::map_to_cta(loaded_bar(own), 0));
             }
         };
-        for (int tile = unit; (wgrad || gather || p.ext_groups > 0) && ok && tile < total; tile += units) {
-            const detail::PairTile t = detail::pair_tile(p, table, tile);
+        detail::PairTile t;
+        for (uint32_t i = 0; loads && ok && queue.pop(i, &t, ctl, true, lane); ++i) {
             const int first_row = static_cast<int>(rank) * t.half;  // of this CTA, in the tile
             if (!wgrad) {
                 const int rows = max(0, min(t.half, t.valid - first_row));  // of this CTA that exist
@@ -550,8 +592,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
         uint32_t buffer = 0;
         uint32_t count = 0;
         bool alive = true;
-        for (int tile = unit; alive && tile < total; tile += units) {
-            const detail::PairTile t = detail::pair_tile(p, table, tile);
+        detail::PairTile t;
+        for (uint32_t i = 0; alive && queue.pop(i, &t, ctl, true, lane); ++i) {
             const uint32_t acc = count & 1u;
             const bool got =
                 detail::wait_barrier(acc_full_bar(acc), (count >> 1) & 1u, ctl, kRoleEpilogue, count);
@@ -568,13 +610,23 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                 static_cast<Elem*>(p.c) + (wgrad ? static_cast<long long>(t.group) * p.c_stride : 0ll);
             const float factor = p.alpha * (p.scales != nullptr ? __ldg(p.scales + t.group) : 1.0f);
             const int z = wgrad ? t.group : 0;
+            // Whole runs of 32 consecutive rows leave by TMA, which clips at the edge of C; in a weight
+            // gradient it clips rows as well.
+            auto leaves_by_tma = [&](int j0) { return p.c_tma != 0 && (wgrad || j0 + 32 <= rows); };
+            // 16-bit runs are read as matrix fragments (two halves of 16 columns of C), everything
+            // else one column per lane.
             uint32_t r[32];
+            uint32_t(&half0)[16] = *reinterpret_cast<uint32_t(*)[16]>(&r[0]);
+            uint32_t(&half1)[16] = *reinterpret_cast<uint32_t(*)[16]>(&r[16]);
             auto fetch = [&](int j0) {
                 if (nothing) {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         r[i] = 0;
                     }
+                } else if (sizeof(Elem) == 2 && leaves_by_tma(j0)) {
+                    ptx::tmem_ld_16x256b_x4(t_row + static_cast<uint32_t>(j0), half0);
+                    ptx::tmem_ld_16x256b_x4(t_row + (16u << 16) + static_cast<uint32_t>(j0), half1);
                 } else {
                     ptx::tmem_ld_32x32(t_row + static_cast<uint32_t>(j0), r);
                 }
@@ -598,9 +650,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                 if (j0 + 32 >= rows) {
                     release();
                 }
-                // Whole runs of 32 consecutive rows leave by TMA, which clips at the edge of C; in a
-                // weight gradient it clips rows as well.
-                const bool by_tma = p.c_tma != 0 && (wgrad || j0 + 32 <= rows);
+                const bool by_tma = leaves_by_tma(j0);
                 if (lane == 0) {
                     // the stores that last used the buffer have read it
                     if (by_tma) {
@@ -613,13 +663,19 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                 if (by_tma) {
                     uint8_t* buf = stg + buffer * 2048u;
                     if constexpr (kRowBytes == 64) {
-                        // 64-byte swizzle: the 16-byte unit is exchanged by row bits 1 and 2
+                        // Eight rows at a time: four 8 x 8 fragments (32 columns) are stored transposed,
+                        // 16 bytes = 8 columns of a row each (2-byte stores lane by lane took the
+                        // 256 x 256 tile's epilogue above its 6 blocks of MMAs).  64-byte swizzle: the
+                        // 16-byte unit is exchanged by row bits 1 and 2.
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            T::store(reinterpret_cast<Elem*>(buf + j * 64 +
-                                                             (((lane >> 3) ^ ((j >> 1) & 3u)) << 4) +
-                                                             (lane & 7u) * 2u),
-                                     factor * __uint_as_float(r[j]));
+                        for (int c = 0; c < 4; ++c) {
+                            const uint32_t row = static_cast<uint32_t>(c) * 8u + (lane & 7u);
+                            const uint32_t at =
+                                stg_addr + buffer * 2048u + row * 64u + (((lane >> 3) ^ ((row >> 1) & 3u)) << 4);
+                            ptx::stmatrix_x4_trans(at, detail::pack16<Elem>(factor, half0[4 * c], half0[4 * c + 1]),
+                                                   detail::pack16<Elem>(factor, half0[4 * c + 2], half0[4 * c + 3]),
+                                                   detail::pack16<Elem>(factor, half1[4 * c], half1[4 * c + 1]),
+                                                   detail::pack16<Elem>(factor, half1[4 * c + 2], half1[4 * c + 3]));
                         }
                     } else {
 #pragma unroll
