@@ -26,7 +26,8 @@
 namespace ckl {
 
 struct GroupedPairConfig {
-    static constexpr int kStages = 6;
+    // Five stages of 32 KB: a sixth brought nothing, its room holds the staging buffers.
+    static constexpr int kStages = 5;
     static constexpr uint32_t kBoxBytes = 64 * 64 * 2;
     static constexpr uint32_t kColsBytes = 2 * kBoxBytes;
     static constexpr uint32_t kRowsBytes = 2 * kBoxBytes;
@@ -34,7 +35,9 @@ struct GroupedPairConfig {
     static constexpr int kFirstLoader = 6;
     static constexpr int kScheduler = kFirstLoader + kStages;  // one loader warp per stage
     static constexpr int kThreads = 32 * (kScheduler + 1);
-    static constexpr uint32_t kWarpStaging = 3 * 2048;  // per epilogue warp
+    static constexpr uint32_t kBufferBytes = 4096;
+    static constexpr int kBuffers = 3;  // per epilogue warp
+    static constexpr uint32_t kWarpStaging = kBuffers * kBufferBytes;
     static constexpr uint32_t kStagingBytes = 4 * kWarpStaging;
     static constexpr int kNumBarriers = 3 * kStages + 5 + 8;
     static constexpr uint32_t kTableBytes = 2 * (kMaxGemmGroups + 2) * 4;
@@ -581,10 +584,6 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
         constexpr int kVec = T::kVec;
         constexpr int kLanesPerRow = 32 / kVec;
         constexpr int kRowsPerPass = 32 / kLanesPerRow;
-        // one buffer of 32 rows x 32 columns: 64-byte rows for 16-bit types (three buffers), 128-byte
-        // rows for FP32 (one; the third 2 KB stay unused)
-        constexpr uint32_t kRowBytes = 32 * sizeof(Elem);
-        constexpr uint32_t kBuffers = kRowBytes == 64 ? 3 : 1;
         const uint32_t quad = static_cast<uint32_t>(warp) & 3u;
         uint8_t* stg = staging_ptr + quad * Cfg::kWarpStaging;
         const uint32_t stg_addr = ring + kStages * Cfg::kStageBytes + quad * Cfg::kWarpStaging;
@@ -610,30 +609,6 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                 static_cast<Elem*>(p.c) + (wgrad ? static_cast<long long>(t.group) * p.c_stride : 0ll);
             const float factor = p.alpha * (p.scales != nullptr ? __ldg(p.scales + t.group) : 1.0f);
             const int z = wgrad ? t.group : 0;
-            // Whole runs of 32 consecutive rows leave by TMA, which clips at the edge of C; in a weight
-            // gradient it clips rows as well.
-            auto leaves_by_tma = [&](int j0) { return p.c_tma != 0 && (wgrad || j0 + 32 <= rows); };
-            // 16-bit runs are read as matrix fragments (two halves of 16 columns of C), everything
-            // else one column per lane.
-            uint32_t r[32];
-            uint32_t(&half0)[16] = *reinterpret_cast<uint32_t(*)[16]>(&r[0]);
-            uint32_t(&half1)[16] = *reinterpret_cast<uint32_t(*)[16]>(&r[16]);
-            auto fetch = [&](int j0) {
-                if (nothing) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        r[i] = 0;
-                    }
-                } else if (sizeof(Elem) == 2 && leaves_by_tma(j0)) {
-                    ptx::tmem_ld_16x256b_x4(t_row + static_cast<uint32_t>(j0), half0);
-                    ptx::tmem_ld_16x256b_x4(t_row + (16u << 16) + static_cast<uint32_t>(j0), half1);
-                } else {
-                    ptx::tmem_ld_32x32(t_row + static_cast<uint32_t>(j0), r);
-                }
-            };
-            if (rows > 0) {
-                fetch(0);
-            }
             bool released = false;
             auto release = [&]() {  // once, when the last accumulator column is in registers
                 if (!released) {
@@ -645,63 +620,109 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                     }
                 }
             };
-            for (int j0 = 0; j0 < rows; j0 += 32) {
-                ptx::tmem_ld_wait();
-                if (j0 + 32 >= rows) {
-                    release();
-                }
-                const bool by_tma = leaves_by_tma(j0);
-                if (lane == 0) {
-                    // the stores that last used the buffer have read it
-                    if (by_tma) {
-                        ptx::bulk_wait_group_read<kBuffers - 1>();
-                    } else {
-                        ptx::bulk_wait_group_read<0>();
-                    }
-                }
-                __syncwarp();
-                if (by_tma) {
-                    uint8_t* buf = stg + buffer * 2048u;
-                    if constexpr (kRowBytes == 64) {
-                        // Eight rows at a time: four 8 x 8 fragments (32 columns) are stored transposed,
-                        // 16 bytes = 8 columns of a row each (2-byte stores lane by lane took the
-                        // 256 x 256 tile's epilogue above its 6 blocks of MMAs).  64-byte swizzle: the
-                        // 16-byte unit is exchanged by row bits 1 and 2.
+            // Whole runs of 32 consecutive rows leave by TMA, which clips at the edge of C; in a weight
+            // gradient it clips rows as well.
+            const int by_tma = p.c_tma == 0 ? 0 : wgrad ? (rows + 31) / 32 * 32 : rows / 32 * 32;
+            int j0 = 0;
+            if constexpr (sizeof(Elem) == 2) {
+                // 64 rows at a time: the accumulator is read as matrix fragments (16 columns of C by
+                // 32 rows), whose 8 x 8 blocks are stored transposed, 16 bytes = 8 columns of a row
+                // each.  (Lane = column and 2-byte stores, 32 rows at a time, took the epilogue of a
+                // 256 x 256 tile to 8000 cycles, twice its 6 blocks of MMAs in a weight gradient.)
+                uint32_t f[64];
+                auto fetch = [&](int j) {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const uint32_t row = static_cast<uint32_t>(c) * 8u + (lane & 7u);
-                            const uint32_t at =
-                                stg_addr + buffer * 2048u + row * 64u + (((lane >> 3) ^ ((row >> 1) & 3u)) << 4);
-                            ptx::stmatrix_x4_trans(at, detail::pack16<Elem>(factor, half0[4 * c], half0[4 * c + 1]),
-                                                   detail::pack16<Elem>(factor, half0[4 * c + 2], half0[4 * c + 3]),
-                                                   detail::pack16<Elem>(factor, half1[4 * c], half1[4 * c + 1]),
-                                                   detail::pack16<Elem>(factor, half1[4 * c + 2], half1[4 * c + 3]));
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            *reinterpret_cast<float*>(buf + j * 128 + (((lane >> 2) ^ (j & 7u)) << 4) +
-                                                      (lane & 3u) * 4u) = factor * __uint_as_float(r[j]);
+                    for (int h = 0; h < 4; ++h) {
+                        if (j + (h >> 1) * 32 < by_tma) {
+                            ptx::tmem_ld_16x256b_x4(
+                                t_row + (static_cast<uint32_t>(h & 1) << 20) + static_cast<uint32_t>(j + (h >> 1) * 32),
+                                *reinterpret_cast<uint32_t(*)[16]>(&f[h * 16]));
                         }
                     }
-                } else {
+                };
+                if (nothing) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        *reinterpret_cast<uint32_t*>(stg + j * 128 + (((lane >> 2) ^ (j & 7u)) << 4) +
-                                                     (lane & 3u) * 4u) = r[j];
+                    for (int i = 0; i < 64; ++i) {
+                        f[i] = 0;
                     }
+                } else if (by_tma > 0) {
+                    fetch(0);
                 }
-                if (j0 + 32 < rows) {
-                    fetch(j0 + 32);
-                }
-                if (by_tma) {
+                for (; j0 < by_tma; j0 += 64) {
+                    ptx::tmem_ld_wait();
+                    uint32_t w[32];  // [32-row run][8-row block][16-byte unit]
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int at = ((i >> 4) * 2 + ((i >> 1) & 1)) * 16 + ((i >> 2) & 3) * 4 + (i & 1) * 2;
+                        w[i] = detail::pack16<Elem>(factor, f[at], f[at + 1]);
+                    }
+                    if (j0 + 64 >= rows) {
+                        release();
+                    } else if (!nothing && j0 + 64 < by_tma) {
+                        fetch(j0 + 64);
+                    }
+                    if (lane == 0) {
+                        // the stores that last used the buffer have read it
+                        ptx::bulk_wait_group_read<Cfg::kBuffers - 1>();
+                    }
+                    __syncwarp();
+                    const uint32_t buf = stg_addr + buffer * Cfg::kBufferBytes;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        // 64-byte swizzle: the 16-byte unit is exchanged by row bits 1 and 2
+                        const uint32_t row = static_cast<uint32_t>(i & 3) * 8u + (lane & 7u);
+                        ptx::stmatrix_x4_trans(
+                            buf + (i >> 2) * 2048u + row * 64u + (((lane >> 3) ^ ((row >> 1) & 3u)) << 4), w[4 * i],
+                            w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                    }
                     ptx::fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        ptx::tma_store_3d(&tmap_c, stg_addr + buffer * 2048u, col0, t.r0 + j0, z);
+                        ptx::tma_store_3d(&tmap_c, buf, col0, t.r0 + j0, z);
+                        if (j0 + 32 < by_tma) {
+                            ptx::tma_store_3d(&tmap_c, buf + 2048u, col0, t.r0 + j0 + 32, z);
+                        }
                         ptx::bulk_commit_group();
                     }
-                    buffer = buffer + 1 == kBuffers ? 0u : buffer + 1;
+                    buffer = buffer + 1 == Cfg::kBuffers ? 0u : buffer + 1;
+                }
+                j0 = by_tma;
+            }
+            // FP32 runs, and rows that are scattered, read before they are written or do not fill a
+            // run: one column per lane.
+            for (; j0 < rows; j0 += 32) {
+                uint32_t r[32];
+                if (nothing) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        r[i] = 0;
+                    }
+                } else {
+                    ptx::tmem_ld_32x32(t_row + static_cast<uint32_t>(j0), r);
+                    ptx::tmem_ld_wait();
+                }
+                if (j0 + 32 >= rows) {
+                    release();
+                }
+                const bool run = j0 < by_tma;
+                if (lane == 0) {
+                    ptx::bulk_wait_group_read<Cfg::kBuffers - 1>();
+                }
+                __syncwarp();
+                uint8_t* buf = stg + buffer * Cfg::kBufferBytes;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    // 128-byte swizzle: the 16-byte unit is exchanged by row bits 0 to 2
+                    *reinterpret_cast<float*>(buf + j * 128 + (((lane >> 2) ^ (j & 7u)) << 4) + (lane & 3u) * 4u) =
+                        __uint_as_float(r[j]) * (run ? factor : 1.0f);
+                }
+                if (run) {
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        ptx::tma_store_3d(&tmap_c, stg_addr + buffer * Cfg::kBufferBytes, col0, t.r0 + j0, z);
+                        ptx::bulk_commit_group();
+                    }
                 } else {
                     __syncwarp();
                     const int col = col0 + sub * kVec;
@@ -719,7 +740,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
 #pragma unroll
                         for (int u = 0; u < kVec / 4; ++u) {
                             const float4 x = *reinterpret_cast<const float4*>(
-                                stg + j * 128 + (((sub * (kVec / 4) + u) ^ (j & 7)) << 4));
+                                buf + j * 128 + (((sub * (kVec / 4) + u) ^ (j & 7)) << 4));
                             v[4 * u] = x.x;
                             v[4 * u + 1] = x.y;
                             v[4 * u + 2] = x.z;
@@ -730,7 +751,11 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                         }
                     }
                     __syncwarp();
+                    if (lane == 0) {
+                        ptx::bulk_commit_group();  // keeps one group per buffer
+                    }
                 }
+                buffer = buffer + 1 == Cfg::kBuffers ? 0u : buffer + 1;
             }
             release();
             ++count;
