@@ -91,19 +91,8 @@ template <auto kKernel>
 int launch_kernel(int device, int threads, size_t smem, int cluster, const Maps& maps, const GroupedParams& p,
                   int grid, cudaStream_t stream) {
     GRP_TRY(allow_smem<kKernel>(device, smem));
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(grid));
-    cfg.blockDim = dim3(static_cast<unsigned>(threads));
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = static_cast<unsigned>(cluster);
-    attr.val.clusterDim.y = 1;
-    attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = cluster > 1 ? 1 : 0;
-    GRP_TRY_CUDA(cudaLaunchKernelEx(&cfg, kKernel, maps.a_box, maps.b_box, maps.e_box, maps.c, p));
+    GRP_TRY_CUDA(launch_dependent(kKernel, dim3(static_cast<unsigned>(grid)), threads, smem, cluster, stream,
+                                  maps.a_box, maps.b_box, maps.e_box, maps.c, p));
     return CKL_OK;
 }
 

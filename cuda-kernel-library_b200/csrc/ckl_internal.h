@@ -30,6 +30,28 @@ int encode_operand(CUtensorMap* map, int dtype, const void* base, uint64_t inner
                    uint64_t pitch, uint64_t depth, uint64_t stack, uint32_t box_inner,
                    uint32_t box_outer);
 
+// Launches a kernel as a programmatic dependent: it may be set up while the kernel before it on
+// the stream finishes, and waits for that one itself before it touches memory.
+template <typename... Params, typename... Args>
+inline cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, size_t smem,
+                                    int cluster, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attrs[1].val.clusterDim.y = 1;
+    attrs[1].val.clusterDim.z = 1;
+    cfg.attrs = attrs;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // The wait fault armed by ckl_test_arm_wait_fault for the calling thread (kind 0: none); disarms it.
 int take_wait_fault(unsigned long long* limit_ns);
 

@@ -56,8 +56,8 @@ int launch_route(const RouteParams& p, cudaStream_t stream) {
         }
     }
     const unsigned grid = static_cast<unsigned>((p.tokens + kRouteWarps - 1) / kRouteWarps);
-    moe_route_kernel<T, NV, kWide><<<grid, 32 * kRouteWarps, smem, stream>>>(p);
-    MOE_TRY_CUDA(cudaGetLastError());
+    MOE_TRY_CUDA(launch_dependent(moe_route_kernel<T, NV, kWide>, dim3(grid), 32 * kRouteWarps,
+                                  static_cast<size_t>(smem), 1, stream, p));
     return CKL_OK;
 }
 
@@ -76,6 +76,24 @@ template <typename T>
 int launch_route_type(const RouteParams& p, cudaStream_t stream) {
     return p.bias != nullptr || p.groups > 1 ? launch_route_size<T, true>(p, stream)
                                              : launch_route_size<T, false>(p, stream);
+}
+
+template <typename T, int NV>
+int launch_route_backward(const RouteBackwardParams& p, cudaStream_t stream) {
+    const unsigned grid = static_cast<unsigned>((p.tokens + kRouteWarps - 1) / kRouteWarps);
+    MOE_TRY_CUDA(launch_dependent(moe_route_backward_kernel<T, NV>, dim3(grid), 32 * kRouteWarps, 0, 1, stream, p));
+    return CKL_OK;
+}
+
+template <typename T>
+int launch_route_backward_size(const RouteBackwardParams& p, cudaStream_t stream) {
+    const int nv = (p.n_experts + 31) / 32;
+    if (nv <= 1) return launch_route_backward<T, 1>(p, stream);
+    if (nv <= 2) return launch_route_backward<T, 2>(p, stream);
+    if (nv <= 4) return launch_route_backward<T, 4>(p, stream);
+    if (nv <= 8) return launch_route_backward<T, 8>(p, stream);
+    if (nv <= 16) return launch_route_backward<T, 16>(p, stream);
+    return launch_route_backward<T, 32>(p, stream);
 }
 
 int check_route(const char* what, int dtype, const void* logits, int ldl, int tokens, int n_experts,
@@ -107,12 +125,8 @@ int launch_combine(const CombineParams& p, bool vec, cudaStream_t stream) {
     if (grid > 0x7fffffffll) {
         return set_error(CKL_ERR_TOO_LARGE, "moe_combine: %d tokens of %d columns", p.tokens, p.n);
     }
-    if (vec) {
-        moe_combine_kernel<T, OutT, true><<<static_cast<unsigned>(grid), kCombineThreads, 0, stream>>>(p);
-    } else {
-        moe_combine_kernel<T, OutT, false><<<static_cast<unsigned>(grid), kCombineThreads, 0, stream>>>(p);
-    }
-    MOE_TRY_CUDA(cudaGetLastError());
+    MOE_TRY_CUDA(launch_dependent(vec ? moe_combine_kernel<T, OutT, true> : moe_combine_kernel<T, OutT, false>,
+                                  dim3(static_cast<unsigned>(grid)), kCombineThreads, 0, 1, stream, p));
     return CKL_OK;
 }
 
@@ -127,13 +141,14 @@ int launch_combine_out(int out_dtype, const CombineParams& p, bool vec, cudaStre
 
 template <typename T, typename OutT>
 int launch_combine_backward(const CombineBackwardParams& p, bool vec, cudaStream_t stream) {
-    const unsigned grid = static_cast<unsigned>(p.tokens);
-    if (vec) {
-        moe_combine_backward_kernel<T, OutT, true><<<grid, kCombineThreads, 0, stream>>>(p);
-    } else {
-        moe_combine_backward_kernel<T, OutT, false><<<grid, kCombineThreads, 0, stream>>>(p);
+    const long long slots = static_cast<long long>(p.tokens) * p.top_k;
+    const long long grid = (slots + kCombineThreads / 32 - 1) / (kCombineThreads / 32);
+    if (grid > 0x7fffffffll) {
+        return set_error(CKL_ERR_TOO_LARGE, "moe_combine_backward: %d tokens, top_k %d", p.tokens, p.top_k);
     }
-    MOE_TRY_CUDA(cudaGetLastError());
+    MOE_TRY_CUDA(launch_dependent(
+        vec ? moe_combine_backward_kernel<T, OutT, true> : moe_combine_backward_kernel<T, OutT, false>,
+        dim3(static_cast<unsigned>(grid)), kCombineThreads, 0, 1, stream, p));
     return CKL_OK;
 }
 
@@ -254,17 +269,11 @@ int ckl_moe_route_backward(int logit_dtype, const void* logits, int ldl, const i
     p.renormalise = renormalise != 0 ? 1 : 0;
     p.scale = scale;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const unsigned grid = static_cast<unsigned>((tokens + kRouteWarps - 1) / kRouteWarps);
-    const int smem = kRouteWarps * n_experts * 4;  // at most 16 KB
     switch (logit_dtype) {
-        case CKL_F16: moe_route_backward_kernel<__half><<<grid, 32 * kRouteWarps, smem, s>>>(p); break;
-        case CKL_BF16:
-            moe_route_backward_kernel<__nv_bfloat16><<<grid, 32 * kRouteWarps, smem, s>>>(p);
-            break;
-        default: moe_route_backward_kernel<float><<<grid, 32 * kRouteWarps, smem, s>>>(p); break;
+        case CKL_F16: return launch_route_backward_size<__half>(p, s);
+        case CKL_BF16: return launch_route_backward_size<__nv_bfloat16>(p, s);
+        default: return launch_route_backward_size<float>(p, s);
     }
-    MOE_TRY_CUDA(cudaGetLastError());
-    return CKL_OK;
 }
 
 int ckl_group_rows(const int* ids, int slots, int groups, int slots_per_row, int* offsets, int* rows,
@@ -307,19 +316,8 @@ int ckl_group_rows(const int* ids, int slots, int groups, int slots_per_row, int
     if (const int rc = allow_smem(group_rows_kernel, most); rc != CKL_OK) {
         return rc;
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(cluster));
-    cfg.blockDim = dim3(kOrderThreads);
-    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
-    cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = static_cast<unsigned>(cluster);
-    attr.val.clusterDim.y = 1;
-    attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    MOE_TRY_CUDA(cudaLaunchKernelEx(&cfg, group_rows_kernel, p));
+    MOE_TRY_CUDA(launch_dependent(group_rows_kernel, dim3(static_cast<unsigned>(cluster)), kOrderThreads,
+                                  static_cast<size_t>(smem), cluster, static_cast<cudaStream_t>(stream), p));
     return CKL_OK;
 }
 

@@ -614,6 +614,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
         ptx::tmem_alloc(tmem_slot, 512);
         ptx::tmem_relinquish();
     }
+    // Up to here only this CTA's own memory: the kernel before this one may still be running.
+    ptx::grid_dependency_wait();
+    ptx::launch_dependents();
     int* offs = reinterpret_cast<int*>(table_ptr);
     const detail::GroupedTable table = detail::make_table(p, offs, offs + kMaxGemmGroups + 2, 128, p.bn, warp,
                                                           lane, Cfg::kThreads);

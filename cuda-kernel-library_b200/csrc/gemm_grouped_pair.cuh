@@ -196,6 +196,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
         ptx::tmem_alloc_pair(tmem_slot, 512);
         ptx::tmem_relinquish_pair();
     }
+    // Up to here only this CTA's own memory: the kernel before this one may still be running.
+    ptx::grid_dependency_wait();
+    ptx::launch_dependents();
     int* offs = reinterpret_cast<int*>(table_ptr);
     const detail::GroupedTable table =
         detail::make_table(p, offs, offs + kMaxGemmGroups + 2, 256, 256, warp, lane, Cfg::kThreads);

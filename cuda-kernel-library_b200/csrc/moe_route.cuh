@@ -42,6 +42,9 @@ __device__ __forceinline__ uint32_t order_key(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
+__device__ __forceinline__ float key_value(uint32_t key) {  // back to the number
+    return __uint_as_float((key & 0x80000000u) ? key & 0x7FFFFFFFu : ~key);
+}
 __device__ __forceinline__ unsigned long long order_key(double x) {
     const unsigned long long u = static_cast<unsigned long long>(__double_as_longlong(x + 0.0));
     return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
@@ -98,157 +101,79 @@ __device__ __forceinline__ float chosen_share(float logit, bool some, bool sigmo
 
 }  // namespace detail
 
-// One warp per token.  Lane l holds the logits of experts l, l + 32, ...; each of the top_k
-// picks is one redux over the lanes' best keys and one over the tied lanes' indices, so ties
-// go to the lowest index.
-//
-// Which experts are chosen is a whole-number answer, so the keys must not be rounded into
-// false ties: without a bias and groups the logits themselves are compared (the scores are
-// monotone in them); with them (kWide) score + bias is formed in 64 bits.
-template <typename T, int NV, bool kWide>
-__global__ void __launch_bounds__(32 * kRouteWarps) moe_route_kernel(const RouteParams p) {
-    using Traits = detail::OutTraits<T>;
-    using Key = typename std::conditional<kWide, unsigned long long, uint32_t>::type;
-    extern __shared__ __align__(16) uint8_t route_smem[];
-    const int warp = static_cast<int>(threadIdx.x >> 5);
-    const int lane = static_cast<int>(threadIdx.x & 31);
-    const int token = static_cast<int>(blockIdx.x) * kRouteWarps + warp;
-    if (token >= p.tokens) {
-        return;
-    }
-    const int e_count = p.n_experts;
-    float* row = reinterpret_cast<float*>(route_smem) + warp * (NV * 32);
-    const T* src = static_cast<const T*>(p.logits) + static_cast<size_t>(token) * p.ldl;
+namespace detail {
 
+// The experts a warp has to choose from: lane l holds experts l, l + 32, ...
+template <int NV>
+struct RouteRow {
     float logit[NV];
-    float top = detail::kNegInf;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int e = i * 32 + lane;
-        logit[i] = e < e_count ? detail::clean_logit(Traits::load(src + e)) : detail::kNegInf;
-        top = fmaxf(top, logit[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        row[i * 32 + lane] = logit[i];
-    }
-    const bool need_sum = !p.sigmoid && (kWide || !p.renormalise);
-    float inv_sum = 0.0f;
-    if (!p.sigmoid) {
-        top = detail::warp_maxf(top);
-        if (!kWide && need_sum) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                sum += logit[i] == detail::kNegInf ? 0.0f : expf(logit[i] - top);
-            }
-            sum = detail::warp_sum(sum);
-            inv_sum = sum > 0.0f ? 1.0f / sum : 0.0f;
-        }
-    }
+    float top;      // softmax: the row's maximum
+    float inv_sum;  // softmax: 1 / sum of exp(l - top), 0 for an empty row
+};
 
-    Key key[NV];
-    if constexpr (kWide) {
-        double score[NV];
-        double sum = 0.0;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            if (logit[i] == detail::kNegInf) {
-                score[i] = 0.0;
-            } else if (p.sigmoid) {
-                score[i] = 1.0 / (1.0 + exp(-static_cast<double>(logit[i])));
-            } else {
-                score[i] = exp(static_cast<double>(logit[i]) - static_cast<double>(top));
-            }
-            sum += score[i];
-        }
-        if (!p.sigmoid) {
-            sum = detail::warp_sum(sum);
-            inv_sum = sum > 0.0 ? static_cast<float>(1.0 / sum) : 0.0f;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                score[i] = sum > 0.0 ? score[i] / sum : 0.0;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int e = i * 32 + lane;
-            if (p.bias != nullptr && e < e_count) {
-                score[i] += static_cast<double>(__ldg(p.bias + e));
-            }
-            // (a bias of -inf or NaN takes its expert out of the choice)
-            key[i] = logit[i] == detail::kNegInf || !(score[i] > -__builtin_huge_val())
-                         ? 0ull
-                         : detail::order_key(score[i]);
-        }
-        if (p.groups > 1) {
-            // A group's score is the sum of its two best keys.  The keys pass through shared
-            // memory so that a few neighbouring lanes can scan one group.
-            double* keys = reinterpret_cast<double*>(route_smem + kRouteWarps * NV * 32 * 4) +
-                           warp * (NV * 32 + kMaxRouteGroups);
-            const int size = e_count / p.groups;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int e = i * 32 + lane;
-                if (e < e_count) {
-                    keys[e + e / size] = key[i] == 0ull ? -__builtin_huge_val() : score[i];
-                }
-            }
-            __syncwarp();
-            int per = 1;  // lanes per group, a power of two
-            while (per * 2 * p.groups <= 32) {
-                per *= 2;
-            }
-            const int g = lane / per;
-            double first = -__builtin_huge_val(), second = first;
-            if (g < p.groups) {
-                for (int i = lane % per; i < size; i += per) {
-                    const double v = keys[g * (size + 1) + i];
-                    second = v > first ? first : (v > second ? v : second);
-                    first = v > first ? v : first;
-                }
-            }
-            for (int d = 1; d < per; d <<= 1) {
-                const double f = __shfl_xor_sync(0xFFFFFFFFu, first, d);
-                const double s = __shfl_xor_sync(0xFFFFFFFFu, second, d);
-                const double lose = f > first ? first : f;
-                const double run = f > first ? s : second;
-                first = f > first ? f : first;
-                second = lose > run ? lose : run;
-            }
-            unsigned long long mine = 0ull;
-            if (g < p.groups && lane % per == 0 && first != -__builtin_huge_val()) {
-                mine = detail::order_key(first + (second == -__builtin_huge_val() ? 0.0 : second));
-            }
-            uint32_t kept = 0;
-            for (int r = 0; r < p.top_groups; ++r) {
-                const unsigned long long best = detail::warp_max(mine);
-                if (best == 0ull) {
-                    break;
-                }
-                const int winner = __ffs(__ballot_sync(0xFFFFFFFFu, mine == best)) - 1;
-                kept |= 1u << (winner / per);
-                if (lane == winner) {
-                    mine = 0ull;
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int e = i * 32 + lane;
-                if (e < e_count && !((kept >> (e / size)) & 1u)) {
-                    key[i] = 0;
-                }
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            key[i] = logit[i] == detail::kNegInf ? 0u : detail::order_key(logit[i]);
+// Which groups take part: bit g.  A group's score is the sum of its two best keys; `keys` is
+// shared memory (index e + e / size), read by a few neighbouring lanes per group.  `margin` gets
+// the distance of the last group kept to the best one left out (infinite if none competes).
+template <typename F>
+__device__ __forceinline__ uint32_t choose_groups(const RouteParams& p, const F* keys, int lane, F* margin) {
+    const F none = static_cast<F>(kNegInf);
+    const int size = p.n_experts / p.groups;
+    int per = 1;  // lanes per group, a power of two
+    while (per * 2 * p.groups <= 32) {
+        per *= 2;
+    }
+    const int g = lane / per;
+    F first = none, second = none;
+    if (g < p.groups) {
+        for (int i = lane % per; i < size; i += per) {
+            const F v = keys[g * (size + 1) + i];
+            second = v > first ? first : (v > second ? v : second);
+            first = v > first ? v : first;
         }
     }
+    for (int d = 1; d < per; d <<= 1) {
+        const F f = __shfl_xor_sync(0xFFFFFFFFu, first, d);
+        const F s = __shfl_xor_sync(0xFFFFFFFFu, second, d);
+        const F lose = f > first ? first : f;
+        const F run = f > first ? s : second;
+        first = f > first ? f : first;
+        second = lose > run ? lose : run;
+    }
+    const bool mine_counts = g < p.groups && lane % per == 0 && first != none;
+    const F score = mine_counts ? first + (second == none ? static_cast<F>(0) : second) : none;
+    auto mine = mine_counts ? order_key(score) : decltype(order_key(score))(0);
+    uint32_t kept = 0;
+    F last = none;
+    for (int r = 0; r <= p.top_groups; ++r) {
+        const auto best = warp_max(mine);
+        if (best == 0) {
+            *margin = static_cast<F>(-kNegInf);
+            return kept;
+        }
+        const int winner = __ffs(__ballot_sync(0xFFFFFFFFu, mine == best)) - 1;
+        const F at = __shfl_sync(0xFFFFFFFFu, score, winner);
+        if (r == p.top_groups) {
+            *margin = last - at;
+            break;
+        }
+        last = at;
+        kept |= 1u << (winner / per);
+        if (lane == winner) {
+            mine = 0;
+        }
+    }
+    return kept;
+}
 
-    int chosen = -1;  // lane j: the j-th choice
-    for (int j = 0; j < p.top_k; ++j) {
+// The top_k largest keys (0: never chosen), ties to the lowest index: lane j gets choice j, or
+// -1.  Each pick is one redux over the lanes' best keys and one over the tied lanes' indices.
+// kGaps: also the smallest distance between the keys of two successive places, down to the first
+// one left out (`value` gives a key's number back).
+template <int NV, bool kGaps, typename Key>
+__device__ __forceinline__ int choose_experts(const RouteParams& p, Key (&key)[NV], int lane, float* gap) {
+    int chosen = -1;
+    float last = -kNegInf, smallest = -kNegInf;
+    for (int j = 0; j < p.top_k + (kGaps ? 1 : 0); ++j) {
         Key best = 0;
         int at = 0;
 #pragma unroll
@@ -258,9 +183,17 @@ __global__ void __launch_bounds__(32 * kRouteWarps) moe_route_kernel(const Route
                 at = i;
             }
         }
-        const Key all = detail::warp_max(best);
+        const Key all = warp_max(best);
         if (all == 0) {
             break;
+        }
+        if constexpr (kGaps) {
+            const float v = key_value(all);
+            smallest = fminf(smallest, last - v);
+            last = v;
+            if (j == p.top_k) {
+                break;
+            }
         }
         const uint32_t e = __reduce_min_sync(
             0xFFFFFFFFu, best == all ? static_cast<uint32_t>(at * 32 + lane) : 0xFFFFFFFFu);
@@ -276,16 +209,195 @@ __global__ void __launch_bounds__(32 * kRouteWarps) moe_route_kernel(const Route
             }
         }
     }
+    if constexpr (kGaps) {
+        *gap = smallest;
+    }
+    return chosen;
+}
+
+// Choice by score + bias inside the best groups, in FP32; false where rounding might decide.
+// Errors: a score s is off by at most 2e-6 s <= 2e-6 (exp 2 ulp, a sum of up to 1024 terms, a
+// quotient), adding the bias rounds to 2^-24 of the key.  Without a bias the choice inside the
+// groups is by the logits themselves, exactly.
+template <int NV>
+__device__ __forceinline__ bool choose_fast(const RouteParams& p, const RouteRow<NV>& row, float* keys, int lane,
+                                            int* chosen) {
+    float key[NV];
+    float largest = 1.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int e = i * 32 + lane;
+        const float l = row.logit[i];
+        float v = l == kNegInf ? kNegInf : p.sigmoid ? sigmoidf(l) : expf(l - row.top) * row.inv_sum;
+        if (p.bias != nullptr && e < p.n_experts) {
+            v += __ldg(p.bias + e);
+            v = v > kNegInf ? v : kNegInf;  // a bias of -inf or NaN takes its expert out
+        }
+        key[i] = v;
+        largest = v > kNegInf ? fmaxf(largest, fabsf(v)) : largest;
+    }
+    const float error = 2e-6f + 1.2e-7f * warp_maxf(largest);
+    uint32_t kept = 0xFFFFFFFFu;
+    if (p.groups > 1) {
+        const int size = p.n_experts / p.groups;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = i * 32 + lane;
+            if (e < p.n_experts) {
+                keys[e + e / size] = key[i];
+            }
+        }
+        __syncwarp();
+        float margin;
+        kept = choose_groups(p, keys, lane, &margin);
+        __syncwarp();
+        if (!(margin > 4.0f * error)) {
+            return false;
+        }
+    }
+    uint32_t order[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int e = i * 32 + lane;
+        const bool in = key[i] > kNegInf && (p.groups == 1 || ((kept >> (e * p.groups / p.n_experts)) & 1u));
+        order[i] = in ? order_key(p.bias != nullptr ? key[i] : row.logit[i]) : 0u;
+    }
+    if (p.bias == nullptr) {
+        *chosen = choose_experts<NV, false>(p, order, lane, nullptr);
+        return true;
+    }
+    float gap;
+    *chosen = choose_experts<NV, true>(p, order, lane, &gap);
+    return gap > 2.0f * error;
+}
+
+// The same choice with scores and sums in 64 bits.  (Reads the row back from shared memory: an array
+// handed to a function that is not inlined would live in local memory for every token.)
+template <int NV>
+__device__ __noinline__ int choose_exact(const RouteParams& p, const float* row, float top, double* keys, int lane) {
+    double score[NV];
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const float l = row[i * 32 + lane];
+        if (l == kNegInf) {
+            score[i] = 0.0;
+        } else if (p.sigmoid) {
+            score[i] = 1.0 / (1.0 + exp(-static_cast<double>(l)));
+        } else {
+            score[i] = exp(static_cast<double>(l) - static_cast<double>(top));
+        }
+        sum += score[i];
+    }
+    if (!p.sigmoid) {
+        sum = warp_sum(sum);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            score[i] = sum > 0.0 ? score[i] / sum : 0.0;
+        }
+    }
+    unsigned long long key[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int e = i * 32 + lane;
+        if (p.bias != nullptr && e < p.n_experts) {
+            score[i] += static_cast<double>(__ldg(p.bias + e));
+        }
+        key[i] = row[e] == kNegInf || !(score[i] > -__builtin_huge_val()) ? 0ull : order_key(score[i]);
+    }
+    if (p.groups > 1) {
+        const int size = p.n_experts / p.groups;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = i * 32 + lane;
+            if (e < p.n_experts) {
+                keys[e + e / size] = key[i] == 0ull ? -__builtin_huge_val() : score[i];
+            }
+        }
+        __syncwarp();
+        double margin;
+        const uint32_t kept = choose_groups(p, static_cast<const double*>(keys), lane, &margin);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = i * 32 + lane;
+            if (e < p.n_experts && !((kept >> (e / size)) & 1u)) {
+                key[i] = 0;
+            }
+        }
+    }
+    return choose_experts<NV, false>(p, key, lane, nullptr);
+}
+
+}  // namespace detail
+
+// One warp per token.  Which experts are chosen is a whole-number answer, so rounding must not
+// decide it: without a bias and groups the logits themselves are compared (the scores are
+// monotone in them); with them (kWide) FP32 keys decide where their distance is beyond their
+// error, and 64-bit ones elsewhere (8192 tokens, 256 experts, 8 groups, bias: 34 us with 64-bit
+// keys for every token).
+template <typename T, int NV, bool kWide>
+__global__ void __launch_bounds__(32 * kRouteWarps) moe_route_kernel(const RouteParams p) {
+    using Traits = detail::OutTraits<T>;
+    extern __shared__ __align__(16) uint8_t route_smem[];
+    ptx::grid_dependency_wait();
+    ptx::launch_dependents();
+    const int warp = static_cast<int>(threadIdx.x >> 5);
+    const int lane = static_cast<int>(threadIdx.x & 31);
+    const int token = static_cast<int>(blockIdx.x) * kRouteWarps + warp;
+    if (token >= p.tokens) {
+        return;
+    }
+    float* smem_row = reinterpret_cast<float*>(route_smem) + warp * (NV * 32);
+    const T* src = static_cast<const T*>(p.logits) + static_cast<size_t>(token) * p.ldl;
+
+    detail::RouteRow<NV> row;
+    row.top = detail::kNegInf;
+    row.inv_sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int e = i * 32 + lane;
+        row.logit[i] = e < p.n_experts ? detail::clean_logit(Traits::load(src + e)) : detail::kNegInf;
+        row.top = fmaxf(row.top, row.logit[i]);
+        smem_row[e] = row.logit[i];
+    }
+    if (!p.sigmoid) {
+        row.top = detail::warp_maxf(row.top);
+        if (kWide || !p.renormalise) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                sum += row.logit[i] == detail::kNegInf ? 0.0f : expf(row.logit[i] - row.top);
+            }
+            sum = detail::warp_sum(sum);
+            row.inv_sum = sum > 0.0f ? 1.0f / sum : 0.0f;
+        }
+    }
+    int chosen;  // lane j: the j-th choice
+    if constexpr (kWide) {
+        double* keys = reinterpret_cast<double*>(route_smem + kRouteWarps * NV * 32 * 4) +
+                       warp * (NV * 32 + kMaxRouteGroups);
+        if (!detail::choose_fast<NV>(p, row, reinterpret_cast<float*>(keys), lane, &chosen)) {
+            chosen = detail::choose_exact<NV>(p, smem_row, row.top, keys, lane);
+        }
+    } else {
+        uint32_t key[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            key[i] = row.logit[i] == detail::kNegInf ? 0u : detail::order_key(row.logit[i]);
+        }
+        chosen = detail::choose_experts<NV, false>(p, key, lane, nullptr);
+    }
     __syncwarp();
     const bool some = chosen >= 0;
-    const float l = some ? row[chosen] : detail::kNegInf;
+    const float l = some ? smem_row[chosen] : detail::kNegInf;
     float w;
     if (p.renormalise) {
         w = detail::chosen_share(l, some, p.sigmoid != 0);
     } else if (p.sigmoid) {
         w = some ? detail::sigmoidf(l) : 0.0f;
     } else {
-        w = some ? expf(l - top) * inv_sum : 0.0f;
+        w = some ? expf(l - row.top) * row.inv_sum : 0.0f;
     }
     if (lane < p.top_k) {
         const size_t at = static_cast<size_t>(token) * p.top_k + lane;
@@ -305,57 +417,63 @@ struct RouteBackwardParams {
     float scale;
 };
 
-// One warp per token.  With p_j the chosen scores' shares and d_j the incoming gradient:
+// One warp per token; lane l holds experts l, l + 32, ...  With p_j the chosen scores' shares and d_j
+// the incoming gradient:
 //   softmax, renormalised   dl_j = scale p_j (d_j - sum d p)                  else 0
 //   sigmoid, renormalised   dl_j = scale p_j (1 - s_j) (d_j - sum d p)        else 0
 //   sigmoid                 dl_j = scale s_j (1 - s_j) d_j                    else 0
 //   softmax                 dl_e = s_e (scale d_e - sum_j scale d_j s_j)      for every e
 // (the choice itself and the bias get no gradient).  Only the last reads the whole row.
-template <typename T>
+template <typename T, int NV>
 __global__ void __launch_bounds__(32 * kRouteWarps)
 moe_route_backward_kernel(const RouteBackwardParams p) {
     using Traits = detail::OutTraits<T>;
-    extern __shared__ __align__(16) uint8_t route_smem[];
+    ptx::grid_dependency_wait();
+    ptx::launch_dependents();
     const int warp = static_cast<int>(threadIdx.x >> 5);
     const int lane = static_cast<int>(threadIdx.x & 31);
     const int token = static_cast<int>(blockIdx.x) * kRouteWarps + warp;
     if (token >= p.tokens) {
         return;
     }
-    float* grad = reinterpret_cast<float*>(route_smem) + warp * p.n_experts;
     const T* src = static_cast<const T*>(p.logits) + static_cast<size_t>(token) * p.ldl;
     T* dst = static_cast<T*>(p.dlogits) + static_cast<size_t>(token) * p.ldd;
-    for (int e = lane; e < p.n_experts; e += 32) {
-        grad[e] = 0.0f;
-    }
+    const bool whole_row = !p.sigmoid && !p.renormalise;
     int chosen = -1;
-    float d = 0.0f, l = detail::kNegInf;
+    float d = 0.0f;
     if (lane < p.top_k) {
         const size_t at = static_cast<size_t>(token) * p.top_k + lane;
         chosen = p.experts[at];
-        if (chosen >= 0 && chosen < p.n_experts) {
-            l = detail::clean_logit(Traits::load(src + chosen));
-            d = p.dweights[at] * p.scale;
-        }
+        d = p.dweights[at] * p.scale;
     }
+    float x[NV], grad[NV];
+    float top = detail::kNegInf;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int e = i * 32 + lane;
+        x[i] = whole_row && e < p.n_experts ? detail::clean_logit(Traits::load(src + e)) : detail::kNegInf;
+        top = fmaxf(top, x[i]);
+        grad[i] = 0.0f;
+    }
+    const bool named = chosen >= 0 && chosen < p.n_experts;
+    const float l = named ? detail::clean_logit(Traits::load(src + chosen)) : detail::kNegInf;
     const bool some = l != detail::kNegInf;
     d = some ? d : 0.0f;
-    float top = 0.0f, inv_sum = 0.0f, dot = 0.0f;
-    const bool whole_row = !p.sigmoid && !p.renormalise;
-    float value = 0.0f;
+    float dot = 0.0f, value;
     if (whole_row) {
-        float m = detail::kNegInf;
-        for (int e = lane; e < p.n_experts; e += 32) {
-            m = fmaxf(m, detail::clean_logit(Traits::load(src + e)));
-        }
-        top = detail::warp_maxf(m);
+        top = detail::warp_maxf(top);
         float sum = 0.0f;
-        for (int e = lane; e < p.n_experts; e += 32) {
-            const float x = detail::clean_logit(Traits::load(src + e));
-            sum += x == detail::kNegInf ? 0.0f : expf(x - top);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            x[i] = x[i] == detail::kNegInf ? 0.0f : expf(x[i] - top);
+            sum += x[i];
         }
         sum = detail::warp_sum(sum);
-        inv_sum = sum > 0.0f ? 1.0f / sum : 0.0f;
+        const float inv_sum = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            x[i] *= inv_sum;  // the scores
+        }
         dot = detail::warp_sum(some ? d * expf(l - top) * inv_sum : 0.0f);
         value = d;
     } else if (p.renormalise) {
@@ -365,24 +483,24 @@ moe_route_backward_kernel(const RouteBackwardParams p) {
     } else {
         value = some ? d * detail::sigmoidf(l) * detail::sigmoidf(-l) : 0.0f;
     }
-    __syncwarp();
     // One choice at a time, so that the result does not depend on the order of threads even
     // where a row names an expert twice.
     for (int j = 0; j < p.top_k; ++j) {
         const float v = __shfl_sync(0xFFFFFFFFu, value, j);
         const int e = __shfl_sync(0xFFFFFFFFu, some ? chosen : -1, j);
-        if (lane == 0 && e >= 0) {
-            grad[e] += v;
+        if (e >= 0 && (e & 31) == lane) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                grad[i] += i == (e >> 5) ? v : 0.0f;
+            }
         }
     }
-    __syncwarp();
-    for (int e = lane; e < p.n_experts; e += 32) {
-        float g = grad[e];
-        if (whole_row) {
-            const float x = detail::clean_logit(Traits::load(src + e));
-            g = x == detail::kNegInf ? 0.0f : expf(x - top) * inv_sum * (g - dot);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int e = i * 32 + lane;
+        if (e < p.n_experts) {
+            Traits::store(dst + e, whole_row ? x[i] * (grad[i] - dot) : grad[i]);
         }
-        Traits::store(dst + e, g);
     }
 }
 
@@ -391,6 +509,7 @@ moe_route_backward_kernel(const RouteBackwardParams p) {
 constexpr int kOrderThreads = 1024;
 constexpr int kOrderWarps = kOrderThreads / 32;
 constexpr int kMaxOrderCluster = 8;
+constexpr int kOrderSteps = 8;  // of 32 slots that a warp holds in registers
 
 struct GroupRowsParams {
     const int* ids;
@@ -423,15 +542,46 @@ __global__ void __launch_bounds__(kOrderThreads) group_rows_kernel(const GroupRo
     for (int i = tid; i < kOrderWarps * bins; i += kOrderThreads) {
         hist[i] = 0;
     }
+    ptx::grid_dependency_wait();
+    ptx::launch_dependents();
     __syncthreads();
     const long long first =
         (static_cast<long long>(rank) * kOrderWarps + warp) * static_cast<long long>(p.warp_slots);
     const int begin = static_cast<int>(min(first, static_cast<long long>(p.slots)));
     const int end = static_cast<int>(min(first + p.warp_slots, static_cast<long long>(p.slots)));
     int* mine = hist + warp * bins;
-    for (int s = begin + lane; s < end; s += 32) {
-        const int id = p.ids[s];
-        atomicAdd(mine + (id >= 0 && id < p.groups ? id : p.groups), 1);
+    // The bins of kOrderSteps x 32 slots at a time, fetched together; the first batch is kept for the
+    // second walk (it is the only one up to 65536 slots).
+    auto fetch = [&](int from, int (&bin)[kOrderSteps]) {
+#pragma unroll
+        for (int i = 0; i < kOrderSteps; ++i) {
+            const int s = from + i * 32 + lane;
+            bin[i] = s < end ? p.ids[s] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < kOrderSteps; ++i) {
+            const int s = from + i * 32 + lane;
+            bin[i] = s >= end ? -1 : bin[i] >= 0 && bin[i] < p.groups ? bin[i] : p.groups;
+        }
+    };
+    int kept_bin[kOrderSteps];
+    fetch(begin, kept_bin);
+    for (int from = begin; from < end; from += 32 * kOrderSteps) {
+        int bin[kOrderSteps];
+        if (from == begin) {
+#pragma unroll
+            for (int i = 0; i < kOrderSteps; ++i) {
+                bin[i] = kept_bin[i];
+            }
+        } else {
+            fetch(from, bin);
+        }
+#pragma unroll
+        for (int i = 0; i < kOrderSteps; ++i) {
+            if (bin[i] >= 0) {
+                atomicAdd(mine + bin[i], 1);
+            }
+        }
     }
     __syncthreads();
     for (int b = tid; b < bins; b += kOrderThreads) {
@@ -506,28 +656,66 @@ __global__ void __launch_bounds__(kOrderThreads) group_rows_kernel(const GroupRo
     // All reads of the other CTAs' totals are done once every CTA is here.
     ptx::cluster_arrive_release();
     ptx::cluster_wait_acquire();
-    for (int s0 = begin; s0 < end; s0 += 32) {
-        const int s = s0 + lane;
-        int bin = -1;
-        if (s < end) {
-            const int id = p.ids[s];
-            bin = id >= 0 && id < p.groups ? id : p.groups;
+    for (int from = begin; from < end; from += 32 * kOrderSteps) {
+        int bin[kOrderSteps];
+        if (from == begin) {
+#pragma unroll
+            for (int i = 0; i < kOrderSteps; ++i) {
+                bin[i] = kept_bin[i];
+            }
+        } else {
+            fetch(from, bin);
         }
-        const uint32_t same = __match_any_sync(0xFFFFFFFFu, bin);
-        if (bin >= 0) {
-            const int pos = start[bin] + mine[bin] + __popc(same & ((1u << lane) - 1u));
-            p.positions[s] = pos;
-            p.rows[pos] = s / p.slots_per_row;
+        uint32_t same[kOrderSteps];
+#pragma unroll
+        for (int i = 0; i < kOrderSteps; ++i) {
+            same[i] = __match_any_sync(0xFFFFFFFFu, bin[i]);
         }
-        __syncwarp();
-        if (bin >= 0 && lane == __ffs(same) - 1) {
-            mine[bin] += __popc(same);
+#pragma unroll
+        for (int i = 0; i < kOrderSteps; ++i) {
+            const int s = from + i * 32 + lane;
+            if (bin[i] >= 0) {
+                const int pos = start[bin[i]] + mine[bin[i]] + __popc(same[i] & ((1u << lane) - 1u));
+                p.positions[s] = pos;
+                p.rows[pos] = s / p.slots_per_row;
+            }
+            __syncwarp();
+            if (bin[i] >= 0 && lane == __ffs(same[i]) - 1) {
+                mine[bin[i]] += __popc(same[i]);
+            }
+            __syncwarp();
         }
-        __syncwarp();
     }
 }
 
 // ---- rows back to their tokens --------------------------------------------------------------
+
+namespace detail {
+
+// Eight consecutive elements on a 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+    constexpr int U = OutTraits<T>::kVec;
+#pragma unroll
+    for (int h = 0; h < 8 / U; ++h) {
+        float u[U];
+        OutTraits<T>::load_vec(p + h * U, u);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            v[h * U + i] = u[i];
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+    constexpr int U = OutTraits<T>::kVec;
+#pragma unroll
+    for (int h = 0; h < 8 / U; ++h) {
+        OutTraits<T>::store_vec(p + h * U, v + h * U);
+    }
+}
+
+}  // namespace detail
 
 constexpr int kCombineThreads = 256;
 
@@ -545,6 +733,8 @@ struct CombineParams {
 // A position outside [0, y_rows) adds nothing.
 template <typename T, typename OutT, bool kVec>
 __global__ void __launch_bounds__(kCombineThreads) moe_combine_kernel(const CombineParams p) {
+    ptx::grid_dependency_wait();
+    ptx::launch_dependents();
     constexpr int V = kVec ? 8 : 1;
     const int units = kVec ? p.n / 8 : p.n;
     const long long id = static_cast<long long>(blockIdx.x) * kCombineThreads + threadIdx.x;
@@ -566,15 +756,11 @@ __global__ void __launch_bounds__(kCombineThreads) moe_combine_kernel(const Comb
         }
         const T* src = y + static_cast<size_t>(at) * p.ldy;
         if constexpr (kVec) {
-            constexpr int U = detail::OutTraits<T>::kVec;
+            float v[V];
+            detail::load8(src, v);
 #pragma unroll
-            for (int h = 0; h < V / U; ++h) {
-                float v[U];
-                detail::OutTraits<T>::load_vec(src + h * U, v);
-#pragma unroll
-                for (int i = 0; i < U; ++i) {
-                    acc[h * U + i] = fmaf(f, v[i], acc[h * U + i]);
-                }
+            for (int i = 0; i < V; ++i) {
+                acc[i] = fmaf(f, v[i], acc[i]);
             }
         } else {
             acc[0] = fmaf(f, detail::OutTraits<T>::load(src), acc[0]);
@@ -582,11 +768,7 @@ __global__ void __launch_bounds__(kCombineThreads) moe_combine_kernel(const Comb
     }
     OutT* dst = static_cast<OutT*>(p.out) + static_cast<size_t>(t) * p.ldo + col;
     if constexpr (kVec) {
-        constexpr int U = detail::OutTraits<OutT>::kVec;
-#pragma unroll
-        for (int h = 0; h < V / U; ++h) {
-            detail::OutTraits<OutT>::store_vec(dst + h * U, acc + h * U);
-        }
+        detail::store8(dst, acc);
     } else {
         detail::OutTraits<OutT>::store(dst, acc[0]);
     }
@@ -603,92 +785,53 @@ struct CombineBackwardParams {
     int ldy, ldo, lddy;
 };
 
-// One CTA per token: dy[positions[t][j]] = weights[t][j] * dout[t] and
-// dweights[t][j] = <dout[t], y[positions[t][j]]> in one pass over y.  Eight choices at a time
-// keep their dot products in registers; more choices walk dout again (it is in L1 by then).
+// One warp per slot (t, j): dy[positions[t][j]] = weights[t][j] * dout[t] and
+// dweights[t][j] = <dout[t], y[positions[t][j]]> in one pass over y.  The slots of a token sit in
+// one CTA, so dout comes from L1 after the first.  No sum leaves its warp: with one CTA per
+// token and the choices' sums in registers, the two block-wide steps per token left the memory
+// idle (2047 x 8 rows of 2048 columns: 43 us).
 template <typename T, typename OutT, bool kVec>
 __global__ void __launch_bounds__(kCombineThreads)
 moe_combine_backward_kernel(const CombineBackwardParams p) {
+    ptx::grid_dependency_wait();
+    ptx::launch_dependents();
     constexpr int V = kVec ? 8 : 1;
-    constexpr int J = 8;
-    __shared__ float part[kCombineThreads / 32][J];
-    const size_t t = blockIdx.x;
-    const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
-    const OutT* dout = static_cast<const OutT*>(p.dout) + t * p.ldo;
-    for (int j0 = 0; j0 < p.top_k; j0 += J) {
-        int at[J];
-        float w[J], dot[J];
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            at[j] = -1;
-            w[j] = dot[j] = 0.0f;
-            if (j0 + j < p.top_k) {
-                at[j] = __ldg(p.positions + t * p.top_k + j0 + j);
-                w[j] = __ldg(p.weights + t * p.top_k + j0 + j);
-                if (at[j] >= p.y_rows) {
-                    at[j] = -1;
-                }
-            }
-        }
-        for (int col = static_cast<int>(threadIdx.x) * V; col < p.n; col += kCombineThreads * V) {
-            float g[V];
+    const int lane = static_cast<int>(threadIdx.x & 31);
+    const long long slot = (static_cast<long long>(blockIdx.x) * kCombineThreads + threadIdx.x) >> 5;
+    const long long t = slot / p.top_k;
+    if (t >= p.tokens) {
+        return;
+    }
+    const int at = __ldg(p.positions + slot);
+    const float w = __ldg(p.weights + slot);
+    const bool exists = at >= 0 && at < p.y_rows;
+    float dot = 0.0f;
+    if (exists) {
+        const OutT* dout = static_cast<const OutT*>(p.dout) + static_cast<size_t>(t) * p.ldo;
+        const T* src = static_cast<const T*>(p.y) + static_cast<size_t>(at) * p.ldy;
+        T* dst = static_cast<T*>(p.dy) + static_cast<size_t>(at) * p.lddy;
+#pragma unroll 4
+        for (int col = lane * V; col < p.n; col += 32 * V) {
             if constexpr (kVec) {
-                constexpr int U = detail::OutTraits<OutT>::kVec;
+                float g[V], v[V];
+                detail::load8(dout + col, g);
+                detail::load8(src + col, v);
 #pragma unroll
-                for (int h = 0; h < V / U; ++h) {
-                    float v[U];
-                    detail::OutTraits<OutT>::load_vec(dout + col + h * U, v);
-#pragma unroll
-                    for (int i = 0; i < U; ++i) {
-                        g[h * U + i] = v[i];
-                    }
+                for (int i = 0; i < V; ++i) {
+                    dot = fmaf(v[i], g[i], dot);
+                    g[i] *= w;
                 }
+                detail::store8(dst + col, g);
             } else {
-                g[0] = detail::OutTraits<OutT>::load(dout + col);
-            }
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                if (at[j] < 0) {
-                    continue;
-                }
-                const T* src = static_cast<const T*>(p.y) + static_cast<size_t>(at[j]) * p.ldy + col;
-                T* dst = static_cast<T*>(p.dy) + static_cast<size_t>(at[j]) * p.lddy + col;
-                if constexpr (kVec) {
-                    constexpr int U = detail::OutTraits<T>::kVec;
-#pragma unroll
-                    for (int h = 0; h < V / U; ++h) {
-                        float v[U], o[U];
-                        detail::OutTraits<T>::load_vec(src + h * U, v);
-#pragma unroll
-                        for (int i = 0; i < U; ++i) {
-                            dot[j] = fmaf(v[i], g[h * U + i], dot[j]);
-                            o[i] = w[j] * g[h * U + i];
-                        }
-                        detail::OutTraits<T>::store_vec(dst + h * U, o);
-                    }
-                } else {
-                    dot[j] = fmaf(detail::OutTraits<T>::load(src), g[0], dot[j]);
-                    detail::OutTraits<T>::store(dst, w[j] * g[0]);
-                }
+                const float g = detail::OutTraits<OutT>::load(dout + col);
+                dot = fmaf(detail::OutTraits<T>::load(src + col), g, dot);
+                detail::OutTraits<T>::store(dst + col, w * g);
             }
         }
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const float s = detail::warp_sum(dot[j]);
-            if (lane == 0) {
-                part[warp][j] = s;
-            }
-        }
-        __syncthreads();
-        if (threadIdx.x < J && j0 + static_cast<int>(threadIdx.x) < p.top_k) {
-            float s = 0.0f;
-#pragma unroll
-            for (int v = 0; v < kCombineThreads / 32; ++v) {
-                s += part[v][threadIdx.x];
-            }
-            p.dweights[t * p.top_k + j0 + threadIdx.x] = s;
-        }
-        __syncthreads();
+    }
+    dot = detail::warp_sum(dot);
+    if (lane == 0) {
+        p.dweights[slot] = dot;
     }
 }
 
