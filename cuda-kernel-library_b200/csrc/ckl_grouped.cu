@@ -194,6 +194,9 @@ int run(Product& q, cudaStream_t stream) {
     p.lda = q.lda;
     p.ldb = q.ldb;
     p.ldt = q.ldt;
+    p.e = q.e;
+    p.lde = q.lde;
+    p.e_stride = q.e_stack;
     unsigned long long limit_ns = 0;
     const int fault = take_wait_fault(&limit_ns);
     p.wait_limit_ns = limit_ns;
@@ -266,6 +269,33 @@ Product shrink(int ab_dtype, const void* a, int lda, int k, const void* b, int l
     return q;
 }
 
+// The same for a few rows, where one CTA per row and 32 ranks is a wave or two.
+int shrink_rows(int ab_dtype, const void* x, int ldx, int k, const void* a, int lda, long long stack, int rank,
+                const float* scales, void* t, const int* offsets, const int* rows, int adapters, int m,
+                cudaStream_t stream) {
+    DeviceView view;
+    GRP_TRY(device_view(&view));
+    LoraRowsParams p = {};
+    p.offsets = offsets;
+    p.rows = rows;
+    p.scales = scales;
+    p.x = static_cast<const unsigned short*>(x);
+    p.a = static_cast<const unsigned short*>(a);
+    p.t = static_cast<unsigned short*>(t);
+    p.a_stride = stack;
+    p.adapters = adapters;
+    p.m = m;
+    p.k = k;
+    p.rank = rank;
+    p.part_cols = padded_rank(rank);
+    p.ldx = ldx;
+    p.lda = lda;
+    const dim3 grid(static_cast<unsigned>(m), static_cast<unsigned>((rank + kLoraRanks - 1) / kLoraRanks));
+    GRP_TRY_CUDA(launch_dependent(ab_dtype == CKL_BF16 ? lora_rows_kernel<__nv_bfloat16> : lora_rows_kernel<__half>,
+                                  grid, kLoraRowsThreads, 0, 1, stream, p));
+    return CKL_OK;
+}
+
 // C[rows[p]] = A[rows[p]] * op(B) + T[p] * op(E_g) + beta * C[rows[p]], C of n columns.
 Product expand(int ab_dtype, int c_dtype, const void* a, int lda, int k, const void* b, int ldb, int n,
                bool trans, const void* t, int rank, const void* e, int lde, long long e_stack, void* c,
@@ -277,6 +307,7 @@ Product expand(int ab_dtype, int c_dtype, const void* a, int lda, int k, const v
     q.p.c = c;
     q.p.groups = q.p.ext_groups = adapters;
     q.p.ext_cols = rp;
+    q.p.ext_rank = rank;
     q.p.rows = q.p.a_count = q.p.c_count = m;
     q.p.n = n;
     q.p.k = k;
@@ -447,9 +478,16 @@ int ckl_gemm_lora(int ab_dtype, const void* x, const void* w, const void* lora_a
         return set_error(CKL_ERR_INVALID_ARG, "%s: y %p, ldy %d for n %d", what, y, ldy, n);
     }
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    Product t = shrink(ab_dtype, x, ldx, k, lora_a, ldla, stride_a, false, rank, scales, workspace, offsets,
-                       rows, adapters, m);
-    GRP_TRY(run(t, s));
+    DeviceView view;
+    GRP_TRY(device_view(&view));
+    if (static_cast<long long>(m) * ((rank + kLoraRanks - 1) / kLoraRanks) <= 2ll * view.sm_count) {
+        GRP_TRY(shrink_rows(ab_dtype, x, ldx, k, lora_a, ldla, stride_a, rank, scales, workspace, offsets, rows,
+                            adapters, m, s));
+    } else {
+        Product t = shrink(ab_dtype, x, ldx, k, lora_a, ldla, stride_a, false, rank, scales, workspace, offsets,
+                           rows, adapters, m);
+        GRP_TRY(run(t, s));
+    }
     Product q = expand(ab_dtype, y_dtype, x, ldx, k, w, ldw, n, false, workspace, rank, lora_b, ldlb, stride_b,
                        y, ldy, offsets, rows, adapters, m, beta);
     return run(q, s);

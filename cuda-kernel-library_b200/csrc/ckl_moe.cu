@@ -223,6 +223,8 @@ int ckl_moe_route(int logit_dtype, const void* logits, int ldl, const float* bia
     // Keeping every group is keeping none apart.
     p.groups = top_groups == groups ? 1 : groups;
     p.top_groups = top_groups == groups ? 1 : top_groups;
+    p.group_size = n_experts / p.groups;
+    p.inv_group_size = 1.0f / static_cast<float>(p.group_size);
     p.sigmoid = score == CKL_SCORE_SIGMOID ? 1 : 0;
     p.renormalise = renormalise != 0 ? 1 : 0;
     p.scale = scale;

@@ -70,6 +70,9 @@ struct GroupedParams {
     int c_part_cols;     // TwoPart output: distance of lo behind hi
     // Extension (ext_groups > 0): offsets/groups describe the adapters.
     int ext_groups, ext_cols;  // adapters; columns of one part of T (a multiple of 16)
+    const void* e;             // E, `ext_rank` x n per adapter (n x ext_rank with trans_b)
+    int ext_rank, lde;
+    long long e_stride;
     uint32_t fmt;        // operand format for the instruction descriptor
     int split;           // CTAs per tile (a split launch)
     int load_a;          // rows of A come through the loaders (gathered, or few per tile)
@@ -193,7 +196,7 @@ __device__ __forceinline__ int total_tiles(const GroupedParams& p, const Grouped
 }
 
 __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, const GroupedTable& t,
-                                                    int tile) {
+                                                    int tile, bool split) {
     GroupedTile o;
     int mt, nt;
     int m_tiles, local;
@@ -229,7 +232,7 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, cons
         o.valid = min(128, seg1 - o.p0);
         o.m0 = 0;
         o.k_blocks = (p.k + 63) / 64;
-        if (p.ext_groups > 0 && o.p0 < t.offs[p.ext_groups]) {
+        if (!split && p.ext_groups > 0 && o.p0 < t.offs[p.ext_groups]) {
             // first adapter that ends behind p0, and the one after the last that starts in here
             o.ext_first = last_at_most(t.offs, p.ext_groups, o.p0);
             o.ext_last = last_at_most(t.offs, p.ext_groups, o.p0 + o.valid - 1) + 1;
@@ -533,6 +536,100 @@ struct Loader {
     }
 };
 
+// v[i] += sum over ranks of T[pos] * E_g, columns col .. of the row behind position pos; T's two
+// parts are added first.  The operands are 16-bit words: BF16 is the upper half of an FP32 word.
+__device__ __forceinline__ float from16(const GroupedParams& p, uint32_t word) {
+    return p.fmt != 0 ? __uint_as_float(word << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(word)));
+}
+template <typename Elem, int kVec>
+__device__ __forceinline__ void add_adapter(const GroupedParams& p, const GroupedTable& table, int pos, int col,
+                                            int have, float (&v)[kVec]) {
+    if (pos >= table.offs[p.ext_groups] || pos < table.offs[0]) {
+        return;
+    }
+    const int g = last_at_most(table.offs, p.ext_groups, pos);
+    if (pos >= table.offs[g + 1]) {
+        return;
+    }
+    const unsigned short* t = static_cast<const unsigned short*>(p.t) + static_cast<size_t>(pos) * p.ldt;
+    const unsigned short* e = static_cast<const unsigned short*>(p.e) + static_cast<size_t>(g) * p.e_stride;
+    // eight ranks at a time: their T is one 16-byte word per part (parts are 16 ranks wide or more)
+    for (int r0 = 0; r0 < p.ext_rank; r0 += 8) {
+        const uint4 hi = *reinterpret_cast<const uint4*>(t + r0);
+        const uint4 lo = *reinterpret_cast<const uint4*>(t + p.ext_cols + r0);
+        const uint32_t h[4] = {hi.x, hi.y, hi.z, hi.w}, l[4] = {lo.x, lo.y, lo.z, lo.w};
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = from16(p, h[i] & 0xffffu) + from16(p, l[i] & 0xffffu);
+            f[2 * i + 1] = from16(p, h[i] >> 16) + from16(p, l[i] >> 16);
+        }
+        if (p.trans_b) {
+            // one column's ranks are neighbours
+#pragma unroll
+            for (int c = 0; c < kVec; ++c) {
+                if (c < have) {
+                    const unsigned short* src = e + static_cast<size_t>(col + c) * p.lde + r0;
+                    if (r0 + 8 <= p.ext_rank) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(src);
+                        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            v[c] = fmaf(f[2 * i], from16(p, x[i] & 0xffffu), v[c]);
+                            v[c] = fmaf(f[2 * i + 1], from16(p, x[i] >> 16), v[c]);
+                        }
+                    } else {
+                        for (int i = 0; r0 + i < p.ext_rank; ++i) {
+                            const float fi = i == 0 ? f[0] : i == 1 ? f[1] : i == 2 ? f[2] : i == 3 ? f[3]
+                                             : i == 4 ? f[4] : i == 5 ? f[5] : f[6];
+                            v[c] = fmaf(fi, from16(p, src[i]), v[c]);
+                        }
+                    }
+                }
+            }
+        } else if (r0 + 8 <= p.ext_rank && have == kVec) {
+            // eight loads in flight, then their sums
+            uint32_t x[8][kVec / 2];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const unsigned short* src = e + static_cast<size_t>(r0 + i) * p.lde + col;
+                if constexpr (kVec == 8) {
+                    const uint4 w = *reinterpret_cast<const uint4*>(src);
+                    x[i][0] = w.x;
+                    x[i][1] = w.y;
+                    x[i][2] = w.z;
+                    x[i][3] = w.w;
+                } else {
+                    const uint2 w = *reinterpret_cast<const uint2*>(src);
+                    x[i][0] = w.x;
+                    x[i][1] = w.y;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+#pragma unroll
+                for (int c = 0; c < kVec / 2; ++c) {
+                    v[2 * c] = fmaf(f[i], from16(p, x[i][c] & 0xffffu), v[2 * c]);
+                    v[2 * c + 1] = fmaf(f[i], from16(p, x[i][c] >> 16), v[2 * c + 1]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (r0 + i < p.ext_rank) {
+                    const unsigned short* src = e + static_cast<size_t>(r0 + i) * p.lde + col;
+#pragma unroll
+                    for (int c = 0; c < kVec; ++c) {
+                        if (c < have) {
+                            v[c] = fmaf(f[i], from16(p, src[c]), v[c]);
+                        }
+                    }
+                }
+            }
+        }
+    }
+}
+
 // Row of C behind row `in_tile` of a tile, -1 for none.
 __device__ __forceinline__ int row_of_c(const GroupedParams& p, const GroupedTile& t, int in_tile) {
     if (p.form == kFormWgrad) {
@@ -581,7 +678,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
     const uint32_t tmem_slot = bars + 8u * Cfg::kNumBarriers;
     volatile uint32_t* tmem_slot_ptr =
         reinterpret_cast<volatile uint32_t*>(bars_ptr + 8 * Cfg::kNumBarriers);
-    const bool loads = p.form == kFormWgrad || p.load_a != 0 || p.ext_groups > 0;  // the loaders work
+    // the loaders work
+    const bool loads = p.form == kFormWgrad || p.load_a != 0 || (!kSplit && p.ext_groups > 0);
 
     detail::Control ctl;
     ctl.abort_flag = reinterpret_cast<volatile int*>(bars_ptr + 8 * Cfg::kNumBarriers + 4);
@@ -879,7 +977,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
             detail::GroupedTile t;
             bool ok = true;
             for (int tile = first_tile; ok && tile < total; tile += tile_step, ++i) {
-                t = detail::grouped_tile(p, table, tile);
+                t = detail::grouped_tile(p, table, tile, kSplit);
                 detail::take_share(p, table, &t, rank, size);
                 ok = queue.push(i, t, ctl);
             }
@@ -1214,7 +1312,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
             constexpr int kLanesPerRow = 128 / kVec;
             constexpr int kRowsPerWarp = 32 / kLanesPerRow;
             constexpr int kWarps = Cfg::kThreads / 32;
-            const detail::GroupedTile t = detail::grouped_tile(p, table, first_tile);
+            const detail::GroupedTile t = detail::grouped_tile(p, table, first_tile, true);
             const int rows = p.form == kFormWgrad ? min(128, p.m - t.m0) : t.valid;
             const int sub = static_cast<int>(lane) % kLanesPerRow;
             const int col = t.n0 + sub * kVec;
@@ -1244,6 +1342,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
                         v[4 * u + 3] += x.w;
                     }
                 }
+                if (p.ext_groups > 0) {
+                    detail::add_adapter<Elem, kVec>(p, table, t.p0 + row, col, have, v);
+                }
                 detail::store_unit<OutT, kVec>(p, c_base, c_row, col, have, factor, v);
             }
         }
@@ -1257,6 +1358,118 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
     if (warp == 1) {
         ptx::tc_fence_after_sync();
         ptx::tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// T of the adapters for a few rows, on the CUDA cores: one CTA per position and 32 ranks reads its
+// adapter's A_g (k x 32 of it) once, at the rate of one SM's L2 port, and no tensor-core tile is
+// filled with rows that do not exist (48 rows of 24 adapters, k 4096, rank 16: 10.7 us through the
+// tensor cores, whose clusters wait for 16 blocks and each other).
+struct LoraRowsParams {
+    const int* offsets;
+    const int* rows;       // or nullptr
+    const float* scales;   // or nullptr
+    const unsigned short* x;
+    const unsigned short* a;
+    unsigned short* t;
+    long long a_stride;
+    int adapters, m, k, rank, part_cols, ldx, lda;
+};
+constexpr int kLoraRowsThreads = 256;
+constexpr int kLoraRanks = 32;
+
+template <typename T>
+__global__ void __launch_bounds__(kLoraRowsThreads) lora_rows_kernel(const LoraRowsParams p) {
+    using Traits = detail::OutTraits<T>;
+    __shared__ int adapter;
+    __shared__ float part[kLoraRowsThreads / 32][kLoraRanks];
+    ptx::grid_dependency_wait();
+    ptx::launch_dependents();
+    const int pos = static_cast<int>(blockIdx.x);
+    const int r0 = static_cast<int>(blockIdx.y) * kLoraRanks;
+    if (threadIdx.x == 0) {
+        adapter = -1;
+    }
+    __syncthreads();
+    for (int g = static_cast<int>(threadIdx.x); g < p.adapters; g += kLoraRowsThreads) {
+        if (min(max(p.offsets[g], 0), p.m) <= pos && pos < min(max(p.offsets[g + 1], 0), p.m)) {
+            adapter = g;
+        }
+    }
+    __syncthreads();
+    const int g = adapter;
+    if (g < 0) {
+        return;
+    }
+    const int row = p.rows != nullptr ? __ldg(p.rows + pos) : pos;
+    const bool exists = row >= 0 && row < p.m;
+    const int ranks = min(kLoraRanks, p.rank - r0);
+    // 16-byte units (8 ranks) per row of A_g: 1, 2 or 4; the other lanes take further rows.
+    const int shift = ranks <= 8 ? 0 : ranks <= 16 ? 1 : 2;
+    const int lane = static_cast<int>(threadIdx.x & 31), warp = static_cast<int>(threadIdx.x >> 5);
+    const int unit = lane & ((1 << shift) - 1);
+    const int step = kLoraRowsThreads >> shift;
+    const T* x = reinterpret_cast<const T*>(p.x) + static_cast<size_t>(exists ? row : 0) * p.ldx;
+    const T* a = reinterpret_cast<const T*>(p.a) + static_cast<size_t>(g) * p.a_stride + r0 + unit * 8;
+    const int have = min(8, ranks - unit * 8);
+    float acc[8] = {};
+    int k = static_cast<int>(threadIdx.x) >> shift;
+    if (exists && have == 8) {
+        // eight loads of either operand in flight
+        for (; k + 7 * step < p.k; k += 8 * step) {
+            float f[8], v[8][8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                f[i] = Traits::load(x + k + i * step);
+                Traits::load_vec(a + static_cast<size_t>(k + i * step) * p.lda, v[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    acc[c] = fmaf(f[i], v[i][c], acc[c]);
+                }
+            }
+        }
+    }
+    if (exists) {
+        for (; k < p.k; k += step) {
+            const float f = Traits::load(x + k);
+            const T* src = a + static_cast<size_t>(k) * p.lda;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (i < have) {
+                    acc[i] = fmaf(f, Traits::load(src + i), acc[i]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        for (int d = 16; d >= (1 << shift); d >>= 1) {
+            acc[i] += __shfl_xor_sync(0xFFFFFFFFu, acc[i], d);
+        }
+        if (lane < (1 << shift)) {
+            part[warp][unit * 8 + i] = acc[i];
+        }
+    }
+    __syncthreads();
+    const int r = static_cast<int>(threadIdx.x);
+    if (r < kLoraRanks && r0 + r < p.part_cols) {
+        float v = 0.0f;
+        if (r < ranks) {
+#pragma unroll
+            for (int w = 0; w < kLoraRowsThreads / 32; ++w) {
+                v += part[w][r];
+            }
+            v *= p.scales != nullptr ? __ldg(p.scales + g) : 1.0f;
+        }
+        T* dst = reinterpret_cast<T*>(p.t) + static_cast<size_t>(pos) * 2 * p.part_cols + r0 + r;
+        T hi;
+        Traits::store(&hi, v);
+        const float h = Traits::load(&hi);
+        *dst = hi;
+        Traits::store(dst + p.part_cols, isinf(h) ? 0.0f : v - h);
     }
 }
 

@@ -627,16 +627,17 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
             // gradient it clips rows as well.
             const int by_tma = p.c_tma == 0 ? 0 : wgrad ? (rows + 31) / 32 * 32 : rows / 32 * 32;
             int j0 = 0;
-            if constexpr (sizeof(Elem) == 2) {
+            if (sizeof(Elem) == 2 && p.beta == 0.0f && p.c_vec != 0) {
                 // 64 rows at a time: the accumulator is read as matrix fragments (16 columns of C by
                 // 32 rows), whose 8 x 8 blocks are stored transposed, 16 bytes = 8 columns of a row
                 // each.  (Lane = column and 2-byte stores, 32 rows at a time, took the epilogue of a
                 // 256 x 256 tile to 8000 cycles, twice its 6 blocks of MMAs in a weight gradient.)
+                // Rows that do not leave by TMA are read back, four lanes a row, and stored one by one.
                 uint32_t f[64];
                 auto fetch = [&](int j) {
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
-                        if (j + (h >> 1) * 32 < by_tma) {
+                        if (j + (h >> 1) * 32 < rows) {
                             ptx::tmem_ld_16x256b_x4(
                                 t_row + (static_cast<uint32_t>(h & 1) << 20) + static_cast<uint32_t>(j + (h >> 1) * 32),
                                 *reinterpret_cast<uint32_t(*)[16]>(&f[h * 16]));
@@ -648,10 +649,10 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                     for (int i = 0; i < 64; ++i) {
                         f[i] = 0;
                     }
-                } else if (by_tma > 0) {
+                } else if (rows > 0) {
                     fetch(0);
                 }
-                for (; j0 < by_tma; j0 += 64) {
+                for (; j0 < rows; j0 += 64) {
                     ptx::tmem_ld_wait();
                     uint32_t w[32];  // [32-row run][8-row block][16-byte unit]
 #pragma unroll
@@ -661,7 +662,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                     }
                     if (j0 + 64 >= rows) {
                         release();
-                    } else if (!nothing && j0 + 64 < by_tma) {
+                    } else if (!nothing) {
                         fetch(j0 + 64);
                     }
                     if (lane == 0) {
@@ -678,21 +679,63 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                             buf + (i >> 2) * 2048u + row * 64u + (((lane >> 3) ^ ((row >> 1) & 3u)) << 4), w[4 * i],
                             w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
                     }
-                    ptx::fence_proxy_async_smem();
+                    if (j0 < by_tma) {
+                        ptx::fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            ptx::tma_store_3d(&tmap_c, buf, col0, t.r0 + j0, z);
+                            if (j0 + 32 < by_tma) {
+                                ptx::tma_store_3d(&tmap_c, buf + 2048u, col0, t.r0 + j0 + 32, z);
+                            }
+                        }
+                    } else {
+                        __syncwarp();
+                    }
+                    const int col = col0 + sub * kVec;
+                    const int have = min(kVec, p.n - col);
+#pragma unroll
+                    for (int run = 0; run < 2; ++run) {
+                        if (j0 + run * 32 < by_tma) {
+                            continue;
+                        }
+#pragma unroll
+                        for (int pass = 0; pass < 4; ++pass) {
+                            const int j = pass * 8 + static_cast<int>(lane >> 2);
+                            const int in_tile = j0 + run * 32 + j;
+                            if (in_tile >= rows || have <= 0) {
+                                continue;
+                            }
+                            int c_row = t.r0 + in_tile;
+                            if (!wgrad && p.c_rows != nullptr) {
+                                c_row = __ldg(p.c_rows + t.p0 + in_tile);
+                                if (c_row < 0 || c_row >= p.c_count) {
+                                    continue;
+                                }
+                            }
+                            const uint4 v = *reinterpret_cast<const uint4*>(
+                                stg + buffer * Cfg::kBufferBytes + run * 2048 + j * 64 +
+                                ((sub ^ ((j >> 1) & 3)) << 4));
+                            Elem* dst = c_base + static_cast<size_t>(c_row) * p.ldc + col;
+                            if (have == kVec) {
+                                *reinterpret_cast<uint4*>(dst) = v;
+                            } else {
+                                for (int i = 0; i < have; ++i) {
+                                    const uint32_t word = i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w;
+                                    reinterpret_cast<unsigned short*>(dst)[i] =
+                                        static_cast<unsigned short>((i & 1) ? word >> 16 : word);
+                                }
+                            }
+                        }
+                    }
                     __syncwarp();
                     if (lane == 0) {
-                        ptx::tma_store_3d(&tmap_c, buf, col0, t.r0 + j0, z);
-                        if (j0 + 32 < by_tma) {
-                            ptx::tma_store_3d(&tmap_c, buf + 2048u, col0, t.r0 + j0 + 32, z);
-                        }
-                        ptx::bulk_commit_group();
+                        ptx::bulk_commit_group();  // one group per buffer, empty or not
                     }
                     buffer = buffer + 1 == Cfg::kBuffers ? 0u : buffer + 1;
                 }
-                j0 = by_tma;
+                j0 = rows;
             }
-            // FP32 runs, and rows that are scattered, read before they are written or do not fill a
-            // run: one column per lane.
+            // FP32 columns, and C that is read or not on 16 bytes: one column per lane.
             for (; j0 < rows; j0 += 32) {
                 uint32_t r[32];
                 if (nothing) {
@@ -724,7 +767,6 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                     __syncwarp();
                     if (lane == 0) {
                         ptx::tma_store_3d(&tmap_c, stg_addr + buffer * Cfg::kBufferBytes, col0, t.r0 + j0, z);
-                        ptx::bulk_commit_group();
                     }
                 } else {
                     __syncwarp();
@@ -754,9 +796,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
                         }
                     }
                     __syncwarp();
-                    if (lane == 0) {
-                        ptx::bulk_commit_group();  // keeps one group per buffer
-                    }
+                }
+                if (lane == 0) {
+                    ptx::bulk_commit_group();
                 }
                 buffer = buffer + 1 == Cfg::kBuffers ? 0u : buffer + 1;
             }

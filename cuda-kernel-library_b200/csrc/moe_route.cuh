@@ -28,6 +28,8 @@ struct RouteParams {
     int ldl;
     int tokens, n_experts, top_k;
     int groups, top_groups;
+    int group_size;         // experts per group
+    float inv_group_size;
     int sigmoid, renormalise;
     float scale;
 };
@@ -111,13 +113,18 @@ struct RouteRow {
     float inv_sum;  // softmax: 1 / sum of exp(l - top), 0 for an empty row
 };
 
+// e / group size, exact for e < 2^20.
+__device__ __forceinline__ int group_of(const RouteParams& p, int e) {
+    return __float2int_rz((static_cast<float>(e) + 0.5f) * p.inv_group_size);
+}
+
 // Which groups take part: bit g.  A group's score is the sum of its two best keys; `keys` is
 // shared memory (index e + e / size), read by a few neighbouring lanes per group.  `margin` gets
 // the distance of the last group kept to the best one left out (infinite if none competes).
 template <typename F>
 __device__ __forceinline__ uint32_t choose_groups(const RouteParams& p, const F* keys, int lane, F* margin) {
     const F none = static_cast<F>(kNegInf);
-    const int size = p.n_experts / p.groups;
+    const int size = p.group_size;
     int per = 1;  // lanes per group, a power of two
     while (per * 2 * p.groups <= 32) {
         per *= 2;
@@ -216,8 +223,10 @@ __device__ __forceinline__ int choose_experts(const RouteParams& p, Key (&key)[N
 }
 
 // Choice by score + bias inside the best groups, in FP32; false where rounding might decide.
-// Errors: a score s is off by at most 2e-6 s <= 2e-6 (exp 2 ulp, a sum of up to 1024 terms, a
-// quotient), adding the bias rounds to 2^-24 of the key.  Without a bias the choice inside the
+// Errors: with the fast exponential of x = -l or l - top, 2^(x log2 e), the product rounds to 2^-24
+// of itself and the power is off by 2^-22, so a score is off by s (|x| + 4) 2^-24 at most plus the
+// quotient's 2^-23 and (softmax) the sum's 1e-6: below 3e-6 in all, as s |x| < 0.4 for the
+// sigmoid's and the softmax's tails.  Adding the bias rounds to 2^-24 of the key.  Without a bias the choice inside the
 // groups is by the logits themselves, exactly.
 template <int NV>
 __device__ __forceinline__ bool choose_fast(const RouteParams& p, const RouteRow<NV>& row, float* keys, int lane,
@@ -228,7 +237,8 @@ __device__ __forceinline__ bool choose_fast(const RouteParams& p, const RouteRow
     for (int i = 0; i < NV; ++i) {
         const int e = i * 32 + lane;
         const float l = row.logit[i];
-        float v = l == kNegInf ? kNegInf : p.sigmoid ? sigmoidf(l) : expf(l - row.top) * row.inv_sum;
+        float v = p.sigmoid ? __fdividef(1.0f, 1.0f + __expf(-l)) : __expf(l - row.top) * row.inv_sum;
+        v = l == kNegInf ? kNegInf : v;
         if (p.bias != nullptr && e < p.n_experts) {
             v += __ldg(p.bias + e);
             v = v > kNegInf ? v : kNegInf;  // a bias of -inf or NaN takes its expert out
@@ -236,15 +246,14 @@ __device__ __forceinline__ bool choose_fast(const RouteParams& p, const RouteRow
         key[i] = v;
         largest = v > kNegInf ? fmaxf(largest, fabsf(v)) : largest;
     }
-    const float error = 2e-6f + 1.2e-7f * warp_maxf(largest);
+    const float error = 3e-6f + 1.2e-7f * warp_maxf(largest);
     uint32_t kept = 0xFFFFFFFFu;
     if (p.groups > 1) {
-        const int size = p.n_experts / p.groups;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int e = i * 32 + lane;
             if (e < p.n_experts) {
-                keys[e + e / size] = key[i];
+                keys[e + group_of(p, e)] = key[i];
             }
         }
         __syncwarp();
@@ -259,7 +268,7 @@ __device__ __forceinline__ bool choose_fast(const RouteParams& p, const RouteRow
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int e = i * 32 + lane;
-        const bool in = key[i] > kNegInf && (p.groups == 1 || ((kept >> (e * p.groups / p.n_experts)) & 1u));
+        const bool in = key[i] > kNegInf && (p.groups == 1 || ((kept >> (group_of(p, e) & 31)) & 1u));
         order[i] = in ? order_key(p.bias != nullptr ? key[i] : row.logit[i]) : 0u;
     }
     if (p.bias == nullptr) {
@@ -271,62 +280,63 @@ __device__ __forceinline__ bool choose_fast(const RouteParams& p, const RouteRow
     return gap > 2.0f * error;
 }
 
-// The same choice with scores and sums in 64 bits.  (Reads the row back from shared memory: an array
-// handed to a function that is not inlined would live in local memory for every token.)
+// The same choice with scores and sums in 64 bits, for the few tokens that need it (a launch ends
+// with its slowest warp: loops are rolled and keys live in shared memory, `keys`, so that this
+// takes few registers from every other token).
 template <int NV>
 __device__ __noinline__ int choose_exact(const RouteParams& p, const float* row, float top, double* keys, int lane) {
-    double score[NV];
+    const double none = -__builtin_huge_val();
     double sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const float l = row[i * 32 + lane];
-        if (l == kNegInf) {
-            score[i] = 0.0;
-        } else if (p.sigmoid) {
-            score[i] = 1.0 / (1.0 + exp(-static_cast<double>(l)));
-        } else {
-            score[i] = exp(static_cast<double>(l) - static_cast<double>(top));
-        }
-        sum += score[i];
-    }
     if (!p.sigmoid) {
+#pragma unroll 1
+        for (int e = lane; e < p.n_experts; e += 32) {
+            sum += row[e] == kNegInf ? 0.0 : exp(static_cast<double>(row[e]) - static_cast<double>(top));
+        }
         sum = warp_sum(sum);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            score[i] = sum > 0.0 ? score[i] / sum : 0.0;
-        }
     }
-    unsigned long long key[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int e = i * 32 + lane;
-        if (p.bias != nullptr && e < p.n_experts) {
-            score[i] += static_cast<double>(__ldg(p.bias + e));
+#pragma unroll 1
+    for (int e = lane; e < p.n_experts; e += 32) {
+        const double l = static_cast<double>(row[e]);
+        double v = exp(p.sigmoid ? -l : l - static_cast<double>(top));
+        v = p.sigmoid ? 1.0 / (1.0 + v) : v / sum;
+        if (p.bias != nullptr) {
+            v += static_cast<double>(__ldg(p.bias + e));
         }
-        key[i] = row[e] == kNegInf || !(score[i] > -__builtin_huge_val()) ? 0ull : order_key(score[i]);
+        keys[e + group_of(p, e)] = row[e] == kNegInf || !(v > none) ? none : v;
     }
+    __syncwarp();
+    uint32_t kept = 0xFFFFFFFFu;
     if (p.groups > 1) {
-        const int size = p.n_experts / p.groups;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int e = i * 32 + lane;
-            if (e < p.n_experts) {
-                keys[e + e / size] = key[i] == 0ull ? -__builtin_huge_val() : score[i];
-            }
-        }
-        __syncwarp();
         double margin;
-        const uint32_t kept = choose_groups(p, static_cast<const double*>(keys), lane, &margin);
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int e = i * 32 + lane;
-            if (e < p.n_experts && !((kept >> (e / size)) & 1u)) {
-                key[i] = 0;
-            }
-        }
+        kept = choose_groups(p, static_cast<const double*>(keys), lane, &margin);
     }
-    return choose_experts<NV, false>(p, key, lane, nullptr);
+    int chosen = -1;
+    for (int j = 0; j < p.top_k; ++j) {
+        unsigned long long best = 0ull;
+        uint32_t at = 0xFFFFFFFFu;
+#pragma unroll 4
+        for (int e = lane; e < p.n_experts; e += 32) {
+            const int g = group_of(p, e);
+            const double v = keys[e + g];
+            const unsigned long long key =
+                v == none || (p.groups > 1 && !((kept >> (g & 31)) & 1u)) ? 0ull : order_key(v);
+            at = key > best ? static_cast<uint32_t>(e) : at;
+            best = key > best ? key : best;
+        }
+        const unsigned long long all = warp_max(best);
+        if (all == 0ull) {
+            break;
+        }
+        const uint32_t e = __reduce_min_sync(0xFFFFFFFFu, best == all ? at : 0xFFFFFFFFu);
+        if (lane == j) {
+            chosen = static_cast<int>(e);
+        }
+        if (static_cast<int>(e & 31u) == lane) {
+            keys[e + group_of(p, static_cast<int>(e))] = none;
+        }
+        __syncwarp();
+    }
+    return chosen;
 }
 
 }  // namespace detail
@@ -337,7 +347,7 @@ __device__ __noinline__ int choose_exact(const RouteParams& p, const float* row,
 // error, and 64-bit ones elsewhere (8192 tokens, 256 experts, 8 groups, bias: 34 us with 64-bit
 // keys for every token).
 template <typename T, int NV, bool kWide>
-__global__ void __launch_bounds__(32 * kRouteWarps) moe_route_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(32 * kRouteWarps, NV <= 8 ? 12 : 4) moe_route_kernel(const RouteParams p) {
     using Traits = detail::OutTraits<T>;
     extern __shared__ __align__(16) uint8_t route_smem[];
     ptx::grid_dependency_wait();
@@ -373,7 +383,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps) moe_route_kernel(const Route
             row.inv_sum = sum > 0.0f ? 1.0f / sum : 0.0f;
         }
     }
-    int chosen;  // lane j: the j-th choice
+    int chosen = -1;  // lane j: the j-th choice
     if constexpr (kWide) {
         double* keys = reinterpret_cast<double*>(route_smem + kRouteWarps * NV * 32 * 4) +
                        warp * (NV * 32 + kMaxRouteGroups);
@@ -666,10 +676,24 @@ __global__ void __launch_bounds__(kOrderThreads) group_rows_kernel(const GroupRo
         } else {
             fetch(from, bin);
         }
+        // Lanes with the same bin, from one ballot per bit of the bin (__match_any_sync took 100
+        // cycles a step with 32 different bins: 26 of this kernel's 35 thousand at 65536 slots).
         uint32_t same[kOrderSteps];
 #pragma unroll
         for (int i = 0; i < kOrderSteps; ++i) {
-            same[i] = __match_any_sync(0xFFFFFFFFu, bin[i]);
+            same[i] = 0xFFFFFFFFu;
+        }
+        for (int b = 0; (p.groups >> b) != 0; ++b) {
+#pragma unroll
+            for (int i = 0; i < kOrderSteps; ++i) {
+                const bool bit = (bin[i] >> b) & 1;
+                const uint32_t set = __ballot_sync(0xFFFFFFFFu, bit);
+                same[i] &= bit ? set : ~set;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kOrderSteps; ++i) {
+            same[i] &= __ballot_sync(0xFFFFFFFFu, bin[i] >= 0);  // lanes without a slot count nowhere
         }
 #pragma unroll
         for (int i = 0; i < kOrderSteps; ++i) {

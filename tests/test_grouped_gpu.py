@@ -527,3 +527,39 @@ def test_lora_pairs(ckl, trans, r):
             ref, mag = ref + t @ p2.double(), mag + ta @ p2.double().abs()
             extra = TWO_PART["f16"] * (t.abs() @ p2.double().abs()) + 2.0 ** -25 * r * p2.double().abs().max()
         check(out[sel], ref, mag, 2 * max(k, n) + 2 * r, "f32", extra)
+
+
+@pytest.mark.parametrize("r", [8, 24, 100])
+@pytest.mark.parametrize("dt,out", [("f16", "f32"), ("bf16", "bf16")])
+def test_lora_few_rows_ranks_and_gradients(ckl, r, dt, out):
+    """As above for odd ranks, an odd n, and the gradient of x, whose adapters are read the other way."""
+    m, g, k, n = 37, 9, 1032, 1041
+    gen = torch.Generator(device="cuda").manual_seed(r)
+    ids = torch.randint(-1, g, (m,), generator=gen, device="cuda", dtype=torch.int32)
+    ldn, ldr = (n + 7) // 8 * 8, (r + 7) // 8 * 8
+    x, dy = rand((m, k), DT[dt], 91), rand((m, ldn), DT[dt], 92)
+    w = rand((k, ldn), DT[dt], 93, k ** -0.5)
+    a, b = rand((g, k, ldr), DT[dt], 94, k ** -0.5), rand((g, r, ldn), DT[dt], 95, r ** -0.5)
+    s = 0.5 + torch.rand(g, device="cuda")
+    offs, rows, _ = plan(ckl, ids, g)
+    size = ckl.gemm_lora_workspace_bytes(m, r, True)
+    ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    y = torch.full((m, n), float("nan"), dtype=DT[out], device="cuda")
+    dx = torch.full((m, k), float("nan"), dtype=DT[out], device="cuda")
+    ld = dict(ldw=ldn, ldla=ldr, ldlb=ldn)
+    ckl.gemm_lora(code(ckl, dt), x, w, a, b, s, y, code(ckl, out), offs, rows, g, m, n, k, r, ws, size, **ld)
+    ckl.gemm_lora_backward(code(ckl, dt), dy, x, w, a, b, s, dx, code(ckl, out), None, None, ckl.F32, offs, rows, g, m, n,
+                           k, r, ws, size, lddy=ldn, **ld)
+    torch.cuda.synchronize()
+    tiny = 2.0 ** -25 if dt == "f16" else 0.0
+    for i in range(-1, g):
+        sel = ids == i
+        aa, bb = a[i, :, :r].double(), b[i, :, :n].double()
+        for v, ww, p1, p2, got in ((x[sel].double(), w[:, :n].double(), aa, bb, y[sel]),
+                                   (dy[sel][:, :n].double(), w[:, :n].double().t(), bb.t(), aa.t(), dx[sel])):
+            ref, mag, extra = v @ ww, v.abs() @ ww.abs(), 0.0
+            if i >= 0:
+                t, ta = s[i].double() * (v @ p1), s[i].double() * (v.abs() @ p1.abs())
+                ref, mag = ref + t @ p2, mag + ta @ p2.abs()
+                extra = TWO_PART[dt] * (t.abs() @ p2.abs()) + tiny * r * p2.abs().max()
+            check(got, ref, mag, 2 * max(k, n) + 2 * r + 10, out, extra)
