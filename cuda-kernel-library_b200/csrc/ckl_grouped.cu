@@ -67,10 +67,6 @@ int check_groups(const char* what, const int* offsets, int groups, int rows) {
     return CKL_OK;
 }
 
-struct Maps {
-    CUtensorMap a_box, b_box, e_box, c;
-};
-
 // A kernel that needs `bytes` of dynamic shared memory is told so once per device.
 template <auto kKernel>
 int allow_smem(int device, size_t bytes) {
@@ -87,32 +83,15 @@ int allow_smem(int device, size_t bytes) {
     return CKL_OK;
 }
 
-template <auto kKernel>
-int launch_kernel(int device, int threads, size_t smem, int cluster, const Maps& maps, const GroupedParams& p,
-                  int grid, cudaStream_t stream) {
+template <auto kKernel, typename Arg>
+int launch_kernel(int device, int threads, size_t smem, int cluster, const Arg& arg, dim3 grid,
+                  cudaStream_t stream) {
     GRP_TRY(allow_smem<kKernel>(device, smem));
-    GRP_TRY_CUDA(launch_dependent(kKernel, dim3(static_cast<unsigned>(grid)), threads, smem, cluster, stream,
-                                  maps.a_box, maps.b_box, maps.e_box, maps.c, p));
+    GRP_TRY_CUDA(launch_dependent(kKernel, grid, threads, smem, cluster, stream, arg));
     return CKL_OK;
 }
 
-template <typename OutT>
-int launch(bool pair, int device, const Maps& maps, const GroupedParams& p, int grid, cudaStream_t stream) {
-    if constexpr (!GroupedStore<OutT>::kTwo) {
-        if (pair) {
-            return launch_kernel<grouped_pair_kernel<OutT>>(device, GroupedPairConfig::kThreads,
-                                                            GroupedPairConfig::kSmemBytes, 2, maps, p, grid, stream);
-        }
-    }
-    if (p.split > 1) {
-        return launch_kernel<grouped_gemm_kernel<OutT, true>>(
-            device, GroupedConfig<true>::kThreads, GroupedConfig<true>::kSmemBytes, p.split, maps, p, grid, stream);
-    }
-    return launch_kernel<grouped_gemm_kernel<OutT, false>>(
-        device, GroupedConfig<false>::kThreads, GroupedConfig<false>::kSmemBytes, 1, maps, p, grid, stream);
-}
-
-// One product in terms of its operands; fills the descriptors and launches.
+// One product in terms of its operands.
 struct Product {
     int ab_dtype, c_dtype;  // c_dtype < 0: two-part C in the operand type
     GroupedParams p;
@@ -122,106 +101,226 @@ struct Product {
     int b_depth;
     long long b_stack, e_stack;
     int e_cols, e_outer;
+    // the plan
+    bool pair, whole;
+    long long tiles, blocks;
 };
 
-int run(Product& q, cudaStream_t stream) {
+long long row_tiles(const Product& q, int height) {
+    // An upper bound: the groups' sizes are known on the device only.
+    const GroupedParams& p = q.p;
+    return p.form == kFormWgrad ? static_cast<long long>(p.groups) * ((p.m + height - 1) / height)
+           : q.whole            ? (p.rows + height - 1) / height
+                                : p.rows / height + std::min(p.groups, p.rows);
+}
+long long single_tiles(const Product& q, int bn) { return row_tiles(q, 128) * ((q.p.n + bn - 1) / bn); }
+
+// Chooses the kernel and its tiles.
+void plan(Product& q, const DeviceView& view) {
     GroupedParams& p = q.p;
-    DeviceView view;
-    GRP_TRY(device_view(&view));
+    const bool wgrad = p.form == kFormWgrad;
     p.status = view.status;
     p.fmt = q.ab_dtype == CKL_BF16 ? 1u : 0u;
-    const bool wgrad = p.form == kFormWgrad;
-    // Upper bound of the row tiles: the groups' sizes are known on the device only.
-    const bool whole = !wgrad && (p.offsets == nullptr || p.ext_groups > 0);
-    const auto row_tiles = [&](int height) -> long long {
-        return wgrad   ? static_cast<long long>(p.groups) * ((p.m + height - 1) / height)
-               : whole ? (p.rows + height - 1) / height
-                       : p.rows / height + std::min(p.groups, p.rows);
-    };
+    q.whole = !wgrad && (p.offsets == nullptr || p.ext_groups > 0);
     // CTA pairs on 256 x 256 tiles where there are enough of them; operands in two parts and a
     // gathered G have only a few columns or rows of output and stay with the single-CTA kernel.
-    const long long pair_tiles = row_tiles(256) * ((p.n + 255) / 256);
-    const bool pair = q.c_dtype >= 0 && p.a_parts == 1 && p.b_parts == 1 && p.b_rows == nullptr && p.n > 128 &&
-                      (!wgrad || p.m > 128) && pair_tiles * 2 > view.max_pairs;
+    const long long pair_tiles = row_tiles(q, 256) * ((p.n + 255) / 256);
+    q.pair = q.c_dtype >= 0 && p.a_parts == 1 && p.b_parts == 1 && p.b_rows == nullptr && p.n > 128 &&
+             (!wgrad || p.m > 128) && pair_tiles * 2 > view.max_pairs;
     // Tile width of the single-CTA kernel: with enough tiles for every SM the wider one, which
     // reads A half as often, unless its last wave leaves more of the machine idle than the narrow
     // one's extra loads cost (a tenth).
-    const auto tiles_of = [&](int bn) { return row_tiles(128) * ((p.n + bn - 1) / bn); };
     const auto cost_of = [&](int bn) {  // waves x columns
-        return static_cast<double>((tiles_of(bn) + view.sm_count - 1) / view.sm_count) * bn;
+        return static_cast<double>((single_tiles(q, bn) + view.sm_count - 1) / view.sm_count) * bn;
     };
     p.bn = p.n > 128 && cost_of(256) <= 1.1 * cost_of(128) ? 256 : p.n > 64 ? 128 : 64;
-    long long tiles = pair ? pair_tiles : tiles_of(p.bn);
-    p.split = 1;
     // Blocks of 64 reduced elements behind one tile, as far as the host can tell.
-    const long long blocks = wgrad ? static_cast<long long>(p.rows / p.groups + 63) / 64 * p.a_parts * p.b_parts
-                                   : (p.k + 63) / 64;
-    if (!pair && tiles_of(std::min(p.bn, 128)) * 2 <= view.sm_count) {
-        // Fewer tiles than half of the SMs: a cluster divides the blocks of each.
-        p.bn = std::min(p.bn, 128);
-        tiles = tiles_of(p.bn);
-        while (p.split < kMaxSplit && tiles * p.split * 2 <= view.sm_count && blocks >= p.split * 2 * 4) {
-            p.split *= 2;
+    q.blocks = wgrad ? static_cast<long long>(p.rows / p.groups + 63) / 64 * p.a_parts * p.b_parts
+                     : (p.k + 63) / 64;
+    p.split = 1;
+    q.tiles = q.pair ? pair_tiles : single_tiles(q, p.bn);
+}
+
+// Fewer tiles than half of the SMs: a cluster divides the blocks of each, at least four per CTA.
+bool may_split(const Product& q, const DeviceView& view) {
+    return !q.pair && single_tiles(q, std::min(q.p.bn, 128)) * 2 <= view.sm_count;
+}
+
+// Clusters of `size` CTAs that are resident at once.  A cluster lives inside one GPC, so sizes that do
+// not divide a GPC's SMs well leave some unused (24 clusters of 6 ran as two waves: 17.5 us, 24 of
+// 4 in one: 10.7).
+int resident_clusters(int device, int size) {
+    static std::mutex mu;
+    static int known[64][kMaxSplit + 1] = {};
+    if (device < 0 || device >= 64) {
+        return 0;
+    }
+    std::lock_guard<std::mutex> lock(mu);
+    int& count = known[device][size];
+    if (count == 0) {
+        using Cfg = GroupedConfig<true>;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(size));
+        cfg.blockDim = dim3(Cfg::kThreads);
+        cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = static_cast<unsigned>(size);
+        attr.val.clusterDim.y = 1;
+        attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        if (allow_smem<grouped_gemm_kernel<float, true>>(device, Cfg::kSmemBytes) != CKL_OK ||
+            cudaOccupancyMaxActiveClusters(&count, grouped_gemm_kernel<float, true>, &cfg) != cudaSuccess) {
+            (void)cudaGetLastError();
+            count = 0;
+        }
+        count = std::max(count, 1);  // (no answer: this size is never chosen)
+    }
+    return count;
+}
+int choose_split(long long tiles, long long blocks, const DeviceView& view) {
+    for (int size = static_cast<int>(std::min<long long>(kMaxSplit, blocks / 4)); size > 1; --size) {
+        if (resident_clusters(view.device, size) >= tiles) {
+            return size;
         }
     }
-    if (tiles * std::max(p.split, 2) > 0x7fffffffll) {
-        return set_error(CKL_ERR_TOO_LARGE, "%lld output tiles", tiles);
-    }
-    if (tiles == 0) {
-        return CKL_OK;
+    return 1;
+}
+
+// Descriptors and remaining parameters of a planned product.
+int describe(Product& q, GroupedProblem* out) {
+    GroupedParams& p = q.p;
+    const bool wgrad = p.form == kFormWgrad;
+    if (q.tiles * std::max(p.split, 2) > 0x7fffffffll) {
+        return set_error(CKL_ERR_TOO_LARGE, "%lld output tiles", q.tiles);
     }
     // Few rows to a tile: the loaders fetch those alone, where a boxed copy would fetch 128.
     p.load_a = p.a_rows != nullptr ||
-               (!wgrad && !pair && p.k > 0 && !whole && p.rows <= 32ll * std::min(p.groups, p.rows));
+               (!wgrad && !q.pair && p.k > 0 && !q.whole && p.rows <= 32ll * std::min(p.groups, p.rows));
+    std::memset(out, 0, sizeof *out);
     // Gathered operands are read by the loader warps, all others through these descriptors.
-    Maps maps;
-    std::memset(&maps, 0, sizeof maps);
     if (p.load_a == 0) {
-        GRP_TRY(encode_operand(&maps.a_box, q.ab_dtype, q.a, q.a_cols, p.a_count, q.lda, 0, 0, 64,
-                               wgrad || pair ? 64 : 128));
+        GRP_TRY(encode_operand(&out->a_box, q.ab_dtype, q.a, q.a_cols, p.a_count, q.lda, 0, 0, 64,
+                               wgrad || q.pair ? 64 : 128));
     }
     if (!wgrad || p.b_rows == nullptr) {
-        GRP_TRY(encode_operand(&maps.b_box, q.ab_dtype, q.b, q.b_cols, wgrad ? p.b_count : q.b_outer, q.ldb,
+        GRP_TRY(encode_operand(&out->b_box, q.ab_dtype, q.b, q.b_cols, wgrad ? p.b_count : q.b_outer, q.ldb,
                                static_cast<uint64_t>(q.b_depth), static_cast<uint64_t>(q.b_stack), 64, 64));
     }
-    if (p.ext_groups > 0) {
-        GRP_TRY(encode_operand(&maps.e_box, q.ab_dtype, q.e, q.e_cols, q.e_outer, q.lde, p.ext_groups,
+    if (p.ext_groups > 0 && p.split == 1) {
+        GRP_TRY(encode_operand(&out->e_box, q.ab_dtype, q.e, q.e_cols, q.e_outer, q.lde, p.ext_groups,
                                static_cast<uint64_t>(q.e_stack), 64, 64));
     }
     p.a = q.a;
     p.b = q.b;
     p.t = q.t;
+    p.e = q.e;
     p.lda = q.lda;
     p.ldb = q.ldb;
     p.ldt = q.ldt;
-    p.e = q.e;
     p.lde = q.lde;
     p.e_stride = q.e_stack;
     unsigned long long limit_ns = 0;
     const int fault = take_wait_fault(&limit_ns);
     p.wait_limit_ns = limit_ns;
     p.overstate_first_stage = fault == 1 ? 1 : 0;
-    const int grid = static_cast<int>(pair          ? 2 * std::min<long long>(view.max_pairs, tiles)
-                                      : p.split > 1 ? tiles * p.split
-                                                    : std::min<long long>(view.sm_count, tiles));
-    if (q.c_dtype < 0) {
-        return q.ab_dtype == CKL_BF16 ? launch<TwoPart<__nv_bfloat16>>(false, view.device, maps, p, grid, stream)
-                                      : launch<TwoPart<__half>>(false, view.device, maps, p, grid, stream);
+    if (q.c_dtype >= 0) {
+        const int bytes = size_of(q.c_dtype);
+        p.c_vec = !misaligned(p.c, 16) && (static_cast<long long>(p.ldc) * bytes) % 16 == 0 &&
+                  (p.c_stride * bytes) % 16 == 0;
+        p.c_tma = p.c_vec && p.beta == 0.0f && p.c_rows == nullptr && p.split == 1;
+        if (p.c_tma) {
+            GRP_TRY(encode_operand(&out->c, q.c_dtype, p.c, p.n, wgrad ? p.m : p.rows, p.ldc, wgrad ? p.groups : 1,
+                                   wgrad ? p.c_stride : static_cast<long long>(p.ldc) * p.rows,
+                                   static_cast<uint32_t>(q.pair ? 32 : 64 / bytes), 32));
+        }
     }
-    const int bytes = size_of(q.c_dtype);
-    p.c_vec = !misaligned(p.c, 16) && (static_cast<long long>(p.ldc) * bytes) % 16 == 0 &&
-              (p.c_stride * bytes) % 16 == 0;
-    p.c_tma = p.c_vec && p.beta == 0.0f && p.c_rows == nullptr && p.split == 1;
-    if (p.c_tma) {
-        GRP_TRY(encode_operand(&maps.c, q.c_dtype, p.c, p.n, wgrad ? p.m : p.rows, p.ldc, wgrad ? p.groups : 1,
-                               wgrad ? p.c_stride : static_cast<long long>(p.ldc) * p.rows,
-                               static_cast<uint32_t>(pair ? 32 : 64 / bytes), 32));
+    out->p = p;
+    return CKL_OK;
+}
+
+template <typename OutT>
+int launch_single(const GroupedProblems& problems, int count, int tiles, const DeviceView& view,
+                  cudaStream_t stream) {
+    const int split = problems.at[0].p.split;
+    if (split > 1) {
+        return launch_kernel<grouped_gemm_kernel<OutT, true>>(
+            view.device, GroupedConfig<true>::kThreads, GroupedConfig<true>::kSmemBytes, split, problems,
+            dim3(static_cast<unsigned>(tiles * split), static_cast<unsigned>(count)), stream);
+    }
+    return launch_kernel<grouped_gemm_kernel<OutT, false>>(
+        view.device, GroupedConfig<false>::kThreads, GroupedConfig<false>::kSmemBytes, 1, problems,
+        dim3(static_cast<unsigned>(std::min(view.sm_count, tiles)), static_cast<unsigned>(count)), stream);
+}
+
+int launch_single(const Product& q, const GroupedProblems& problems, int count, long long tiles,
+                  const DeviceView& view, cudaStream_t stream) {
+    const int n = static_cast<int>(tiles);
+    if (q.c_dtype < 0) {
+        return q.ab_dtype == CKL_BF16 ? launch_single<TwoPart<__nv_bfloat16>>(problems, count, n, view, stream)
+                                      : launch_single<TwoPart<__half>>(problems, count, n, view, stream);
     }
     switch (q.c_dtype) {
-        case CKL_F16: return launch<__half>(pair, view.device, maps, p, grid, stream);
-        case CKL_BF16: return launch<__nv_bfloat16>(pair, view.device, maps, p, grid, stream);
-        default: return launch<float>(pair, view.device, maps, p, grid, stream);
+        case CKL_F16: return launch_single<__half>(problems, count, n, view, stream);
+        case CKL_BF16: return launch_single<__nv_bfloat16>(problems, count, n, view, stream);
+        default: return launch_single<float>(problems, count, n, view, stream);
     }
+}
+
+template <typename OutT>
+int launch_pair(const GroupedProblem& problem, long long tiles, const DeviceView& view, cudaStream_t stream) {
+    return launch_kernel<grouped_pair_kernel<OutT>>(
+        view.device, GroupedPairConfig::kThreads, GroupedPairConfig::kSmemBytes, 2, problem,
+        dim3(static_cast<unsigned>(2 * std::min<long long>(view.max_pairs, tiles))), stream);
+}
+
+int run(Product& q, cudaStream_t stream) {
+    DeviceView view;
+    GRP_TRY(device_view(&view));
+    plan(q, view);
+    if (may_split(q, view)) {
+        q.p.bn = std::min(q.p.bn, 128);
+        q.tiles = single_tiles(q, q.p.bn);
+        q.p.split = choose_split(q.tiles, q.blocks, view);
+    }
+    if (q.tiles == 0) {
+        return CKL_OK;
+    }
+    GroupedProblems problems;
+    GRP_TRY(describe(q, &problems.at[0]));
+    if (!q.pair) {
+        return launch_single(q, problems, 1, q.tiles, view, stream);
+    }
+    switch (q.c_dtype) {
+        case CKL_F16: return launch_pair<__half>(problems.at[0], q.tiles, view, stream);
+        case CKL_BF16: return launch_pair<__nv_bfloat16>(problems.at[0], q.tiles, view, stream);
+        default: return launch_pair<float>(problems.at[0], q.tiles, view, stream);
+    }
+}
+
+// Two products of the same output type that do not depend on each other: in one launch where both
+// are small, which spends a launch's fixed 5 us once and fills the SMs better.
+int run_two(Product& q, Product& r, cudaStream_t stream) {
+    DeviceView view;
+    GRP_TRY(device_view(&view));
+    plan(q, view);
+    plan(r, view);
+    if (!may_split(q, view) || !may_split(r, view) || q.tiles == 0 || r.tiles == 0) {
+        GRP_TRY(run(q, stream));
+        return run(r, stream);
+    }
+    long long tiles = 0;
+    for (Product* x : {&q, &r}) {
+        x->p.bn = std::min(x->p.bn, 128);
+        x->tiles = single_tiles(*x, x->p.bn);
+        tiles = std::max(tiles, x->tiles);
+    }
+    q.p.split = r.p.split = choose_split(q.tiles + r.tiles, std::min(q.blocks, r.blocks), view);
+    GroupedProblems problems;
+    GRP_TRY(describe(q, &problems.at[0]));
+    GRP_TRY(describe(r, &problems.at[1]));
+    return launch_single(q, problems, 2, tiles, view, stream);
 }
 
 Product blank(int ab_dtype, int c_dtype, int form) {
@@ -525,65 +624,68 @@ int ckl_gemm_lora_backward(int ab_dtype, const void* dy, const void* x, const vo
     void* u = workspace;
     void* t = static_cast<unsigned char*>(workspace) + two_part_bytes(m, rank);
     const int rp = padded_rank(rank);
-    if (m > 0 && (dx != nullptr || da != nullptr)) {
-        Product q = shrink(ab_dtype, dy, lddy, n, lora_b, ldlb, stride_b, true, rank, scales, u, offsets, rows,
-                           adapters, m);
-        GRP_TRY(run(q, s));
+    const bool need_u = m > 0 && (dx != nullptr || da != nullptr), need_t = m > 0 && db != nullptr;
+    Product pu = shrink(ab_dtype, dy, lddy, n, lora_b, ldlb, stride_b, true, rank, scales, u, offsets, rows,
+                        adapters, m);
+    Product pt = shrink(ab_dtype, x, ldx, k, lora_a, ldla, stride_a, false, rank, scales, t, offsets, rows,
+                        adapters, m);
+    if (need_u && need_t) {
+        GRP_TRY(run_two(pu, pt, s));
+    } else if (need_u) {
+        GRP_TRY(run(pu, s));
+    } else if (need_t) {
+        GRP_TRY(run(pt, s));
+    }
+    Product pa = blank(ab_dtype, dab_dtype, kFormWgrad);
+    pa.p.offsets = offsets;
+    pa.p.a_rows = rows;
+    pa.p.c = da;
+    pa.p.c_stride = stride_da;
+    pa.p.groups = adapters;
+    pa.p.rows = pa.p.a_count = pa.p.b_count = m;
+    pa.p.m = k;
+    pa.p.n = rank;
+    pa.p.ldc = ldda;
+    pa.p.beta = beta;
+    pa.p.b_parts = 2;
+    pa.p.b_part_cols = rp;
+    pa.a = x;
+    pa.lda = ldx;
+    pa.a_cols = k;
+    pa.b = u;
+    pa.ldb = pa.b_cols = 2 * rp;
+    pa.b_depth = 1;
+    pa.b_stack = static_cast<long long>(pa.ldb) * std::max(m, 1);
+    Product pb = blank(ab_dtype, dab_dtype, kFormWgrad);
+    pb.p.offsets = offsets;
+    pb.p.b_rows = rows;
+    pb.p.c = db;
+    pb.p.c_stride = stride_db;
+    pb.p.groups = adapters;
+    pb.p.rows = pb.p.a_count = pb.p.b_count = m;
+    pb.p.m = rank;
+    pb.p.n = n;
+    pb.p.ldc = lddb;
+    pb.p.beta = beta;
+    pb.p.a_parts = 2;
+    pb.p.a_part_cols = rp;
+    pb.a = t;
+    pb.lda = pb.a_cols = 2 * rp;
+    pb.b = dy;
+    pb.ldb = lddy;
+    pb.b_cols = n;
+    pb.b_depth = 1;
+    pb.b_stack = static_cast<long long>(lddy) * std::max(m, 1);
+    if (da != nullptr && db != nullptr) {
+        GRP_TRY(run_two(pa, pb, s));
+    } else if (da != nullptr) {
+        GRP_TRY(run(pa, s));
+    } else if (db != nullptr) {
+        GRP_TRY(run(pb, s));
     }
     if (m > 0 && dx != nullptr) {
         Product q = expand(ab_dtype, dx_dtype, dy, lddy, n, w, ldw, k, true, u, rank, lora_a, ldla, stride_a, dx,
                            lddx, offsets, rows, adapters, m, 0.0f);
-        GRP_TRY(run(q, s));
-    }
-    if (da != nullptr) {
-        Product q = blank(ab_dtype, dab_dtype, kFormWgrad);
-        q.p.offsets = offsets;
-        q.p.a_rows = rows;
-        q.p.c = da;
-        q.p.c_stride = stride_da;
-        q.p.groups = adapters;
-        q.p.rows = q.p.a_count = q.p.b_count = m;
-        q.p.m = k;
-        q.p.n = rank;
-        q.p.ldc = ldda;
-        q.p.beta = beta;
-        q.p.b_parts = 2;
-        q.p.b_part_cols = rp;
-        q.a = x;
-        q.lda = ldx;
-        q.a_cols = k;
-        q.b = u;
-        q.ldb = q.b_cols = 2 * rp;
-        q.b_depth = 1;
-        q.b_stack = static_cast<long long>(q.ldb) * std::max(m, 1);
-        GRP_TRY(run(q, s));
-    }
-    if (db != nullptr) {
-        if (m > 0) {
-            Product q = shrink(ab_dtype, x, ldx, k, lora_a, ldla, stride_a, false, rank, scales, t, offsets, rows,
-                               adapters, m);
-            GRP_TRY(run(q, s));
-        }
-        Product q = blank(ab_dtype, dab_dtype, kFormWgrad);
-        q.p.offsets = offsets;
-        q.p.b_rows = rows;
-        q.p.c = db;
-        q.p.c_stride = stride_db;
-        q.p.groups = adapters;
-        q.p.rows = q.p.a_count = q.p.b_count = m;
-        q.p.m = rank;
-        q.p.n = n;
-        q.p.ldc = lddb;
-        q.p.beta = beta;
-        q.p.a_parts = 2;
-        q.p.a_part_cols = rp;
-        q.a = t;
-        q.lda = q.a_cols = 2 * rp;
-        q.b = dy;
-        q.ldb = lddy;
-        q.b_cols = n;
-        q.b_depth = 1;
-        q.b_stack = static_cast<long long>(lddy) * std::max(m, 1);
         GRP_TRY(run(q, s));
     }
     return CKL_OK;

@@ -83,6 +83,17 @@ struct GroupedParams {
     int overstate_first_stage;  // test hook, see GemmParams
 };
 
+// One product: descriptors (operands that are boxed, C) and parameters.  A launch of the single-CTA
+// kernel runs one or two that do not depend on each other (blockIdx.y), as the two intermediates and
+// the two weight gradients of the adapters.
+struct GroupedProblem {
+    CUtensorMap a_box, b_box, e_box, c;
+    GroupedParams p;
+};
+struct GroupedProblems {
+    GroupedProblem at[2];
+};
+
 // kSplit: a cluster of CTAs shares one tile of at most 128 columns and divides its blocks; the
 // FP32 partial tiles meet in distributed shared memory.  For launches with fewer tiles than SMs.
 template <bool kSplit>
@@ -646,10 +657,11 @@ __device__ __forceinline__ int row_of_c(const GroupedParams& p, const GroupedTil
 
 template <typename OutT, bool kSplit>
 __global__ void __launch_bounds__(GroupedConfig<kSplit>::kThreads, 1)
-grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
-                    const __grid_constant__ CUtensorMap tmap_b_box,
-                    const __grid_constant__ CUtensorMap tmap_e_box,
-                    const __grid_constant__ CUtensorMap tmap_c, const GroupedParams p) {
+grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
+    const GroupedProblem& problem = problems.at[blockIdx.y];
+    const GroupedParams& p = problem.p;
+    const CUtensorMap &tmap_a_box = problem.a_box, &tmap_b_box = problem.b_box;
+    const CUtensorMap &tmap_e_box = problem.e_box, &tmap_c = problem.c;
     using Cfg = GroupedConfig<kSplit>;
     using Elem = typename GroupedStore<OutT>::Elem;
     constexpr bool kTwo = GroupedStore<OutT>::kTwo;
@@ -707,6 +719,11 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a_box,
         queue.init(6u + (loads ? kStages : 0u));  // producer, MMA, four epilogue warps, loaders
         *ctl.abort_flag = 0;
         ptx::fence_barrier_init();
+    }
+    if (threadIdx.x == 64) {
+        ptx::prefetch_tensormap(&tmap_a_box);
+        ptx::prefetch_tensormap(&tmap_b_box);
+        ptx::prefetch_tensormap(&tmap_c);
     }
     if (warp == 1) {
         ptx::tmem_alloc(tmem_slot, 512);
@@ -1375,7 +1392,7 @@ struct LoraRowsParams {
     long long a_stride;
     int adapters, m, k, rank, part_cols, ldx, lda;
 };
-constexpr int kLoraRowsThreads = 256;
+constexpr int kLoraRowsThreads = 1024;  // k 4096, rank 16: one batch of eight loads per thread
 constexpr int kLoraRanks = 32;
 
 template <typename T>

@@ -128,10 +128,10 @@ __device__ __forceinline__ uint32_t pack16(float factor, uint32_t a, uint32_t b)
 
 template <typename OutT>
 __global__ void __launch_bounds__(GroupedPairConfig::kThreads, 1)
-grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
-                    const __grid_constant__ CUtensorMap tmap_cols,
-                    const __grid_constant__ CUtensorMap tmap_ext,
-                    const __grid_constant__ CUtensorMap tmap_c, const GroupedParams p) {
+grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
+    const GroupedParams& p = problem.p;
+    const CUtensorMap &tmap_rows = problem.a_box, &tmap_cols = problem.b_box;
+    const CUtensorMap &tmap_ext = problem.e_box, &tmap_c = problem.c;
     using Cfg = GroupedPairConfig;
     using Elem = typename GroupedStore<OutT>::Elem;
     constexpr int kStages = Cfg::kStages;
@@ -191,6 +191,11 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_rows,
         queue.init(5u + (leader ? 1u : 0u) + (loads ? kStages : 0u));
         *ctl.abort_flag = 0;
         ptx::fence_barrier_init();
+    }
+    if (threadIdx.x == 64) {
+        ptx::prefetch_tensormap(&tmap_rows);
+        ptx::prefetch_tensormap(&tmap_cols);
+        ptx::prefetch_tensormap(&tmap_c);
     }
     if (warp == 1) {
         ptx::tmem_alloc_pair(tmem_slot, 512);
