@@ -28,15 +28,15 @@ bool aligned16(const void* p, long long pitch, int dtype) {
 bool misaligned(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % bytes != 0; }
 
 // Kernels that may need more than 48 KB of dynamic shared memory are told so once per device.
-template <typename F>
-int allow_smem(F* kernel, int bytes) {
+template <auto kKernel>
+int allow_smem(int bytes) {
     static std::mutex mu;
     static int granted[64] = {};
     int dev = 0;
     MOE_TRY_CUDA(cudaGetDevice(&dev));
     std::lock_guard<std::mutex> lock(mu);
     if (dev < 0 || dev >= 64 || granted[dev] < bytes) {
-        MOE_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        MOE_TRY_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
         if (dev >= 0 && dev < 64) {
             granted[dev] = bytes;
         }
@@ -46,12 +46,9 @@ int allow_smem(F* kernel, int bytes) {
 
 template <typename T, int NV, bool kWide>
 int launch_route(const RouteParams& p, cudaStream_t stream) {
-    int smem = kRouteWarps * NV * 32 * 4;
-    if (kWide) {
-        smem += kRouteWarps * (NV * 32 + kMaxRouteGroups) * 8;
-    }
+    const int smem = kRouteWarps * ((NV * 32 + kMaxRouteGroups) * 8 + NV * 32 * 4);
     if (smem > 48 * 1024) {
-        if (const int rc = allow_smem(moe_route_kernel<T, NV, kWide>, smem); rc != CKL_OK) {
+        if (const int rc = allow_smem<moe_route_kernel<T, NV, kWide>>(smem); rc != CKL_OK) {
             return rc;
         }
     }
@@ -315,7 +312,7 @@ int ckl_group_rows(const int* ids, int slots, int groups, int slots_per_row, int
     const int bins = groups + 1;
     const int smem = (kOrderWarps * bins + 2 * bins + kOrderWarps) * 4;
     const int most = (kOrderWarps * (kMaxExperts + 1) + 2 * (kMaxExperts + 1) + kOrderWarps) * 4;
-    if (const int rc = allow_smem(group_rows_kernel, most); rc != CKL_OK) {
+    if (const int rc = allow_smem<group_rows_kernel>(most); rc != CKL_OK) {
         return rc;
     }
     MOE_TRY_CUDA(launch_dependent(group_rows_kernel, dim3(static_cast<unsigned>(cluster)), kOrderThreads,

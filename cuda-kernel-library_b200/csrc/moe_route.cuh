@@ -44,9 +44,6 @@ __device__ __forceinline__ uint32_t order_key(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-__device__ __forceinline__ float key_value(uint32_t key) {  // back to the number
-    return __uint_as_float((key & 0x80000000u) ? key & 0x7FFFFFFFu : ~key);
-}
 __device__ __forceinline__ unsigned long long order_key(double x) {
     const unsigned long long u = static_cast<unsigned long long>(__double_as_longlong(x + 0.0));
     return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
@@ -105,83 +102,135 @@ __device__ __forceinline__ float chosen_share(float logit, bool some, bool sigmo
 
 namespace detail {
 
-// The experts a warp has to choose from: lane l holds experts l, l + 32, ...
-template <int NV>
-struct RouteRow {
-    float logit[NV];
-    float top;      // softmax: the row's maximum
-    float inv_sum;  // softmax: 1 / sum of exp(l - top), 0 for an empty row
-};
-
 // e / group size, exact for e < 2^20.
 __device__ __forceinline__ int group_of(const RouteParams& p, int e) {
     return __float2int_rz((static_cast<float>(e) + 0.5f) * p.inv_group_size);
 }
 
-// Which groups take part: bit g.  A group's score is the sum of its two best keys; `keys` is
-// shared memory (index e + e / size), read by a few neighbouring lanes per group.  `margin` gets
-// the distance of the last group kept to the best one left out (infinite if none competes).
-template <typename F>
-__device__ __forceinline__ uint32_t choose_groups(const RouteParams& p, const F* keys, int lane, F* margin) {
-    const F none = static_cast<F>(kNegInf);
+// Which groups take part: bit g.  A group's score is the sum of its two best keys; `keys` is shared
+// memory (index e + group of e, so that the lanes' scans start in different banks), read by a few
+// neighbouring lanes per group.
+__device__ __forceinline__ uint32_t choose_groups(const RouteParams& p, const double* keys, int lane) {
+    const double none = -__builtin_huge_val();
     const int size = p.group_size;
-    int per = 1;  // lanes per group, a power of two
-    while (per * 2 * p.groups <= 32) {
-        per *= 2;
+    int shift = 0;  // 2^shift lanes per group
+    while ((2 << shift) * p.groups <= 32) {
+        ++shift;
     }
-    const int g = lane / per;
-    F first = none, second = none;
+    const int per = 1 << shift;
+    const int g = lane >> shift;
+    double first = none, second = none;
     if (g < p.groups) {
-        for (int i = lane % per; i < size; i += per) {
-            const F v = keys[g * (size + 1) + i];
+        for (int i = lane & (per - 1); i < size; i += per) {
+            const double v = keys[g * (size + 1) + i];
             second = v > first ? first : (v > second ? v : second);
             first = v > first ? v : first;
         }
     }
     for (int d = 1; d < per; d <<= 1) {
-        const F f = __shfl_xor_sync(0xFFFFFFFFu, first, d);
-        const F s = __shfl_xor_sync(0xFFFFFFFFu, second, d);
-        const F lose = f > first ? first : f;
-        const F run = f > first ? s : second;
+        const double f = __shfl_xor_sync(0xFFFFFFFFu, first, d);
+        const double s = __shfl_xor_sync(0xFFFFFFFFu, second, d);
+        const double lose = f > first ? first : f;
+        const double run = f > first ? s : second;
         first = f > first ? f : first;
         second = lose > run ? lose : run;
     }
-    const bool mine_counts = g < p.groups && lane % per == 0 && first != none;
-    const F score = mine_counts ? first + (second == none ? static_cast<F>(0) : second) : none;
-    auto mine = mine_counts ? order_key(score) : decltype(order_key(score))(0);
+    unsigned long long mine = 0ull;
+    if (g < p.groups && (lane & (per - 1)) == 0 && first != none) {
+        mine = order_key(first + (second == none ? 0.0 : second));
+    }
     uint32_t kept = 0;
-    F last = none;
-    for (int r = 0; r <= p.top_groups; ++r) {
-        const auto best = warp_max(mine);
-        if (best == 0) {
-            *margin = static_cast<F>(-kNegInf);
-            return kept;
-        }
-        const int winner = __ffs(__ballot_sync(0xFFFFFFFFu, mine == best)) - 1;
-        const F at = __shfl_sync(0xFFFFFFFFu, score, winner);
-        if (r == p.top_groups) {
-            *margin = last - at;
+    for (int r = 0; r < p.top_groups; ++r) {
+        const unsigned long long best = warp_max(mine);
+        if (best == 0ull) {
             break;
         }
-        last = at;
-        kept |= 1u << (winner / per);
+        const int winner = __ffs(__ballot_sync(0xFFFFFFFFu, mine == best)) - 1;
+        kept |= 1u << (winner >> shift);
         if (lane == winner) {
-            mine = 0;
+            mine = 0ull;
         }
     }
     return kept;
 }
 
-// The top_k largest keys (0: never chosen), ties to the lowest index: lane j gets choice j, or
-// -1.  Each pick is one redux over the lanes' best keys and one over the tied lanes' indices.
-// kGaps: also the smallest distance between the keys of two successive places, down to the first
-// one left out (`value` gives a key's number back).
-template <int NV, bool kGaps, typename Key>
-__device__ __forceinline__ int choose_experts(const RouteParams& p, Key (&key)[NV], int lane, float* gap) {
+// Bitonic sort over the lanes of a warp, largest first, equal keys by index.
+__device__ __forceinline__ void sort_lanes(unsigned long long* key, uint32_t* index, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2) {
+#pragma unroll
+        for (int stride = size / 2; stride > 0; stride /= 2) {
+            const unsigned long long k = __shfl_xor_sync(0xFFFFFFFFu, *key, stride);
+            const uint32_t i = __shfl_xor_sync(0xFFFFFFFFu, *index, stride);
+            const bool mine_first = *key > k || (*key == k && *index < i);
+            const bool want_first = ((lane & stride) == 0) == ((lane & size) == 0);
+            if (mine_first != want_first) {
+                *key = k;
+                *index = i;
+            }
+        }
+    }
+}
+__device__ __forceinline__ uint32_t sort_lanes(uint32_t key, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2) {
+#pragma unroll
+        for (int stride = size / 2; stride > 0; stride /= 2) {
+            const uint32_t k = __shfl_xor_sync(0xFFFFFFFFu, key, stride);
+            const bool want_larger = ((lane & stride) == 0) == ((lane & size) == 0);
+            key = want_larger ? max(key, k) : min(key, k);
+        }
+    }
+    return key;
+}
+
+// The top_k largest keys (0: never chosen), ties to the lowest index: lane j gets choice j, or -1.
+// The top_k-th largest of the lanes' best keys (their upper words) bounds the answer from below; the
+// few keys that reach it are gathered, one per lane, and sorted.  `room` is shared memory for 32
+// keys and indices.  More than 32 such keys (large top_k, many equal upper words): one pick after
+// the other.
+template <int NV>
+__device__ __forceinline__ int choose_experts(const RouteParams& p, unsigned long long (&key)[NV],
+                                              unsigned long long* room, int lane) {
+    unsigned long long candidate;
+    uint32_t index;
+    int count;
+    if constexpr (NV == 1) {
+        candidate = key[0];
+        index = static_cast<uint32_t>(lane);
+        count = 32;
+    } else {
+        uint32_t best = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            best = max(best, static_cast<uint32_t>(key[i] >> 32));
+        }
+        const uint32_t bound = max(1u, __shfl_sync(0xFFFFFFFFu, sort_lanes(best, lane), p.top_k - 1));
+        uint32_t* room_index = reinterpret_cast<uint32_t*>(room + 32);
+        count = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const bool reaches = static_cast<uint32_t>(key[i] >> 32) >= bound;
+            const uint32_t which = __ballot_sync(0xFFFFFFFFu, reaches);
+            const int at = count + __popc(which & ((1u << lane) - 1u));
+            if (reaches && at < 32) {
+                room[at] = key[i];
+                room_index[at] = static_cast<uint32_t>(i * 32 + lane);
+            }
+            count += __popc(which);
+        }
+        __syncwarp();
+        candidate = lane < count ? room[lane] : 0ull;
+        index = lane < count ? room_index[lane] : 0xFFFFFFFFu;
+        __syncwarp();
+    }
+    if (count <= 32) {
+        sort_lanes(&candidate, &index, lane);
+        return lane < p.top_k && candidate != 0ull ? static_cast<int>(index) : -1;
+    }
     int chosen = -1;
-    float last = -kNegInf, smallest = -kNegInf;
-    for (int j = 0; j < p.top_k + (kGaps ? 1 : 0); ++j) {
-        Key best = 0;
+    for (int j = 0; j < p.top_k; ++j) {
+        unsigned long long best = 0ull;
         int at = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -190,164 +239,41 @@ __device__ __forceinline__ int choose_experts(const RouteParams& p, Key (&key)[N
                 at = i;
             }
         }
-        const Key all = warp_max(best);
-        if (all == 0) {
+        const unsigned long long all = warp_max(best);
+        if (all == 0ull) {
             break;
-        }
-        if constexpr (kGaps) {
-            const float v = key_value(all);
-            smallest = fminf(smallest, last - v);
-            last = v;
-            if (j == p.top_k) {
-                break;
-            }
         }
         const uint32_t e = __reduce_min_sync(
             0xFFFFFFFFu, best == all ? static_cast<uint32_t>(at * 32 + lane) : 0xFFFFFFFFu);
         if (lane == j) {
             chosen = static_cast<int>(e);
         }
-        if (static_cast<int>(e & 31u) == lane) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                if (i == static_cast<int>(e >> 5)) {
-                    key[i] = 0;
-                }
-            }
-        }
-    }
-    if constexpr (kGaps) {
-        *gap = smallest;
-    }
-    return chosen;
-}
-
-// Choice by score + bias inside the best groups, in FP32; false where rounding might decide.
-// Errors: with the fast exponential of x = -l or l - top, 2^(x log2 e), the product rounds to 2^-24
-// of itself and the power is off by 2^-22, so a score is off by s (|x| + 4) 2^-24 at most plus the
-// quotient's 2^-23 and (softmax) the sum's 1e-6: below 3e-6 in all, as s |x| < 0.4 for the
-// sigmoid's and the softmax's tails.  Adding the bias rounds to 2^-24 of the key.  Without a bias the choice inside the
-// groups is by the logits themselves, exactly.
-template <int NV>
-__device__ __forceinline__ bool choose_fast(const RouteParams& p, const RouteRow<NV>& row, float* keys, int lane,
-                                            int* chosen) {
-    float key[NV];
-    float largest = 1.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int e = i * 32 + lane;
-        const float l = row.logit[i];
-        float v = p.sigmoid ? __fdividef(1.0f, 1.0f + __expf(-l)) : __expf(l - row.top) * row.inv_sum;
-        v = l == kNegInf ? kNegInf : v;
-        if (p.bias != nullptr && e < p.n_experts) {
-            v += __ldg(p.bias + e);
-            v = v > kNegInf ? v : kNegInf;  // a bias of -inf or NaN takes its expert out
-        }
-        key[i] = v;
-        largest = v > kNegInf ? fmaxf(largest, fabsf(v)) : largest;
-    }
-    const float error = 3e-6f + 1.2e-7f * warp_maxf(largest);
-    uint32_t kept = 0xFFFFFFFFu;
-    if (p.groups > 1) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int e = i * 32 + lane;
-            if (e < p.n_experts) {
-                keys[e + group_of(p, e)] = key[i];
-            }
+            key[i] = static_cast<int>(e) == i * 32 + lane ? 0ull : key[i];
         }
-        __syncwarp();
-        float margin;
-        kept = choose_groups(p, keys, lane, &margin);
-        __syncwarp();
-        if (!(margin > 4.0f * error)) {
-            return false;
-        }
-    }
-    uint32_t order[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int e = i * 32 + lane;
-        const bool in = key[i] > kNegInf && (p.groups == 1 || ((kept >> (group_of(p, e) & 31)) & 1u));
-        order[i] = in ? order_key(p.bias != nullptr ? key[i] : row.logit[i]) : 0u;
-    }
-    if (p.bias == nullptr) {
-        *chosen = choose_experts<NV, false>(p, order, lane, nullptr);
-        return true;
-    }
-    float gap;
-    *chosen = choose_experts<NV, true>(p, order, lane, &gap);
-    return gap > 2.0f * error;
-}
-
-// The same choice with scores and sums in 64 bits, for the few tokens that need it (a launch ends
-// with its slowest warp: loops are rolled and keys live in shared memory, `keys`, so that this
-// takes few registers from every other token).
-template <int NV>
-__device__ __noinline__ int choose_exact(const RouteParams& p, const float* row, float top, double* keys, int lane) {
-    const double none = -__builtin_huge_val();
-    double sum = 0.0;
-    if (!p.sigmoid) {
-#pragma unroll 1
-        for (int e = lane; e < p.n_experts; e += 32) {
-            sum += row[e] == kNegInf ? 0.0 : exp(static_cast<double>(row[e]) - static_cast<double>(top));
-        }
-        sum = warp_sum(sum);
-    }
-#pragma unroll 1
-    for (int e = lane; e < p.n_experts; e += 32) {
-        const double l = static_cast<double>(row[e]);
-        double v = exp(p.sigmoid ? -l : l - static_cast<double>(top));
-        v = p.sigmoid ? 1.0 / (1.0 + v) : v / sum;
-        if (p.bias != nullptr) {
-            v += static_cast<double>(__ldg(p.bias + e));
-        }
-        keys[e + group_of(p, e)] = row[e] == kNegInf || !(v > none) ? none : v;
-    }
-    __syncwarp();
-    uint32_t kept = 0xFFFFFFFFu;
-    if (p.groups > 1) {
-        double margin;
-        kept = choose_groups(p, static_cast<const double*>(keys), lane, &margin);
-    }
-    int chosen = -1;
-    for (int j = 0; j < p.top_k; ++j) {
-        unsigned long long best = 0ull;
-        uint32_t at = 0xFFFFFFFFu;
-#pragma unroll 4
-        for (int e = lane; e < p.n_experts; e += 32) {
-            const int g = group_of(p, e);
-            const double v = keys[e + g];
-            const unsigned long long key =
-                v == none || (p.groups > 1 && !((kept >> (g & 31)) & 1u)) ? 0ull : order_key(v);
-            at = key > best ? static_cast<uint32_t>(e) : at;
-            best = key > best ? key : best;
-        }
-        const unsigned long long all = warp_max(best);
-        if (all == 0ull) {
-            break;
-        }
-        const uint32_t e = __reduce_min_sync(0xFFFFFFFFu, best == all ? at : 0xFFFFFFFFu);
-        if (lane == j) {
-            chosen = static_cast<int>(e);
-        }
-        if (static_cast<int>(e & 31u) == lane) {
-            keys[e + group_of(p, static_cast<int>(e))] = none;
-        }
-        __syncwarp();
     }
     return chosen;
+}
+
+// 1 / d to 64 bits for d in [1, 1e30]: the FP32 reciprocal and two Newton steps (2^-23, 2^-46, then
+// rounding).
+__device__ __forceinline__ double reciprocal(double d) {
+    double y = static_cast<double>(__frcp_rn(static_cast<float>(d)));
+    y = fma(y, fma(-d, y, 1.0), y);
+    return fma(y, fma(-d, y, 1.0), y);
 }
 
 }  // namespace detail
 
-// One warp per token.  Which experts are chosen is a whole-number answer, so rounding must not
-// decide it: without a bias and groups the logits themselves are compared (the scores are
-// monotone in them); with them (kWide) FP32 keys decide where their distance is beyond their
-// error, and 64-bit ones elsewhere (8192 tokens, 256 experts, 8 groups, bias: 34 us with 64-bit
-// keys for every token).
+// One warp per token; lane l holds experts l, l + 32, ...  Which experts are chosen is a whole-number
+// answer, so rounding must not decide it: without a bias and groups the logits themselves are
+// compared (the scores are monotone in them); with them (kWide) score + bias and the groups' sums
+// are formed in 64 bits, for every token: FP32 keys with an error bound and 64-bit ones where they
+// could not decide (27 of 8192 tokens) were slower, since those few warps fetched the rarely used
+// code while the launch waited for them (12 of 32 us).
 template <typename T, int NV, bool kWide>
-__global__ void __launch_bounds__(32 * kRouteWarps, NV <= 8 ? 12 : 4) moe_route_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(32 * kRouteWarps, NV <= 8 ? 10 : 4) moe_route_kernel(const RouteParams p) {
     using Traits = detail::OutTraits<T>;
     extern __shared__ __align__(16) uint8_t route_smem[];
     ptx::grid_dependency_wait();
@@ -358,56 +284,105 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NV <= 8 ? 12 : 4) moe_route_
     if (token >= p.tokens) {
         return;
     }
-    float* smem_row = reinterpret_cast<float*>(route_smem) + warp * (NV * 32);
+    // per warp: 64-bit keys by expert (room for 32 candidates at least), then the row
+    constexpr int kKeys = NV * 32 + kMaxRouteGroups;
+    double* keys = reinterpret_cast<double*>(route_smem) + warp * kKeys;
+    float* row = reinterpret_cast<float*>(route_smem + kRouteWarps * kKeys * 8) + warp * (NV * 32);
     const T* src = static_cast<const T*>(p.logits) + static_cast<size_t>(token) * p.ldl;
 
-    detail::RouteRow<NV> row;
-    row.top = detail::kNegInf;
-    row.inv_sum = 0.0f;
+    float logit[NV];
+    float top = detail::kNegInf;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int e = i * 32 + lane;
-        row.logit[i] = e < p.n_experts ? detail::clean_logit(Traits::load(src + e)) : detail::kNegInf;
-        row.top = fmaxf(row.top, row.logit[i]);
-        smem_row[e] = row.logit[i];
+        logit[i] = e < p.n_experts ? detail::clean_logit(Traits::load(src + e)) : detail::kNegInf;
+        top = fmaxf(top, logit[i]);
+        row[e] = logit[i];
     }
+    float inv_sum = 0.0f;
     if (!p.sigmoid) {
-        row.top = detail::warp_maxf(row.top);
-        if (kWide || !p.renormalise) {
+        top = detail::warp_maxf(top);
+        if (!kWide && !p.renormalise) {
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                sum += row.logit[i] == detail::kNegInf ? 0.0f : expf(row.logit[i] - row.top);
+                sum += logit[i] == detail::kNegInf ? 0.0f : expf(logit[i] - top);
             }
             sum = detail::warp_sum(sum);
-            row.inv_sum = sum > 0.0f ? 1.0f / sum : 0.0f;
+            inv_sum = sum > 0.0f ? 1.0f / sum : 0.0f;
         }
     }
-    int chosen = -1;  // lane j: the j-th choice
+    unsigned long long key[NV];
     if constexpr (kWide) {
-        double* keys = reinterpret_cast<double*>(route_smem + kRouteWarps * NV * 32 * 4) +
-                       warp * (NV * 32 + kMaxRouteGroups);
-        if (!detail::choose_fast<NV>(p, row, reinterpret_cast<float*>(keys), lane, &chosen)) {
-            chosen = detail::choose_exact<NV>(p, smem_row, row.top, keys, lane);
-        }
-    } else {
-        uint32_t key[NV];
+        const double none = -__builtin_huge_val();
+        double score[NV];
+        double sum = 0.0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            key[i] = row.logit[i] == detail::kNegInf ? 0u : detail::order_key(row.logit[i]);
+            const double l = static_cast<double>(logit[i]);
+            const double x = exp(p.sigmoid ? -l : l - static_cast<double>(top));
+            if (p.sigmoid) {
+                const double d = 1.0 + x;
+                score[i] = d < 1e30 ? detail::reciprocal(d) : 1.0 / d;
+            } else {
+                score[i] = logit[i] == detail::kNegInf ? 0.0 : x;
+                sum += score[i];
+            }
         }
-        chosen = detail::choose_experts<NV, false>(p, key, lane, nullptr);
+        if (!p.sigmoid) {
+            sum = detail::warp_sum(sum);
+            const double inv = sum > 0.0 ? 1.0 / sum : 0.0;
+            inv_sum = static_cast<float>(inv);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                score[i] *= inv;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = i * 32 + lane;
+            if (p.bias != nullptr && e < p.n_experts) {
+                score[i] += static_cast<double>(__ldg(p.bias + e));
+            }
+            // (a bias of -inf or NaN takes its expert out of the choice)
+            const bool may = logit[i] != detail::kNegInf && score[i] > none;
+            key[i] = may ? detail::order_key(score[i]) : 0ull;
+            if (p.groups > 1 && e < p.n_experts) {
+                keys[e + detail::group_of(p, e)] = may ? score[i] : none;
+            }
+        }
+        if (p.groups > 1) {
+            __syncwarp();
+            const uint32_t kept = detail::choose_groups(p, keys, lane);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int e = i * 32 + lane;
+                if (e < p.n_experts && !((kept >> detail::group_of(p, e)) & 1u)) {
+                    key[i] = 0ull;
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            key[i] = logit[i] == detail::kNegInf
+                         ? 0ull
+                         : static_cast<unsigned long long>(detail::order_key(logit[i])) << 32;
+        }
     }
+    const int chosen =
+        detail::choose_experts<NV>(p, key, reinterpret_cast<unsigned long long*>(keys), lane);  // lane j: choice j
     __syncwarp();
     const bool some = chosen >= 0;
-    const float l = some ? smem_row[chosen] : detail::kNegInf;
+    const float l = some ? row[chosen] : detail::kNegInf;
     float w;
     if (p.renormalise) {
         w = detail::chosen_share(l, some, p.sigmoid != 0);
     } else if (p.sigmoid) {
         w = some ? detail::sigmoidf(l) : 0.0f;
     } else {
-        w = some ? expf(l - row.top) * row.inv_sum : 0.0f;
+        w = some ? expf(l - top) * inv_sum : 0.0f;
     }
     if (lane < p.top_k) {
         const size_t at = static_cast<size_t>(token) * p.top_k + lane;
