@@ -308,11 +308,15 @@ int ckl_group_rows(const int* ids, int slots, int groups, int slots_per_row, int
     p.slots = slots;
     p.groups = groups;
     p.slots_per_row = slots_per_row;
+    p.inv_row = slots_per_row < 512 ? (1ull << 40) / static_cast<unsigned long long>(slots_per_row) + 1 : 0;
     p.warp_slots = static_cast<int>(((slots + warps - 1) / warps + 31) / 32 * 32);
-    const int bins = groups + 1;
-    const int smem = (kOrderWarps * bins + 2 * bins + kOrderWarps) * 4;
-    const int most = (kOrderWarps * (kMaxExperts + 1) + 2 * (kMaxExperts + 1) + kOrderWarps) * 4;
-    if (const int rc = allow_smem<group_rows_kernel>(most); rc != CKL_OK) {
+    const auto smem_of = [](int bins, int staged_slots) {
+        return (kOrderWarps * bins + 2 * bins + kOrderWarps + (bins + 1) / 2 * 2 + 2) * 4 + staged_slots * 8;
+    };
+    const int cta_slots = p.warp_slots * kOrderWarps;
+    p.staged = slots > kOrderThreads && cta_slots <= kOrderStaged ? 1 : 0;
+    const int smem = smem_of(groups + 1, p.staged ? cta_slots : 0);
+    if (const int rc = allow_smem<group_rows_kernel>(smem_of(kMaxExperts + 1, kOrderStaged)); rc != CKL_OK) {
         return rc;
     }
     MOE_TRY_CUDA(launch_dependent(group_rows_kernel, dim3(static_cast<unsigned>(cluster)), kOrderThreads,

@@ -494,6 +494,7 @@ moe_route_backward_kernel(const RouteBackwardParams p) {
 constexpr int kOrderThreads = 1024;
 constexpr int kOrderWarps = kOrderThreads / 32;
 constexpr int kMaxOrderCluster = 8;
+constexpr int kOrderStaged = kOrderThreads * 8;  // slots of a CTA that are sorted in shared memory
 constexpr int kOrderSteps = 8;  // of 32 slots that a warp holds in registers
 
 struct GroupRowsParams {
@@ -502,6 +503,8 @@ struct GroupRowsParams {
     int* rows;
     int* positions;
     int slots, groups, slots_per_row;
+    unsigned long long inv_row;  // floor(2^40 / slots_per_row) + 1, or 0: divide
+    int staged;      // a CTA's slots fit in shared memory, sorted
     int warp_slots;  // consecutive slots of one warp, a multiple of 32
 };
 
@@ -518,6 +521,8 @@ __global__ void __launch_bounds__(kOrderThreads) group_rows_kernel(const GroupRo
     int* total = hist + kOrderWarps * bins;       // [bin] of this CTA, read by the cluster
     int* start = total + bins;                    // [bin]
     int* warp_sums = start + bins;                // [32]
+    int* local = warp_sums + kOrderWarps;         // [bin] first place in `sorted`
+    int2* sorted = reinterpret_cast<int2*>(local + (bins + 1) / 2 * 2);  // (position, row), p.staged
     const int tid = static_cast<int>(threadIdx.x);
     const int warp = tid >> 5, lane = tid & 31;
     uint32_t rank, size;
@@ -617,6 +622,37 @@ __global__ void __launch_bounds__(kOrderThreads) group_rows_kernel(const GroupRo
     __syncthreads();
     const int base = scan - all + (warp > 0 ? warp_sums[warp - 1] : 0);
     const int kept = warp_sums[kOrderWarps - 1];
+    if (p.staged) {
+        // The same scan over this CTA's own counts: where its slots of a bin lie in `sorted`.
+        __syncthreads();
+        const int own = tid < p.groups ? total[tid] : 0;
+        int v = own;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
+            v += lane >= d ? u : 0;
+        }
+        if (lane == 31) {
+            warp_sums[warp] = v;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            int w = warp_sums[lane];
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int u = __shfl_up_sync(0xFFFFFFFFu, w, d);
+                w += lane >= d ? u : 0;
+            }
+            warp_sums[lane] = w;
+        }
+        __syncthreads();
+        if (tid < p.groups) {
+            local[tid] = v - own + (warp > 0 ? warp_sums[warp - 1] : 0);
+        }
+        if (tid == 0) {
+            local[p.groups] = warp_sums[kOrderWarps - 1];
+        }
+    }
     if (tid < p.groups) {
         start[tid] = base + before;
         if (rank == 0) {
@@ -674,15 +710,34 @@ __global__ void __launch_bounds__(kOrderThreads) group_rows_kernel(const GroupRo
         for (int i = 0; i < kOrderSteps; ++i) {
             const int s = from + i * 32 + lane;
             if (bin[i] >= 0) {
-                const int pos = start[bin[i]] + mine[bin[i]] + __popc(same[i] & ((1u << lane) - 1u));
+                const int in_bin = mine[bin[i]] + __popc(same[i] & ((1u << lane) - 1u));
+                const int pos = start[bin[i]] + in_bin;
                 p.positions[s] = pos;
-                p.rows[pos] = s / p.slots_per_row;
+                // s / slots_per_row, exact for slots_per_row < 512 as s < 2^31
+                const int row = p.inv_row != 0 ? static_cast<int>(s * p.inv_row >> 40) : s / p.slots_per_row;
+                if (p.staged) {
+                    sorted[local[bin[i]] + in_bin] = make_int2(pos, row);
+                } else {
+                    p.rows[pos] = row;
+                }
             }
             __syncwarp();
             if (bin[i] >= 0 && lane == __ffs(same[i]) - 1) {
                 mine[bin[i]] += __popc(same[i]);
             }
             __syncwarp();
+        }
+    }
+    if (p.staged) {
+        // Neighbours in `sorted` are neighbours in `rows` up to the end of a bin: the stores are runs
+        // instead of 32 places per instruction.
+        __syncthreads();
+        const long long cta_first = static_cast<long long>(rank) * kOrderWarps * p.warp_slots;
+        const int count = static_cast<int>(max(0ll, min(static_cast<long long>(kOrderWarps) * p.warp_slots,
+                                                        static_cast<long long>(p.slots) - cta_first)));
+        for (int i = tid; i < count; i += kOrderThreads) {
+            const int2 v = sorted[i];
+            p.rows[v.x] = v.y;
         }
     }
 }
