@@ -111,7 +111,7 @@ long long row_tiles(const Product& q, int height) {
     const GroupedParams& p = q.p;
     return p.form == kFormWgrad ? static_cast<long long>(p.groups) * ((p.m + height - 1) / height)
            : q.whole            ? (p.rows + height - 1) / height
-                                : p.rows / height + std::min(p.groups, p.rows);
+                                : p.rows / height + std::min(p.groups + (p.ext_mode == kExtBlocks ? 1 : 0), p.rows);
 }
 long long single_tiles(const Product& q, int bn) { return row_tiles(q, 128) * ((q.p.n + bn - 1) / bn); }
 
@@ -121,7 +121,7 @@ void plan(Product& q, const DeviceView& view) {
     const bool wgrad = p.form == kFormWgrad;
     p.status = view.status;
     p.fmt = q.ab_dtype == CKL_BF16 ? 1u : 0u;
-    q.whole = !wgrad && (p.offsets == nullptr || p.ext_groups > 0);
+    q.whole = !wgrad && (p.offsets == nullptr || p.ext_mode == kExtAdd);
     // CTA pairs on 256 x 256 tiles where there are enough of them; operands in two parts and a
     // gathered G have only a few columns or rows of output and stay with the single-CTA kernel.
     const long long pair_tiles = row_tiles(q, 256) * ((p.n + 255) / 256);
@@ -197,7 +197,7 @@ int describe(Product& q, GroupedProblem* out) {
     }
     // Few rows to a tile: the loaders fetch those alone, where a boxed copy would fetch 128.
     p.load_a = p.a_rows != nullptr ||
-               (!wgrad && !q.pair && p.k > 0 && !q.whole && p.rows <= 32ll * std::min(p.groups, p.rows));
+               (!wgrad && !q.pair && p.k > 0 && p.ext_mode == kExtNone && !q.whole && p.rows <= 32ll * std::min(p.groups, p.rows));
     std::memset(out, 0, sizeof *out);
     // Gathered operands are read by the loader warps, all others through these descriptors.
     if (p.load_a == 0) {
@@ -208,8 +208,8 @@ int describe(Product& q, GroupedProblem* out) {
         GRP_TRY(encode_operand(&out->b_box, q.ab_dtype, q.b, q.b_cols, wgrad ? p.b_count : q.b_outer, q.ldb,
                                static_cast<uint64_t>(q.b_depth), static_cast<uint64_t>(q.b_stack), 64, 64));
     }
-    if (p.ext_groups > 0 && p.split == 1) {
-        GRP_TRY(encode_operand(&out->e_box, q.ab_dtype, q.e, q.e_cols, q.e_outer, q.lde, p.ext_groups,
+    if (p.ext_mode == kExtBlocks) {
+        GRP_TRY(encode_operand(&out->e_box, q.ab_dtype, q.e, q.e_cols, q.e_outer, q.lde, p.groups,
                                static_cast<uint64_t>(q.e_stack), 64, 64));
     }
     p.a = q.a;
@@ -229,7 +229,7 @@ int describe(Product& q, GroupedProblem* out) {
         const int bytes = size_of(q.c_dtype);
         p.c_vec = !misaligned(p.c, 16) && (static_cast<long long>(p.ldc) * bytes) % 16 == 0 &&
                   (p.c_stride * bytes) % 16 == 0;
-        p.c_tma = p.c_vec && p.beta == 0.0f && p.c_rows == nullptr && p.split == 1;
+        p.c_tma = p.c_vec && p.beta == 0.0f && p.c_rows == nullptr && p.split == 1 && p.ext_mode != kExtAdd;
         if (p.c_tma) {
             GRP_TRY(encode_operand(&out->c, q.c_dtype, p.c, p.n, wgrad ? p.m : p.rows, p.ldc, wgrad ? p.groups : 1,
                                    wgrad ? p.c_stride : static_cast<long long>(p.ldc) * p.rows,
@@ -280,6 +280,11 @@ int run(Product& q, cudaStream_t stream) {
     GRP_TRY(device_view(&view));
     plan(q, view);
     if (may_split(q, view)) {
+        if (q.p.ext_mode == kExtBlocks) {
+            // (the parts of a split tile meet row by row: adapters are added there)
+            q.p.ext_mode = kExtAdd;
+            plan(q, view);
+        }
         q.p.bn = std::min(q.p.bn, 128);
         q.tiles = single_tiles(q, q.p.bn);
         q.p.split = choose_split(q.tiles, q.blocks, view);
@@ -333,6 +338,9 @@ Product blank(int ab_dtype, int c_dtype, int form) {
     q.p.a_parts = q.p.b_parts = 1;
     return q;
 }
+
+// Rows per adapter from which tiles end with them.
+constexpr int kExtRows = 64;
 
 int padded_rank(int rank) { return (rank + 15) / 16 * 16; }
 size_t two_part_bytes(int m, int rank) {
@@ -404,7 +412,10 @@ Product expand(int ab_dtype, int c_dtype, const void* a, int lda, int k, const v
     q.p.offsets = offsets;
     q.p.a_rows = q.p.c_rows = rows;
     q.p.c = c;
-    q.p.groups = q.p.ext_groups = adapters;
+    q.p.groups = adapters;
+    // Tiles that end with their adapter cost half a tile's time per adapter, one product per row and
+    // rank on the CUDA cores about as much as a tile's epilogue from rank 32 on.
+    q.p.ext_mode = m >= kExtRows * adapters ? kExtBlocks : kExtAdd;
     q.p.ext_cols = rp;
     q.p.ext_rank = rank;
     q.p.rows = q.p.a_count = q.p.c_count = m;

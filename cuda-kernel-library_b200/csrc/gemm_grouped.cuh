@@ -7,17 +7,22 @@
 //   kFormWgrad  W_g = alpha * sum over p in g of A[row(p)]^T G[row(p)]: the ragged dimension is
 //               the one that is summed; tiles of 128 x bn of each W_g.
 //
-// Either form may be "extended" (kFormRows only): all positions form one group for a shared B,
-// and behind the k blocks of that product a tile runs, for each adapter g whose rows it holds,
-// the k blocks of T[p] * op(E_g) into the same accumulator, with the rows of other adapters
-// read as zeros.  Low-rank adapters thereby cost neither a second pass over C nor tiles cut at
-// the borders of requests.
+// kFormRows may be "extended": one B for all groups (a shared projection), and for the rows of adapter
+// g (groups and adapters are then the same thing; rows behind the last belong to none) T[p] * op(E_g)
+// besides.  Two ways, chosen by how many rows an adapter has:
+//   kExtBlocks  tiles end with the adapters, as with any other groups, and behind the k blocks of the
+//               product a tile runs those of its adapter's T and E_g into the same accumulator;
+//   kExtAdd     tiles are cut from all rows alike, and the few products a row needs are added in FP32
+//               on the CUDA cores while the tile is stored.
+// (Running every adapter's blocks over a tile that several share, the rows of the others read as
+// zeros, would cost less than kExtAdd at high ranks, but zero times an infinity or NaN in one
+// request's adapter is NaN in another's rows.)
 //
 // Consecutive rows arrive by boxed TMA copies.  Gathered rows arrive by cp.async from four loader
 // warps that write the same swizzled layout: TMA's own row gather (tile::gather4) took about 100
 // cycles per four rows, 3300 per 128 x 64 stage against the 512 the stage's MMAs need (4096^3:
-// 355 TFLOP/s gathered, 1113 boxed).  The loaders also write the zeros that masked rows need:
-// rows of other adapters, and in a weight gradient the positions behind the end of a group.
+// 355 TFLOP/s gathered, 1113 boxed).  The loaders also write the zeros that a weight gradient needs
+// behind the end of a group.
 //
 // Operand layout in shared memory is that of the dense kernel (gemm_umma.cuh): 128-byte rows of
 // 64 elements under the 128-byte swizzle.  The matrix whose reduced dimension is contiguous in
@@ -35,6 +40,7 @@ constexpr int kMaxGemmGroups = 1024;
 constexpr int kMaxLoraRank = 128;
 
 enum GroupedForm : int { kFormRows = 0, kFormWgrad = 1 };
+enum ExtMode : int { kExtNone = 0, kExtBlocks = 1, kExtAdd = 2 };
 
 // Element type of C, or the two-part form: an FP32 value v stored as 16-bit hi = round(v) and
 // lo = round(v - hi), lo `part` columns behind hi.  Holds 16 (BF16) or 22 (FP16) bits of v, so an
@@ -68,8 +74,9 @@ struct GroupedParams {
     int a_parts, a_part_cols;
     int b_parts, b_part_cols;
     int c_part_cols;     // TwoPart output: distance of lo behind hi
-    // Extension (ext_groups > 0): offsets/groups describe the adapters.
-    int ext_groups, ext_cols;  // adapters; columns of one part of T (a multiple of 16)
+    // Extension: offsets/groups describe the adapters.
+    int ext_mode;              // ExtMode
+    int ext_cols;              // columns of one part of T (a multiple of 16)
     const void* e;             // E, `ext_rank` x n per adapter (n x ext_rank with trans_b)
     int ext_rank, lde;
     long long e_stride;
@@ -124,7 +131,7 @@ struct GroupedTile {
     int m0, n0;     // kFormWgrad: first row of W_g; first column
     int cols;       // columns of the tile that exist
     int k_blocks;   // 64-wide blocks of the main product
-    int ext_first, ext_last;  // adapters [first, last) that may have rows in the tile
+    int adapter;    // whose blocks the tile runs besides (kExtBlocks), -1: none
     int begin, end;  // this CTA's share of the tile's blocks (main product, then adapters)
 };
 
@@ -159,6 +166,9 @@ __device__ __forceinline__ GroupedTable make_table(const GroupedParams& p, int* 
         for (int g = static_cast<int>(threadIdx.x); g <= p.groups; g += threads) {
             offs[g] = min(max(p.offsets[g], 0), p.rows);
         }
+        if (threadIdx.x == 0) {
+            offs[p.groups + 1] = p.rows;  // kExtBlocks: rows of no adapter are a last segment
+        }
     } else if (threadIdx.x == 0) {
         offs[0] = 0;
         offs[1] = p.rows;
@@ -167,8 +177,8 @@ __device__ __forceinline__ GroupedTable make_table(const GroupedParams& p, int* 
     GroupedTable t;
     t.offs = offs;
     t.tiles = tiles;
-    t.whole = p.offsets == nullptr || p.ext_groups > 0;
-    t.segments = t.whole ? 1 : p.groups;
+    t.whole = p.offsets == nullptr || p.ext_mode == kExtAdd;
+    t.segments = t.whole ? 1 : p.groups + (p.ext_mode == kExtBlocks ? 1 : 0);
     t.n_tiles = (p.n + tile_cols - 1) / tile_cols;
     t.m_tiles = (p.m + tile_rows - 1) / tile_rows;
     if (warp == 0) {
@@ -179,23 +189,23 @@ __device__ __forceinline__ GroupedTable make_table(const GroupedParams& p, int* 
             }
         } else {
             int run = 0;
-            for (int g0 = 0; g0 < p.groups; g0 += 32) {
+            for (int g0 = 0; g0 < t.segments; g0 += 32) {
                 const int g = g0 + static_cast<int>(lane);
                 const int count =
-                    g < p.groups ? (max(0, offs[g + 1] - offs[g]) + tile_rows - 1) / tile_rows : 0;
+                    g < t.segments ? (max(0, offs[g + 1] - offs[g]) + tile_rows - 1) / tile_rows : 0;
                 int v = count;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
                     const int u = __shfl_up_sync(0xFFFFFFFFu, v, d);
                     v += static_cast<int>(lane) >= d ? u : 0;
                 }
-                if (g < p.groups) {
+                if (g < t.segments) {
                     tiles[g] = run + v - count;
                 }
                 run += __shfl_sync(0xFFFFFFFFu, v, 31);
             }
             if (lane == 0) {
-                tiles[p.groups] = run;
+                tiles[t.segments] = run;
             }
         }
     }
@@ -207,7 +217,7 @@ __device__ __forceinline__ int total_tiles(const GroupedParams& p, const Grouped
 }
 
 __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, const GroupedTable& t,
-                                                    int tile, bool split) {
+                                                    int tile) {
     GroupedTile o;
     int mt, nt;
     int m_tiles, local;
@@ -230,7 +240,7 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, cons
     mt = band * kBand + in_band - nt * height;
     o.n0 = nt * p.bn;
     o.cols = min(p.bn, p.n - o.n0);
-    o.ext_first = o.ext_last = 0;
+    o.adapter = p.ext_mode == kExtBlocks && o.group < p.groups ? o.group : -1;
     if (p.form == kFormWgrad) {
         o.p0 = t.offs[o.group];
         o.valid = max(0, t.offs[o.group + 1] - o.p0);
@@ -243,11 +253,6 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, cons
         o.valid = min(128, seg1 - o.p0);
         o.m0 = 0;
         o.k_blocks = (p.k + 63) / 64;
-        if (!split && p.ext_groups > 0 && o.p0 < t.offs[p.ext_groups]) {
-            // first adapter that ends behind p0, and the one after the last that starts in here
-            o.ext_first = last_at_most(t.offs, p.ext_groups, o.p0);
-            o.ext_last = last_at_most(t.offs, p.ext_groups, o.p0 + o.valid - 1) + 1;
-        }
     }
     return o;
 }
@@ -319,22 +324,9 @@ struct TileQueue {
     }
 };
 
-// Positions [lo, hi) of tile t that belong to adapter g.
-struct Span {
-    int lo, hi;
-};
-__device__ __forceinline__ Span adapter_span(const GroupedTable& table, const GroupedTile& t, int g) {
-    return {max(table.offs[g], t.p0), min(table.offs[g + 1], t.p0 + t.valid)};
-}
-
 // Fills in the share of a tile's blocks that CTA `rank` of `size` runs.
-__device__ __forceinline__ void take_share(const GroupedParams& p, const GroupedTable& table, GroupedTile* t,
-                                           int rank, int size) {
-    int blocks = t->k_blocks;
-    for (int g = t->ext_first; g < t->ext_last; ++g) {
-        const Span s = adapter_span(table, *t, g);
-        blocks += s.lo < s.hi ? 2 * ((p.ext_cols + 63) / 64) : 0;
-    }
+__device__ __forceinline__ void take_share(const GroupedParams& p, GroupedTile* t, int rank, int size) {
+    const int blocks = t->k_blocks + (t->adapter >= 0 ? 2 * ((p.ext_cols + 63) / 64) : 0);
     t->begin = static_cast<int>(static_cast<long long>(blocks) * rank / size);
     t->end = static_cast<int>(static_cast<long long>(blocks) * (rank + 1) / size);
 }
@@ -476,10 +468,10 @@ struct Loader {
         }
     }
 
-    // Columns [k0, k0 + 64) of one part of T behind positions pos0 ..; positions outside [lo, hi) and
-    // columns behind the part are zeros.
+    // Columns [k0, k0 + 64) of one part of T behind positions pos0 .. pos0 + rows; columns behind the
+    // part are zeros, positions behind the rows are skipped.
     __device__ __forceinline__ void adapter_rows(uint32_t offset, const GroupedParams& p, int pos0, int rows,
-                                                 int lo, int hi, int part, int k0) const {
+                                                 int part, int k0) const {
         const int col = k0 + unit * 8;
         const bool exists = col < p.ext_cols;
         const char* base = static_cast<const char*>(p.t) +
@@ -492,10 +484,10 @@ struct Loader {
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int pos = pos0 + q * 32 + i * 4 + sub;
-                const bool take = pos >= lo && pos < hi && exists;
+                const int r = q * 32 + i * 4 + sub;
+                const bool take = r < rows && exists;
                 ptx::cp_async_16(stage + offset + q * 4096u + (i >> 1) * 1024u + ((i & 1) ? odd : even),
-                                 base + (take ? pos : 0) * pitch, take);
+                                 base + (take ? pos0 + r : 0) * pitch, take);
             }
         }
     }
@@ -555,10 +547,10 @@ __device__ __forceinline__ float from16(const GroupedParams& p, uint32_t word) {
 template <typename Elem, int kVec>
 __device__ __forceinline__ void add_adapter(const GroupedParams& p, const GroupedTable& table, int pos, int col,
                                             int have, float (&v)[kVec]) {
-    if (pos >= table.offs[p.ext_groups] || pos < table.offs[0]) {
+    if (pos >= table.offs[p.groups] || pos < table.offs[0]) {
         return;
     }
-    const int g = last_at_most(table.offs, p.ext_groups, pos);
+    const int g = last_at_most(table.offs, p.groups, pos);
     if (pos >= table.offs[g + 1]) {
         return;
     }
@@ -691,7 +683,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
     volatile uint32_t* tmem_slot_ptr =
         reinterpret_cast<volatile uint32_t*>(bars_ptr + 8 * Cfg::kNumBarriers);
     // the loaders work
-    const bool loads = p.form == kFormWgrad || p.load_a != 0 || (!kSplit && p.ext_groups > 0);
+    const bool loads = p.form == kFormWgrad || p.load_a != 0 || p.ext_mode == kExtBlocks;
 
     detail::Control ctl;
     ctl.abort_flag = reinterpret_cast<volatile int*>(bars_ptr + 8 * Cfg::kNumBarriers + 4);
@@ -740,7 +732,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
     ptx::tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot_ptr;
     const int total = detail::total_tiles(p, table);
-    const int ext_blocks = 2 * ((p.ext_cols + 63) / 64);  // of one adapter: both parts of T
+    const int ext_blocks = 2 * ((p.ext_cols + 63) / 64);  // of an adapter (kExtBlocks): both parts of T
     // A split launch has one tile per cluster.
     const int rank = kSplit ? static_cast<int>(ptx::cluster_cta_rank()) : 0;
     const int size = kSplit ? p.split : 1;
@@ -790,7 +782,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                     }
                 };
                 if (p.form == kFormRows) {
-                    const int group = table.whole ? 0 : t.group;
+                    const int group = table.whole || p.ext_mode != kExtNone ? 0 : t.group;
                     for (int kb = t.begin; kb < min(t.end, t.k_blocks); ++kb) {
                         if (!acquire_stage(b_bytes + (gather_a ? 0u : Cfg::kABytes))) {
                             ok = false;
@@ -805,22 +797,14 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         load_b(a_dst + Cfg::kABytes, &tmap_b_box, kb * 64, group);
                         advance();
                     }
-                    int at = t.k_blocks;  // index of the adapter's first block in the tile
-                    for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
-                        const detail::Span span = detail::adapter_span(table, t, g);
-                        if (span.lo >= span.hi) {
-                            continue;
+                    for (int eb = max(0, t.begin - t.k_blocks); ok && eb < t.end - t.k_blocks; ++eb) {
+                        if (!acquire_stage(b_bytes)) {
+                            ok = false;
+                            break;
                         }
-                        for (int eb = max(0, t.begin - at); eb < min(ext_blocks, t.end - at); ++eb) {
-                            if (!acquire_stage(b_bytes)) {
-                                ok = false;
-                                break;
-                            }
-                            load_b(ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes + Cfg::kABytes,
-                                   &tmap_e_box, (eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb) * 64, g);
-                            advance();
-                        }
-                        at += ext_blocks;
+                        load_b(ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes + Cfg::kABytes, &tmap_e_box,
+                               (eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb) * 64, t.adapter);
+                        advance();
                     }
                 } else {
                     // Weight gradient: 64 positions per block, both operands MN-major.
@@ -951,20 +935,9 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         break;
                     }
                 }
-                int at = t.k_blocks;
-                for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
-                    const detail::Span span = detail::adapter_span(table, t, g);
-                    if (span.lo >= span.hi) {
-                        continue;
-                    }
-                    for (int eb = max(0, t.begin - at); eb < min(ext_blocks, t.end - at); ++eb) {
-                        const int in_part = eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb;
-                        if (!block(min(4, (p.ext_cols - in_part * 64) / 16), true)) {
-                            ok = false;
-                            break;
-                        }
-                    }
-                    at += ext_blocks;
+                for (int eb = max(0, t.begin - t.k_blocks); ok && eb < t.end - t.k_blocks; ++eb) {
+                    const int in_part = eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb;
+                    ok = block(min(4, (p.ext_cols - in_part * 64) / 16), true);
                 }
                 if (ok) {
                     if (accumulate != 0) {
@@ -994,8 +967,8 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
             detail::GroupedTile t;
             bool ok = true;
             for (int tile = first_tile; ok && tile < total; tile += tile_step, ++i) {
-                t = detail::grouped_tile(p, table, tile, kSplit);
-                detail::take_share(p, table, &t, rank, size);
+                t = detail::grouped_tile(p, table, tile);
+                detail::take_share(p, &t, rank, size);
                 ok = queue.push(i, t, ctl);
             }
             t.group = -1;  // no more
@@ -1058,27 +1031,17 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         hand_over();
                     }
                 }
-                int first_block = t.k_blocks;
-                for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
-                    const detail::Span span = detail::adapter_span(table, t, g);
-                    if (span.lo >= span.hi) {
+                for (int eb = max(0, t.begin - t.k_blocks); ok && eb < t.end - t.k_blocks; ++eb, ++it) {
+                    if (static_cast<int>(it % kStages) != own) {
                         continue;
                     }
-                    const int eb_end = min(ext_blocks, t.end - first_block);
-                    for (int eb = max(0, t.begin - first_block); eb < eb_end; ++eb, ++it) {
-                        if (static_cast<int>(it % kStages) != own) {
-                            continue;
-                        }
-                        if (!acquire()) {
-                            ok = false;
-                            break;
-                        }
-                        const int part = eb >= ext_blocks / 2 ? 1 : 0;
-                        load.adapter_rows(0, p, t.p0, t.valid, span.lo, span.hi, part,
-                                          (eb - part * (ext_blocks / 2)) * 64);
-                        hand_over();
+                    if (!acquire()) {
+                        ok = false;
+                        break;
                     }
-                    first_block += ext_blocks;
+                    const int part = eb >= ext_blocks / 2 ? 1 : 0;
+                    load.adapter_rows(0, p, t.p0, t.valid, part, (eb - part * (ext_blocks / 2)) * 64);
+                    hand_over();
                 }
             } else {
                 const int row_blocks = (t.valid + 63) / 64;
@@ -1305,6 +1268,10 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                             v[4 * u] = x.x; v[4 * u + 1] = x.y; v[4 * u + 2] = x.z; v[4 * u + 3] = x.w;
                         }
                         if (c_row >= 0 && have > 0) {
+                            if (p.ext_mode == kExtAdd) {
+                                detail::add_adapter<Elem, kVec>(
+                                    p, table, t.p0 + static_cast<int>(quad) * 32 + row, col, have, v);
+                            }
                             detail::store_unit<OutT, kVec>(p, c_base, c_row, col, have, factor, v);
                         }
                     }
@@ -1329,7 +1296,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
             constexpr int kLanesPerRow = 128 / kVec;
             constexpr int kRowsPerWarp = 32 / kLanesPerRow;
             constexpr int kWarps = Cfg::kThreads / 32;
-            const detail::GroupedTile t = detail::grouped_tile(p, table, first_tile, true);
+            const detail::GroupedTile t = detail::grouped_tile(p, table, first_tile);
             const int rows = p.form == kFormWgrad ? min(128, p.m - t.m0) : t.valid;
             const int sub = static_cast<int>(lane) % kLanesPerRow;
             const int col = t.n0 + sub * kVec;
@@ -1359,7 +1326,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         v[4 * u + 3] += x.w;
                     }
                 }
-                if (p.ext_groups > 0) {
+                if (p.ext_mode == kExtAdd) {
                     detail::add_adapter<Elem, kVec>(p, table, t.p0 + row, col, have, v);
                 }
                 detail::store_unit<OutT, kVec>(p, c_base, c_row, col, have, factor, v);

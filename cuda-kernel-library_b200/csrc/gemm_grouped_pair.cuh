@@ -55,7 +55,7 @@ struct PairTile {
     int c0;         // first column
     int half;       // rows per CTA: 16, 32, ... 128 (kFormWgrad: 64 or 128)
     int k_blocks;
-    int ext_first, ext_last;
+    int adapter;    // whose blocks the tile runs besides (kExtBlocks), -1: none
 };
 
 __device__ __forceinline__ PairTile pair_tile(const GroupedParams& p, const GroupedTable& t, int tile) {
@@ -88,7 +88,7 @@ __device__ __forceinline__ PairTile pair_tile(const GroupedParams& p, const Grou
     o.r0 = seg0 + rt * step;
     o.rows = max(0, min(step, total_rows - rt * step));
     o.half = max(unit, (o.rows + unit - 1) / unit * unit) / 2;
-    o.ext_first = o.ext_last = 0;
+    o.adapter = p.ext_mode == kExtBlocks && o.group < p.groups && o.rows > 0 ? o.group : -1;
     if (p.form == kFormWgrad) {
         o.p0 = t.offs[o.group];
         o.valid = max(0, t.offs[o.group + 1] - o.p0);
@@ -97,16 +97,8 @@ __device__ __forceinline__ PairTile pair_tile(const GroupedParams& p, const Grou
         o.p0 = o.r0;
         o.valid = o.rows;
         o.k_blocks = o.rows > 0 ? (p.k + 63) / 64 : 0;
-        if (p.ext_groups > 0 && o.rows > 0 && o.p0 < t.offs[p.ext_groups]) {
-            o.ext_first = last_at_most(t.offs, p.ext_groups, o.p0);
-            o.ext_last = last_at_most(t.offs, p.ext_groups, o.p0 + o.valid - 1) + 1;
-        }
     }
     return o;
-}
-
-__device__ __forceinline__ Span adapter_span(const GroupedTable& table, const PairTile& t, int g) {
-    return {max(table.offs[g], t.p0), min(table.offs[g + 1], t.p0 + t.valid)};
 }
 
 // factor * a and factor * b (FP32 bits), rounded and packed with a in the low half.
@@ -165,7 +157,7 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
     const bool leader = rank == 0;
     const bool wgrad = p.form == kFormWgrad;
     const bool gather = p.load_a != 0;
-    const bool loads = wgrad || gather || p.ext_groups > 0;  // the loaders work
+    const bool loads = wgrad || gather || p.ext_mode == kExtBlocks;  // the loaders work
 
     detail::Control ctl;
     ctl.abort_flag = reinterpret_cast<volatile int*>(bars_ptr + 8 * Cfg::kNumBarriers + 4);
@@ -266,7 +258,7 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                     }
                 };
                 if (!wgrad) {
-                    const int group = table.whole ? 0 : t.group;
+                    const int group = table.whole || p.ext_mode != kExtNone ? 0 : t.group;
                     const int row0 = t.p0 + static_cast<int>(rank) * t.half;
                     const int row_boxes = gather ? 0 : (t.half + 63) / 64;
                     const uint32_t rows_bytes = 2u * static_cast<uint32_t>(row_boxes) * Cfg::kBoxBytes;
@@ -287,20 +279,14 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                         }
                         advance();
                     }
-                    for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
-                        const detail::Span span = detail::adapter_span(table, t, g);
-                        if (span.lo >= span.hi) {
-                            continue;
+                    for (int eb = 0; ok && t.adapter >= 0 && eb < ext_blocks; ++eb) {
+                        if (!acquire_stage(cols_bytes)) {
+                            ok = false;
+                            break;
                         }
-                        for (int eb = 0; eb < ext_blocks; ++eb) {
-                            if (!acquire_stage(cols_bytes)) {
-                                ok = false;
-                                break;
-                            }
-                            load_cols(ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes, &tmap_ext,
-                                      (eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb) * 64, g);
-                            advance();
-                        }
+                        load_cols(ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes, &tmap_ext,
+                                  (eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb) * 64, t.adapter);
+                        advance();
                     }
                 } else {
                     const int row0 = t.r0 + static_cast<int>(rank) * t.half;
@@ -426,18 +412,9 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                         break;
                     }
                 }
-                for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
-                    const detail::Span span = detail::adapter_span(table, t, g);
-                    if (span.lo >= span.hi) {
-                        continue;
-                    }
-                    for (int eb = 0; eb < ext_blocks; ++eb) {
-                        const int in_part = eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb;
-                        if (!block(min(4, (p.ext_cols - in_part * 64) / 16), true)) {
-                            ok = false;
-                            break;
-                        }
-                    }
+                for (int eb = 0; ok && t.adapter >= 0 && eb < ext_blocks; ++eb) {
+                    const int in_part = eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb;
+                    ok = block(min(4, (p.ext_cols - in_part * 64) / 16), true);
                 }
                 if (ok) {
                     if (accumulate != 0) {
@@ -527,24 +504,18 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                         hand_over();
                     }
                 }
-                for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
-                    const detail::Span span = detail::adapter_span(table, t, g);
-                    if (span.lo >= span.hi) {
+                for (int eb = 0; ok && t.adapter >= 0 && eb < ext_blocks; ++eb, ++it) {
+                    if (static_cast<int>(it % kStages) != own) {
                         continue;
                     }
-                    for (int eb = 0; eb < ext_blocks; ++eb, ++it) {
-                        if (static_cast<int>(it % kStages) != own) {
-                            continue;
-                        }
-                        if (!acquire()) {
-                            ok = false;
-                            break;
-                        }
-                        const int part = eb >= ext_blocks / 2 ? 1 : 0;
-                        load.adapter_rows(Cfg::kColsBytes, p, t.p0 + first_row, rows, span.lo, span.hi, part,
-                                          (eb - part * (ext_blocks / 2)) * 64);
-                        hand_over();
+                    if (!acquire()) {
+                        ok = false;
+                        break;
                     }
+                    const int part = eb >= ext_blocks / 2 ? 1 : 0;
+                    load.adapter_rows(Cfg::kColsBytes, p, t.p0 + first_row, rows, part,
+                                      (eb - part * (ext_blocks / 2)) * 64);
+                    hand_over();
                 }
             } else {
                 const int first = (own - static_cast<int>(it % kStages) + kStages) % kStages;
@@ -632,7 +603,7 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
             // gradient it clips rows as well.
             const int by_tma = p.c_tma == 0 ? 0 : wgrad ? (rows + 31) / 32 * 32 : rows / 32 * 32;
             int j0 = 0;
-            if (sizeof(Elem) == 2 && p.beta == 0.0f && p.c_vec != 0) {
+            if (sizeof(Elem) == 2 && p.beta == 0.0f && p.c_vec != 0 && p.ext_mode != kExtAdd) {
                 // 64 rows at a time: the accumulator is read as matrix fragments (16 columns of C by
                 // 32 rows), whose 8 x 8 blocks are stored transposed, 16 bytes = 8 columns of a row
                 // each.  (Lane = column and 2-byte stores, 32 rows at a time, took the epilogue of a
@@ -797,6 +768,9 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                             v[4 * u + 3] = x.w;
                         }
                         if (c_row >= 0 && have > 0) {
+                            if (p.ext_mode == kExtAdd) {
+                                detail::add_adapter<Elem, kVec>(p, table, t.p0 + j0 + j, col, have, v);
+                            }
                             detail::store_unit<OutT, kVec>(p, c_base, c_row, col, have, factor, v);
                         }
                     }

@@ -563,3 +563,42 @@ def test_lora_few_rows_ranks_and_gradients(ckl, r, dt, out):
                 ref, mag = ref + t @ p2, mag + ta @ p2.abs()
                 extra = TWO_PART[dt] * (t.abs() @ p2.abs()) + tiny * r * p2.abs().max()
             check(got, ref, mag, 2 * max(k, n) + 2 * r + 10, out, extra)
+
+
+@pytest.mark.parametrize("m,g,n,k", [(40, 6, 520, 2048), (900, 5, 200, 64), (3000, 9, 1040, 72), (2000, 200, 1040, 72)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_lora_adapters_do_not_reach_each_other(ckl, m, g, n, k, bad):
+    """An adapter that holds NaN or infinities, or a row of x that does, spoils its own rows only."""
+    r = 16
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    ids = torch.randint(-1, g, (m,), generator=gen, device="cuda", dtype=torch.int32)
+    ids[0], ids[1], ids[2], ids[3] = 0, 1, 2, -1
+    m, x, w, a, b, s, offs, rows = lora_case(ckl, ids, g, k, n, r, "bf16", 96)
+    dy = rand((m, n), torch.bfloat16, 97)
+    a[0, 3, 5], b[1, 7, 11] = bad, bad
+    x[2, 4] = bad
+    dy[2, 4] = bad
+    size = ckl.gemm_lora_workspace_bytes(m, r, True)
+    ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    y = torch.empty(m, n, device="cuda")
+    dx, da, db = torch.empty(m, k, device="cuda"), torch.empty(g, k, r, device="cuda"), torch.empty(g, r, n, device="cuda")
+    ckl.gemm_lora(ckl.BF16, x, w, a, b, s, y, ckl.F32, offs, rows, g, m, n, k, r, ws, size)
+    ckl.gemm_lora_backward(ckl.BF16, dy, x, w, a, b, s, dx, ckl.F32, da, db, ckl.F32, offs, rows, g, m, n, k, r, ws, size)
+    torch.cuda.synchronize()
+    clean = (ids != 0) & (ids != 1)
+    clean[2] = False
+    assert torch.isfinite(y[clean]).all() and torch.isfinite(dx[clean]).all()
+    assert not torch.isfinite(y[ids == 0]).any() and not torch.isfinite(y[ids == 1][:, 11]).any()
+    fine = [i for i in range(3, g)]
+    assert torch.isfinite(da[fine]).all() and torch.isfinite(db[fine]).all()
+    v, ww = x[clean].double(), w.double()
+    t = torch.zeros(m, r, dtype=torch.float64, device="cuda")
+    ref, mag = v @ ww, v.abs() @ ww.abs()
+    which = ids[clean]
+    for i in range(2, g):
+        sel = which == i
+        t = s[i].double() * (v[sel] @ a[i].double())
+        ta = s[i].double() * (v[sel].abs() @ a[i].double().abs())
+        ref[sel] += t @ b[i].double()
+        mag[sel] += ta @ b[i].double().abs()
+    check(y[clean], ref, mag, 2 * k + 2 * r + 10, "f32", TWO_PART["bf16"] * mag)
