@@ -111,7 +111,7 @@ long long row_tiles(const Product& q, int height) {
     const GroupedParams& p = q.p;
     return p.form == kFormWgrad ? static_cast<long long>(p.groups) * ((p.m + height - 1) / height)
            : q.whole            ? (p.rows + height - 1) / height
-                                : p.rows / height + std::min(p.groups + (p.ext_mode == kExtBlocks ? 1 : 0), p.rows);
+                                : p.rows / height + std::min(p.groups, p.rows);
 }
 long long single_tiles(const Product& q, int bn) { return row_tiles(q, 128) * ((q.p.n + bn - 1) / bn); }
 
@@ -121,7 +121,7 @@ void plan(Product& q, const DeviceView& view) {
     const bool wgrad = p.form == kFormWgrad;
     p.status = view.status;
     p.fmt = q.ab_dtype == CKL_BF16 ? 1u : 0u;
-    q.whole = !wgrad && (p.offsets == nullptr || p.ext_mode == kExtAdd);
+    q.whole = !wgrad && (p.offsets == nullptr || q.e != nullptr);
     // CTA pairs on 256 x 256 tiles where there are enough of them; operands in two parts and a
     // gathered G have only a few columns or rows of output and stay with the single-CTA kernel.
     const long long pair_tiles = row_tiles(q, 256) * ((p.n + 255) / 256);
@@ -197,7 +197,7 @@ int describe(Product& q, GroupedProblem* out) {
     }
     // Few rows to a tile: the loaders fetch those alone, where a boxed copy would fetch 128.
     p.load_a = p.a_rows != nullptr ||
-               (!wgrad && !q.pair && p.k > 0 && p.ext_mode == kExtNone && !q.whole && p.rows <= 32ll * std::min(p.groups, p.rows));
+               (!wgrad && !q.pair && p.k > 0 && !q.whole && p.rows <= 32ll * std::min(p.groups, p.rows));
     std::memset(out, 0, sizeof *out);
     // Gathered operands are read by the loader warps, all others through these descriptors.
     if (p.load_a == 0) {
@@ -229,7 +229,7 @@ int describe(Product& q, GroupedProblem* out) {
         const int bytes = size_of(q.c_dtype);
         p.c_vec = !misaligned(p.c, 16) && (static_cast<long long>(p.ldc) * bytes) % 16 == 0 &&
                   (p.c_stride * bytes) % 16 == 0;
-        p.c_tma = p.c_vec && p.beta == 0.0f && p.c_rows == nullptr && p.split == 1 && p.ext_mode != kExtAdd;
+        p.c_tma = p.c_vec && p.beta == 0.0f && p.c_rows == nullptr && p.split == 1;
         if (p.c_tma) {
             GRP_TRY(encode_operand(&out->c, q.c_dtype, p.c, p.n, wgrad ? p.m : p.rows, p.ldc, wgrad ? p.groups : 1,
                                    wgrad ? p.c_stride : static_cast<long long>(p.ldc) * p.rows,
@@ -275,22 +275,44 @@ int launch_pair(const GroupedProblem& problem, long long tiles, const DeviceView
         dim3(static_cast<unsigned>(2 * std::min<long long>(view.max_pairs, tiles))), stream);
 }
 
+// Finds the adapters that are not finite, see ExtMode.
+int check_adapters(const Product& q, cudaStream_t stream) {
+    ExtCheckParams c = {};
+    c.offsets = q.p.offsets;
+    c.e = static_cast<const unsigned short*>(q.e);
+    c.flags = reinterpret_cast<unsigned char*>(const_cast<uint32_t*>(q.p.ext_flags));
+    c.stride = q.e_stack;
+    c.adapters = q.p.groups;
+    c.rows = q.e_outer;
+    c.cols = q.e_cols;
+    c.ld = q.lde;
+    c.exponent = q.ab_dtype == CKL_BF16 ? 0x7f80u : 0x7c00u;
+    GRP_TRY_CUDA(launch_dependent(ext_check_kernel, dim3(static_cast<unsigned>(c.adapters), kExtChecks),
+                                  kExtCheckThreads, 0, 1,
+                                  stream, c));
+    return CKL_OK;
+}
+
 int run(Product& q, cudaStream_t stream) {
     DeviceView view;
     GRP_TRY(device_view(&view));
     plan(q, view);
     if (may_split(q, view)) {
-        if (q.p.ext_mode == kExtBlocks) {
-            // (the parts of a split tile meet row by row: adapters are added there)
-            q.p.ext_mode = kExtAdd;
-            plan(q, view);
-        }
         q.p.bn = std::min(q.p.bn, 128);
         q.tiles = single_tiles(q, q.p.bn);
         q.p.split = choose_split(q.tiles, q.blocks, view);
     }
     if (q.tiles == 0) {
         return CKL_OK;
+    }
+    if (q.e != nullptr) {
+        // Adapters row by row cost about 0.6 ps per row, rank and column (500 rows, 8 adapters, rank
+        // 64, n 2048: 50 us, 34 with blocks); up to 5 us of that a split launch saves their blocks.
+        const long long products = static_cast<long long>(q.p.rows) * q.p.ext_rank * q.p.n;
+        q.p.ext_mode = q.p.split > 1 && products <= (1ll << 23) ? kExtAdd : kExtBlocks;
+        if (q.p.ext_mode == kExtBlocks) {
+            GRP_TRY(check_adapters(q, stream));
+        }
     }
     GroupedProblems problems;
     GRP_TRY(describe(q, &problems.at[0]));
@@ -339,10 +361,10 @@ Product blank(int ab_dtype, int c_dtype, int form) {
     return q;
 }
 
-// Rows per adapter from which tiles end with them.
-constexpr int kExtRows = 64;
-
 int padded_rank(int rank) { return (rank + 15) / 16 * 16; }
+// The workspace begins with the adapters' flags.
+constexpr size_t kFlagBytes = static_cast<size_t>(kMaxGemmGroups) * sizeof(uint32_t);
+static_assert(kExtChecks == sizeof(uint32_t), "a byte per check");
 size_t two_part_bytes(int m, int rank) {
     return (static_cast<size_t>(std::max(m, 0)) * 2 * padded_rank(rank) * 2 + 255) / 256 * 256;
 }
@@ -405,19 +427,17 @@ int shrink_rows(int ab_dtype, const void* x, int ldx, int k, const void* a, int 
 
 // C[rows[p]] = A[rows[p]] * op(B) + T[p] * op(E_g) + beta * C[rows[p]], C of n columns.
 Product expand(int ab_dtype, int c_dtype, const void* a, int lda, int k, const void* b, int ldb, int n,
-               bool trans, const void* t, int rank, const void* e, int lde, long long e_stack, void* c,
-               int ldc, const int* offsets, const int* rows, int adapters, int m, float beta) {
+               bool trans, const void* flags, const void* t, int rank, const void* e, int lde, long long e_stack,
+               void* c, int ldc, const int* offsets, const int* rows, int adapters, int m, float beta) {
     Product q = blank(ab_dtype, c_dtype, kFormRows);
     const int rp = padded_rank(rank);
     q.p.offsets = offsets;
     q.p.a_rows = q.p.c_rows = rows;
     q.p.c = c;
     q.p.groups = adapters;
-    // Tiles that end with their adapter cost half a tile's time per adapter, one product per row and
-    // rank on the CUDA cores about as much as a tile's epilogue from rank 32 on.
-    q.p.ext_mode = m >= kExtRows * adapters ? kExtBlocks : kExtAdd;
     q.p.ext_cols = rp;
     q.p.ext_rank = rank;
+    q.p.ext_flags = static_cast<const uint32_t*>(flags);
     q.p.rows = q.p.a_count = q.p.c_count = m;
     q.p.n = n;
     q.p.k = k;
@@ -568,7 +588,9 @@ int ckl_gemm_grouped_wgrad(int ab_dtype, const void* a, const int* a_rows, int a
 }
 
 size_t ckl_gemm_lora_workspace_bytes(int m, int rank, int backward) {
-    return rank < 1 || rank > kMaxLoraRank ? 0 : two_part_bytes(m, rank) * (backward != 0 ? 2 : 1);
+    return m < 1 || rank < 1 || rank > kMaxLoraRank
+               ? 0
+               : kFlagBytes + two_part_bytes(m, rank) * (backward != 0 ? 2 : 1);
 }
 
 int ckl_gemm_lora(int ab_dtype, const void* x, const void* w, const void* lora_a, const void* lora_b,
@@ -588,17 +610,18 @@ int ckl_gemm_lora(int ab_dtype, const void* x, const void* w, const void* lora_a
         return set_error(CKL_ERR_INVALID_ARG, "%s: y %p, ldy %d for n %d", what, y, ldy, n);
     }
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    void* t = static_cast<unsigned char*>(workspace) + kFlagBytes;
     DeviceView view;
     GRP_TRY(device_view(&view));
     if (static_cast<long long>(m) * ((rank + kLoraRanks - 1) / kLoraRanks) <= 2ll * view.sm_count) {
-        GRP_TRY(shrink_rows(ab_dtype, x, ldx, k, lora_a, ldla, stride_a, rank, scales, workspace, offsets, rows,
+        GRP_TRY(shrink_rows(ab_dtype, x, ldx, k, lora_a, ldla, stride_a, rank, scales, t, offsets, rows,
                             adapters, m, s));
     } else {
-        Product t = shrink(ab_dtype, x, ldx, k, lora_a, ldla, stride_a, false, rank, scales, workspace, offsets,
-                           rows, adapters, m);
-        GRP_TRY(run(t, s));
+        Product p = shrink(ab_dtype, x, ldx, k, lora_a, ldla, stride_a, false, rank, scales, t, offsets, rows,
+                           adapters, m);
+        GRP_TRY(run(p, s));
     }
-    Product q = expand(ab_dtype, y_dtype, x, ldx, k, w, ldw, n, false, workspace, rank, lora_b, ldlb, stride_b,
+    Product q = expand(ab_dtype, y_dtype, x, ldx, k, w, ldw, n, false, workspace, t, rank, lora_b, ldlb, stride_b,
                        y, ldy, offsets, rows, adapters, m, beta);
     return run(q, s);
 }
@@ -632,8 +655,8 @@ int ckl_gemm_lora_backward(int ab_dtype, const void* dy, const void* x, const vo
                          what, lddx, ldda, lddb);
     }
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    void* u = workspace;
-    void* t = static_cast<unsigned char*>(workspace) + two_part_bytes(m, rank);
+    void* u = static_cast<unsigned char*>(workspace) + kFlagBytes;
+    void* t = static_cast<unsigned char*>(u) + two_part_bytes(m, rank);
     const int rp = padded_rank(rank);
     const bool need_u = m > 0 && (dx != nullptr || da != nullptr), need_t = m > 0 && db != nullptr;
     Product pu = shrink(ab_dtype, dy, lddy, n, lora_b, ldlb, stride_b, true, rank, scales, u, offsets, rows,
@@ -695,7 +718,7 @@ int ckl_gemm_lora_backward(int ab_dtype, const void* dy, const void* x, const vo
         GRP_TRY(run(pb, s));
     }
     if (m > 0 && dx != nullptr) {
-        Product q = expand(ab_dtype, dx_dtype, dy, lddy, n, w, ldw, k, true, u, rank, lora_a, ldla, stride_a, dx,
+        Product q = expand(ab_dtype, dx_dtype, dy, lddy, n, w, ldw, k, true, workspace, u, rank, lora_a, ldla, stride_a, dx,
                            lddx, offsets, rows, adapters, m, 0.0f);
         GRP_TRY(run(q, s));
     }

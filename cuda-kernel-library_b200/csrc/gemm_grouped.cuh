@@ -7,22 +7,25 @@
 //   kFormWgrad  W_g = alpha * sum over p in g of A[row(p)]^T G[row(p)]: the ragged dimension is
 //               the one that is summed; tiles of 128 x bn of each W_g.
 //
-// kFormRows may be "extended": one B for all groups (a shared projection), and for the rows of adapter
-// g (groups and adapters are then the same thing; rows behind the last belong to none) T[p] * op(E_g)
-// besides.  Two ways, chosen by how many rows an adapter has:
-//   kExtBlocks  tiles end with the adapters, as with any other groups, and behind the k blocks of the
-//               product a tile runs those of its adapter's T and E_g into the same accumulator;
-//   kExtAdd     tiles are cut from all rows alike, and the few products a row needs are added in FP32
-//               on the CUDA cores while the tile is stored.
-// (Running every adapter's blocks over a tile that several share, the rows of the others read as
-// zeros, would cost less than kExtAdd at high ranks, but zero times an infinity or NaN in one
-// request's adapter is NaN in another's rows.)
+// kFormRows may be "extended": one B for all positions (a shared projection), and for the rows of
+// adapter g (offsets are then the adapters') T[p] * op(E_g) besides.
+//   kExtBlocks  behind the k blocks of the product a tile runs, for each adapter whose rows it holds,
+//               those of T and E_g into the same accumulator, the rows of other adapters read as
+//               zeros: no second pass over C, and no tiles cut at the borders of requests (which
+//               reads the shared weights again for each: 2000 rows, 30 adapters, 4096 x 4096:
+//               157 us against 47 for the product alone).  Zero times an infinity or NaN in one
+//               adapter would be NaN in another's rows, so an adapter whose E_g holds any
+//               (ext_flags, found by ext_check_kernel) is left out there and added row by row when
+//               the tile is stored.
+//   kExtAdd     all adapters are added row by row, in FP32 on the CUDA cores: a split launch of few
+//               rows, where 64-wide blocks that hold a rank of 16 for one or two rows each
+//               outnumbered those of the product.
 //
 // Consecutive rows arrive by boxed TMA copies.  Gathered rows arrive by cp.async from four loader
 // warps that write the same swizzled layout: TMA's own row gather (tile::gather4) took about 100
 // cycles per four rows, 3300 per 128 x 64 stage against the 512 the stage's MMAs need (4096^3:
-// 355 TFLOP/s gathered, 1113 boxed).  The loaders also write the zeros that a weight gradient needs
-// behind the end of a group.
+// 355 TFLOP/s gathered, 1113 boxed).  The loaders also write the zeros that masked rows need:
+// rows of other adapters, and in a weight gradient the positions behind the end of a group.
 //
 // Operand layout in shared memory is that of the dense kernel (gemm_umma.cuh): 128-byte rows of
 // 64 elements under the 128-byte swizzle.  The matrix whose reduced dimension is contiguous in
@@ -40,6 +43,7 @@ constexpr int kMaxGemmGroups = 1024;
 constexpr int kMaxLoraRank = 128;
 
 enum GroupedForm : int { kFormRows = 0, kFormWgrad = 1 };
+constexpr int kExtChecks = 4;
 enum ExtMode : int { kExtNone = 0, kExtBlocks = 1, kExtAdd = 2 };
 
 // Element type of C, or the two-part form: an FP32 value v stored as 16-bit hi = round(v) and
@@ -77,6 +81,7 @@ struct GroupedParams {
     // Extension: offsets/groups describe the adapters.
     int ext_mode;              // ExtMode
     int ext_cols;              // columns of one part of T (a multiple of 16)
+    const uint32_t* ext_flags; // kExtBlocks: a word of kExtChecks bytes per adapter, not 0: E_g is not finite
     const void* e;             // E, `ext_rank` x n per adapter (n x ext_rank with trans_b)
     int ext_rank, lde;
     long long e_stride;
@@ -114,7 +119,7 @@ struct GroupedConfig {
     static constexpr int kBuffers = 3;  // of 2 KB (32 rows x 64 bytes) per epilogue warp
     static constexpr uint32_t kStagingBytes = kSplit ? 128 * 128 * 4 : 4 * kBuffers * 2048;
     static constexpr int kNumBarriers = 3 * kStages + 5 + 8;
-    static constexpr uint32_t kTableBytes = 2 * (kMaxGemmGroups + 2) * 4;
+    static constexpr uint32_t kTableBytes = 2 * (kMaxGemmGroups + 2) * 4 + kMaxGemmGroups / 8;
     static constexpr uint32_t kQueueBytes = 4 * 64;
     static constexpr uint32_t kSmemBytes =
         kStages * kStageBytes + kStagingBytes + kTableBytes + kQueueBytes + kNumBarriers * 8 + 16 + 1024;
@@ -131,12 +136,13 @@ struct GroupedTile {
     int m0, n0;     // kFormWgrad: first row of W_g; first column
     int cols;       // columns of the tile that exist
     int k_blocks;   // 64-wide blocks of the main product
-    int adapter;    // whose blocks the tile runs besides (kExtBlocks), -1: none
+    int ext_first, ext_last;  // kExtBlocks: adapters [first, last) that may have rows in the tile
     int begin, end;  // this CTA's share of the tile's blocks (main product, then adapters)
 };
 
 struct GroupedTable {
     const int* offs;   // [groups + 1], clamped to [0, rows]
+    const uint32_t* flagged;  // kExtBlocks: bit per adapter
     const int* tiles;  // [groups + 1] running count of row tiles (kFormRows)
     int segments;      // groups that are cut into tiles
     bool whole;        // one segment of all positions (extended, or no offsets)
@@ -166,19 +172,28 @@ __device__ __forceinline__ GroupedTable make_table(const GroupedParams& p, int* 
         for (int g = static_cast<int>(threadIdx.x); g <= p.groups; g += threads) {
             offs[g] = min(max(p.offsets[g], 0), p.rows);
         }
-        if (threadIdx.x == 0) {
-            offs[p.groups + 1] = p.rows;  // kExtBlocks: rows of no adapter are a last segment
-        }
     } else if (threadIdx.x == 0) {
         offs[0] = 0;
         offs[1] = p.rows;
     }
+    uint32_t* flagged = reinterpret_cast<uint32_t*>(tiles + kMaxGemmGroups + 2);
+    if (p.ext_mode == kExtBlocks) {
+        for (int g0 = warp * 32; g0 < p.groups; g0 += threads) {
+            const int g = g0 + static_cast<int>(lane);
+            const uint32_t any = g < p.groups ? p.ext_flags[g] : 0u;
+            const uint32_t bits = __ballot_sync(0xFFFFFFFFu, any != 0);
+            if (lane == 0) {
+                flagged[g0 / 32] = bits;
+            }
+        }
+    }
     __syncthreads();
     GroupedTable t;
     t.offs = offs;
+    t.flagged = flagged;
     t.tiles = tiles;
-    t.whole = p.offsets == nullptr || p.ext_mode == kExtAdd;
-    t.segments = t.whole ? 1 : p.groups + (p.ext_mode == kExtBlocks ? 1 : 0);
+    t.whole = p.offsets == nullptr || p.ext_mode != kExtNone;
+    t.segments = t.whole ? 1 : p.groups;
     t.n_tiles = (p.n + tile_cols - 1) / tile_cols;
     t.m_tiles = (p.m + tile_rows - 1) / tile_rows;
     if (warp == 0) {
@@ -240,7 +255,7 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, cons
     mt = band * kBand + in_band - nt * height;
     o.n0 = nt * p.bn;
     o.cols = min(p.bn, p.n - o.n0);
-    o.adapter = p.ext_mode == kExtBlocks && o.group < p.groups ? o.group : -1;
+    o.ext_first = o.ext_last = 0;
     if (p.form == kFormWgrad) {
         o.p0 = t.offs[o.group];
         o.valid = max(0, t.offs[o.group + 1] - o.p0);
@@ -253,6 +268,10 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, cons
         o.valid = min(128, seg1 - o.p0);
         o.m0 = 0;
         o.k_blocks = (p.k + 63) / 64;
+        if (p.ext_mode == kExtBlocks && o.p0 < t.offs[p.groups]) {
+            o.ext_first = last_at_most(t.offs, p.groups, o.p0);
+            o.ext_last = last_at_most(t.offs, p.groups, o.p0 + o.valid - 1) + 1;
+        }
     }
     return o;
 }
@@ -324,9 +343,34 @@ struct TileQueue {
     }
 };
 
+// Positions [lo, hi) of a tile that belong to adapter g, none for an adapter that is added row by row.
+struct Span {
+    int lo, hi;
+};
+template <typename Tile>
+__device__ __forceinline__ Span adapter_span(const GroupedTable& table, const Tile& t, int g) {
+    const bool runs = ((table.flagged[g >> 5] >> (g & 31)) & 1u) == 0;
+    return {max(table.offs[g], t.p0), runs ? min(table.offs[g + 1], t.p0 + t.valid) : t.p0};
+}
+// Whether the tile holds rows of an adapter that is added row by row.
+template <typename Tile>
+__device__ __forceinline__ bool has_flagged(const GroupedTable& table, const Tile& t) {
+    for (int g = t.ext_first; g < t.ext_last; ++g) {
+        if ((table.flagged[g >> 5] >> (g & 31)) & 1u) {
+            return true;
+        }
+    }
+    return false;
+}
+
 // Fills in the share of a tile's blocks that CTA `rank` of `size` runs.
-__device__ __forceinline__ void take_share(const GroupedParams& p, GroupedTile* t, int rank, int size) {
-    const int blocks = t->k_blocks + (t->adapter >= 0 ? 2 * ((p.ext_cols + 63) / 64) : 0);
+__device__ __forceinline__ void take_share(const GroupedParams& p, const GroupedTable& table, GroupedTile* t,
+                                           int rank, int size) {
+    int blocks = t->k_blocks;
+    for (int g = t->ext_first; g < t->ext_last; ++g) {
+        const Span s = adapter_span(table, *t, g);
+        blocks += s.lo < s.hi ? 2 * ((p.ext_cols + 63) / 64) : 0;
+    }
     t->begin = static_cast<int>(static_cast<long long>(blocks) * rank / size);
     t->end = static_cast<int>(static_cast<long long>(blocks) * (rank + 1) / size);
 }
@@ -468,10 +512,10 @@ struct Loader {
         }
     }
 
-    // Columns [k0, k0 + 64) of one part of T behind positions pos0 .. pos0 + rows; columns behind the
-    // part are zeros, positions behind the rows are skipped.
+    // Columns [k0, k0 + 64) of one part of T behind positions pos0 ..; positions outside [lo, hi) and
+    // columns behind the part are zeros.
     __device__ __forceinline__ void adapter_rows(uint32_t offset, const GroupedParams& p, int pos0, int rows,
-                                                 int part, int k0) const {
+                                                 int lo, int hi, int part, int k0) const {
         const int col = k0 + unit * 8;
         const bool exists = col < p.ext_cols;
         const char* base = static_cast<const char*>(p.t) +
@@ -484,10 +528,10 @@ struct Loader {
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int r = q * 32 + i * 4 + sub;
-                const bool take = r < rows && exists;
+                const int pos = pos0 + q * 32 + i * 4 + sub;
+                const bool take = pos >= lo && pos < hi && exists;
                 ptx::cp_async_16(stage + offset + q * 4096u + (i >> 1) * 1024u + ((i & 1) ? odd : even),
-                                 base + (take ? pos0 + r : 0) * pitch, take);
+                                 base + (take ? pos : 0) * pitch, take);
             }
         }
     }
@@ -551,12 +595,14 @@ __device__ __forceinline__ void add_adapter(const GroupedParams& p, const Groupe
         return;
     }
     const int g = last_at_most(table.offs, p.groups, pos);
-    if (pos >= table.offs[g + 1]) {
+    if (pos >= table.offs[g + 1] ||
+        (p.ext_mode == kExtBlocks && ((table.flagged[g >> 5] >> (g & 31)) & 1u) == 0)) {
         return;
     }
     const unsigned short* t = static_cast<const unsigned short*>(p.t) + static_cast<size_t>(pos) * p.ldt;
     const unsigned short* e = static_cast<const unsigned short*>(p.e) + static_cast<size_t>(g) * p.e_stride;
     // eight ranks at a time: their T is one 16-byte word per part (parts are 16 ranks wide or more)
+#pragma unroll 2
     for (int r0 = 0; r0 < p.ext_rank; r0 += 8) {
         const uint4 hi = *reinterpret_cast<const uint4*>(t + r0);
         const uint4 lo = *reinterpret_cast<const uint4*>(t + p.ext_cols + r0);
@@ -797,14 +843,22 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         load_b(a_dst + Cfg::kABytes, &tmap_b_box, kb * 64, group);
                         advance();
                     }
-                    for (int eb = max(0, t.begin - t.k_blocks); ok && eb < t.end - t.k_blocks; ++eb) {
-                        if (!acquire_stage(b_bytes)) {
-                            ok = false;
-                            break;
+                    int at = t.k_blocks;  // index of the adapter's first block in the tile
+                    for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
+                        const detail::Span span = detail::adapter_span(table, t, g);
+                        if (span.lo >= span.hi) {
+                            continue;
                         }
-                        load_b(ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes + Cfg::kABytes, &tmap_e_box,
-                               (eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb) * 64, t.adapter);
-                        advance();
+                        for (int eb = max(0, t.begin - at); eb < min(ext_blocks, t.end - at); ++eb) {
+                            if (!acquire_stage(b_bytes)) {
+                                ok = false;
+                                break;
+                            }
+                            load_b(ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes + Cfg::kABytes,
+                                   &tmap_e_box, (eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb) * 64, g);
+                            advance();
+                        }
+                        at += ext_blocks;
                     }
                 } else {
                     // Weight gradient: 64 positions per block, both operands MN-major.
@@ -935,9 +989,17 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         break;
                     }
                 }
-                for (int eb = max(0, t.begin - t.k_blocks); ok && eb < t.end - t.k_blocks; ++eb) {
-                    const int in_part = eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb;
-                    ok = block(min(4, (p.ext_cols - in_part * 64) / 16), true);
+                int at = t.k_blocks;
+                for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
+                    const detail::Span span = detail::adapter_span(table, t, g);
+                    if (span.lo >= span.hi) {
+                        continue;
+                    }
+                    for (int eb = max(0, t.begin - at); ok && eb < min(ext_blocks, t.end - at); ++eb) {
+                        const int in_part = eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb;
+                        ok = block(min(4, (p.ext_cols - in_part * 64) / 16), true);
+                    }
+                    at += ext_blocks;
                 }
                 if (ok) {
                     if (accumulate != 0) {
@@ -968,7 +1030,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
             bool ok = true;
             for (int tile = first_tile; ok && tile < total; tile += tile_step, ++i) {
                 t = detail::grouped_tile(p, table, tile);
-                detail::take_share(p, &t, rank, size);
+                detail::take_share(p, table, &t, rank, size);
                 ok = queue.push(i, t, ctl);
             }
             t.group = -1;  // no more
@@ -1031,17 +1093,27 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         hand_over();
                     }
                 }
-                for (int eb = max(0, t.begin - t.k_blocks); ok && eb < t.end - t.k_blocks; ++eb, ++it) {
-                    if (static_cast<int>(it % kStages) != own) {
+                int first_block = t.k_blocks;
+                for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
+                    const detail::Span span = detail::adapter_span(table, t, g);
+                    if (span.lo >= span.hi) {
                         continue;
                     }
-                    if (!acquire()) {
-                        ok = false;
-                        break;
+                    const int eb_end = min(ext_blocks, t.end - first_block);
+                    for (int eb = max(0, t.begin - first_block); eb < eb_end; ++eb, ++it) {
+                        if (static_cast<int>(it % kStages) != own) {
+                            continue;
+                        }
+                        if (!acquire()) {
+                            ok = false;
+                            break;
+                        }
+                        const int part = eb >= ext_blocks / 2 ? 1 : 0;
+                        load.adapter_rows(0, p, t.p0, t.valid, span.lo, span.hi, part,
+                                          (eb - part * (ext_blocks / 2)) * 64);
+                        hand_over();
                     }
-                    const int part = eb >= ext_blocks / 2 ? 1 : 0;
-                    load.adapter_rows(0, p, t.p0, t.valid, part, (eb - part * (ext_blocks / 2)) * 64);
-                    hand_over();
+                    first_block += ext_blocks;
                 }
             } else {
                 const int row_blocks = (t.valid + 63) / 64;
@@ -1125,6 +1197,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
             }
             ptx::tc_fence_after_sync();
             const bool nothing = t.begin == t.end;
+            const bool flagged = !kSplit && detail::has_flagged(table, t);
             const uint32_t t_row = tmem_base + ((quad * 32u) << 16) + acc * 256u;
             // Hands the accumulator back to the MMA warp, once, when its last column is in registers.
             bool released = false;
@@ -1166,7 +1239,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
             // All 32 rows of this warp are consecutive rows of C: 32-column chunks (64 or 128 bytes
             // a row) go through a swizzled buffer and out by TMA, which clips at the edge
             // of C.  Otherwise rows are written one by one.
-            const bool by_tma = !kTwo && p.c_tma != 0 &&
+            const bool by_tma = !kTwo && p.c_tma != 0 && !flagged &&
                                 (p.form == kFormWgrad ? t.m0 + static_cast<int>(quad) * 32 < p.m
                                                       : static_cast<int>(quad) * 32 + 32 <= t.valid);
             if (by_tma) {
@@ -1268,7 +1341,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                             v[4 * u] = x.x; v[4 * u + 1] = x.y; v[4 * u + 2] = x.z; v[4 * u + 3] = x.w;
                         }
                         if (c_row >= 0 && have > 0) {
-                            if (p.ext_mode == kExtAdd) {
+                            if (flagged) {
                                 detail::add_adapter<Elem, kVec>(
                                     p, table, t.p0 + static_cast<int>(quad) * 32 + row, col, have, v);
                             }
@@ -1305,6 +1378,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
             Elem* c_base = static_cast<Elem*>(p.c) +
                            (p.form == kFormWgrad ? static_cast<long long>(t.group) * p.c_stride : 0ll);
             const uint32_t parts = ring + kStages * Cfg::kStageBytes;
+            const bool add = p.ext_mode == kExtAdd || detail::has_flagged(table, t);
             for (int i = warp * kRowsPerWarp + static_cast<int>(lane) / kLanesPerRow; i * size + rank < rows;
                  i += kWarps * kRowsPerWarp) {
                 const int row = i * size + rank;
@@ -1326,7 +1400,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         v[4 * u + 3] += x.w;
                     }
                 }
-                if (p.ext_mode == kExtAdd) {
+                if (add) {
                     detail::add_adapter<Elem, kVec>(p, table, t.p0 + row, col, have, v);
                 }
                 detail::store_unit<OutT, kVec>(p, c_base, c_row, col, have, factor, v);
@@ -1342,6 +1416,70 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
     if (warp == 1) {
         ptx::tc_fence_after_sync();
         ptx::tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// Whether E_g holds an infinity or NaN: kExtChecks CTAs per adapter, a byte each for the answer.
+// Adapters without rows are not read.
+struct ExtCheckParams {
+    const int* offsets;
+    const unsigned short* e;
+    unsigned char* flags;
+    long long stride;
+    int adapters, rows, cols, ld;  // of E_g as stored
+    unsigned int exponent;         // all ones: 0x7f80 (BF16) or 0x7c00 (FP16)
+};
+constexpr int kExtCheckThreads = 1024;
+__global__ void __launch_bounds__(kExtCheckThreads) ext_check_kernel(const ExtCheckParams p) {
+    ptx::grid_dependency_wait();
+    ptx::launch_dependents();
+    const int g = static_cast<int>(blockIdx.x);
+    const unsigned short* e = p.e + static_cast<size_t>(g) * p.stride;
+    bool bad = false;
+    if (p.offsets[g] < p.offsets[g + 1]) {
+        // 16-byte units, dealt to the threads of the adapter's CTAs; (row, unit) advances without
+        // a division.
+        const int units = (p.cols + 7) / 8;
+        const int step = kExtChecks * kExtCheckThreads;
+        const int first = static_cast<int>(blockIdx.y) * kExtCheckThreads + static_cast<int>(threadIdx.x);
+        const int rows_per_step = step / units, units_per_step = step - rows_per_step * units;
+        int r = first / units, u = first - r * units;
+        const unsigned int both = p.exponent * 0x10001u;
+        auto odd = [&](uint32_t w) {
+            const uint32_t x = (w & both) ^ both;  // a half that is zero has its exponent all ones
+            return (x & 0xffffu) == 0 || (x >> 16) == 0;
+        };
+        while (r < p.rows) {
+            uint4 w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = make_uint4(0, 0, 0, 0);
+                if (r < p.rows) {
+                    const unsigned short* src = e + static_cast<size_t>(r) * p.ld + u * 8;
+                    if (u * 8 + 8 <= p.cols) {
+                        w[i] = *reinterpret_cast<const uint4*>(src);
+                    } else {
+                        for (int k = 0; u * 8 + k < p.cols; ++k) {
+                            bad |= (src[k] & p.exponent) == p.exponent;
+                        }
+                    }
+                }
+                r += rows_per_step;
+                u += units_per_step;
+                if (u >= units) {
+                    u -= units;
+                    ++r;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                bad |= odd(w[i].x) || odd(w[i].y) || odd(w[i].z) || odd(w[i].w);
+            }
+        }
+    }
+    const int any = __syncthreads_or(bad);
+    if (threadIdx.x == 0) {
+        p.flags[g * kExtChecks + blockIdx.y] = any != 0 ? 1 : 0;
     }
 }
 

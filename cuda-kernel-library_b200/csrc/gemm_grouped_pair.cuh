@@ -40,7 +40,7 @@ struct GroupedPairConfig {
     static constexpr uint32_t kWarpStaging = kBuffers * kBufferBytes;
     static constexpr uint32_t kStagingBytes = 4 * kWarpStaging;
     static constexpr int kNumBarriers = 3 * kStages + 5 + 8;
-    static constexpr uint32_t kTableBytes = 2 * (kMaxGemmGroups + 2) * 4;
+    static constexpr uint32_t kTableBytes = 2 * (kMaxGemmGroups + 2) * 4 + kMaxGemmGroups / 8;
     static constexpr uint32_t kQueueBytes = 4 * 64;
     static constexpr uint32_t kSmemBytes =
         kStages * kStageBytes + kStagingBytes + kTableBytes + kQueueBytes + kNumBarriers * 8 + 16 + 1024;
@@ -55,7 +55,7 @@ struct PairTile {
     int c0;         // first column
     int half;       // rows per CTA: 16, 32, ... 128 (kFormWgrad: 64 or 128)
     int k_blocks;
-    int adapter;    // whose blocks the tile runs besides (kExtBlocks), -1: none
+    int ext_first, ext_last;  // kExtBlocks: adapters that may have rows in the tile
 };
 
 __device__ __forceinline__ PairTile pair_tile(const GroupedParams& p, const GroupedTable& t, int tile) {
@@ -88,7 +88,7 @@ __device__ __forceinline__ PairTile pair_tile(const GroupedParams& p, const Grou
     o.r0 = seg0 + rt * step;
     o.rows = max(0, min(step, total_rows - rt * step));
     o.half = max(unit, (o.rows + unit - 1) / unit * unit) / 2;
-    o.adapter = p.ext_mode == kExtBlocks && o.group < p.groups && o.rows > 0 ? o.group : -1;
+    o.ext_first = o.ext_last = 0;
     if (p.form == kFormWgrad) {
         o.p0 = t.offs[o.group];
         o.valid = max(0, t.offs[o.group + 1] - o.p0);
@@ -97,6 +97,10 @@ __device__ __forceinline__ PairTile pair_tile(const GroupedParams& p, const Grou
         o.p0 = o.r0;
         o.valid = o.rows;
         o.k_blocks = o.rows > 0 ? (p.k + 63) / 64 : 0;
+        if (p.ext_mode == kExtBlocks && o.rows > 0 && o.p0 < t.offs[p.groups]) {
+            o.ext_first = last_at_most(t.offs, p.groups, o.p0);
+            o.ext_last = last_at_most(t.offs, p.groups, o.p0 + o.valid - 1) + 1;
+        }
     }
     return o;
 }
@@ -279,14 +283,17 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                         }
                         advance();
                     }
-                    for (int eb = 0; ok && t.adapter >= 0 && eb < ext_blocks; ++eb) {
-                        if (!acquire_stage(cols_bytes)) {
-                            ok = false;
-                            break;
+                    for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
+                        const detail::Span span = detail::adapter_span(table, t, g);
+                        for (int eb = 0; span.lo < span.hi && eb < ext_blocks; ++eb) {
+                            if (!acquire_stage(cols_bytes)) {
+                                ok = false;
+                                break;
+                            }
+                            load_cols(ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes, &tmap_ext,
+                                      (eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb) * 64, g);
+                            advance();
                         }
-                        load_cols(ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes, &tmap_ext,
-                                  (eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb) * 64, t.adapter);
-                        advance();
                     }
                 } else {
                     const int row0 = t.r0 + static_cast<int>(rank) * t.half;
@@ -412,9 +419,12 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                         break;
                     }
                 }
-                for (int eb = 0; ok && t.adapter >= 0 && eb < ext_blocks; ++eb) {
-                    const int in_part = eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb;
-                    ok = block(min(4, (p.ext_cols - in_part * 64) / 16), true);
+                for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
+                    const detail::Span span = detail::adapter_span(table, t, g);
+                    for (int eb = 0; ok && span.lo < span.hi && eb < ext_blocks; ++eb) {
+                        const int in_part = eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb;
+                        ok = block(min(4, (p.ext_cols - in_part * 64) / 16), true);
+                    }
                 }
                 if (ok) {
                     if (accumulate != 0) {
@@ -504,18 +514,21 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                         hand_over();
                     }
                 }
-                for (int eb = 0; ok && t.adapter >= 0 && eb < ext_blocks; ++eb, ++it) {
-                    if (static_cast<int>(it % kStages) != own) {
-                        continue;
+                for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
+                    const detail::Span span = detail::adapter_span(table, t, g);
+                    for (int eb = 0; span.lo < span.hi && eb < ext_blocks; ++eb, ++it) {
+                        if (static_cast<int>(it % kStages) != own) {
+                            continue;
+                        }
+                        if (!acquire()) {
+                            ok = false;
+                            break;
+                        }
+                        const int part = eb >= ext_blocks / 2 ? 1 : 0;
+                        load.adapter_rows(Cfg::kColsBytes, p, t.p0 + first_row, rows, span.lo, span.hi, part,
+                                          (eb - part * (ext_blocks / 2)) * 64);
+                        hand_over();
                     }
-                    if (!acquire()) {
-                        ok = false;
-                        break;
-                    }
-                    const int part = eb >= ext_blocks / 2 ? 1 : 0;
-                    load.adapter_rows(Cfg::kColsBytes, p, t.p0 + first_row, rows, part,
-                                      (eb - part * (ext_blocks / 2)) * 64);
-                    hand_over();
                 }
             } else {
                 const int first = (own - static_cast<int>(it % kStages) + kStages) % kStages;
@@ -601,9 +614,10 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
             };
             // Whole runs of 32 consecutive rows leave by TMA, which clips at the edge of C; in a weight
             // gradient it clips rows as well.
-            const int by_tma = p.c_tma == 0 ? 0 : wgrad ? (rows + 31) / 32 * 32 : rows / 32 * 32;
+            const bool flagged = detail::has_flagged(table, t);
+            const int by_tma = p.c_tma == 0 || flagged ? 0 : wgrad ? (rows + 31) / 32 * 32 : rows / 32 * 32;
             int j0 = 0;
-            if (sizeof(Elem) == 2 && p.beta == 0.0f && p.c_vec != 0 && p.ext_mode != kExtAdd) {
+            if (sizeof(Elem) == 2 && p.beta == 0.0f && p.c_vec != 0 && !flagged) {
                 // 64 rows at a time: the accumulator is read as matrix fragments (16 columns of C by
                 // 32 rows), whose 8 x 8 blocks are stored transposed, 16 bytes = 8 columns of a row
                 // each.  (Lane = column and 2-byte stores, 32 rows at a time, took the epilogue of a
@@ -768,7 +782,7 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                             v[4 * u + 3] = x.w;
                         }
                         if (c_row >= 0 && have > 0) {
-                            if (p.ext_mode == kExtAdd) {
+                            if (flagged) {
                                 detail::add_adapter<Elem, kVec>(p, table, t.p0 + j0 + j, col, have, v);
                             }
                             detail::store_unit<OutT, kVec>(p, c_base, c_row, col, have, factor, v);
