@@ -166,3 +166,37 @@ def test_exported_from_the_library(ckl):
                  "ckl_gemm_grouped_wgrad", "ckl_moe_combine", "ckl_moe_combine_backward", "ckl_gemm_lora",
                  "ckl_gemm_lora_backward", "ckl_gemm_lora_workspace_bytes"):
         assert hasattr(lib, name)
+
+
+def test_cpp_header_compiles(tmp_path, ckl):
+    """include/ckl/grouped.hpp compiles as C++17 and links against the library."""
+    import os
+    import shutil
+    import subprocess
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    if not os.path.exists(nvcc):
+        pytest.skip("no nvcc here")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = tmp_path / "use_grouped.cu"
+    src.write_text("""
+#include "ckl/grouped.hpp"
+int main(int argc, char**) {
+    if (argc < 100) return ckl::gemm_lora_workspace_bytes(1, 16) == 0;
+    __half* h = nullptr; __nv_bfloat16* b = nullptr; float* f = nullptr; int* i = nullptr;
+    ckl::group_rows(i, 1, 1, 1, i, i, i);
+    ckl::moe_route(f, f, i, 1, 8, 2);
+    ckl::moe_route(h, f, i, 1, 8, 2, ckl::RouteOptions{});
+    ckl::moe_route_backward(b, i, f, b, 1, 8, 2);
+    ckl::gemm_grouped(h, i, 1, h, f, i, 1, 1, 8, 8);
+    ckl::gemm_grouped_wgrad(b, i, 1, b, b, i, 1, 1, 8, 8);
+    ckl::moe_combine(h, i, f, f, 1, 1, 8, 1);
+    ckl::moe_combine_backward(h, i, f, f, h, f, 1, 1, 8, 1);
+    ckl::gemm_lora(h, h, h, h, f, f, i, i, 1, 1, 8, 8, 8, f, 4096);
+    ckl::gemm_lora_backward(h, h, h, h, h, f, f, f, f, i, i, 1, 1, 8, 8, 8, f, 4096);
+}
+""")
+    exe = tmp_path / "use_grouped"
+    subprocess.run([nvcc, "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-I",
+                    os.path.join(root, "include"), "-o", str(exe), str(src), ckl.LIB_PATH,
+                    "-Xlinker", f"-rpath={os.path.dirname(ckl.LIB_PATH)}"], check=True)
+    assert subprocess.run([str(exe)]).returncode == 0
