@@ -108,16 +108,18 @@ struct GroupedProblems {
 
 // kSplit: a cluster of CTAs shares one tile of at most 128 columns and divides its blocks; the
 // FP32 partial tiles meet in distributed shared memory.  For launches with fewer tiles than SMs.
+// A split launch has one tile per CTA, whose partial then takes the place of the ring: six stages of
+// 32 KB instead of four beside a 64 KB buffer.
 template <bool kSplit>
 struct GroupedConfig {
-    static constexpr int kStages = 4;
+    static constexpr int kStages = kSplit ? 6 : 4;
     static constexpr uint32_t kABytes = 128 * 64 * 2;
     static constexpr uint32_t kBoxBytes = 64 * 64 * 2;
     static constexpr uint32_t kBBytes = (kSplit ? 2 : 4) * kBoxBytes;
     static constexpr uint32_t kStageBytes = kABytes + kBBytes;
     static constexpr int kThreads = 192 + 32 * kStages + 32;  // one loader warp per stage, a scheduler
     static constexpr int kBuffers = 3;  // of 2 KB (32 rows x 64 bytes) per epilogue warp
-    static constexpr uint32_t kStagingBytes = kSplit ? 128 * 128 * 4 : 4 * kBuffers * 2048;
+    static constexpr uint32_t kStagingBytes = kSplit ? 0 : 4 * kBuffers * 2048;
     static constexpr int kNumBarriers = 3 * kStages + 5 + 8;
     static constexpr uint32_t kTableBytes = 2 * (kMaxGemmGroups + 2) * 4 + kMaxGemmGroups / 8;
     static constexpr uint32_t kQueueBytes = 4 * 64;
@@ -679,6 +681,22 @@ __device__ __forceinline__ void add_adapter(const GroupedParams& p, const Groupe
     }
 }
 
+// Pulls columns [col, col + cols) of one rank of the adapter of position pos into L2.
+__device__ __forceinline__ void prefetch_adapter(const GroupedParams& p, const GroupedTable& table, int pos, int r,
+                                                 int col, int cols) {
+    if (pos >= table.offs[p.groups] || pos < table.offs[0]) {
+        return;
+    }
+    const int g = last_at_most(table.offs, p.groups, pos);
+    if (pos < table.offs[g + 1]) {
+        const unsigned short* src = static_cast<const unsigned short*>(p.e) +
+                                    static_cast<size_t>(g) * p.e_stride + static_cast<size_t>(r) * p.lde + col;
+        for (int c = 0; c < cols; c += 64) {
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(src + c));
+        }
+    }
+}
+
 // Row of C behind row `in_tile` of a tile, -1 for none.
 __device__ __forceinline__ int row_of_c(const GroupedParams& p, const GroupedTile& t, int in_tile) {
     if (p.form == kFormWgrad) {
@@ -1175,10 +1193,20 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
         const int sub = static_cast<int>(lane) % kLanesPerRow;
         uint32_t count = 0;
         const uint32_t stg_addr = ring + kStages * Cfg::kStageBytes + quad * (Cfg::kBuffers * 2048u);
-        const uint32_t stg_all = ring + kStages * Cfg::kStageBytes;
         uint32_t buffer = 0;
         bool alive = true;
         detail::GroupedTile t;
+        if constexpr (kSplit) {
+            if (p.ext_mode == kExtAdd && p.trans_b == 0 && first_tile < total) {
+                // What add_adapter will read of E_g for this CTA's rows travels to L2 meanwhile.
+                t = detail::grouped_tile(p, table, first_tile);
+                const int mine = (t.valid - rank + size - 1) / size * p.ext_rank;
+                for (int i = static_cast<int>(threadIdx.x) - 64; i < mine; i += 128) {
+                    const int row = i / p.ext_rank;
+                    detail::prefetch_adapter(p, table, t.p0 + row * size + rank, i - row * p.ext_rank, t.n0, t.cols);
+                }
+            }
+        }
         for (uint32_t i = 0; alive && queue.pop(i, &t, ctl, true, lane); ++i) {
             const uint32_t acc = count & 1u;
             const uint32_t parity = (count >> 1) & 1u;
@@ -1212,9 +1240,10 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                 }
             };
             if constexpr (kSplit) {
-                // Park the partial tile: 512 bytes a row, the 16-byte units exchanged by the row
-                // so that the 32 rows of a store hit all banks.
-                const uint32_t row_addr = stg_all + static_cast<uint32_t>(in_tile) * 512u;
+                // Park the partial tile where the ring was (every block has been multiplied): 512 bytes a
+                // row, the 16-byte units exchanged by the row so that the 32 rows of a store hit all
+                // banks.
+                const uint32_t row_addr = ring + static_cast<uint32_t>(in_tile) * 512u;
                 for (int c0 = 0; c0 < t.cols; c0 += 32) {
                     uint32_t r[32];
                     if (nothing) {
@@ -1377,7 +1406,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
             const float factor = p.alpha * (p.scales != nullptr ? __ldg(p.scales + t.group) : 1.0f);
             Elem* c_base = static_cast<Elem*>(p.c) +
                            (p.form == kFormWgrad ? static_cast<long long>(t.group) * p.c_stride : 0ll);
-            const uint32_t parts = ring + kStages * Cfg::kStageBytes;
+            const uint32_t parts = ring;
             const bool add = p.ext_mode == kExtAdd || detail::has_flagged(table, t);
             for (int i = warp * kRowsPerWarp + static_cast<int>(lane) / kLanesPerRow; i * size + rank < rows;
                  i += kWarps * kRowsPerWarp) {
