@@ -56,13 +56,17 @@ int check_types(const char* what, int ab_dtype, int c_dtype) {
     return CKL_OK;
 }
 
-int check_groups(const char* what, const int* offsets, int groups, int rows) {
+int check_groups(const char* what, const int* offsets, int groups, int rows, int cols, int depth) {
     if (groups < 1 || rows < 0 || offsets == nullptr || misaligned(offsets, 4)) {
         return set_error(CKL_ERR_INVALID_ARG, "%s: offsets %p of %d groups, %d rows", what,
                          static_cast<const void*>(offsets), groups, rows);
     }
     if (groups > kMaxGemmGroups) {
         return set_error(CKL_ERR_TOO_LARGE, "%s: %d groups (at most %d)", what, groups, kMaxGemmGroups);
+    }
+    if (std::max(rows, std::max(cols, depth)) > kMaxExtent) {
+        return set_error(CKL_ERR_TOO_LARGE, "%s: extents %d, %d, %d (at most %d)", what, rows, cols, depth,
+                         kMaxExtent);
     }
     return CKL_OK;
 }
@@ -288,8 +292,7 @@ int check_adapters(const Product& q, cudaStream_t stream) {
     c.ld = q.lde;
     c.exponent = q.ab_dtype == CKL_BF16 ? 0x7f80u : 0x7c00u;
     GRP_TRY_CUDA(launch_dependent(ext_check_kernel, dim3(static_cast<unsigned>(c.adapters), kExtChecks),
-                                  kExtCheckThreads, 0, 1,
-                                  stream, c));
+                                  kExtCheckThreads, 0, 1, stream, c));
     return CKL_OK;
 }
 
@@ -307,7 +310,7 @@ int run(Product& q, cudaStream_t stream) {
     }
     if (q.e != nullptr) {
         // Adapters row by row cost about 0.6 ps per row, rank and column (500 rows, 8 adapters, rank
-        // 64, n 2048: 50 us, 34 with blocks); up to 5 us of that a split launch saves their blocks.
+        // 64, n 2048: 50 us, 40 with blocks and their check); up to 5 us of that a split launch saves their blocks.
         const long long products = static_cast<long long>(q.p.rows) * q.p.ext_rank * q.p.n;
         q.p.ext_mode = q.p.split > 1 && products <= (1ll << 23) ? kExtAdd : kExtBlocks;
         if (q.p.ext_mode == kExtBlocks) {
@@ -468,7 +471,7 @@ int check_lora(const char* what, int ab_dtype, int out_dtype, const void* w, int
                const float* scales, const int* offsets, const int* rows, int adapters, int m, int n,
                int k, int rank, const void* workspace, size_t have, size_t need) {
     GRP_TRY(check_types(what, ab_dtype, out_dtype));
-    GRP_TRY(check_groups(what, offsets, adapters, m));
+    GRP_TRY(check_groups(what, offsets, adapters, m, n, k));
     if (rank < 1 || rank > kMaxLoraRank) {
         return set_error(rank < 1 ? CKL_ERR_INVALID_ARG : CKL_ERR_TOO_LARGE, "%s: rank %d (1 to %d)", what,
                          rank, kMaxLoraRank);
@@ -482,7 +485,7 @@ int check_lora(const char* what, int ab_dtype, int out_dtype, const void* w, int
     if (misaligned(scales, 4) || misaligned(rows, 4)) {
         return set_error(CKL_ERR_INVALID_ARG, "%s: misaligned scales or rows", what);
     }
-    if (workspace == nullptr || misaligned(workspace, 256) || have < need) {
+    if (need > 0 && (workspace == nullptr || misaligned(workspace, 256) || have < need)) {
         return set_error(CKL_ERR_INVALID_ARG,
                          "%s: the workspace is %p of %zu bytes, needed are %zu on a 256-byte boundary", what,
                          workspace, have, need);
@@ -503,7 +506,7 @@ int ckl_gemm_grouped(int ab_dtype, const void* a, const int* a_rows, int a_count
         return CKL_OK;
     }
     GRP_TRY(check_types(what, ab_dtype, c_dtype));
-    GRP_TRY(check_groups(what, offsets, groups, rows));
+    GRP_TRY(check_groups(what, offsets, groups, rows, n, k));
     k = std::max(k, 0);
     if (k > 0) {
         GRP_TRY(check_operand(what, "a", a, lda, k, 0));
@@ -550,7 +553,7 @@ int ckl_gemm_grouped_wgrad(int ab_dtype, const void* a, const int* a_rows, int a
     }
     rows = std::max(rows, 0);
     GRP_TRY(check_types(what, ab_dtype, dw_dtype));
-    GRP_TRY(check_groups(what, offsets, groups, rows));
+    GRP_TRY(check_groups(what, offsets, groups, rows, n, m));
     if (rows > 0) {
         GRP_TRY(check_operand(what, "a", a, lda, m, 0));
         GRP_TRY(check_operand(what, "g", g, ldg, n, 0));

@@ -30,6 +30,10 @@ int encode_operand(CUtensorMap* map, int dtype, const void* base, uint64_t inner
                    uint64_t pitch, uint64_t depth, uint64_t stack, uint32_t box_inner,
                    uint32_t box_outer);
 
+// Largest count of rows, columns, tokens or slots of the routed operators: their kernels round such
+// counts up and step past them in 32 bits by less than the rest.
+constexpr int kMaxExtent = 0x7fffffff - 4095;
+
 // Launches a kernel as a programmatic dependent: it may be set up while the kernel before it on
 // the stream finishes, and waits for that one itself before it touches memory.
 template <typename... Params, typename... Args>

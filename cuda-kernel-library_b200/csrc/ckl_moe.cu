@@ -101,9 +101,9 @@ int check_route(const char* what, int dtype, const void* logits, int ldl, int to
     if (n_experts < 1 || top_k < 1 || top_k > n_experts) {
         return set_error(CKL_ERR_INVALID_ARG, "%s: %d experts, top_k %d", what, n_experts, top_k);
     }
-    if (n_experts > kMaxExperts || top_k > kMaxTopK) {
-        return set_error(CKL_ERR_TOO_LARGE, "%s: %d experts (at most %d), top_k %d (at most %d)", what,
-                         n_experts, kMaxExperts, top_k, kMaxTopK);
+    if (n_experts > kMaxExperts || top_k > kMaxTopK || tokens > kMaxExtent) {
+        return set_error(CKL_ERR_TOO_LARGE, "%s: %d experts (at most %d), top_k %d (at most %d), %d tokens", what,
+                         n_experts, kMaxExperts, top_k, kMaxTopK, tokens);
     }
     if (score != CKL_SCORE_SOFTMAX && score != CKL_SCORE_SIGMOID) {
         return set_error(CKL_ERR_INVALID_ARG, "%s: bad score %d", what, score);
@@ -164,6 +164,9 @@ int check_combine(const char* what, int y_dtype, const void* y, const int* posit
                   int ldy, int ldo) {
     if (!known_dtype(y_dtype) || !known_dtype(out_dtype)) {
         return set_error(CKL_ERR_INVALID_ARG, "%s: bad dtype %d or %d", what, y_dtype, out_dtype);
+    }
+    if (n > kMaxExtent) {
+        return set_error(CKL_ERR_TOO_LARGE, "%s: %d columns", what, n);
     }
     if (top_k < 1 || y_rows < 0 || ldy < n || ldo < n) {
         return set_error(CKL_ERR_INVALID_ARG, "%s: top_k %d, y_rows %d, n %d, ldy %d, ldo %d", what, top_k,
@@ -281,8 +284,9 @@ int ckl_group_rows(const int* ids, int slots, int groups, int slots_per_row, int
         return set_error(CKL_ERR_INVALID_ARG, "group_rows: %d slots, %d groups, %d slots per row", slots,
                          groups, slots_per_row);
     }
-    if (groups > kMaxExperts) {
-        return set_error(CKL_ERR_TOO_LARGE, "group_rows: %d groups (at most %d)", groups, kMaxExperts);
+    if (groups > kMaxExperts || slots > kMaxExtent) {
+        return set_error(CKL_ERR_TOO_LARGE, "group_rows: %d groups (at most %d), %d slots", groups, kMaxExperts,
+                         slots);
     }
     if (offsets == nullptr || (slots > 0 && (ids == nullptr || rows == nullptr || positions == nullptr))) {
         return set_error(CKL_ERR_INVALID_ARG, "group_rows: null pointer");

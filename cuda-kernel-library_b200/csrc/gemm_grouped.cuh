@@ -21,8 +21,8 @@
 //               rows, where 64-wide blocks that hold a rank of 16 for one or two rows each
 //               outnumbered those of the product.
 //
-// Consecutive rows arrive by boxed TMA copies.  Gathered rows arrive by cp.async from four loader
-// warps that write the same swizzled layout: TMA's own row gather (tile::gather4) took about 100
+// Consecutive rows arrive by boxed TMA copies.  Gathered rows arrive by cp.async from loader warps,
+// one per stage, that write the same swizzled layout: TMA's own row gather (tile::gather4) took about 100
 // cycles per four rows, 3300 per 128 x 64 stage against the 512 the stage's MMAs need (4096^3:
 // 355 TFLOP/s gathered, 1113 boxed).  The loaders also write the zeros that masked rows need:
 // rows of other adapters, and in a weight gradient the positions behind the end of a group.
@@ -31,8 +31,8 @@
 // 64 elements under the 128-byte swizzle.  The matrix whose reduced dimension is contiguous in
 // memory is read K-major, the other one MN-major, so nothing is ever transposed in memory.
 //
-// Warp roles: warp 0 TMA producer, warp 1 MMA, warps 2-5 epilogue as in the dense kernel, warps
-// 6-9 loaders; two accumulators in tensor memory; every wait bounded.
+// Warp roles: warp 0 TMA producer, warp 1 MMA, warps 2-5 epilogue as in the dense kernel, then a
+// loader warp per stage and the scheduler; two accumulators in tensor memory; every wait bounded.
 #pragma once
 
 #include "gemm_umma.cuh"
@@ -1058,7 +1058,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
         }
         __syncwarp();
     } else if (warp >= 6) {
-        // Loaders: warp 6 + s owns stage s, so four stages are in flight at once and each is handed
+        // Loaders: warp 6 + s owns stage s, so all stages are in flight at once and each is handed
         // over the moment its own copies have landed (one warp for all stages, or all warps for each
         // stage, would hand over only in order and lag behind: 700 TFLOP/s at 4096^3).  Eight lanes
         // copy the 128 bytes of one row (lane & 7 picks the 16-byte unit), four rows per instruction;

@@ -295,7 +295,8 @@ int ckl_scatter_column_block(void* const* dsts, int parts, const void* src, int 
  * All of these: pointers are device memory of the current device, work is enqueued on `stream`,
  * nothing is allocated per call and nothing is kept between calls; the first call on a device
  * creates its small state (make it outside stream capture).  Two calls may overlap as long as they
- * do not share outputs or a workspace.  No result depends on the order in which threads run. */
+ * do not share outputs or a workspace.  No result depends on the order in which threads run.
+ * Counts of rows, columns, tokens and slots are at most 2^31 - 4096 (CKL_ERR_TOO_LARGE). */
 
 /* Stable order of `slots` ids by group.  ids[s] names the group of slot s; an id outside
  * [0, groups) names none.  offsets[g] .. offsets[g+1] (groups + 1 values) are the positions of

@@ -602,3 +602,61 @@ def test_lora_adapters_do_not_reach_each_other(ckl, m, g, n, k, bad):
         ref[sel] += t @ b[i].double()
         mag[sel] += ta @ b[i].double().abs()
     check(y[clean], ref, mag, 2 * k + 2 * r + 10, "f32", TWO_PART["bf16"] * mag)
+
+
+def test_gradients_without_rows(ckl):
+    """An empty batch: gradients become beta times their old values, an empty workspace will do."""
+    g, k, n, r = 3, 64, 520, 24
+    offs = torch.zeros(g + 1, dtype=torch.int32, device="cuda")
+    w, a, b = (rand(s, torch.bfloat16, 60 + i) for i, s in enumerate([(k, n), (g, k, r), (g, r, n)]))
+    da, db = rand((g, k, r), torch.float32, 63), rand((g, r, n), torch.float32, 64)
+    want = 0.5 * da, 0.5 * db
+    none = torch.empty(0, dtype=torch.uint8, device="cuda")
+    assert ckl.gemm_lora_workspace_bytes(0, r, True) == 0
+    ckl.gemm_lora_backward(ckl.BF16, None, None, w, a, b, None, None, ckl.F32, da, db, ckl.F32, offs, None, g, 0, n,
+                           k, r, none, 0, beta=0.5)
+    assert torch.equal(da, want[0]) and torch.equal(db, want[1])
+    for m in (72, 520):  # one CTA and a pair per tile
+        dw = rand((40, m, n), torch.float32, 65)
+        want = 0.5 * dw
+        ckl.gemm_grouped_wgrad(ckl.BF16, None, None, dw, ckl.F32, torch.zeros(41, dtype=torch.int32, device="cuda"),
+                               40, 0, m, n, beta=0.5)
+        assert torch.equal(dw, want)
+        ckl.gemm_grouped_wgrad(ckl.BF16, None, None, dw, ckl.F32, torch.zeros(41, dtype=torch.int32, device="cuda"),
+                               40, 0, m, n)
+        assert not dw.any()
+
+
+@pytest.mark.parametrize("sizes", [(3, 0, 40), (300, 0, 2000)], ids=["few", "many"])
+def test_offsets_that_pass_32_bits(ckl, sizes):
+    """Matrices of a stack 2^31 + 8 elements apart, rows of A and C 2^20 and 2^21 apart."""
+    n, k, far = 264, 136, 2 ** 31 + 8
+    rows = sum(sizes)
+    offs = offsets_of(sizes)
+    stack = torch.empty(2 * far + n * k, dtype=torch.bfloat16, device="cuda")
+    small = rand((3, k, n), torch.bfloat16, 70)
+    for g in range(3):
+        stack[g * far:g * far + k * n] = small[g].reshape(-1)
+    pitch = 2 ** 21 if rows > 1000 else 2 ** 26
+    a_far = torch.empty(rows * pitch, dtype=torch.bfloat16, device="cuda").view(rows, pitch)
+    a = rand((rows, k), torch.bfloat16, 71)
+    a_far[:, :k] = a
+    back = torch.arange(rows - 1, -1, -1, dtype=torch.int32, device="cuda")
+    c_far = torch.empty(rows * pitch, dtype=torch.bfloat16, device="cuda").view(rows, pitch)
+    ref = torch.cat([x.double() @ w.double() for x, w in zip(a.split(sizes), small)])
+    mag = torch.cat([x.double().abs() @ w.double().abs() for x, w in zip(a.split(sizes), small)])
+    for idx, src in ((None, a), (back, a.flip(0))):
+        a_far[:, :k] = src
+        c_far[:, :n] = float("nan")
+        ckl.gemm_grouped(ckl.BF16, a_far, stack, c_far, ckl.BF16, offs, 3, rows, n, k, a_rows=idx, a_count=rows,
+                         lda=pitch, stride_b=far, ldc=pitch)
+        check(c_far[:, :n].float(), ref, mag, k, "bf16")
+    # the gradient of the weights into the same stack
+    gr = rand((rows, n), torch.bfloat16, 72)
+    ckl.gemm_grouped_wgrad(ckl.BF16, a_far, gr, stack, ckl.BF16, offs, 3, rows, k, n, a_rows=back, a_count=rows,
+                           lda=pitch, stride_dw=far)
+    at = 0
+    for g, size in enumerate(sizes):
+        x, d = a[at:at + size].double(), gr[at:at + size].double()
+        check(stack[g * far:g * far + k * n].view(k, n).float(), x.T @ d, x.T.abs() @ d.abs(), max(size, 1), "bf16")
+        at += size

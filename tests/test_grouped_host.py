@@ -168,6 +168,16 @@ def test_exported_from_the_library(ckl):
         assert hasattr(lib, name)
 
 
+def test_counts_that_32_bit_steps_would_pass(ckl):
+    big = 2 ** 31 - 1
+    for f in (lambda: grouped(ckl, rows=big), lambda: grouped(ckl, n=big, ldb=big - 7, ldc=big, trans_b=True),
+              lambda: grouped(ckl, k=big), lambda: wgrad(ckl, rows=big), lambda: wgrad(ckl, m=big),
+              lambda: lora(ckl, m=big), lambda: ckl.group_rows(P, big, 4, P, P, P),
+              lambda: ckl.moe_route(ckl.F32, P, P, P, big, 8, 2),
+              lambda: ckl.moe_combine(ckl.F32, P, P, P, P, ckl.F32, 4, 2, big, 8)):
+        assert status(ckl, f) == ckl.ERR_TOO_LARGE
+
+
 def test_cpp_header_compiles(tmp_path, ckl):
     """include/ckl/grouped.hpp compiles as C++17 and links against the library."""
     import os
