@@ -1450,6 +1450,10 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
 
 // Whether E_g holds an infinity or NaN: kExtChecks CTAs per adapter, a byte each for the answer.
 // Adapters without rows are not read.
+// It reads beside the kernel before it on the stream, which is one of the same call: that one writes
+// none of what is read here, and lets this one start only after its own wait, when everything before
+// it has completed.  The reads go to L2 for that reason, and the wait comes at the end, so that
+// nobody who waits for this kernel overtakes the other.
 struct ExtCheckParams {
     const int* offsets;
     const unsigned short* e;
@@ -1460,12 +1464,11 @@ struct ExtCheckParams {
 };
 constexpr int kExtCheckThreads = 1024;
 __global__ void __launch_bounds__(kExtCheckThreads) ext_check_kernel(const ExtCheckParams p) {
-    ptx::grid_dependency_wait();
     ptx::launch_dependents();
     const int g = static_cast<int>(blockIdx.x);
     const unsigned short* e = p.e + static_cast<size_t>(g) * p.stride;
     bool bad = false;
-    if (p.offsets[g] < p.offsets[g + 1]) {
+    if (__ldcg(p.offsets + g) < __ldcg(p.offsets + g + 1)) {
         // 16-byte units, dealt to the threads of the adapter's CTAs; (row, unit) advances without
         // a division.
         const int units = (p.cols + 7) / 8;
@@ -1486,10 +1489,10 @@ __global__ void __launch_bounds__(kExtCheckThreads) ext_check_kernel(const ExtCh
                 if (r < p.rows) {
                     const unsigned short* src = e + static_cast<size_t>(r) * p.ld + u * 8;
                     if (u * 8 + 8 <= p.cols) {
-                        w[i] = *reinterpret_cast<const uint4*>(src);
+                        w[i] = __ldcg(reinterpret_cast<const uint4*>(src));
                     } else {
                         for (int k = 0; u * 8 + k < p.cols; ++k) {
-                            bad |= (src[k] & p.exponent) == p.exponent;
+                            bad |= (__ldcg(src + k) & p.exponent) == p.exponent;
                         }
                     }
                 }
@@ -1507,6 +1510,7 @@ __global__ void __launch_bounds__(kExtCheckThreads) ext_check_kernel(const ExtCh
         }
     }
     const int any = __syncthreads_or(bad);
+    ptx::grid_dependency_wait();
     if (threadIdx.x == 0) {
         p.flags[g * kExtChecks + blockIdx.y] = any != 0 ? 1 : 0;
     }
