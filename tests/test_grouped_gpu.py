@@ -660,3 +660,27 @@ def test_offsets_that_pass_32_bits(ckl, sizes):
         x, d = a[at:at + size].double(), gr[at:at + size].double()
         check(stack[g * far:g * far + k * n].view(k, n).float(), x.T @ d, x.T.abs() @ d.abs(), max(size, 1), "bf16")
         at += size
+
+
+def test_lora_weights_written_just_before_the_call(ckl):
+    """The check for adapters that are not finite reads beside the kernel before it: it must see what the
+    stream wrote last.  One adapter's weights change between finite and NaN before every call."""
+    g, m, n, k, r = 9, 900, 1040, 72, 24
+    ids = torch.randint(0, g, (m,), device="cuda", dtype=torch.int32,
+                        generator=torch.Generator(device="cuda").manual_seed(80))
+    m, x, w, a, b, s, offs, rows = lora_case(ckl, ids, g, k, n, r, "bf16", 81)
+    size = ckl.gemm_lora_workspace_bytes(m, r)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    y = torch.empty(24, m, n, device="cuda", dtype=torch.bfloat16)
+    good, bad = b[4].clone(), torch.full_like(b[4], float("nan"))
+    for i in range(24):
+        b[4].copy_(bad if i % 3 == 1 else good)
+        ckl.gemm_lora(ckl.BF16, x, w, a, b, s, y[i], ckl.BF16, offs, rows, g, m, n, k, r, ws, size,
+                      stream=torch.cuda.current_stream())
+    mine = ids == 4
+    for i in range(24):
+        assert torch.equal(y[i][~mine], y[0][~mine])
+        if i % 3 == 1:
+            assert y[i][mine].isnan().all()
+        else:
+            assert torch.equal(y[i][mine], y[0][mine])
