@@ -311,8 +311,7 @@ int ckl_group_rows(const int* ids, int slots, int groups, int slots_per_row, int
     p.positions = positions;
     p.slots = slots;
     p.groups = groups;
-    p.slots_per_row = slots_per_row;
-    p.inv_row = slots_per_row < 512 ? (1ull << 40) / static_cast<unsigned long long>(slots_per_row) + 1 : 0;
+    p.inv_row = detail::reciprocal_of(slots_per_row);
     p.warp_slots = static_cast<int>(((slots + warps - 1) / warps + 31) / 32 * 32);
     const auto smem_of = [](int bins, int staged_slots) {
         return (kOrderWarps * bins + 2 * bins + kOrderWarps + (bins + 1) / 2 * 2 + 2) * 4 + staged_slots * 8;

@@ -497,13 +497,32 @@ constexpr int kMaxOrderCluster = 8;
 constexpr int kOrderStaged = kOrderThreads * 8;  // slots of a CTA that are sorted in shared memory
 constexpr int kOrderSteps = 8;  // of 32 slots that a warp holds in registers
 
+namespace detail {
+
+// s / d for 0 <= s < 2^31 and 1 <= d < 2^31 by a multiplication: with r = 2^64 / d rounded up,
+// s r = 2^64 s / d + s e where 0 <= e < 1, and s e < 2^64 / d, so the upper word of s r is the quotient.
+// (r of d = 1 does not fit in 64 bits: 0 stands for it.)
+__host__ __device__ inline unsigned long long reciprocal_of(int d) {
+    return d == 1 ? 0ull : ~0ull / static_cast<unsigned long long>(d) + 1ull;
+}
+__host__ __device__ inline int quotient(int s, unsigned long long r) {
+    if (r == 0ull) {
+        return s;
+    }
+    // the two halves of r one after the other: s < 2^32, so neither product passes 64 bits
+    const unsigned long long n = static_cast<unsigned int>(s);
+    return static_cast<int>((n * (r >> 32) + ((n * (r & 0xffffffffull)) >> 32)) >> 32);
+}
+
+}  // namespace detail
+
 struct GroupRowsParams {
     const int* ids;
     int* offsets;
     int* rows;
     int* positions;
-    int slots, groups, slots_per_row;
-    unsigned long long inv_row;  // floor(2^40 / slots_per_row) + 1, or 0: divide
+    int slots, groups;
+    unsigned long long inv_row;  // reciprocal_of(slots_per_row)
     int staged;      // a CTA's slots fit in shared memory, sorted
     int warp_slots;  // consecutive slots of one warp, a multiple of 32
 };
@@ -713,8 +732,7 @@ __global__ void __launch_bounds__(kOrderThreads) group_rows_kernel(const GroupRo
                 const int in_bin = mine[bin[i]] + __popc(same[i] & ((1u << lane) - 1u));
                 const int pos = start[bin[i]] + in_bin;
                 p.positions[s] = pos;
-                // s / slots_per_row, exact for slots_per_row < 512 as s < 2^31
-                const int row = p.inv_row != 0 ? static_cast<int>(s * p.inv_row >> 40) : s / p.slots_per_row;
+                const int row = detail::quotient(s, p.inv_row);
                 if (p.staged) {
                     sorted[local[bin[i]] + in_bin] = make_int2(pos, row);
                 } else {

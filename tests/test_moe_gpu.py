@@ -254,3 +254,21 @@ def test_combine_and_gradient(ckl, t, k, n, dt, out):
     ref = torch.full((rows, n), 9.0, dtype=torch.float64, device="cuda")
     ref[perm[ok].long()] = (w.double().unsqueeze(2) * dout.double().unsqueeze(1))[ok]
     assert ((dy.double() - ref).abs() <= (HALF_STEP[dt] + 2.0 ** -23) * ref.abs() + (2.0 ** -25 if dt == "f16" else 0)).all()
+
+
+@pytest.mark.parametrize("slots,per_row", [(2 ** 24 + 3001, 1), (2 ** 25 + 11, 2), (2 ** 27 + 4103, 8)])
+def test_group_rows_past_row_2_24(ckl, slots, per_row):
+    """Rows from 2^24 on.  Five slots of group 1 come first and end up last, so every place is known."""
+    ids = torch.zeros(slots, dtype=torch.int32, device="cuda")
+    ids[:5] = 1
+    offs = torch.empty(3, dtype=torch.int32, device="cuda")
+    rows, pos = (torch.full((slots,), -5, dtype=torch.int32, device="cuda") for _ in range(2))
+    ckl.group_rows(ids, slots, 2, offs, rows, pos, slots_per_row=per_row)
+    assert offs.tolist() == [0, slots - 5, slots]
+    step = 1 << 24
+    for at in range(0, slots, step):
+        s = torch.arange(at, min(at + step, slots), device="cuda")
+        want = torch.where(s < 5, s + slots - 5, s - 5)
+        assert torch.equal(pos[at:at + step].long(), want)
+        slot = torch.where(s < slots - 5, s + 5, s - (slots - 5))  # the slot at position s
+        assert torch.equal(rows[at:at + step].long(), slot // per_row)
