@@ -309,9 +309,9 @@ _lib.ckl_gemm_grouped.argtypes = [_i, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _
                                   _f, _f, _vp]
 _lib.ckl_gemm_grouped_wgrad.argtypes = [_i, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _ll,
                                         _f, _f, _vp]
-_lib.ckl_moe_combine.argtypes = [_i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp]
-_lib.ckl_moe_combine_backward.argtypes = [_i, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i,
-                                          _vp]
+_lib.ckl_moe_combine_ex.argtypes = [_i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp]
+_lib.ckl_moe_combine_backward_ex.argtypes = [_i, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i,
+                                             _vp, _vp]
 _lib.ckl_gemm_lora_workspace_bytes.argtypes = [_i, _i, _i]
 _lib.ckl_gemm_lora.argtypes = [_i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i,
                                _ll, _i, _ll, _i, _f, _vp, _sz, _vp]
@@ -319,7 +319,7 @@ _lib.ckl_gemm_lora_backward.argtypes = [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _
                                         _i, _i, _i, _i, _i, _i, _i, _i, _ll, _i, _ll, _i, _i, _ll, _i, _ll, _f,
                                         _vp, _sz, _vp]
 for _name in ("ckl_group_rows", "ckl_moe_route", "ckl_moe_route_backward", "ckl_gemm_grouped",
-              "ckl_gemm_grouped_wgrad", "ckl_moe_combine", "ckl_moe_combine_backward", "ckl_gemm_lora",
+              "ckl_gemm_grouped_wgrad", "ckl_moe_combine_ex", "ckl_moe_combine_backward_ex", "ckl_gemm_lora",
               "ckl_gemm_lora_backward"):
     getattr(_lib, _name).restype = ctypes.c_int
 _lib.ckl_gemm_lora_workspace_bytes.restype = _sz
@@ -376,20 +376,22 @@ def gemm_grouped_wgrad(ab_dtype, a, g, dw, dw_dtype, offsets, groups, rows, m, n
 
 
 def moe_combine(y_dtype, y, positions, weights, out, out_dtype, tokens, top_k, n, y_rows, ldy=None, ldo=None,
-                stream=None) -> None:
-    """out[t] = sum_j weights[t][j] * y[positions[t][j]]."""
-    _check(_lib.ckl_moe_combine(y_dtype, _ptr(y), _ptr(positions), _ptr(weights), _ptr(out), out_dtype, tokens,
-                                top_k, n, y_rows, n if ldy is None else ldy, n if ldo is None else ldo,
-                                _stream(stream)))
+                stream=None, kept=None) -> None:
+    """out[t] = sum_j weights[t][j] * y[positions[t][j]]; a weight of 0 adds nothing.  With ``kept``
+    (``offsets[groups:]`` on the device) positions from there on name no row."""
+    _check(_lib.ckl_moe_combine_ex(y_dtype, _ptr(y), _ptr(positions), _ptr(weights), _ptr(out), out_dtype, tokens,
+                                   top_k, n, y_rows, n if ldy is None else ldy, n if ldo is None else ldo,
+                                   _ptr(kept), _stream(stream)))
 
 
 def moe_combine_backward(y_dtype, y, positions, weights, dout, dout_dtype, dy, dweights, tokens, top_k, n,
-                         y_rows, ldy=None, ldo=None, lddy=None, stream=None) -> None:
-    """dy (y's type) and dweights (FP32) from the gradient of moe_combine's output."""
-    _check(_lib.ckl_moe_combine_backward(y_dtype, _ptr(y), _ptr(positions), _ptr(weights), _ptr(dout), dout_dtype,
-                                         _ptr(dy), _ptr(dweights), tokens, top_k, n, y_rows,
-                                         n if ldy is None else ldy, n if ldo is None else ldo,
-                                         n if lddy is None else lddy, _stream(stream)))
+                         y_rows, ldy=None, ldo=None, lddy=None, stream=None, kept=None) -> None:
+    """dy (y's type) and dweights (FP32) from the gradient of moe_combine's output.  With ``kept`` the
+    places behind the groups get 0 in dweights and leave dy as it is."""
+    _check(_lib.ckl_moe_combine_backward_ex(y_dtype, _ptr(y), _ptr(positions), _ptr(weights), _ptr(dout),
+                                            dout_dtype, _ptr(dy), _ptr(dweights), tokens, top_k, n, y_rows,
+                                            n if ldy is None else ldy, n if ldo is None else ldo,
+                                            n if lddy is None else lddy, _ptr(kept), _stream(stream)))
 
 
 def gemm_lora_workspace_bytes(m: int, rank: int, backward: bool = False) -> int:

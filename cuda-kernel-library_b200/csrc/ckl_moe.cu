@@ -161,7 +161,7 @@ int launch_combine_backward_out(int out_dtype, const CombineBackwardParams& p, b
 
 int check_combine(const char* what, int y_dtype, const void* y, const int* positions,
                   const float* weights, int out_dtype, const void* out, int top_k, int n, int y_rows,
-                  int ldy, int ldo) {
+                  int ldy, int ldo, const int* kept) {
     if (!known_dtype(y_dtype) || !known_dtype(out_dtype)) {
         return set_error(CKL_ERR_INVALID_ARG, "%s: bad dtype %d or %d", what, y_dtype, out_dtype);
     }
@@ -176,7 +176,7 @@ int check_combine(const char* what, int y_dtype, const void* y, const int* posit
         return set_error(CKL_ERR_INVALID_ARG, "%s: null pointer", what);
     }
     if (misaligned(y, size_of(y_dtype)) || misaligned(out, size_of(out_dtype)) ||
-        misaligned(positions, 4) || misaligned(weights, 4)) {
+        misaligned(positions, 4) || misaligned(weights, 4) || misaligned(kept, 4)) {
         return set_error(CKL_ERR_INVALID_ARG, "%s: a pointer is not aligned to its element", what);
     }
     return CKL_OK;
@@ -327,14 +327,14 @@ int ckl_group_rows(const int* ids, int slots, int groups, int slots_per_row, int
     return CKL_OK;
 }
 
-int ckl_moe_combine(int y_dtype, const void* y, const int* positions, const float* weights, void* out,
-                    int out_dtype, int tokens, int top_k, int n, int y_rows, int ldy, int ldo,
-                    ckl_stream_t stream) {
+int ckl_moe_combine_ex(int y_dtype, const void* y, const int* positions, const float* weights, void* out,
+                       int out_dtype, int tokens, int top_k, int n, int y_rows, int ldy, int ldo,
+                       const int* kept, ckl_stream_t stream) {
     if (tokens <= 0 || n <= 0) {
         return CKL_OK;
     }
     if (const int rc = check_combine("moe_combine", y_dtype, y, positions, weights, out_dtype, out, top_k, n,
-                                     y_rows, ldy, ldo);
+                                     y_rows, ldy, ldo, kept);
         rc != CKL_OK) {
         return rc;
     }
@@ -342,7 +342,7 @@ int ckl_moe_combine(int y_dtype, const void* y, const int* positions, const floa
     if (const int rc = device_view(&view); rc != CKL_OK) {
         return rc;
     }
-    const CombineParams p = {y, positions, weights, out, tokens, top_k, n, y_rows, ldy, ldo};
+    const CombineParams p = {y, positions, weights, out, tokens, top_k, n, y_rows, ldy, ldo, kept};
     const bool vec = n % 8 == 0 && aligned16(y, ldy, y_dtype) && aligned16(out, ldo, out_dtype);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (y_dtype) {
@@ -352,15 +352,15 @@ int ckl_moe_combine(int y_dtype, const void* y, const int* positions, const floa
     }
 }
 
-int ckl_moe_combine_backward(int y_dtype, const void* y, const int* positions, const float* weights,
-                             const void* dout, int dout_dtype, void* dy, float* dweights, int tokens,
-                             int top_k, int n, int y_rows, int ldy, int ldo, int lddy,
-                             ckl_stream_t stream) {
+int ckl_moe_combine_backward_ex(int y_dtype, const void* y, const int* positions, const float* weights,
+                                const void* dout, int dout_dtype, void* dy, float* dweights, int tokens,
+                                int top_k, int n, int y_rows, int ldy, int ldo, int lddy,
+                                const int* kept, ckl_stream_t stream) {
     if (tokens <= 0 || n <= 0) {
         return CKL_OK;
     }
     if (const int rc = check_combine("moe_combine_backward", y_dtype, y, positions, weights, dout_dtype, dout,
-                                     top_k, n, y_rows, ldy, ldo);
+                                     top_k, n, y_rows, ldy, ldo, kept);
         rc != CKL_OK) {
         return rc;
     }
@@ -375,7 +375,7 @@ int ckl_moe_combine_backward(int y_dtype, const void* y, const int* positions, c
         return rc;
     }
     const CombineBackwardParams p = {y, positions, weights, dout, dy, dweights, tokens, top_k, n, y_rows,
-                                     ldy, ldo, lddy};
+                                     ldy, ldo, lddy, kept};
     const bool vec = n % 8 == 0 && aligned16(y, ldy, y_dtype) && aligned16(dout, ldo, dout_dtype) &&
                      aligned16(dy, lddy, y_dtype);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -384,6 +384,20 @@ int ckl_moe_combine_backward(int y_dtype, const void* y, const int* positions, c
         case CKL_BF16: return launch_combine_backward_out<__nv_bfloat16>(dout_dtype, p, vec, s);
         default: return launch_combine_backward_out<float>(dout_dtype, p, vec, s);
     }
+}
+
+int ckl_moe_combine(int y_dtype, const void* y, const int* positions, const float* weights, void* out,
+                    int out_dtype, int tokens, int top_k, int n, int y_rows, int ldy, int ldo,
+                    ckl_stream_t stream) {
+    return ckl_moe_combine_ex(y_dtype, y, positions, weights, out, out_dtype, tokens, top_k, n, y_rows, ldy, ldo,
+                              nullptr, stream);
+}
+
+int ckl_moe_combine_backward(int y_dtype, const void* y, const int* positions, const float* weights,
+                             const void* dout, int dout_dtype, void* dy, float* dweights, int tokens,
+                             int top_k, int n, int y_rows, int ldy, int ldo, int lddy, ckl_stream_t stream) {
+    return ckl_moe_combine_backward_ex(y_dtype, y, positions, weights, dout, dout_dtype, dy, dweights, tokens, top_k,
+                                       n, y_rows, ldy, ldo, lddy, nullptr, stream);
 }
 
 }  // extern "C"

@@ -798,11 +798,23 @@ struct CombineParams {
     void* out;
     int tokens, top_k, n, y_rows;
     int ldy, ldo;
+    const int* kept;  // or nullptr
 };
+
+namespace detail {
+
+// Rows of y that exist: y_rows, or fewer where the device knows better (the positions behind the last
+// group hold no expert's row, and nobody wrote them).
+__device__ __forceinline__ int rows_that_exist(int y_rows, const int* kept) {
+    return kept != nullptr ? min(y_rows, *kept) : y_rows;
+}
+
+}  // namespace detail
 
 // out[t] = sum_j weights[t][j] * y[positions[t][j]], summed in FP32 in the order of j.  One
 // thread per 8 columns of one token (kVec) or per column; memory-bound: y is read once.
-// A position outside [0, y_rows) adds nothing.
+// A position that names no row adds nothing, nor does a weight of 0: it may stand for a place that
+// routing could not fill, whose row of y is whatever the memory held before.
 template <typename T, typename OutT, bool kVec>
 __global__ void __launch_bounds__(kCombineThreads) moe_combine_kernel(const CombineParams p) {
     ptx::grid_dependency_wait();
@@ -818,12 +830,13 @@ __global__ void __launch_bounds__(kCombineThreads) moe_combine_kernel(const Comb
     const T* y = static_cast<const T*>(p.y) + col;
     const int* pos = p.positions + t * p.top_k;
     const float* w = p.weights + t * p.top_k;
+    const int rows = detail::rows_that_exist(p.y_rows, p.kept);
     float acc[V] = {};
 #pragma unroll 8
     for (int j = 0; j < p.top_k; ++j) {
         const int at = __ldg(pos + j);
         const float f = __ldg(w + j);
-        if (at < 0 || at >= p.y_rows) {
+        if (at < 0 || at >= rows || f == 0.0f) {
             continue;
         }
         const T* src = y + static_cast<size_t>(at) * p.ldy;
@@ -855,6 +868,7 @@ struct CombineBackwardParams {
     float* dweights;
     int tokens, top_k, n, y_rows;
     int ldy, ldo, lddy;
+    const int* kept;  // or nullptr
 };
 
 // One warp per slot (t, j): dy[positions[t][j]] = weights[t][j] * dout[t] and
@@ -876,7 +890,7 @@ moe_combine_backward_kernel(const CombineBackwardParams p) {
     }
     const int at = __ldg(p.positions + slot);
     const float w = __ldg(p.weights + slot);
-    const bool exists = at >= 0 && at < p.y_rows;
+    const bool exists = at >= 0 && at < detail::rows_that_exist(p.y_rows, p.kept);
     float dot = 0.0f;
     if (exists) {
         const OutT* dout = static_cast<const OutT*>(p.dout) + static_cast<size_t>(t) * p.ldo;

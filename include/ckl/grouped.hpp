@@ -72,19 +72,19 @@ inline void gemm_grouped_wgrad(const InT* a, const int* a_rows, int a_count, con
 
 template <typename T, typename OutT>
 inline void moe_combine(const T* y, const int* positions, const float* weights, OutT* out, int tokens, int top_k,
-                        int n, int y_rows, cudaStream_t stream = nullptr) {
-    detail::throw_on_error(ckl_moe_combine(detail::dtype_of(y), y, positions, weights, out, detail::dtype_of(out),
-                                           tokens, top_k, n, y_rows, n, n, stream),
+                        int n, int y_rows, cudaStream_t stream = nullptr, const int* kept = nullptr) {
+    detail::throw_on_error(ckl_moe_combine_ex(detail::dtype_of(y), y, positions, weights, out, detail::dtype_of(out),
+                                              tokens, top_k, n, y_rows, n, n, kept, stream),
                            "moe_combine");
 }
 
 template <typename T, typename OutT>
 inline void moe_combine_backward(const T* y, const int* positions, const float* weights, const OutT* dout, T* dy,
                                  float* dweights, int tokens, int top_k, int n, int y_rows,
-                                 cudaStream_t stream = nullptr) {
+                                 cudaStream_t stream = nullptr, const int* kept = nullptr) {
     detail::throw_on_error(
-        ckl_moe_combine_backward(detail::dtype_of(y), y, positions, weights, dout, detail::dtype_of(dout), dy,
-                                 dweights, tokens, top_k, n, y_rows, n, n, n, stream),
+        ckl_moe_combine_backward_ex(detail::dtype_of(y), y, positions, weights, dout, detail::dtype_of(dout), dy,
+                                    dweights, tokens, top_k, n, y_rows, n, n, n, kept, stream),
         "moe_combine_backward");
 }
 

@@ -355,19 +355,32 @@ int ckl_gemm_grouped_wgrad(int ab_dtype, const void* a, const int* a_rows, int a
                            ckl_stream_t stream);
 
 /* Rows back to their tokens: out[t] = sum over j < top_k of weights[t][j] * y[positions[t][j]],
- * summed in FP32 in the order of j.  y: y_rows x n, out: tokens x n, any types; a position outside
- * [0, y_rows) adds nothing.  tokens <= 0 or n <= 0 is a no-op. */
+ * summed in FP32 in the order of j.  y: y_rows x n, out: tokens x n, any types.  A position outside
+ * [0, y_rows) adds nothing, and a weight of 0 adds nothing whatever its row holds: the places that
+ * ckl_moe_route could not fill have weight 0 and positions behind the last group, in rows that
+ * ckl_gemm_grouped leaves as they were.  tokens <= 0 or n <= 0 is a no-op.
+ * The _ex form also takes `kept`, NULL or a pointer to offsets[groups] on the device: positions from
+ * there on name no row, whatever their weight. */
 int ckl_moe_combine(int y_dtype, const void* y, const int* positions, const float* weights, void* out,
                     int out_dtype, int tokens, int top_k, int n, int y_rows, int ldy, int ldo,
                     ckl_stream_t stream);
+int ckl_moe_combine_ex(int y_dtype, const void* y, const int* positions, const float* weights, void* out,
+                       int out_dtype, int tokens, int top_k, int n, int y_rows, int ldy, int ldo,
+                       const int* kept, ckl_stream_t stream);
 
 /* Its gradient: dy[positions[t][j]] = weights[t][j] * dout[t] (dy in y's type; rows that no position
  * names are left as they are; a row named twice holds one of the two) and
- * dweights[t][j] = <dout[t], y[positions[t][j]]>. */
+ * dweights[t][j] = <dout[t], y[positions[t][j]]>, 0 for a position that names no row.  Without `kept`
+ * the places that routing could not fill get their product with whatever their row of y holds;
+ * ckl_moe_route_backward does not look at it. */
 int ckl_moe_combine_backward(int y_dtype, const void* y, const int* positions, const float* weights,
                              const void* dout, int dout_dtype, void* dy, float* dweights, int tokens,
                              int top_k, int n, int y_rows, int ldy, int ldo, int lddy,
                              ckl_stream_t stream);
+int ckl_moe_combine_backward_ex(int y_dtype, const void* y, const int* positions, const float* weights,
+                                const void* dout, int dout_dtype, void* dy, float* dweights, int tokens,
+                                int top_k, int n, int y_rows, int ldy, int ldo, int lddy, const int* kept,
+                                ckl_stream_t stream);
 
 /* Low-rank adapters beside a shared projection.  Row i of x uses adapter g (or none):
  *     y[i] = x[i] W + scales[g] * (x[i] A_g) B_g + beta * y[i]

@@ -272,3 +272,47 @@ def test_group_rows_past_row_2_24(ckl, slots, per_row):
         assert torch.equal(pos[at:at + step].long(), want)
         slot = torch.where(s < slots - 5, s + 5, s - (slots - 5))  # the slot at position s
         assert torch.equal(rows[at:at + step].long(), slot // per_row)
+
+
+
+@pytest.mark.parametrize("t,k,n,dt,out", [(5, 3, 64, "bf16", "bf16"), (9, 4, 7, "f32", "f16"), (300, 8, 136, "f16", "f32")])
+@pytest.mark.parametrize("known", [False, True], ids=["weight_0", "kept"])
+def test_combine_leaves_out_rows_that_no_group_holds(ckl, t, k, n, dt, out, known):
+    """Slots of no group stand behind the groups, where y was never written.  A weight of 0 adds nothing
+    there; with `kept` a weight of any size does not, and the gradients know it too."""
+    g = torch.Generator(device="cuda").manual_seed(t + n)
+    slots, groups = t * k, 4
+    ids = torch.randint(-1, groups, (t, k), generator=g, device="cuda", dtype=torch.int32)
+    ids[0] = -1  # a token of no group at all
+    offs = torch.empty(groups + 1, dtype=torch.int32, device="cuda")
+    rows, pos = (torch.empty(slots, dtype=torch.int32, device="cuda") for _ in range(2))
+    ckl.group_rows(ids, slots, groups, offs, rows, pos, slots_per_row=k)
+    kept = int(offs[-1])
+    y = torch.full((slots, n), math.nan, device="cuda").to(DT[dt])
+    y[:kept] = torch.randn(kept, n, generator=g, device="cuda").to(DT[dt])
+    some = ids >= 0
+    w = torch.randn(t, k, generator=g, device="cuda")
+    if not known:
+        w = torch.where(some, w, 0.0)
+    end = dict(kept=offs[groups:]) if known else {}
+    res = torch.full((t, n), 3.0, dtype=DT[out], device="cuda")
+    ckl.moe_combine(code(ckl, dt), y, pos, w, res, code(ckl, out), t, k, n, slots, **end)
+    at = pos.view(t, k).long()
+    picked = torch.where(some.unsqueeze(2), y[at].double(), 0.0)
+    terms = w.double().unsqueeze(2) * picked
+    ref = terms.sum(1)
+    tiny = 2.0 ** -25 if out == "f16" else 0.0
+    assert ((res.double() - ref).abs() <= HALF_STEP[out] * ref.abs() + (k + 1) * 2.0 ** -24 * terms.abs().sum(1) + tiny).all()
+    assert (res[0] == 0).all()
+    if not known:
+        return
+    dout = torch.randn(t, n, generator=g, device="cuda").to(DT[out])
+    dy = torch.full((slots, n), 9.0, dtype=DT[dt], device="cuda")
+    dw = torch.full((t, k), math.nan, device="cuda")
+    ckl.moe_combine_backward(code(ckl, dt), y, pos, w, dout, code(ckl, out), dy, dw, t, k, n, slots, **end)
+    prod = picked * dout.double().unsqueeze(1)
+    assert ((dw.double() - prod.sum(2)).abs() <= (n + 2) * 2.0 ** -24 * prod.abs().sum(2)).all()
+    assert (dw[~some] == 0).all() and (dy[kept:] == 9.0).all()
+    want = (w.double().unsqueeze(2) * dout.double().unsqueeze(1))[some]
+    tiny = 2.0 ** -25 if dt == "f16" else 0.0
+    assert ((dy[at[some]].double() - want).abs() <= (HALF_STEP[dt] + 2.0 ** -23) * want.abs() + tiny).all()

@@ -52,3 +52,12 @@ int main() {
     return 0;
 }
 """)
+
+
+def test_combine_refuses_a_misaligned_row_count(ckl):
+    p = 1 << 20
+    for call in (lambda: ckl.moe_combine(ckl.F32, p, p, p, p, ckl.F32, 4, 2, 64, 8, kept=p + 2),
+                 lambda: ckl.moe_combine_backward(ckl.F32, p, p, p, p, ckl.F32, p, p, 4, 2, 64, 8, kept=p + 1)):
+        with pytest.raises(ckl.CklError) as e:
+            call()
+        assert e.value.status == ckl.ERR_INVALID_ARG

@@ -226,3 +226,25 @@ def test_adapters_in_a_graph_beside_the_dense_kernel(ckl):
         torch.cuda.synchronize()
         for t, u in zip((y, dx, da, db, dense), want):
             assert torch.equal(t, u)
+
+
+
+def test_layer_with_tokens_that_route_nowhere(ckl):
+    """Padded tokens (every logit -inf) and tokens with fewer experts than places, in buffers that hold NaN
+    from before: the same bits as in zeroed buffers, and nothing from a place that holds no expert."""
+    got = []
+    for old in (0.0, float("nan")):
+        s = Layer(ckl, 60)
+        s.logits[T - 7:] = -float("inf")
+        s.logits[11, 2:] = -float("inf")  # two experts for three places
+        for buf in (s.h, s.y, s.out, s.dy, s.dh, s.dxr, s.dw1, s.dw2, s.dlogits, s.weights):
+            buf.fill_(old)
+        s.forward(torch.cuda.current_stream())
+        s.backward(torch.cuda.current_stream())
+        torch.cuda.synchronize()
+        kept = int(s.offsets[-1])
+        assert kept == T * K - 7 * K - 1 and (s.experts[T - 7:] == -1).all() and (s.experts[11, 2:] == -1).all()
+        assert (s.out[T - 7:] == 0).all() and (s.dlogits[T - 7:] == 0).all()
+        got.append([s.out, s.weights, s.experts, s.positions, s.dxr[:kept], s.dw1, s.dw2, s.dlogits])
+    for a, b in zip(*got):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
