@@ -1463,45 +1463,65 @@ struct ExtCheckParams {
     unsigned int exponent;         // all ones: 0x7f80 (BF16) or 0x7c00 (FP16)
 };
 constexpr int kExtCheckThreads = 1024;
+
+namespace detail {
+
+// Walks the 16-byte units of a matrix, `units` a row, in steps of `step` of them without a division.
+// Rows are counted without a sign: a walk may take a few steps of up to `step` rows past the last one
+// before it is looked at again, which from 2^31 - 4096 rows would turn a signed count negative.
+struct UnitWalk {
+    unsigned int r;
+    int u, units, rows_per_step, units_per_step;
+
+    __host__ __device__ UnitWalk(int first, int step, int units_in_row)
+        : r(static_cast<unsigned int>(first / units_in_row)),
+          u(first % units_in_row),
+          units(units_in_row),
+          rows_per_step(step / units_in_row),
+          units_per_step(step % units_in_row) {}
+    __host__ __device__ bool inside(int rows) const { return r < static_cast<unsigned int>(rows); }
+    __host__ __device__ void advance() {
+        r += static_cast<unsigned int>(rows_per_step);
+        u += units_per_step;
+        if (u >= units) {
+            u -= units;
+            ++r;
+        }
+    }
+};
+
+}  // namespace detail
+
 __global__ void __launch_bounds__(kExtCheckThreads) ext_check_kernel(const ExtCheckParams p) {
     ptx::launch_dependents();
     const int g = static_cast<int>(blockIdx.x);
     const unsigned short* e = p.e + static_cast<size_t>(g) * p.stride;
     bool bad = false;
     if (__ldcg(p.offsets + g) < __ldcg(p.offsets + g + 1)) {
-        // 16-byte units, dealt to the threads of the adapter's CTAs; (row, unit) advances without
-        // a division.
-        const int units = (p.cols + 7) / 8;
-        const int step = kExtChecks * kExtCheckThreads;
-        const int first = static_cast<int>(blockIdx.y) * kExtCheckThreads + static_cast<int>(threadIdx.x);
-        const int rows_per_step = step / units, units_per_step = step - rows_per_step * units;
-        int r = first / units, u = first - r * units;
+        // 16-byte units, dealt to the threads of the adapter's CTAs.
+        detail::UnitWalk at(static_cast<int>(blockIdx.y) * kExtCheckThreads + static_cast<int>(threadIdx.x),
+                            kExtChecks * kExtCheckThreads, (p.cols + 7) / 8);
         const unsigned int both = p.exponent * 0x10001u;
         auto odd = [&](uint32_t w) {
             const uint32_t x = (w & both) ^ both;  // a half that is zero has its exponent all ones
             return (x & 0xffffu) == 0 || (x >> 16) == 0;
         };
-        while (r < p.rows) {
+        while (at.inside(p.rows)) {
             uint4 w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 w[i] = make_uint4(0, 0, 0, 0);
-                if (r < p.rows) {
-                    const unsigned short* src = e + static_cast<size_t>(r) * p.ld + u * 8;
-                    if (u * 8 + 8 <= p.cols) {
+                if (at.inside(p.rows)) {
+                    const unsigned short* src = e + static_cast<size_t>(at.r) * p.ld + at.u * 8;
+                    if (at.u * 8 + 8 <= p.cols) {
                         w[i] = __ldcg(reinterpret_cast<const uint4*>(src));
                     } else {
-                        for (int k = 0; u * 8 + k < p.cols; ++k) {
+                        for (int k = 0; at.u * 8 + k < p.cols; ++k) {
                             bad |= (__ldcg(src + k) & p.exponent) == p.exponent;
                         }
                     }
                 }
-                r += rows_per_step;
-                u += units_per_step;
-                if (u >= units) {
-                    u -= units;
-                    ++r;
-                }
+                at.advance();
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -1532,6 +1552,11 @@ struct LoraRowsParams {
 };
 constexpr int kLoraRowsThreads = 1024;  // k 4096, rank 16: one batch of eight loads per thread
 constexpr int kLoraRanks = 32;
+
+namespace detail {
+// Whether k, k + step, ... k + 7 step all lie below `limit`, and k + 8 step can be formed where they do.
+__host__ __device__ inline bool eight_steps_inside(int k, int step, int limit) { return k < limit - 7 * step; }
+}  // namespace detail
 
 template <typename T>
 __global__ void __launch_bounds__(kLoraRowsThreads) lora_rows_kernel(const LoraRowsParams p) {
@@ -1571,7 +1596,7 @@ __global__ void __launch_bounds__(kLoraRowsThreads) lora_rows_kernel(const LoraR
     int k = static_cast<int>(threadIdx.x) >> shift;
     if (exists && have == 8) {
         // eight loads of either operand in flight
-        for (; k + 7 * step < p.k; k += 8 * step) {
+        for (; detail::eight_steps_inside(k, step, p.k); k += 8 * step) {
             float f[8], v[8][8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {

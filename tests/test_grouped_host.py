@@ -210,3 +210,49 @@ int main(int argc, char**) {
                     os.path.join(root, "include"), "-o", str(exe), str(src), ckl.LIB_PATH,
                     "-Xlinker", f"-rpath={os.path.dirname(ckl.LIB_PATH)}"], check=True)
     assert subprocess.run([str(exe)]).returncode == 0
+
+
+def test_steps_at_the_largest_extent(tmp_path):
+    """The walks of the adapters' kernels at the largest row count that is accepted: compiled for the host,
+    no step may come back below the limit after it has passed it."""
+    from test_moe_host import run_host
+    run_host(tmp_path, """
+#include <cstdio>
+#include "gemm_grouped.cuh"
+#include "ckl_internal.h"
+int main() {
+    const int limit = ckl::kMaxExtent, step = ckl::kExtChecks * ckl::kExtCheckThreads;
+    for (int units : {1, 2, 3, 16, 17, 520, step, step + 1, 1 << 20}) {
+        for (int first : {0, 1, 37, step - 1}) {
+            for (int rows : {1, 5, 4096, limit - 1, limit}) {
+                ckl::detail::UnitWalk at(first, step, units);
+                if (rows > 1 << 20) {  // straight to the last rows
+                    const unsigned long long steps = (static_cast<unsigned long long>(rows - 1) * units) / step;
+                    const unsigned long long unit = first + steps * step;
+                    at.r = static_cast<unsigned int>(unit / units);
+                    at.u = static_cast<int>(unit % units);
+                }
+                unsigned long long unit = static_cast<unsigned long long>(at.r) * units + at.u;
+                for (int i = 0; i < 12; ++i, unit += step) {  // inside a batch of four, and as far again behind it
+                    const bool inside = unit / units < static_cast<unsigned long long>(rows);
+                    if (at.inside(rows) != inside || (inside && (at.r != unit / units || at.u != int(unit % units)))) {
+                        std::printf("rows %d, units %d, first %d, step %d\\n", rows, units, first, i);
+                        return 1;
+                    }
+                    at.advance();
+                }
+            }
+        }
+    }
+    for (int s : {128, 256, 1024}) {
+        for (int k = limit - 9 * s; k < limit; ++k) {
+            const bool inside = k + 7ll * s < limit;
+            if (ckl::detail::eight_steps_inside(k, s, limit) != inside || (inside && k + 8ll * s > 0x7fffffffll)) return 2;
+        }
+        for (int k = 0; k < 9 * s; ++k) {
+            for (int n : {1, 7, s, 8 * s}) if (ckl::detail::eight_steps_inside(k, s, n) != (k + 7 * s < n)) return 3;
+        }
+    }
+    return 0;
+}
+""")
