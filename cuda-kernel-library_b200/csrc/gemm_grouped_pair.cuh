@@ -386,8 +386,8 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                         return false;
                     }
                     if (loaded) {
-                        if (!detail::wait_barrier(loaded_bar(stage), (loaded_phase >> stage) & 1u, ctl, kRoleMma,
-                                                  0x40000000u | it)) {
+                        if (!detail::wait_barrier<true>(loaded_bar(stage), (loaded_phase >> stage) & 1u, ctl,
+                                                        kRoleMma, 0x40000000u | it)) {
                             return false;
                         }
                         loaded_phase ^= 1u << stage;
@@ -483,10 +483,9 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
         auto hand_over = [&]() {
             load.finish();
             if (lane == 0) {
-                // The stage lies in this CTA's shared memory and this SM's tensor core reads it: the
-                // proxy fence in finish() has made the writes visible to it, the arrival only tells
-                // the issuing thread.  (The cluster-scope release form waits about 2500 cycles.)
-                ptx::mbar_arrive_cluster(ptx::map_to_cta(loaded_bar(own), 0));
+                // The stage lies in this CTA's shared memory, the thread that issues its MMAs may be the
+                // other CTA's.
+                ptx::mbar_arrive_cluster_publish(ptx::map_to_cta(loaded_bar(own), 0));
             }
         };
         detail::PairTile t;

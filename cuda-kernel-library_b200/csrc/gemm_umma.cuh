@@ -181,15 +181,25 @@ __device__ __forceinline__ void raise_abort(const Control& ctl, unsigned int rol
 
 // Bounded wait.  Returns false when the limit ran out here or another role
 // already aborted; the caller must then leave its loop.
+//
+// kCluster: arrivals publish shared memory of other CTAs of the cluster (mbar_arrive_cluster_publish).
+template <bool kCluster = false>
 __device__ __forceinline__ bool wait_barrier(uint32_t bar, uint32_t parity, const Control& ctl,
                                              unsigned int role, unsigned int detail_word) {
-    if (ptx::mbar_try_wait(bar, parity)) {
+    if (kCluster ? ptx::mbar_try_wait_cluster(bar, parity) : ptx::mbar_try_wait(bar, parity)) {
+        if (kCluster) {
+            ptx::fence_acquire_cluster_smem();
+        }
         return true;
     }
     unsigned long long t0 = 0;
     unsigned int spins = 0;
     while (true) {
-        if (ptx::mbar_try_wait_parked(bar, parity, 4000u)) {
+        if (kCluster ? ptx::mbar_try_wait_cluster_parked(bar, parity, 4000u)
+                     : ptx::mbar_try_wait_parked(bar, parity, 4000u)) {
+            if (kCluster) {
+                ptx::fence_acquire_cluster_smem();
+            }
             return true;
         }
         if ((++spins & 15u) == 0u) {

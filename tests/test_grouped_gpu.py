@@ -684,3 +684,74 @@ def test_lora_weights_written_just_before_the_call(ckl):
             assert y[i][mine].isnan().all()
         else:
             assert torch.equal(y[i][mine], y[0][mine])
+
+
+@pytest.mark.parametrize("trans", [False, True], ids=["nn", "nt"])
+@pytest.mark.parametrize("k", [1000, 2069])
+def test_grouped_pairs_long_sums(ckl, trans, k):
+    """Gathered rows on CTA pairs with sums that go round the ring of stages many times and end inside a
+    block; every repetition gives the same bits."""
+    sizes, n, tokens = many_groups(8, 40, 500), 264, 900
+    offs, rows = offsets_of(sizes), sum(sizes)
+    ldk = (k + 7) // 8 * 8
+    a = rand((tokens, ldk), torch.bfloat16, 1)
+    idx = torch.randint(0, tokens, (rows,), device="cuda", dtype=torch.int32)
+    b = rand((40, n, ldk) if trans else (40, k, n), torch.bfloat16, 2, k ** -0.5)
+    c = torch.empty(20, rows, n, device="cuda")
+    for out in c:
+        ckl.gemm_grouped(ckl.BF16, a, b, out, ckl.F32, offs, 40, rows, n, k, lda=ldk, ldb=ldk if trans else n,
+                         stride_b=b.stride(0), a_rows=idx, a_count=tokens, trans_b=trans)
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, c[0]) for out in c)
+    o = offs.tolist()
+    for g in range(40):
+        x, w = a[idx[o[g]:o[g + 1]].long(), :k].double(), (b[g, :, :k].t() if trans else b[g]).double()
+        check(c[0, o[g]:o[g + 1]], x @ w, x.abs() @ w.abs(), k, "f32")
+
+
+@pytest.mark.parametrize("gather", [False, True], ids=["rows", "gather"])
+def test_weight_gradient_pairs_long_sums(ckl, gather):
+    sizes, m, n, tokens = [1500, 0, 701, 64, 3001, 2048, 63, 833] * 3, 1032, 264, 700
+    offs, rows = offsets_of(sizes), sum(sizes)
+    a, d = rand((tokens if gather else rows, m), torch.float16, 1), rand((rows, n), torch.float16, 2)
+    idx = torch.randint(0, tokens, (rows,), device="cuda", dtype=torch.int32) if gather else None
+    w = torch.empty(20, len(sizes), m, n, device="cuda")
+    for out in w:
+        ckl.gemm_grouped_wgrad(ckl.F16, a, d, out, ckl.F32, offs, len(sizes), rows, m, n, a_rows=idx,
+                               a_count=tokens if gather else None)
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, w[0]) for out in w)
+    src, o = a[idx.long()] if gather else a, offs.tolist()
+    for g, size in enumerate(sizes):
+        x, y = src[o[g]:o[g + 1]].double(), d[o[g]:o[g + 1]].double()
+        check(w[0, g], x.t() @ y, x.abs().t() @ y.abs(), size, "f32")
+
+
+def test_lora_pairs_long_sums(ckl):
+    """A prefill batch over a long k, its rows scattered, adapters of rank 72: forward and the gradient of x."""
+    m, g, k, n, r = 2100, 7, 2056, 1032, 72
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    ids = torch.randint(-1, g, (m,), generator=gen, device="cuda", dtype=torch.int32)
+    m, x, w, a, b, s, offs, rows = lora_case(ckl, ids, g, k, n, r, "bf16", 130)
+    dy = rand((m, n), torch.bfloat16, 135)
+    size = ckl.gemm_lora_workspace_bytes(m, r, True)
+    ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    y, dx = torch.empty(10, m, n, device="cuda"), torch.empty(10, m, k, device="cuda")
+    for i in range(10):
+        ckl.gemm_lora(ckl.BF16, x, w, a, b, s, y[i], ckl.F32, offs, rows, g, m, n, k, r, ws, size)
+        ckl.gemm_lora_backward(ckl.BF16, dy, x, w, a, b, s, dx[i], ckl.F32, None, None, ckl.F32, offs, rows, g, m, n, k,
+                               r, ws, size)
+    torch.cuda.synchronize()
+    for i in range(10):
+        assert torch.equal(y[i], y[0]) and torch.equal(dx[i], dx[0])
+    for i in range(-1, g):
+        sel = ids == i
+        for v, ww, p1, p2, got in ((x, w, a, b, y[0]), (dy, w.t(), b.transpose(1, 2), a.transpose(1, 2), dx[0])):
+            v, ww = v[sel].double(), ww.double()
+            ref, mag, extra = v @ ww, v.abs() @ ww.abs(), 0.0
+            if i >= 0:
+                q1, q2 = p1[i].double(), p2[i].double()
+                t, ta = s[i].double() * (v @ q1), s[i].double() * (v.abs() @ q1.abs())
+                ref, mag = ref + t @ q2, mag + ta @ q2.abs()
+                extra = TWO_PART["bf16"] * (t.abs() @ q2.abs())
+            check(got[sel], ref, mag, 2 * max(k, n) + 2 * r, "f32", extra)
