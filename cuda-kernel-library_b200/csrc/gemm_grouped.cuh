@@ -467,7 +467,7 @@ struct Loader {
     __device__ __forceinline__ void part_of_unit(uint32_t dst, const void* row, int col, int have) const {
         uint32_t w[4] = {0, 0, 0, 0};
         for (int e = 0; e < have; ++e) {
-            const uint32_t v = __ldg(static_cast<const unsigned short*>(row) + col + e);
+            const uint32_t v = ptx::ld_global(static_cast<const unsigned short*>(row) + col + e);
             w[0] |= e == 0 ? v : e == 1 ? v << 16 : 0u;
             w[1] |= e == 2 ? v : e == 3 ? v << 16 : 0u;
             w[2] |= e == 4 ? v : e == 5 ? v << 16 : 0u;
@@ -705,7 +705,7 @@ __device__ __forceinline__ int row_of_c(const GroupedParams& p, const GroupedTil
     if (in_tile >= t.valid) {
         return -1;
     }
-    const int row = p.c_rows != nullptr ? __ldg(p.c_rows + t.p0 + in_tile) : t.p0 + in_tile;
+    const int row = p.c_rows != nullptr ? p.c_rows[t.p0 + in_tile] : t.p0 + in_tile;
     return row >= 0 && row < p.c_count ? row : -1;
 }
 
@@ -1093,7 +1093,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                     for (int q = 0; q < 4; ++q) {
                         const int r = q * 32 + static_cast<int>(lane);
                         const int at = r >= t.valid          ? -1
-                                       : p.a_rows != nullptr ? __ldg(p.a_rows + t.p0 + r)
+                                       : p.a_rows != nullptr ? p.a_rows[t.p0 + r]
                                                              : t.p0 + r;
                         src[q] = at < p.a_count ? at : -1;
                     }
@@ -1146,8 +1146,8 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                     for (int q = 0; q < 2; ++q) {
                         const int r = i0 + q * 32 + static_cast<int>(lane);
                         const bool in = kb < t.end && r < t.valid;
-                        const int at_a = !in ? -1 : p.a_rows != nullptr ? __ldg(p.a_rows + t.p0 + r) : t.p0 + r;
-                        const int at_b = !in ? -1 : p.b_rows != nullptr ? __ldg(p.b_rows + t.p0 + r) : t.p0 + r;
+                        const int at_a = !in ? -1 : p.a_rows != nullptr ? p.a_rows[t.p0 + r] : t.p0 + r;
+                        const int at_b = !in ? -1 : p.b_rows != nullptr ? p.b_rows[t.p0 + r] : t.p0 + r;
                         next_a[q] = at_a < p.a_count ? at_a : -1;
                         next_b[q] = at_b < p.b_count ? at_b : -1;
                     }
@@ -1215,7 +1215,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
             const int my_row = detail::row_of_c(p, t, in_tile);
             Elem* c_base = static_cast<Elem*>(p.c) +
                            (p.form == kFormWgrad ? static_cast<long long>(t.group) * p.c_stride : 0ll);
-            const float factor = p.alpha * (p.scales != nullptr ? __ldg(p.scales + t.group) : 1.0f);
+            const float factor = p.alpha * (p.scales != nullptr ? p.scales[t.group] : 1.0f);
             // All lanes wait: after a wait by one lane the warp may stay split in two, and the
             // code behind it then runs several times slower.
             const bool got = detail::wait_barrier(acc_full_bar(acc), parity, ctl, kRoleEpilogue, count);
@@ -1403,7 +1403,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
             const int sub = static_cast<int>(lane) % kLanesPerRow;
             const int col = t.n0 + sub * kVec;
             const int have = min(kVec, t.n0 + t.cols - col);
-            const float factor = p.alpha * (p.scales != nullptr ? __ldg(p.scales + t.group) : 1.0f);
+            const float factor = p.alpha * (p.scales != nullptr ? p.scales[t.group] : 1.0f);
             Elem* c_base = static_cast<Elem*>(p.c) +
                            (p.form == kFormWgrad ? static_cast<long long>(t.group) * p.c_stride : 0ll);
             const uint32_t parts = ring;
@@ -1581,7 +1581,7 @@ __global__ void __launch_bounds__(kLoraRowsThreads) lora_rows_kernel(const LoraR
     if (g < 0) {
         return;
     }
-    const int row = p.rows != nullptr ? __ldg(p.rows + pos) : pos;
+    const int row = p.rows != nullptr ? p.rows[pos] : pos;
     const bool exists = row >= 0 && row < p.m;
     const int ranks = min(kLoraRanks, p.rank - r0);
     // 16-byte units (8 ranks) per row of A_g: 1, 2 or 4; the other lanes take further rows.
@@ -1642,7 +1642,7 @@ __global__ void __launch_bounds__(kLoraRowsThreads) lora_rows_kernel(const LoraR
             for (int w = 0; w < kLoraRowsThreads / 32; ++w) {
                 v += part[w][r];
             }
-            v *= p.scales != nullptr ? __ldg(p.scales + g) : 1.0f;
+            v *= p.scales != nullptr ? p.scales[g] : 1.0f;
         }
         T* dst = reinterpret_cast<T*>(p.t) + static_cast<size_t>(pos) * 2 * p.part_cols + r0 + r;
         T hi;

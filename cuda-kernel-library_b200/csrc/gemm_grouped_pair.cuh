@@ -499,7 +499,7 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                     for (int q = 0; q < 4; ++q) {
                         const int r = q * 32 + static_cast<int>(lane);
                         const int at = r >= rows             ? -1
-                                       : p.a_rows != nullptr ? __ldg(p.a_rows + t.p0 + first_row + r)
+                                       : p.a_rows != nullptr ? ptx::ld_global(p.a_rows + t.p0 + first_row + r)
                                                              : t.p0 + first_row + r;
                         src[q] = at < p.a_count ? at : -1;
                     }
@@ -541,7 +541,7 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                     for (int q = 0; q < 2; ++q) {
                         const int r = kb * 64 + q * 32 + static_cast<int>(lane);
                         const int at = r >= t.valid          ? -1
-                                       : p.a_rows != nullptr ? __ldg(p.a_rows + t.p0 + r)
+                                       : p.a_rows != nullptr ? p.a_rows[t.p0 + r]
                                                              : t.p0 + r;
                         next[q] = at < p.a_count ? at : -1;
                     }
@@ -597,7 +597,7 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
 #pragma unroll
                 for (int q = 0; q < 8; ++q) {
                     const int r = q * 32 + static_cast<int>(lane);
-                    const int row = r < t.rows ? __ldg(p.c_rows + t.p0 + r) : -1;
+                    const int row = r < t.rows ? ptx::ld_global(p.c_rows + t.p0 + r) : -1;
                     row_table[r] = row < p.c_count ? row : -1;
                 }
                 __syncwarp();
@@ -615,7 +615,7 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
             const int rows = col0 < p.n ? t.rows : 0;  // rows this warp stores
             Elem* c_base =
                 static_cast<Elem*>(p.c) + (wgrad ? static_cast<long long>(t.group) * p.c_stride : 0ll);
-            const float factor = p.alpha * (p.scales != nullptr ? __ldg(p.scales + t.group) : 1.0f);
+            const float factor = p.alpha * (p.scales != nullptr ? p.scales[t.group] : 1.0f);
             const int z = wgrad ? t.group : 0;
             auto row_of = [&](int j) -> int {  // row of C behind row j of the tile, negative: none
                 return j >= rows ? -1 : scattered ? row_table[j] : t.r0 + j;

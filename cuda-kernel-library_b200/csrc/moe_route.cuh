@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, NV <= 8 ? 10 : 4) moe_route_
         for (int i = 0; i < NV; ++i) {
             const int e = i * 32 + lane;
             if (p.bias != nullptr && e < p.n_experts) {
-                score[i] += static_cast<double>(__ldg(p.bias + e));
+                score[i] += static_cast<double>(p.bias[e]);
             }
             // (a bias of -inf or NaN takes its expert out of the choice)
             const bool may = logit[i] != detail::kNegInf && score[i] > none;
@@ -834,8 +834,8 @@ __global__ void __launch_bounds__(kCombineThreads) moe_combine_kernel(const Comb
     float acc[V] = {};
 #pragma unroll 8
     for (int j = 0; j < p.top_k; ++j) {
-        const int at = __ldg(pos + j);
-        const float f = __ldg(w + j);
+        const int at = pos[j];
+        const float f = w[j];
         if (at < 0 || at >= rows || f == 0.0f) {
             continue;
         }
@@ -888,8 +888,8 @@ moe_combine_backward_kernel(const CombineBackwardParams p) {
     if (t >= p.tokens) {
         return;
     }
-    const int at = __ldg(p.positions + slot);
-    const float w = __ldg(p.weights + slot);
+    const int at = p.positions[slot];
+    const float w = p.weights[slot];
     const bool exists = at >= 0 && at < detail::rows_that_exist(p.y_rows, p.kept);
     float dot = 0.0f;
     if (exists) {

@@ -248,3 +248,43 @@ def test_layer_with_tokens_that_route_nowhere(ckl):
         got.append([s.out, s.weights, s.experts, s.positions, s.dxr[:kept], s.dw1, s.dw2, s.dlogits])
     for a, b in zip(*got):
         assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+def test_every_kernel_reads_what_the_one_before_it_wrote(ckl):
+    """Each launch may be set up while its predecessor runs.  Ids, scores and rows change in every step of a
+    long chain without a pause; each step must give what it gives alone."""
+    t, k, e, n, steps = 64, 4, 8, 64, 40
+    gen = torch.Generator(device="cuda").manual_seed(70)
+    logits = torch.randn(steps, t, e, generator=gen, device="cuda")
+    y = torch.randn(t * k, n, generator=gen, device="cuda")
+    dout = torch.randn(t, n, generator=gen, device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    w, experts = torch.empty(t, k, device="cuda"), torch.empty(t, k, **i32)
+    offs, rows, pos = torch.empty(e + 1, **i32), torch.empty(t * k, **i32), torch.empty(t * k, **i32)
+    x = torch.randn(t, n, generator=gen, device="cuda").bfloat16()
+    b = torch.randn(e, n, n, generator=gen, device="cuda").bfloat16()
+
+    def chain(pause):
+        got = []
+        for i in range(steps):
+            out, dy, dw = torch.empty(t, n, device="cuda"), torch.empty(t * k, n, device="cuda"), torch.empty(t, k, device="cuda")
+            c = torch.empty(t * k, n, device="cuda")
+            s = torch.cuda.current_stream()
+            ckl.moe_route(ckl.F32, logits[i], w, experts, t, e, k, stream=s)
+            pause()
+            ckl.group_rows(experts, t * k, e, offs, rows, pos, slots_per_row=k, stream=s)
+            pause()
+            ckl.moe_combine(ckl.F32, y, pos, w, out, ckl.F32, t, k, n, t * k, stream=s, kept=offs[e:])
+            pause()
+            ckl.moe_combine_backward(ckl.F32, y, pos, w, dout, ckl.F32, dy, dw, t, k, n, t * k, stream=s)
+            pause()
+            ckl.gemm_grouped(ckl.BF16, x, b, c, ckl.F32, offs, e, t * k, n, n, a_rows=rows, a_count=t, stream=s)
+            pause()
+            got += [out, dy, dw, c]
+        torch.cuda.synchronize()
+        return got
+
+    alone = chain(torch.cuda.synchronize)
+    for _ in range(3):
+        for a, b_ in zip(chain(lambda: None), alone):
+            assert torch.equal(a, b_)
