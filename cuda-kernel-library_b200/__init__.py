@@ -86,21 +86,23 @@ for _name in ("ckl_gemm_f16", "ckl_gemm_bf16", "ckl_gemm_ex", "ckl_gemm_bias_rel
 
 
 def _ptr(x) -> int | None:
-    if x is None:
-        return None
-    try:  # (a third of the time of asking first: small calls are bound by the host)
-        return x.data_ptr()
+    if x is None or type(x) is int:
+        return x
+    try:  # (two thirds of the time of asking first: small calls are bound by the host)
+        x = x.data_ptr()
     except AttributeError:
-        return int(x)
+        pass
+    return x if type(x) is int else int(x)
 
 
 def _stream(s) -> int | None:
-    if s is None:
-        return None
+    if s is None or type(s) is int:
+        return s
     try:
-        return s.cuda_stream
+        s = s.cuda_stream
     except AttributeError:
-        return int(s)
+        pass
+    return s if type(s) is int else int(s)
 
 
 def _check(status: int) -> None:

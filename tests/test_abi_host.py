@@ -330,3 +330,20 @@ int main() {
     assert out.returncode == 0, out.stderr[-3000:]
     run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert run.returncode == 0 and run.stdout.split() == ["0", "5376", "1792", "1"], run.stdout + run.stderr
+
+
+def test_pointers_and_streams_of_any_integer_kind(ckl):
+    """Integers of Python and numpy, and objects whose data_ptr or cuda_stream is either."""
+    np = pytest.importorskip("numpy")
+
+    class Holder:
+        def __init__(self, value):
+            self.cuda_stream = value
+
+        def data_ptr(self):
+            return self.cuda_stream
+
+    for p in (4096, np.int64(4096), np.uint64(4096), Holder(4096), Holder(np.int64(4096)), Holder(np.uint64(4096))):
+        ckl.moe_combine(ckl.F32, p, p, p, p, ckl.F32, 0, 2, 64, 8, stream=p)  # no tokens: nothing is read
+        with pytest.raises(ckl.CklError):
+            ckl.moe_combine(ckl.F32, p, p, p, p, ckl.F32, 4, 0, 64, 8, stream=p)
