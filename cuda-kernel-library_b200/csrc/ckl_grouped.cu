@@ -384,7 +384,8 @@ Product shrink(int ab_dtype, const void* a, int lda, int k, const void* b, int l
     q.p.scales = scales;
     q.p.groups = adapters;
     q.p.rows = q.p.a_count = q.p.c_count = m;
-    q.p.n = rp;  // columns rank .. rp read weights outside their matrix, which are zeros
+    q.p.n = rp;  // columns rank .. rp read weights outside their matrix, and are stored as zeros
+    q.p.ext_rank = rank;
     q.p.k = k;
     q.p.ldc = 2 * rp;
     q.p.c_part_cols = rp;

@@ -83,7 +83,7 @@ struct GroupedParams {
     int ext_cols;              // columns of one part of T (a multiple of 16)
     const uint32_t* ext_flags; // kExtBlocks: a word of kExtChecks bytes per adapter, not 0: E_g is not finite
     const void* e;             // E, `ext_rank` x n per adapter (n x ext_rank with trans_b)
-    int ext_rank, lde;
+    int ext_rank, lde;         // (a TwoPart C: columns from ext_rank on are written as zeros)
     long long e_stride;
     uint32_t fmt;        // operand format for the instruction descriptor
     int split;           // CTAs per tile (a split launch)
@@ -405,6 +405,11 @@ __device__ __forceinline__ void store_unit(const GroupedParams& p,
         v[i] *= factor;
     }
     if constexpr (GroupedStore<OutT>::kTwo) {
+        // Columns behind the rank only fill it up: their sums are of zeros, but infinity times zero is NaN.
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+            v[i] = col + i < p.ext_rank ? v[i] : 0.0f;
+        }
         float lo[kVec];
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {

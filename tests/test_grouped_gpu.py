@@ -755,3 +755,31 @@ def test_lora_pairs_long_sums(ckl):
                 ref, mag = ref + t @ q2, mag + ta @ q2.abs()
                 extra = TWO_PART["bf16"] * (t.abs() @ q2.abs())
             check(got[sel], ref, mag, 2 * max(k, n) + 2 * r, "f32", extra)
+
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("r", [16, 24, 72])
+@pytest.mark.parametrize("m,k,n", [(3, 1032, 520), (40, 2048, 520), (900, 64, 200), (3000, 72, 1040)])
+def test_lora_infinite_row(ckl, dt, r, m, k, n):
+    """An infinity in a row of x (of dy) under positive weights gives that row infinities, whatever the rank:
+    columns that only fill up the rank to a tile's width take no part."""
+    g = 3
+    ids = torch.arange(m, device="cuda", dtype=torch.int32) % g
+    m, x, w, a, b, s, offs, rows = lora_case(ckl, ids, g, k, n, r, dt, 120)
+    dy = rand((m, n), DT[dt], 125)
+    x[2], dy[2] = 1.0, 1.0
+    x[2, 4], dy[2, 7] = float("inf"), float("inf")
+    w.abs_(), a[2].abs_(), b[2].abs_()
+    for t in (w, a, b):
+        t[t == 0] = 1.0
+    size = ckl.gemm_lora_workspace_bytes(m, r, True)
+    ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    y, dx = torch.empty(m, n, device="cuda"), torch.empty(m, k, device="cuda")
+    ckl.gemm_lora(code(ckl, dt), x, w, a, b, s, y, ckl.F32, offs, rows, g, m, n, k, r, ws, size)
+    ckl.gemm_lora_backward(code(ckl, dt), dy, x, w, a, b, s, dx, ckl.F32, None, None, ckl.F32, offs, rows, g, m, n, k, r,
+                           ws, size)
+    torch.cuda.synchronize()
+    assert (y[2] == float("inf")).all() and (dx[2] == float("inf")).all()
+    others = torch.arange(m, device="cuda") != 2
+    assert torch.isfinite(y[others]).all() and torch.isfinite(dx[others]).all()
