@@ -120,7 +120,7 @@ struct GroupedConfig {
     static constexpr int kThreads = 192 + 32 * kStages + 32;  // one loader warp per stage, a scheduler
     static constexpr int kBuffers = 3;  // of 2 KB (32 rows x 64 bytes) per epilogue warp
     static constexpr uint32_t kStagingBytes = kSplit ? 0 : 4 * kBuffers * 2048;
-    static constexpr int kNumBarriers = 3 * kStages + 5 + 8;
+    static constexpr int kNumBarriers = 4 * kStages + 5 + 8;
     static constexpr uint32_t kTableBytes = 2 * (kMaxGemmGroups + 2) * 4 + kMaxGemmGroups / 8;
     static constexpr uint32_t kQueueBytes = 4 * 64;
     static constexpr uint32_t kSmemBytes =
@@ -745,6 +745,8 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
     const uint32_t drain_bar = bars + 8u * (2 * kStages + 4);
     // a stage's rows written by the loaders (stages that need none never use it)
     auto loaded_bar = [&](int s) { return bars + 8u * static_cast<uint32_t>(2 * kStages + 5 + s); };
+    // a stage that the loaders have to write has been acquired (where not every stage is one)
+    auto wanted_bar = [&](int s) { return bars + 8u * static_cast<uint32_t>(3 * kStages + 13 + s); };
     using Queue = detail::TileQueue<detail::GroupedTile>;
     static_assert(Queue::kBytes <= Cfg::kQueueBytes && 2 * detail::kTileSlots == 8, "queue layout");
     const Queue queue = {reinterpret_cast<int4*>(queue_ptr), bars + 8u * (3 * kStages + 5)};
@@ -771,6 +773,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
             ptx::mbar_init(full_bar(s), 1);
             ptx::mbar_init(empty_bar(s), 1);
             ptx::mbar_init(loaded_bar(s), 1);
+            ptx::mbar_init(wanted_bar(s), 1);
         }
         for (uint32_t a = 0; a < 2; ++a) {
             ptx::mbar_init(acc_full_bar(a), 1);
@@ -811,6 +814,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
     // ---- roles ------------------------------------------------------------------------------
     const bool gather_a = p.load_a != 0;
     const bool gather_b = p.form == kFormWgrad && p.b_rows != nullptr;
+    const bool every = gather_a || gather_b;  // the loaders write a part of every block
     if (warp == 0) {
         if (ptx::elect_one_sync()) {
             // TMA producer.
@@ -818,9 +822,12 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
-            auto acquire_stage = [&](uint32_t bytes) -> bool {
+            auto acquire_stage = [&](uint32_t bytes, bool wanted) -> bool {
                 if (!detail::wait_barrier(empty_bar(stage), phase ^ 1u, ctl, kRoleProducer, it)) {
                     return false;
+                }
+                if (wanted) {
+                    ptx::mbar_arrive(wanted_bar(stage));
                 }
                 const bool wrong = p.overstate_first_stage != 0 && it == 0 && blockIdx.x == 0;
                 ptx::mbar_arrive_expect_tx(full_bar(stage), bytes + (wrong ? 16u : 0u));
@@ -853,7 +860,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                 if (p.form == kFormRows) {
                     const int group = table.whole || p.ext_mode != kExtNone ? 0 : t.group;
                     for (int kb = t.begin; kb < min(t.end, t.k_blocks); ++kb) {
-                        if (!acquire_stage(b_bytes + (gather_a ? 0u : Cfg::kABytes))) {
+                        if (!acquire_stage(b_bytes + (gather_a ? 0u : Cfg::kABytes), false)) {
                             ok = false;
                             break;
                         }
@@ -873,7 +880,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                             continue;
                         }
                         for (int eb = max(0, t.begin - at); eb < min(ext_blocks, t.end - at); ++eb) {
-                            if (!acquire_stage(b_bytes)) {
+                            if (!acquire_stage(b_bytes, !every)) {
                                 ok = false;
                                 break;
                             }
@@ -896,7 +903,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         // A last block that is not whole comes through the loaders in both operands,
                         // with zeros behind the group's end (a zero in one alone would leave 0 * NaN).
                         const bool whole = t.valid - at >= 64;
-                        if (!acquire_stage(whole ? bytes : 0u)) {
+                        if (!acquire_stage(whole ? bytes : 0u, !every && !whole)) {
                             ok = false;
                             break;
                         }
@@ -1075,11 +1082,12 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
         uint32_t it = 0;     // blocks of this CTA so far, whoever owns their stage
         uint32_t phase = 0;  // of the own stage
         bool ok = true;
-        // Every block of the own stage is waited for, even one that needs nothing from here: a
-        // barrier tells two adjacent phases apart, no more.
+        // A barrier tells two adjacent phases apart, no more.  Where every block is written here none can
+        // be multiplied without this warp, so it sees each phase of its stage's barrier.  Where only a
+        // few are, the others pass whether it looks or not: then the producer says which.
         auto acquire = [&]() -> bool {
-            const bool got =
-                detail::wait_barrier(empty_bar(own), phase ^ 1u, ctl, kRoleProducer, 0x20000000u | it);
+            const bool got = detail::wait_barrier(every ? empty_bar(own) : wanted_bar(own), every ? phase ^ 1u : phase,
+                                                  ctl, kRoleProducer, 0x20000000u | it);
             phase ^= 1u;
             return __all_sync(0xFFFFFFFFu, got) != 0;
         };
@@ -1104,17 +1112,15 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                     }
                 }
                 for (int kb = t.begin; kb < min(t.end, t.k_blocks); ++kb, ++it) {
-                    if (static_cast<int>(it % kStages) != own) {
+                    if (!gather_a || static_cast<int>(it % kStages) != own) {
                         continue;
                     }
                     if (!acquire()) {
                         ok = false;
                         break;
                     }
-                    if (gather_a) {
-                        load.rows128(0, p.a, p.lda, src, t.valid, kb * 64, p.k);
-                        hand_over();
-                    }
+                    load.rows128(0, p.a, p.lda, src, t.valid, kb * 64, p.k);
+                    hand_over();
                 }
                 int first_block = t.k_blocks;
                 for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
@@ -1166,6 +1172,9 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                     const bool tail = t.valid - (kb - part * row_blocks) * 64 < 64;
                     const int ra[2] = {next_a[0], next_a[1]}, rb[2] = {next_b[0], next_b[1]};
                     fetch(kb + kStages);
+                    if (!every && !tail) {
+                        continue;
+                    }
                     if (!acquire()) {
                         ok = false;
                         break;
@@ -1178,9 +1187,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         load.rows64(Cfg::kABytes, p.b, p.ldb, rb, b_boxes, t.n0 + part * p.b_part_cols,
                                     p.n + part * p.b_part_cols);
                     }
-                    if (gather_a || gather_b || tail) {
-                        hand_over();
-                    }
+                    hand_over();
                 }
                 it += static_cast<uint32_t>(t.end - t.begin);
             }

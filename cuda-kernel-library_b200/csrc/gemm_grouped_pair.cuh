@@ -39,7 +39,7 @@ struct GroupedPairConfig {
     static constexpr int kBuffers = 3;  // per epilogue warp
     static constexpr uint32_t kWarpStaging = kBuffers * kBufferBytes;
     static constexpr uint32_t kStagingBytes = 4 * kWarpStaging;
-    static constexpr int kNumBarriers = 3 * kStages + 5 + 8;
+    static constexpr int kNumBarriers = 4 * kStages + 5 + 8;
     static constexpr uint32_t kTableBytes = 2 * (kMaxGemmGroups + 2) * 4 + kMaxGemmGroups / 8;
     static constexpr uint32_t kQueueBytes = 4 * 64;
     static constexpr uint32_t kRowTableBytes = 4 * 256 * 4;  // rows of C, per epilogue warp
@@ -152,6 +152,8 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
     auto acc_full_bar = [&](uint32_t a) { return bars + 8u * (3 * kStages + a); };
     auto acc_empty_bar = [&](uint32_t a) { return bars + 8u * (3 * kStages + 2 + a); };
     const uint32_t drain_bar = bars + 8u * (3 * kStages + 4);
+    // a stage that the loaders have to write has been acquired (where not every stage is one)
+    auto wanted_bar = [&](int s) { return bars + 8u * static_cast<uint32_t>(3 * kStages + 13 + s); };
     using Queue = detail::TileQueue<detail::PairTile>;
     static_assert(Queue::kBytes <= Cfg::kQueueBytes && 2 * detail::kTileSlots == 8, "queue layout");
     const Queue queue = {reinterpret_cast<int4*>(queue_ptr), bars + 8u * (3 * kStages + 5)};
@@ -178,9 +180,10 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
     // ---- set-up -------------------------------------------------------------------------------
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
-            ptx::mbar_init(full_bar(s), 1);
+            ptx::mbar_init(full_bar(s), 2);    // the producers of both CTAs, at the leader
             ptx::mbar_init(empty_bar(s), 1);
             ptx::mbar_init(loaded_bar(s), 2);  // the loaders of both CTAs, at the leader
+            ptx::mbar_init(wanted_bar(s), 1);
         }
         for (uint32_t a = 0; a < 2; ++a) {
             ptx::mbar_init(acc_full_bar(a), 1);
@@ -228,15 +231,23 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
             uint32_t phase = 0;
             bool ok = true;
             uint32_t bar = 0;
-            auto acquire_stage = [&](uint32_t bytes_of_both) -> bool {
+            // Both producers arrive for every stage, also one that they copy nothing into (columns behind
+            // the last, gathered rows): a stage cannot be filled again before both have seen it free,
+            // so neither falls two phases behind, which a barrier does not tell from none.
+            auto acquire_stage = [&](uint32_t bytes_of_both, bool wanted) -> bool {
                 if (!detail::wait_barrier(empty_bar(stage), phase ^ 1u, ctl, kRoleProducer, it)) {
                     return false;
                 }
+                if (wanted) {
+                    ptx::mbar_arrive(wanted_bar(stage));
+                }
+                bar = ptx::map_to_cta(full_bar(stage), 0);
                 if (leader) {
                     const bool wrong = p.overstate_first_stage != 0 && it == 0 && blockIdx.x == 0;
                     ptx::mbar_arrive_expect_tx(full_bar(stage), bytes_of_both + (wrong ? 16u : 0u));
+                } else {
+                    ptx::mbar_arrive_cluster(bar);
                 }
-                bar = ptx::map_to_cta(full_bar(stage), 0);
                 return true;
             };
             auto advance = [&]() {
@@ -271,7 +282,7 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                     const int row_boxes = gather ? 0 : (t.half + 63) / 64;
                     const uint32_t rows_bytes = 2u * static_cast<uint32_t>(row_boxes) * Cfg::kBoxBytes;
                     for (int kb = 0; kb < t.k_blocks; ++kb) {
-                        if (!acquire_stage(cols_bytes + rows_bytes)) {
+                        if (!acquire_stage(cols_bytes + rows_bytes, false)) {
                             ok = false;
                             break;
                         }
@@ -290,7 +301,7 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                     for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
                         const detail::Span span = detail::adapter_span(table, t, g);
                         for (int eb = 0; span.lo < span.hi && eb < ext_blocks; ++eb) {
-                            if (!acquire_stage(cols_bytes)) {
+                            if (!acquire_stage(cols_bytes, !gather)) {
                                 ok = false;
                                 break;
                             }
@@ -310,7 +321,7 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                     for (int kb = 0; kb < t.k_blocks; ++kb) {
                         // a last block that is not whole comes through the loaders
                         const bool whole = t.valid - kb * 64 >= 64;
-                        if (!acquire_stage(whole ? cols_bytes + rows_bytes : 0u)) {
+                        if (!acquire_stage(whole ? cols_bytes + rows_bytes : 0u, !gather && !whole)) {
                             ok = false;
                             break;
                         }
@@ -474,9 +485,9 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
         uint32_t it = 0;     // blocks so far, whoever owns their stage
         uint32_t phase = 0;  // of the own stage
         bool ok = true;
-        auto acquire = [&]() -> bool {
-            const bool got =
-                detail::wait_barrier(empty_bar(own), phase ^ 1u, ctl, kRoleProducer, 0x20000000u | it);
+        auto acquire = [&]() -> bool {  // (see the single-CTA kernel)
+            const bool got = detail::wait_barrier(gather ? empty_bar(own) : wanted_bar(own), gather ? phase ^ 1u : phase,
+                                                  ctl, kRoleProducer, 0x20000000u | it);
             phase ^= 1u;
             return __all_sync(0xFFFFFFFFu, got) != 0;
         };
@@ -505,17 +516,15 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                     }
                 }
                 for (int kb = 0; kb < t.k_blocks; ++kb, ++it) {
-                    if (static_cast<int>(it % kStages) != own) {
+                    if (!gather || static_cast<int>(it % kStages) != own) {
                         continue;
                     }
                     if (!acquire()) {
                         ok = false;
                         break;
                     }
-                    if (gather) {
-                        load.rows128(Cfg::kColsBytes, p.a, p.lda, src, rows, kb * 64, p.k);
-                        hand_over();
-                    }
+                    load.rows128(Cfg::kColsBytes, p.a, p.lda, src, rows, kb * 64, p.k);
+                    hand_over();
                 }
                 for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
                     const detail::Span span = detail::adapter_span(table, t, g);
@@ -551,23 +560,24 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                     const int left = t.valid - kb * 64;
                     const int rows[2] = {next[0], next[1]};
                     fetch(kb + kStages);
+                    if (!gather && left >= 64) {
+                        continue;
+                    }
                     if (!acquire()) {
                         ok = false;
                         break;
                     }
-                    if (gather || left < 64) {
-                        load.rows64(Cfg::kColsBytes, p.a, p.lda, rows, t.half / 64, t.r0 + first_row, p.m);
-                        if (left < 64) {
-                            int at[2];
+                    load.rows64(Cfg::kColsBytes, p.a, p.lda, rows, t.half / 64, t.r0 + first_row, p.m);
+                    if (left < 64) {
+                        int at[2];
 #pragma unroll
-                            for (int q = 0; q < 2; ++q) {
-                                const int r = q * 32 + static_cast<int>(lane);
-                                at[q] = r < left ? t.p0 + kb * 64 + r : -1;
-                            }
-                            load.rows64(0, p.b, p.ldb, at, 2, t.c0 + static_cast<int>(rank) * 128, p.n);
+                        for (int q = 0; q < 2; ++q) {
+                            const int r = q * 32 + static_cast<int>(lane);
+                            at[q] = r < left ? t.p0 + kb * 64 + r : -1;
                         }
-                        hand_over();
+                        load.rows64(0, p.b, p.ldb, at, 2, t.c0 + static_cast<int>(rank) * 128, p.n);
                     }
+                    hand_over();
                 }
                 it += static_cast<uint32_t>(t.k_blocks);
             }

@@ -783,3 +783,73 @@ def test_lora_infinite_row(ckl, dt, r, m, k, n):
     assert (y[2] == float("inf")).all() and (dx[2] == float("inf")).all()
     others = torch.arange(m, device="cuda") != 2
     assert torch.isfinite(y[others]).all() and torch.isfinite(dx[others]).all()
+
+
+@pytest.mark.parametrize("m,n", [(37, 9), (128, 200), (264, 520)])
+def test_weight_gradient_ends_found_in_time(ckl, m, n):
+    """Rows in place: only the last block of a group needs the loader warps, which must find it however late
+    they come.  Many launches, each the same bits, none that gives up a wait."""
+    sizes = [1500, 0, 701, 3001] if m < 200 else [1500, 0, 701, 1] * 12
+    offs, rows = offsets_of(sizes), sum(sizes)
+    lda, ldd = (m + 7) // 8 * 8, (n + 7) // 8 * 8
+    a, d = rand((rows, lda), torch.bfloat16, 1), rand((rows, ldd), torch.bfloat16, 2)
+    first, w = (torch.empty(len(sizes), m, n, device="cuda") for _ in range(2))
+    same = torch.ones((), dtype=torch.bool, device="cuda")
+    for i in range(400):
+        out = w if i else first
+        ckl.gemm_grouped_wgrad(ckl.BF16, a, d, out, ckl.F32, offs, len(sizes), rows, m, n, lda=lda, ldg=ldd)
+        same &= (out == first).all()
+    assert bool(same)
+    o = offs.tolist()
+    for g in range(len(sizes)):
+        x, y = a[o[g]:o[g + 1], :m].double(), d[o[g]:o[g + 1], :n].double()
+        check(first[g], x.t() @ y, x.abs().t() @ y.abs(), sizes[g] + 10, "f32")
+
+
+def test_grouped_pairs_half_a_tile_of_columns(ckl):
+    """The last tile has columns for one CTA of the pair only, and gathered rows: the other copies nothing.
+    Many launches, each the same bits, none that gives up a wait."""
+    sizes, n, k, tokens = [300, 5, 256, 1000] * 10, 296, 1032, 500
+    offs, rows = offsets_of(sizes), sum(sizes)
+    a = rand((tokens, k), torch.float16, 1)
+    idx = torch.randint(0, tokens, (rows,), device="cuda", dtype=torch.int32)
+    b = rand((40, k, n), torch.float16, 2, k ** -0.5)
+    first, c = (torch.empty(rows, n, device="cuda") for _ in range(2))
+    same = torch.ones((), dtype=torch.bool, device="cuda")
+    for i in range(200):
+        out = c if i else first
+        ckl.gemm_grouped(ckl.F16, a, b, out, ckl.F32, offs, 40, rows, n, k, a_rows=idx, a_count=tokens)
+        same &= (out == first).all()
+    assert bool(same)
+    o = offs.tolist()
+    for g in range(40):
+        x, w = a[idx[o[g]:o[g + 1]].long()].double(), b[g].double()
+        check(first[o[g]:o[g + 1]], x @ w, x.abs() @ w.abs(), k, "f32")
+
+
+def test_lora_rows_in_place_many_times(ckl):
+    """Rows already in adapter order: only the adapters' blocks pass through the loader warps."""
+    g, r = 5, 24
+    for m, k, n in ((300, 1032, 328), (3000, 1032, 1040)):
+        ids = torch.sort(torch.randint(0, g, (m,), device="cuda", dtype=torch.int32)).values.int()
+        m, x, w, a, b, s, offs, _ = lora_case(ckl, ids, g, k, n, r, "bf16", 140)
+        size = ckl.gemm_lora_workspace_bytes(m, r)
+        ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+        first, y = (torch.empty(m, n, device="cuda") for _ in range(2))
+        same = torch.ones((), dtype=torch.bool, device="cuda")
+        for i in range(200):
+            out = y if i else first
+            ckl.gemm_lora(ckl.BF16, x, w, a, b, s, out, ckl.F32, offs, None, g, m, n, k, r, ws, size)
+            same &= (out == first).all()
+        assert bool(same)
+        f = s[ids.long()].double().unsqueeze(1)
+        t, ta = torch.zeros(m, r, dtype=torch.float64, device="cuda"), torch.zeros(m, r, dtype=torch.float64, device="cuda")
+        ref, mag = x.double() @ w.double(), x.double().abs() @ w.double().abs()
+        extra = torch.zeros_like(ref)
+        for i in range(g):
+            sel = ids == i
+            t, ta = f[sel] * (x[sel].double() @ a[i].double()), f[sel] * (x[sel].double().abs() @ a[i].double().abs())
+            ref[sel] += t @ b[i].double()
+            mag[sel] += ta @ b[i].double().abs()
+            extra[sel] = TWO_PART["bf16"] * (t.abs() @ b[i].double().abs())
+        check(first, ref, mag, 2 * k + 2 * r + 10, "f32", extra)
