@@ -126,10 +126,10 @@ void plan(Product& q, const DeviceView& view) {
     p.status = view.status;
     p.fmt = q.ab_dtype == CKL_BF16 ? 1u : 0u;
     q.whole = !wgrad && (p.offsets == nullptr || q.e != nullptr);
-    // CTA pairs on 256 x 256 tiles where there are enough of them; operands in two parts and a
-    // gathered G have only a few columns or rows of output and stay with the single-CTA kernel.
+    // CTA pairs on 256 x 256 tiles where there are enough of them; weight gradients with a two-word operand
+    // or a gathered G have only a few columns or rows of output and stay with the single-CTA kernel.
     const long long pair_tiles = row_tiles(q, 256) * ((p.n + 255) / 256);
-    q.pair = q.c_dtype >= 0 && p.a_parts == 1 && p.b_parts == 1 && p.b_rows == nullptr && p.n > 128 &&
+    q.pair = q.c_dtype >= 0 && p.layered == kLayeredNone && p.b_rows == nullptr && p.n > 128 &&
              (!wgrad || p.m > 128) && pair_tiles * 2 > view.max_pairs;
     // Tile width of the single-CTA kernel: with enough tiles for every SM the wider one, which
     // reads A half as often, unless its last wave leaves more of the machine idle than the narrow
@@ -139,7 +139,7 @@ void plan(Product& q, const DeviceView& view) {
     };
     p.bn = p.n > 128 && cost_of(256) <= 1.1 * cost_of(128) ? 256 : p.n > 64 ? 128 : 64;
     // Blocks of 64 reduced elements behind one tile, as far as the host can tell.
-    q.blocks = wgrad ? static_cast<long long>(p.rows / p.groups + 63) / 64 * p.a_parts * p.b_parts
+    q.blocks = wgrad ? static_cast<long long>(p.rows / p.groups + 63) / 64 * p.parts
                      : (p.k + 63) / 64;
     p.split = 1;
     q.tiles = q.pair ? pair_tiles : single_tiles(q, p.bn);
@@ -174,8 +174,8 @@ int resident_clusters(int device, int size) {
         attr.val.clusterDim.z = 1;
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
-        if (allow_smem<grouped_gemm_kernel<float, true>>(device, Cfg::kSmemBytes) != CKL_OK ||
-            cudaOccupancyMaxActiveClusters(&count, grouped_gemm_kernel<float, true>, &cfg) != cudaSuccess) {
+        if (allow_smem<grouped_gemm_kernel<float, true, false>>(device, Cfg::kSmemBytes) != CKL_OK ||
+            cudaOccupancyMaxActiveClusters(&count, grouped_gemm_kernel<float, true, false>, &cfg) != cudaSuccess) {
             (void)cudaGetLastError();
             count = 0;
         }
@@ -200,7 +200,8 @@ int describe(Product& q, GroupedProblem* out) {
         return set_error(CKL_ERR_TOO_LARGE, "%lld output tiles", q.tiles);
     }
     // Few rows to a tile: the loaders fetch those alone, where a boxed copy would fetch 128.
-    p.load_a = p.a_rows != nullptr ||
+    const bool layers = q.ab_dtype == CKL_F16;  // the loaders read a two-word operand (BF16: columns like others)
+    p.load_a = p.a_rows != nullptr || (layers && p.layered == kLayeredA) ||
                (!wgrad && !q.pair && p.k > 0 && !q.whole && p.rows <= 32ll * std::min(p.groups, p.rows));
     std::memset(out, 0, sizeof *out);
     // Gathered operands are read by the loader warps, all others through these descriptors.
@@ -208,7 +209,7 @@ int describe(Product& q, GroupedProblem* out) {
         GRP_TRY(encode_operand(&out->a_box, q.ab_dtype, q.a, q.a_cols, p.a_count, q.lda, 0, 0, 64,
                                wgrad || q.pair ? 64 : 128));
     }
-    if (!wgrad || p.b_rows == nullptr) {
+    if (!wgrad || (p.b_rows == nullptr && !(layers && p.layered == kLayeredB))) {
         GRP_TRY(encode_operand(&out->b_box, q.ab_dtype, q.b, q.b_cols, wgrad ? p.b_count : q.b_outer, q.ldb,
                                static_cast<uint64_t>(q.b_depth), static_cast<uint64_t>(q.b_stack), 64, 64));
     }
@@ -244,16 +245,16 @@ int describe(Product& q, GroupedProblem* out) {
     return CKL_OK;
 }
 
-template <typename OutT>
+template <typename OutT, bool kAdapters>
 int launch_single(const GroupedProblems& problems, int count, int tiles, const DeviceView& view,
                   cudaStream_t stream) {
     const int split = problems.at[0].p.split;
     if (split > 1) {
-        return launch_kernel<grouped_gemm_kernel<OutT, true>>(
+        return launch_kernel<grouped_gemm_kernel<OutT, true, kAdapters>>(
             view.device, GroupedConfig<true>::kThreads, GroupedConfig<true>::kSmemBytes, split, problems,
             dim3(static_cast<unsigned>(tiles * split), static_cast<unsigned>(count)), stream);
     }
-    return launch_kernel<grouped_gemm_kernel<OutT, false>>(
+    return launch_kernel<grouped_gemm_kernel<OutT, false, kAdapters>>(
         view.device, GroupedConfig<false>::kThreads, GroupedConfig<false>::kSmemBytes, 1, problems,
         dim3(static_cast<unsigned>(std::min(view.sm_count, tiles)), static_cast<unsigned>(count)), stream);
 }
@@ -262,19 +263,28 @@ int launch_single(const Product& q, const GroupedProblems& problems, int count, 
                   const DeviceView& view, cudaStream_t stream) {
     const int n = static_cast<int>(tiles);
     if (q.c_dtype < 0) {
-        return q.ab_dtype == CKL_BF16 ? launch_single<TwoPart<__nv_bfloat16>>(problems, count, n, view, stream)
-                                      : launch_single<TwoPart<__half>>(problems, count, n, view, stream);
+        return q.ab_dtype == CKL_BF16 ? launch_single<TwoPart<__nv_bfloat16>, false>(problems, count, n, view, stream)
+                                      : launch_single<TwoPart<__half>, false>(problems, count, n, view, stream);
+    }
+    if (q.e != nullptr || q.p.layered != kLayeredNone) {
+        switch (q.c_dtype) {
+            case CKL_F16: return launch_single<__half, true>(problems, count, n, view, stream);
+            case CKL_BF16: return launch_single<__nv_bfloat16, true>(problems, count, n, view, stream);
+            default: return launch_single<float, true>(problems, count, n, view, stream);
+        }
     }
     switch (q.c_dtype) {
-        case CKL_F16: return launch_single<__half>(problems, count, n, view, stream);
-        case CKL_BF16: return launch_single<__nv_bfloat16>(problems, count, n, view, stream);
-        default: return launch_single<float>(problems, count, n, view, stream);
+        case CKL_F16: return launch_single<__half, false>(problems, count, n, view, stream);
+        case CKL_BF16: return launch_single<__nv_bfloat16, false>(problems, count, n, view, stream);
+        default: return launch_single<float, false>(problems, count, n, view, stream);
     }
 }
 
 template <typename OutT>
 int launch_pair(const GroupedProblem& problem, long long tiles, const DeviceView& view, cudaStream_t stream) {
-    return launch_kernel<grouped_pair_kernel<OutT>>(
+    const bool ext = problem.p.ext_mode != kExtNone;
+    return (ext ? launch_kernel<grouped_pair_kernel<OutT, true>, GroupedProblem>
+                : launch_kernel<grouped_pair_kernel<OutT, false>, GroupedProblem>)(
         view.device, GroupedPairConfig::kThreads, GroupedPairConfig::kSmemBytes, 2, problem,
         dim3(static_cast<unsigned>(2 * std::min<long long>(view.max_pairs, tiles))), stream);
 }
@@ -360,7 +370,7 @@ Product blank(int ab_dtype, int c_dtype, int form) {
     q.c_dtype = c_dtype;
     q.p.form = form;
     q.p.alpha = 1.0f;
-    q.p.a_parts = q.p.b_parts = 1;
+    q.p.parts = 1;
     return q;
 }
 
@@ -372,7 +382,9 @@ size_t two_part_bytes(int m, int rank) {
     return (static_cast<size_t>(std::max(m, 0)) * 2 * padded_rank(rank) * 2 + 255) / 256 * 256;
 }
 
-// T[p] = scales[g] * A[rows[p]] * op(B_g) in two parts, for the positions of every adapter.
+int parts_of(int ab_dtype) { return ab_dtype == CKL_BF16 ? kBf16Parts : kF16Parts; }
+
+// T[p] = scales[g] * A[rows[p]] * op(B_g) in two words, for the positions of every adapter.
 Product shrink(int ab_dtype, const void* a, int lda, int k, const void* b, int ldb, long long stack,
                bool trans, int rank, const float* scales, void* t, const int* offsets, const int* rows,
                int adapters, int m) {
@@ -439,6 +451,7 @@ Product expand(int ab_dtype, int c_dtype, const void* a, int lda, int k, const v
     q.p.a_rows = q.p.c_rows = rows;
     q.p.c = c;
     q.p.groups = adapters;
+    q.p.parts = parts_of(ab_dtype);
     q.p.ext_cols = rp;
     q.p.ext_rank = rank;
     q.p.ext_flags = static_cast<const uint32_t*>(flags);
@@ -685,8 +698,9 @@ int ckl_gemm_lora_backward(int ab_dtype, const void* dy, const void* x, const vo
     pa.p.n = rank;
     pa.p.ldc = ldda;
     pa.p.beta = beta;
-    pa.p.b_parts = 2;
-    pa.p.b_part_cols = rp;
+    pa.p.parts = parts_of(ab_dtype);
+    pa.p.layered = kLayeredB;
+    pa.p.part_cols = rp;
     pa.a = x;
     pa.lda = ldx;
     pa.a_cols = k;
@@ -705,8 +719,9 @@ int ckl_gemm_lora_backward(int ab_dtype, const void* dy, const void* x, const vo
     pb.p.n = n;
     pb.p.ldc = lddb;
     pb.p.beta = beta;
-    pb.p.a_parts = 2;
-    pb.p.a_part_cols = rp;
+    pb.p.parts = parts_of(ab_dtype);
+    pb.p.layered = kLayeredA;
+    pb.p.part_cols = rp;
     pb.a = t;
     pb.lda = pb.a_cols = 2 * rp;
     pb.b = dy;

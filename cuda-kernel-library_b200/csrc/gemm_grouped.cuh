@@ -9,7 +9,7 @@
 //
 // kFormRows may be "extended": one B for all positions (a shared projection), and for the rows of
 // adapter g (offsets are then the adapters') T[p] * op(E_g) besides.
-//   kExtBlocks  behind the k blocks of the product a tile runs, for each adapter whose rows it holds,
+//   kExtBlocks  before the k blocks of the product a tile runs, for each adapter whose rows it holds,
 //               those of T and E_g into the same accumulator, the rows of other adapters read as
 //               zeros: no second pass over C, and no tiles cut at the borders of requests (which
 //               reads the shared weights again for each: 2000 rows, 30 adapters, 4096 x 4096:
@@ -20,6 +20,19 @@
 //   kExtAdd     all adapters are added row by row, in FP32 on the CUDA cores: a split launch of few
 //               rows, where 64-wide blocks that hold a rank of 16 for one or two rows each
 //               outnumbered those of the product.
+//
+// T is kept in two 16-bit words a value (two_words), which the tensor core takes as operand-type parts:
+// passes over the same blocks into the same accumulator.  BF16: the value rounded and what that left, 16
+// bits.  FP16 has 40 binary orders of magnitude in all, and a gradient early in an adapter's training
+// lies below them (4e-7 under incoming gradients of 1e-4: two plain FP16 parts, which end at 2^-25,
+// kept 4 bits of it).  So there are three parts in units of 1, 2^-11 and 2^-22, of which a value uses
+// the first two or, below 2^-14, the last two: 21 bits from 2^-25 to 65504, and 2^-46 beneath.  The
+// finest pass runs first, and the first MMA of the next one takes the accumulator times 2^-11.
+// (The tensor core does not normalise subnormal FP16 operands: it aligns their products as if they were
+// 2^-14 and cuts the sum's lower bits accordingly; zeros cost nothing.  Measured: adding 2^-24 x 1 to a
+// sum of 2^-24 loses the bits that 2^-14 x 1 does.  That is why a value below 2^-14 leaves the first
+// part empty.)  FP32 words taken apart by the loaders held more bits, but one warp a stage took too
+// long over them (lora, 4100 rows: 154 -> 216 us; gradients, 2050 rows: 60 -> 325).
 //
 // Consecutive rows arrive by boxed TMA copies.  Gathered rows arrive by cp.async from loader warps,
 // one per stage, that write the same swizzled layout: TMA's own row gather (tile::gather4) took about 100
@@ -46,11 +59,13 @@ enum GroupedForm : int { kFormRows = 0, kFormWgrad = 1 };
 constexpr int kExtChecks = 4;
 enum ExtMode : int { kExtNone = 0, kExtBlocks = 1, kExtAdd = 2 };
 
-// Element type of C, or the two-part form: an FP32 value v stored as 16-bit hi = round(v) and
-// lo = round(v - hi), lo `part` columns behind hi.  Holds 16 (BF16) or 22 (FP16) bits of v, so an
-// intermediate that feeds another tensor-core product is not cut to the operand type.
+// Element type of C, or an FP32 value in two words, the second `c_part_cols` columns behind the first.
 template <typename T>
 struct TwoPart {};
+constexpr int kBf16Parts = 2, kF16Parts = 3;
+constexpr int kPartShift = 11;  // FP16: a part's unit is 2^-11 of that of the part before
+// kFormWgrad: the operand that is two words a value, read by the loaders (FP16) or as columns (BF16).
+enum LayeredOperand : int { kLayeredNone = 0, kLayeredA = 1, kLayeredB = 2 };
 
 struct GroupedParams {
     const int* offsets;  // groups + 1, nullptr: one group of all rows
@@ -73,14 +88,13 @@ struct GroupedParams {
     int form;
     int trans_b;         // kFormRows: B_g is stored n x k
     int bn;              // tile columns: 64, 128 or 256
-    // Two-part operands of kFormWgrad: the reduction runs over the rows once per part, the parts
-    // `part_cols` columns apart.
-    int a_parts, a_part_cols;
-    int b_parts, b_part_cols;
-    int c_part_cols;     // TwoPart output: distance of lo behind hi
+    int parts;           // passes that a two-word operand takes, else 1
+    int layered;         // kFormWgrad: LayeredOperand
+    int part_cols;       // columns from its first words to its second ones
+    int c_part_cols;     // the same of a TwoPart C
     // Extension: offsets/groups describe the adapters.
     int ext_mode;              // ExtMode
-    int ext_cols;              // columns of one part of T (a multiple of 16)
+    int ext_cols;              // columns from T's first words to its second ones (a multiple of 16)
     const uint32_t* ext_flags; // kExtBlocks: a word of kExtChecks bytes per adapter, not 0: E_g is not finite
     const void* e;             // E, `ext_rank` x n per adapter (n x ext_rank with trans_b)
     int ext_rank, lde;         // (a TwoPart C: columns from ext_rank on are written as zeros)
@@ -139,7 +153,8 @@ struct GroupedTile {
     int cols;       // columns of the tile that exist
     int k_blocks;   // 64-wide blocks of the main product
     int ext_first, ext_last;  // kExtBlocks: adapters [first, last) that may have rows in the tile
-    int begin, end;  // this CTA's share of the tile's blocks (main product, then adapters)
+    int begin, end;  // this CTA's share of the tile's blocks (adapters, then the main product)
+    int finer;       // part in whose unit the share's sum ends up (FP16 passes), 0: the result's
 };
 
 struct GroupedTable {
@@ -262,7 +277,7 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, cons
         o.p0 = t.offs[o.group];
         o.valid = max(0, t.offs[o.group + 1] - o.p0);
         o.m0 = mt * 128;
-        o.k_blocks = ((o.valid + 63) / 64) * p.a_parts * p.b_parts;
+        o.k_blocks = ((o.valid + 63) / 64) * p.parts;
     } else {
         const int seg0 = t.whole ? 0 : t.offs[o.group];
         const int seg1 = t.whole ? p.rows : t.offs[o.group + 1];
@@ -368,13 +383,23 @@ __device__ __forceinline__ bool has_flagged(const GroupedTable& table, const Til
 // Fills in the share of a tile's blocks that CTA `rank` of `size` runs.
 __device__ __forceinline__ void take_share(const GroupedParams& p, const GroupedTable& table, GroupedTile* t,
                                            int rank, int size) {
-    int blocks = t->k_blocks;
+    int pass = 0;  // blocks of one pass over the two-word operand
     for (int g = t->ext_first; g < t->ext_last; ++g) {
         const Span s = adapter_span(table, *t, g);
-        blocks += s.lo < s.hi ? 2 * ((p.ext_cols + 63) / 64) : 0;
+        pass += s.lo < s.hi ? (p.ext_cols + 63) / 64 : 0;
     }
+    const int blocks = t->k_blocks + p.parts * pass;
     t->begin = static_cast<int>(static_cast<long long>(blocks) * rank / size);
     t->end = static_cast<int>(static_cast<long long>(blocks) * (rank + 1) / size);
+    t->finer = 0;
+    if (p.fmt == 0 && p.parts > 1 && t->begin < t->end) {
+        if (p.form == kFormWgrad) {
+            pass = (t->valid + 63) / 64;
+        }
+        for (int part = p.parts - 1; part > 0; --part) {  // the last part whose pass has not ended
+            t->finer += pass > 0 && t->end <= (p.parts - part) * pass ? 1 : 0;
+        }
+    }
 }
 
 }  // namespace detail
@@ -391,6 +416,70 @@ struct GroupedStore<TwoPart<T>> {
 };
 
 namespace detail {
+
+// An FP32 value as two words of the operand type.
+//   BF16  v rounded, and what that left of v.
+//   FP16  from 2^-14 on the same, what was left times 2^11; below, both words of v times 2^11, and the
+//         lowest bit of the second word is set (else it is 0: the nearest number of the right kind is taken,
+//         at most one of its steps away).  Differences and products by 2^11 are exact.
+__device__ __forceinline__ void two_words(float v, __nv_bfloat16* first, __nv_bfloat16* second) {
+    *first = __float2bfloat16_rn(v);
+    const float f = __bfloat162float(*first);
+    *second = __float2bfloat16_rn(isinf(f) ? 0.0f : v - f);  // out of range stays infinite, inf - inf would not
+}
+__device__ __forceinline__ void two_words(float v, __half* first, __half* second) {
+    constexpr float kUnit = static_cast<float>(1 << kPartShift), kSmallest = 1.0f / (1 << 14);
+    const bool fine = fabsf(v) < kSmallest && v != 0.0f;
+    const float x = fine ? v * kUnit : v;
+    *first = __float2half_rn(x);
+    const float f = __half2float(*first);
+    const float r = isfinite(f) ? (x - f) * kUnit : 0.0f;
+    const __half h = __float2half_rn(r);
+    unsigned int bits = __half_as_ushort(h);
+    if ((bits & 1u) != (fine ? 1u : 0u)) {
+        bits += fabsf(r) >= fabsf(__half2float(h)) ? 1u : ~0u;  // (0 goes up: its magnitude is not above r's)
+    }
+    *second = __ushort_as_half(static_cast<unsigned short>(bits));
+}
+// Part `part` of pairs of values from their words (FP16).
+__device__ __forceinline__ uint32_t layer_of(uint32_t first, uint32_t second, int part) {
+    const uint32_t fine = (second & 0x00010001u) * 0xffffu;  // all ones in the halves that are fine
+    return part == 0 ? first & ~fine : part == 1 ? (second & ~fine) | (first & fine) : second & fine;
+}
+__device__ __forceinline__ uint4 layer_of(const uint4& a, const uint4& b, int part) {
+    return make_uint4(layer_of(a.x, b.x, part), layer_of(a.y, b.y, part), layer_of(a.z, b.z, part),
+                      layer_of(a.w, b.w, part));
+}
+
+// Walks the blocks of a tile's adapters that fall into the share [begin, end): one pass per part, the
+// finest first, and in each the adapters that have rows in the tile, `per` blocks each.
+// f(part, adapter, span, block, first of its pass) returns false to stop.  Returns the number of
+// adapters' blocks of the whole tile, which the main product's follow, or -1 where f stopped.
+// (Kernels for products without adapters have kAdapters off and none of this.)
+template <bool kAdapters, typename Tile, typename F>
+__device__ __forceinline__ int for_adapter_blocks(const GroupedParams& p, const GroupedTable& table, const Tile& t,
+                                                  int per, int begin, int end, F&& f) {
+    int at = 0;
+    if (kAdapters && t.ext_first < t.ext_last) {
+        for (int part = p.parts - 1; part >= 0; --part) {
+            bool first = true;
+            for (int g = t.ext_first; g < t.ext_last; ++g) {
+                const Span span = adapter_span(table, t, g);
+                if (span.lo >= span.hi) {
+                    continue;
+                }
+                for (int eb = max(0, begin - at); eb < min(per, end - at); ++eb) {
+                    if (!f(part, g, span, eb, first)) {
+                        return -1;
+                    }
+                    first = false;
+                }
+                at += per;
+            }
+        }
+    }
+    return at;
+}
 
 // One 16-byte unit of row c_row of C: `have` of its columns exist, v holds the raw sums.
 template <typename OutT, int kVec>
@@ -410,16 +499,16 @@ __device__ __forceinline__ void store_unit(const GroupedParams& p,
         for (int i = 0; i < kVec; ++i) {
             v[i] = col + i < p.ext_rank ? v[i] : 0.0f;
         }
-        float lo[kVec];
+        union {
+            Elem e[kVec];
+            uint4 unit;
+        } first, second;
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
-            Elem h;
-            T::store(&h, v[i]);
-            const float hi = T::load(&h);
-            lo[i] = isinf(hi) ? 0.0f : v[i] - hi;  // out of range stays infinite, inf - inf would not
+            two_words(v[i], &first.e[i], &second.e[i]);
         }
-        T::store_vec(dst, v);  // widths are multiples of 16 columns
-        T::store_vec(dst + p.c_part_cols, lo);
+        *reinterpret_cast<uint4*>(dst) = first.unit;  // widths are multiples of 16 columns
+        *reinterpret_cast<uint4*>(dst + p.c_part_cols) = second.unit;
     } else {
         const bool full = p.c_vec != 0 && have == kVec;
         if (p.beta != 0.0f) {
@@ -450,10 +539,46 @@ __device__ __forceinline__ void store_unit(const GroupedParams& p,
     }
 }
 
+// One part of `rows` rows (a multiple of 32) of a two-word FP16 matrix, `units` 16-byte units of 8 columns
+// each, into a box of 128-byte swizzled rows; rows outside [lo, hi) are zeros.  A whole warp, two, four or
+// eight lanes a row, kBatch rows a lane in flight.
+template <int kBatch>
+__device__ __forceinline__ void store_layer(uint32_t dst, const unsigned short* from, int ld, int second, int row0,
+                                         int rows, int lo, int hi, int units, int part) {
+    const int lane = static_cast<int>(threadIdx.x & 31);
+    const int shift = units <= 2 ? 1 : units <= 4 ? 2 : 3;
+    const int unit = lane & ((1 << shift) - 1), sub = lane >> shift, step = 32 >> shift;
+    const bool exists = unit < units;
+    const unsigned short* base = from + (exists ? unit * 8 : 0);
+    for (int j0 = sub; j0 < rows; j0 += kBatch * step) {
+        uint4 a[kBatch], b[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int row = row0 + j0 + i * step;
+            a[i] = b[i] = make_uint4(0, 0, 0, 0);
+            if (exists && row >= lo && row < hi) {
+                const unsigned short* src = base + static_cast<size_t>(row) * ld;
+                a[i] = *reinterpret_cast<const uint4*>(src);
+                b[i] = *reinterpret_cast<const uint4*>(src + second);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int j = j0 + i * step;
+            if (exists && j < rows) {
+                ptx::st_shared_16(dst + static_cast<uint32_t>((j >> 3) * 1024 + (j & 7) * 128 + ((unit ^ (j & 7)) << 4)),
+                                  layer_of(a[i], b[i], part));
+            }
+        }
+    }
+    __syncwarp();
+}
+
 // Writes one stage for a loader warp.  Eight lanes copy the 128 bytes of one row (lane & 7 picks the
 // 16-byte unit), four rows per instruction; a unit's place under the 128-byte swizzle depends on
 // the row modulo 8.  Shuffles and copies go in batches of eight: one after the other each pair
 // would cost its full latency (110 cycles).
+template <int kBatch>
 struct Loader {
     uint32_t stage;      // shared address
     int unit, sub;       // lane & 7, lane >> 3
@@ -525,6 +650,11 @@ struct Loader {
                                                  int lo, int hi, int part, int k0) const {
         const int col = k0 + unit * 8;
         const bool exists = col < p.ext_cols;
+        if (p.fmt == 0) {
+            store_layer<kBatch>(stage + offset, static_cast<const unsigned short*>(p.t) + k0, p.ldt, p.ext_cols, pos0,
+                        (rows + 31) / 32 * 32, lo, hi, min(8, (p.ext_cols - k0) / 8), part);
+            return;
+        }
         const char* base = static_cast<const char*>(p.t) +
                            (static_cast<size_t>(part) * p.ext_cols + (exists ? col : 0)) * 2;
         const size_t pitch = static_cast<size_t>(p.ldt) * 2;
@@ -540,6 +670,17 @@ struct Loader {
                 ptx::cp_async_16(stage + offset + q * 4096u + (i >> 1) * 1024u + ((i & 1) ? odd : even),
                                  base + (take ? pos : 0) * pitch, take);
             }
+        }
+    }
+
+    // One part of 64 rows of a two-word FP16 matrix, of which `left` exist, MN-major: `boxes` boxes of 64
+    // columns from col0 on.  Columns behind the words are not written: no result reads them.
+    __device__ __forceinline__ void layered64(uint32_t offset, const void* from, int ld, int row0, int left,
+                                              int boxes, int col0, int part_cols, int part) const {
+        for (int box = 0; box < boxes; ++box) {
+            const int col = col0 + box * 64;
+            store_layer<kBatch>(stage + offset + box * 8192u, static_cast<const unsigned short*>(from) + col, ld, part_cols,
+                        row0, 64, row0, row0 + left, min(8, (part_cols - col) / 8), part);
         }
     }
 
@@ -591,9 +732,15 @@ struct Loader {
 };
 
 // v[i] += sum over ranks of T[pos] * E_g, columns col .. of the row behind position pos; T's two
-// parts are added first.  The operands are 16-bit words: BF16 is the upper half of an FP32 word.
+// words are put together first.  The operands are 16-bit words: BF16 is the upper half of an FP32 word.
 __device__ __forceinline__ float from16(const GroupedParams& p, uint32_t word) {
     return p.fmt != 0 ? __uint_as_float(word << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(word)));
+}
+__device__ __forceinline__ float from_two_halves(uint32_t first, uint32_t second) {
+    constexpr float kUnit = 1.0f / (1 << kPartShift);
+    const float f = __half2float(__ushort_as_half(static_cast<unsigned short>(first)));
+    const float s = __half2float(__ushort_as_half(static_cast<unsigned short>(second)));
+    return fmaf(s, kUnit, f) * ((second & 1u) != 0 ? kUnit : 1.0f);
 }
 template <typename Elem, int kVec>
 __device__ __forceinline__ void add_adapter(const GroupedParams& p, const GroupedTable& table, int pos, int col,
@@ -617,8 +764,13 @@ __device__ __forceinline__ void add_adapter(const GroupedParams& p, const Groupe
         float f[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            f[2 * i] = from16(p, h[i] & 0xffffu) + from16(p, l[i] & 0xffffu);
-            f[2 * i + 1] = from16(p, h[i] >> 16) + from16(p, l[i] >> 16);
+            if (p.fmt != 0) {
+                f[2 * i] = __uint_as_float(h[i] << 16) + __uint_as_float(l[i] << 16);
+                f[2 * i + 1] = __uint_as_float(h[i] & 0xffff0000u) + __uint_as_float(l[i] & 0xffff0000u);
+            } else {
+                f[2 * i] = from_two_halves(h[i] & 0xffffu, l[i] & 0xffffu);
+                f[2 * i + 1] = from_two_halves(h[i] >> 16, l[i] >> 16);
+            }
         }
         if (p.trans_b) {
             // one column's ranks are neighbours
@@ -716,7 +868,9 @@ __device__ __forceinline__ int row_of_c(const GroupedParams& p, const GroupedTil
 
 }  // namespace detail
 
-template <typename OutT, bool kSplit>
+// kAdapters: extended products and the adapters' weight gradients.  (One kernel for these and the plain
+// products held 5 % more time for the latter.)
+template <typename OutT, bool kSplit, bool kAdapters>
 __global__ void __launch_bounds__(GroupedConfig<kSplit>::kThreads, 1)
 grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
     const GroupedProblem& problem = problems.at[blockIdx.y];
@@ -754,7 +908,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
     volatile uint32_t* tmem_slot_ptr =
         reinterpret_cast<volatile uint32_t*>(bars_ptr + 8 * Cfg::kNumBarriers);
     // the loaders work
-    const bool loads = p.form == kFormWgrad || p.load_a != 0 || p.ext_mode == kExtBlocks;
+    const bool loads = p.form == kFormWgrad || p.load_a != 0 || (kAdapters && p.ext_mode == kExtBlocks);
 
     detail::Control ctl;
     ctl.abort_flag = reinterpret_cast<volatile int*>(bars_ptr + 8 * Cfg::kNumBarriers + 4);
@@ -804,7 +958,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
     ptx::tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot_ptr;
     const int total = detail::total_tiles(p, table);
-    const int ext_blocks = 2 * ((p.ext_cols + 63) / 64);  // of an adapter (kExtBlocks): both parts of T
+    const int ext_blocks = (p.ext_cols + 63) / 64;  // of an adapter and a part of T (kExtBlocks)
     // A split launch has one tile per cluster.
     const int rank = kSplit ? static_cast<int>(ptx::cluster_cta_rank()) : 0;
     const int size = kSplit ? p.split : 1;
@@ -813,7 +967,14 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
 
     // ---- roles ------------------------------------------------------------------------------
     const bool gather_a = p.load_a != 0;
-    const bool gather_b = p.form == kFormWgrad && p.b_rows != nullptr;
+    const bool layers_a = kAdapters && p.layered == kLayeredA && p.fmt == 0;  // (load_a is set as well)
+    const bool layers_b = kAdapters && p.layered == kLayeredB && p.fmt == 0;
+    const bool gather_b = p.form == kFormWgrad && (p.b_rows != nullptr || layers_b);
+    // kFormWgrad: the pass over the rows that block kb belongs to
+    auto pass_of = [&](int kb, int row_blocks) {
+        return !kAdapters || p.parts == 1 ? 0 : (kb >= row_blocks) + (kb >= 2 * row_blocks);
+    };
+    const bool shifts = kAdapters && p.fmt == 0 && p.parts > 1;  // each pass after the first begins with a shift
     const bool every = gather_a || gather_b;  // the loaders write a part of every block
     if (warp == 0) {
         if (ptx::elect_one_sync()) {
@@ -858,8 +1019,23 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                     }
                 };
                 if (p.form == kFormRows) {
-                    const int group = table.whole || p.ext_mode != kExtNone ? 0 : t.group;
-                    for (int kb = t.begin; kb < min(t.end, t.k_blocks); ++kb) {
+                    const int group = kAdapters || table.whole ? 0 : t.group;
+                    const int before = detail::for_adapter_blocks<kAdapters>(
+                        p, table, t, ext_blocks, t.begin, t.end,
+                        [&](int, int g, const detail::Span&, int eb, bool) -> bool {
+                            if (!acquire_stage(b_bytes, !every)) {
+                                return false;
+                            }
+                            load_b(ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes + Cfg::kABytes, &tmap_e_box,
+                                   eb * 64, g);
+                            advance();
+                            return true;
+                        });
+                    if (before < 0) {
+                        ok = false;
+                        break;
+                    }
+                    for (int kb = max(0, t.begin - before); kb < min(t.k_blocks, t.end - before); ++kb) {
                         if (!acquire_stage(b_bytes + (gather_a ? 0u : Cfg::kABytes), false)) {
                             ok = false;
                             break;
@@ -873,23 +1049,6 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         load_b(a_dst + Cfg::kABytes, &tmap_b_box, kb * 64, group);
                         advance();
                     }
-                    int at = t.k_blocks;  // index of the adapter's first block in the tile
-                    for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
-                        const detail::Span span = detail::adapter_span(table, t, g);
-                        if (span.lo >= span.hi) {
-                            continue;
-                        }
-                        for (int eb = max(0, t.begin - at); eb < min(ext_blocks, t.end - at); ++eb) {
-                            if (!acquire_stage(b_bytes, !every)) {
-                                ok = false;
-                                break;
-                            }
-                            load_b(ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes + Cfg::kABytes,
-                                   &tmap_e_box, (eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb) * 64, g);
-                            advance();
-                        }
-                        at += ext_blocks;
-                    }
                 } else {
                     // Weight gradient: 64 positions per block, both operands MN-major.
                     const int row_blocks = (t.valid + 63) / 64;
@@ -898,8 +1057,9 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         (gather_b ? 0u : b_bytes) +
                         (gather_a ? 0u : static_cast<uint32_t>(a_boxes) * Cfg::kBoxBytes);
                     for (int kb = t.begin; kb < t.end; ++kb) {
-                        const int part = kb >= row_blocks ? 1 : 0;
-                        const int at = (kb - part * row_blocks) * 64;
+                        const int pass = pass_of(kb, row_blocks);
+                        const int at = (kb - pass * row_blocks) * 64;
+                        const int far = kAdapters ? (p.parts - 1 - pass) * p.part_cols : 0;  // (BF16: the words as columns)
                         // A last block that is not whole comes through the loaders in both operands,
                         // with zeros behind the group's end (a zero in one alone would leave 0 * NaN).
                         const bool whole = t.valid - at >= 64;
@@ -912,15 +1072,15 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         for (int b = 0; b < 2; ++b) {
                             if (whole && !gather_a && b < a_boxes) {
                                 ptx::tma_load_2d(a_dst + b * Cfg::kBoxBytes, &tmap_a_box, full_bar(stage),
-                                                 t.m0 + part * p.a_part_cols + b * 64, t.p0 + at);
+                                                 t.m0 + (kAdapters && p.layered == kLayeredA ? far : 0) + b * 64, t.p0 + at);
                             }
                         }
 #pragma unroll
                         for (int b = 0; b < 4; ++b) {
                             if (whole && !gather_b && b < boxes) {
                                 ptx::tma_load_3d(a_dst + Cfg::kABytes + b * Cfg::kBoxBytes, &tmap_b_box,
-                                                 full_bar(stage), t.n0 + part * p.b_part_cols + b * 64, t.p0 + at,
-                                                 0);
+                                                 full_bar(stage), t.n0 + (kAdapters && p.layered == kLayeredB ? far : 0) + b * 64,
+                                                 t.p0 + at, 0);
                             }
                         }
                         advance();
@@ -972,7 +1132,8 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                 const uint32_t idesc =
                     ptx::make_idesc_f16(p.fmt, a_mn ? 1u : 0u, b_mn ? 1u : 0u, 128, width);
                 uint32_t accumulate = 0;
-                auto block = [&](int steps, bool loaded) -> bool {
+                // `shift`: a new pass begins, what has been summed is 2^11 times finer
+                auto block = [&](int steps, bool loaded, bool shift) -> bool {
                     if (!ready && !detail::wait_barrier(full_bar(stage), phase, ctl, kRoleMma, it)) {
                         return false;
                     }
@@ -991,7 +1152,9 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         ptx::make_smem_desc_sw128(b_src, b_mn ? Cfg::kBoxBytes : 16u, 1024);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        if (j < steps) {
+                        if (j == 0 && shift && accumulate != 0) {
+                            ptx::umma_f16_shift<kPartShift>(d_tmem, a_desc, b_desc, idesc);
+                        } else if (j < steps) {
                             ptx::umma_f16(d_tmem, a_desc + static_cast<uint64_t>(j * a_step),
                                           b_desc + static_cast<uint64_t>(j * b_step), idesc, accumulate);
                             accumulate = 1;
@@ -1011,25 +1174,15 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                     return true;
                 };
                 const int row_blocks = a_mn ? (t.valid + 63) / 64 : 0;
-                for (int kb = t.begin; kb < min(t.end, t.k_blocks); ++kb) {
-                    const bool loaded = gather_a || gather_b ||
-                                        (a_mn && (t.valid & 63) != 0 && (kb + 1) % row_blocks == 0);
-                    if (!block(4, loaded)) {
-                        ok = false;
-                        break;
-                    }
-                }
-                int at = t.k_blocks;
-                for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
-                    const detail::Span span = detail::adapter_span(table, t, g);
-                    if (span.lo >= span.hi) {
-                        continue;
-                    }
-                    for (int eb = max(0, t.begin - at); ok && eb < min(ext_blocks, t.end - at); ++eb) {
-                        const int in_part = eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb;
-                        ok = block(min(4, (p.ext_cols - in_part * 64) / 16), true);
-                    }
-                    at += ext_blocks;
+                const int before = detail::for_adapter_blocks<kAdapters>(
+                    p, table, t, ext_blocks, t.begin, t.end, [&](int, int, const detail::Span&, int eb, bool first) {
+                        return block(min(4, (p.ext_cols - eb * 64) / 16), true, shifts && first);
+                    });
+                ok = before >= 0;
+                for (int kb = max(0, t.begin - before); ok && kb < min(t.k_blocks, t.end - before); ++kb) {
+                    const int in_pass = a_mn ? kb - pass_of(kb, row_blocks) * row_blocks : 0;
+                    const bool tail = a_mn && (t.valid & 63) != 0 && in_pass + 1 == row_blocks;
+                    ok = block(4, gather_a || gather_b || tail, a_mn && shifts && in_pass == 0);
                 }
                 if (ok) {
                     if (accumulate != 0) {
@@ -1078,7 +1231,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
         // generic-proxy writes: after they have landed a proxy fence orders them before the tensor
         // core's reads, then one lane arrives.
         const int own = warp - 6;
-        const detail::Loader load(ring + static_cast<uint32_t>(own) * Cfg::kStageBytes, lane);
+        const detail::Loader<kSplit ? 4 : 8> load(ring + static_cast<uint32_t>(own) * Cfg::kStageBytes, lane);
         uint32_t it = 0;     // blocks of this CTA so far, whoever owns their stage
         uint32_t phase = 0;  // of the own stage
         bool ok = true;
@@ -1111,7 +1264,24 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         src[q] = at < p.a_count ? at : -1;
                     }
                 }
-                for (int kb = t.begin; kb < min(t.end, t.k_blocks); ++kb, ++it) {
+                const int before = detail::for_adapter_blocks<kAdapters>(
+                    p, table, t, ext_blocks, t.begin, t.end,
+                    [&](int part, int, const detail::Span& span, int eb, bool) -> bool {
+                        if (static_cast<int>(it++ % kStages) != own) {
+                            return true;
+                        }
+                        if (!acquire()) {
+                            return false;
+                        }
+                        load.adapter_rows(0, p, t.p0, t.valid, span.lo, span.hi, part, eb * 64);
+                        hand_over();
+                        return true;
+                    });
+                if (before < 0) {
+                    ok = false;
+                    break;
+                }
+                for (int kb = max(0, t.begin - before); kb < min(t.k_blocks, t.end - before); ++kb, ++it) {
                     if (!gather_a || static_cast<int>(it % kStages) != own) {
                         continue;
                     }
@@ -1122,28 +1292,6 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                     load.rows128(0, p.a, p.lda, src, t.valid, kb * 64, p.k);
                     hand_over();
                 }
-                int first_block = t.k_blocks;
-                for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
-                    const detail::Span span = detail::adapter_span(table, t, g);
-                    if (span.lo >= span.hi) {
-                        continue;
-                    }
-                    const int eb_end = min(ext_blocks, t.end - first_block);
-                    for (int eb = max(0, t.begin - first_block); eb < eb_end; ++eb, ++it) {
-                        if (static_cast<int>(it % kStages) != own) {
-                            continue;
-                        }
-                        if (!acquire()) {
-                            ok = false;
-                            break;
-                        }
-                        const int part = eb >= ext_blocks / 2 ? 1 : 0;
-                        load.adapter_rows(0, p, t.p0, t.valid, span.lo, span.hi, part,
-                                          (eb - part * (ext_blocks / 2)) * 64);
-                        hand_over();
-                    }
-                    first_block += ext_blocks;
-                }
             } else {
                 const int row_blocks = (t.valid + 63) / 64;
                 const int a_boxes = (min(128, p.m - t.m0) + 63) / 64;
@@ -1152,7 +1300,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                 // end of the group.
                 int next_a[2], next_b[2];
                 auto fetch = [&](int kb) {
-                    const int i0 = (kb >= row_blocks ? kb - row_blocks : kb) * 64;
+                    const int i0 = (kb - pass_of(kb, row_blocks) * row_blocks) * 64;
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         const int r = i0 + q * 32 + static_cast<int>(lane);
@@ -1168,8 +1316,12 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                     t.begin + (own - static_cast<int>(it % kStages) + kStages) % kStages;
                 fetch(first);
                 for (int kb = first; kb < t.end; kb += kStages) {
-                    const int part = kb >= row_blocks ? 1 : 0;
-                    const bool tail = t.valid - (kb - part * row_blocks) * 64 < 64;
+                    const int pass = pass_of(kb, row_blocks);
+                    const int i0 = (kb - pass * row_blocks) * 64, left = t.valid - i0;
+                    const bool tail = left < 64;
+                    const int part = p.parts - 1 - pass;
+                    const int far_a = kAdapters && p.layered == kLayeredA ? part * p.part_cols : 0;
+                    const int far_b = kAdapters && p.layered == kLayeredB ? part * p.part_cols : 0;
                     const int ra[2] = {next_a[0], next_a[1]}, rb[2] = {next_b[0], next_b[1]};
                     fetch(kb + kStages);
                     if (!every && !tail) {
@@ -1179,13 +1331,18 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         ok = false;
                         break;
                     }
-                    if (gather_a || tail) {
-                        load.rows64(0, p.a, p.lda, ra, a_boxes, t.m0 + part * p.a_part_cols,
-                                    p.m + part * p.a_part_cols);
+                    // the copies of the one operand fly while the other's words are taken apart
+                    if ((gather_a || tail) && !layers_a) {
+                        load.rows64(0, p.a, p.lda, ra, a_boxes, t.m0 + far_a, p.m + far_a);
                     }
-                    if (gather_b || tail) {
-                        load.rows64(Cfg::kABytes, p.b, p.ldb, rb, b_boxes, t.n0 + part * p.b_part_cols,
-                                    p.n + part * p.b_part_cols);
+                    if ((gather_b || tail) && !layers_b) {
+                        load.rows64(Cfg::kABytes, p.b, p.ldb, rb, b_boxes, t.n0 + far_b, p.n + far_b);
+                    }
+                    if (layers_a) {
+                        load.layered64(0, p.a, p.lda, t.p0 + i0, min(64, left), a_boxes, t.m0, p.part_cols, part);
+                    } else if (layers_b) {
+                        load.layered64(Cfg::kABytes, p.b, p.ldb, t.p0 + i0, min(64, left), b_boxes, t.n0, p.part_cols,
+                                       part);
                     }
                     hand_over();
                 }
@@ -1208,7 +1365,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
         uint32_t buffer = 0;
         bool alive = true;
         detail::GroupedTile t;
-        if constexpr (kSplit) {
+        if constexpr (kSplit && kAdapters) {
             if (p.ext_mode == kExtAdd && p.trans_b == 0 && first_tile < total) {
                 // What add_adapter will read of E_g for this CTA's rows travels to L2 meanwhile.
                 t = detail::grouped_tile(p, table, first_tile);
@@ -1237,7 +1394,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
             }
             ptx::tc_fence_after_sync();
             const bool nothing = t.begin == t.end;
-            const bool flagged = !kSplit && detail::has_flagged(table, t);
+            const bool flagged = kAdapters && !kSplit && detail::has_flagged(table, t);
             const uint32_t t_row = tmem_base + ((quad * 32u) << 16) + acc * 256u;
             // Hands the accumulator back to the MMA warp, once, when its last column is in registers.
             bool released = false;
@@ -1256,6 +1413,10 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                 // row, the 16-byte units exchanged by the row so that the 32 rows of a store hit all
                 // banks.
                 const uint32_t row_addr = ring + static_cast<uint32_t>(in_tile) * 512u;
+                // A share that ends in one of the finer passes is still in that pass's unit.
+                const float unit = !kAdapters || t.finer == 0 ? 1.0f
+                                   : t.finer == 1             ? 1.0f / (1 << kPartShift)
+                                                              : 1.0f / (1 << 2 * kPartShift);
                 for (int c0 = 0; c0 < t.cols; c0 += 32) {
                     uint32_t r[32];
                     if (nothing) {
@@ -1270,7 +1431,10 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
 #pragma unroll
                     for (int u = 0; u < 8; ++u) {
                         ptx::st_shared_16(row_addr + (((c0 / 4 + u) ^ lane) << 4),
-                                          make_uint4(r[4 * u], r[4 * u + 1], r[4 * u + 2], r[4 * u + 3]));
+                                          make_uint4(__float_as_uint(unit * __uint_as_float(r[4 * u])),
+                                                     __float_as_uint(unit * __uint_as_float(r[4 * u + 1])),
+                                                     __float_as_uint(unit * __uint_as_float(r[4 * u + 2])),
+                                                     __float_as_uint(unit * __uint_as_float(r[4 * u + 3]))));
                     }
                 }
                 release();
@@ -1419,7 +1583,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
             Elem* c_base = static_cast<Elem*>(p.c) +
                            (p.form == kFormWgrad ? static_cast<long long>(t.group) * p.c_stride : 0ll);
             const uint32_t parts = ring;
-            const bool add = p.ext_mode == kExtAdd || detail::has_flagged(table, t);
+            const bool add = kAdapters && (p.ext_mode == kExtAdd || detail::has_flagged(table, t));
             for (int i = warp * kRowsPerWarp + static_cast<int>(lane) / kLanesPerRow; i * size + rank < rows;
                  i += kWarps * kRowsPerWarp) {
                 const int row = i * size + rank;
@@ -1657,11 +1821,7 @@ __global__ void __launch_bounds__(kLoraRowsThreads) lora_rows_kernel(const LoraR
             v *= p.scales != nullptr ? p.scales[g] : 1.0f;
         }
         T* dst = reinterpret_cast<T*>(p.t) + static_cast<size_t>(pos) * 2 * p.part_cols + r0 + r;
-        T hi;
-        Traits::store(&hi, v);
-        const float h = Traits::load(&hi);
-        *dst = hi;
-        Traits::store(dst + p.part_cols, isinf(h) ? 0.0f : v - h);
+        detail::two_words(v, dst, dst + p.part_cols);
     }
 }
 

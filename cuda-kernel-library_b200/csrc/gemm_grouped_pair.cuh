@@ -124,7 +124,8 @@ __device__ __forceinline__ uint32_t pack16(float factor, uint32_t a, uint32_t b)
 
 }  // namespace detail
 
-template <typename OutT>
+// kExt: an extended product (the single-CTA kernel says why that is a kernel of its own).
+template <typename OutT, bool kExt>
 __global__ void __launch_bounds__(GroupedPairConfig::kThreads, 1)
 grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
     const GroupedParams& p = problem.p;
@@ -165,9 +166,9 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
     const uint32_t lane = ptx::lane_id();
     const uint32_t rank = ptx::cluster_cta_rank();
     const bool leader = rank == 0;
-    const bool wgrad = p.form == kFormWgrad;
+    const bool wgrad = !kExt && p.form == kFormWgrad;
     const bool gather = p.load_a != 0;
-    const bool loads = wgrad || gather || p.ext_mode == kExtBlocks;  // the loaders work
+    const bool loads = kExt || wgrad || gather;  // the loaders work
 
     detail::Control ctl;
     ctl.abort_flag = reinterpret_cast<volatile int*>(bars_ptr + 8 * Cfg::kNumBarriers + 4);
@@ -217,7 +218,8 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
     ptx::tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_slot_ptr;
     const int total = detail::total_tiles(p, table);
-    const int ext_blocks = 2 * ((p.ext_cols + 63) / 64);
+    const int ext_blocks = (p.ext_cols + 63) / 64;
+    const bool shifts = kExt && p.fmt == 0;
     const int unit = static_cast<int>(blockIdx.x >> 1);
     const int units = static_cast<int>(gridDim.x >> 1);
 
@@ -277,10 +279,24 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                     }
                 };
                 if (!wgrad) {
-                    const int group = table.whole || p.ext_mode != kExtNone ? 0 : t.group;
+                    const int group = kExt || table.whole ? 0 : t.group;
                     const int row0 = t.p0 + static_cast<int>(rank) * t.half;
                     const int row_boxes = gather ? 0 : (t.half + 63) / 64;
                     const uint32_t rows_bytes = 2u * static_cast<uint32_t>(row_boxes) * Cfg::kBoxBytes;
+                    const int before = detail::for_adapter_blocks<kExt>(
+                        p, table, t, ext_blocks, 0, 0x7fffffff,
+                        [&](int, int g, const detail::Span&, int eb, bool) -> bool {
+                            if (!acquire_stage(cols_bytes, !gather)) {
+                                return false;
+                            }
+                            load_cols(ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes, &tmap_ext, eb * 64, g);
+                            advance();
+                            return true;
+                        });
+                    if (before < 0) {
+                        ok = false;
+                        break;
+                    }
                     for (int kb = 0; kb < t.k_blocks; ++kb) {
                         if (!acquire_stage(cols_bytes + rows_bytes, false)) {
                             ok = false;
@@ -297,18 +313,6 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                             }
                         }
                         advance();
-                    }
-                    for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
-                        const detail::Span span = detail::adapter_span(table, t, g);
-                        for (int eb = 0; span.lo < span.hi && eb < ext_blocks; ++eb) {
-                            if (!acquire_stage(cols_bytes, !gather)) {
-                                ok = false;
-                                break;
-                            }
-                            load_cols(ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes, &tmap_ext,
-                                      (eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb) * 64, g);
-                            advance();
-                        }
                     }
                 } else {
                     const int row0 = t.r0 + static_cast<int>(rank) * t.half;
@@ -392,7 +396,7 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                 const uint32_t idesc = ptx::make_idesc_f16(p.fmt, cols_mn ? 1u : 0u, rows_mn ? 1u : 0u, 256,
                                                            static_cast<uint32_t>(2 * t.half));
                 uint32_t accumulate = 0;
-                auto block = [&](int steps, bool loaded) -> bool {
+                auto block = [&](int steps, bool loaded, bool shift) -> bool {
                     if (!ready && !detail::wait_barrier(full_bar(stage), phase, ctl, kRoleMma, it)) {
                         return false;
                     }
@@ -410,7 +414,9 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                         cols_src + Cfg::kColsBytes, rows_mn ? Cfg::kBoxBytes : 16u, 1024);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        if (j < steps) {
+                        if (j == 0 && shift && accumulate != 0) {
+                            ptx::umma_f16_pair_shift<kPartShift>(d_tmem, cols_desc, rows_desc, idesc);
+                        } else if (j < steps) {
                             ptx::umma_f16_pair(d_tmem, cols_desc + static_cast<uint64_t>(j * cols_step),
                                                rows_desc + static_cast<uint64_t>(j * rows_step), idesc, accumulate);
                             accumulate = 1;
@@ -428,18 +434,13 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                     }
                     return true;
                 };
-                for (int kb = 0; kb < t.k_blocks; ++kb) {
-                    if (!block(4, gather || (wgrad && t.valid - kb * 64 < 64))) {
-                        ok = false;
-                        break;
-                    }
-                }
-                for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
-                    const detail::Span span = detail::adapter_span(table, t, g);
-                    for (int eb = 0; ok && span.lo < span.hi && eb < ext_blocks; ++eb) {
-                        const int in_part = eb >= ext_blocks / 2 ? eb - ext_blocks / 2 : eb;
-                        ok = block(min(4, (p.ext_cols - in_part * 64) / 16), true);
-                    }
+                ok = detail::for_adapter_blocks<kExt>(
+                         p, table, t, ext_blocks, 0, 0x7fffffff,
+                         [&](int, int, const detail::Span&, int eb, bool first) {
+                             return block(min(4, (p.ext_cols - eb * 64) / 16), true, shifts && first);
+                         }) >= 0;
+                for (int kb = 0; ok && kb < t.k_blocks; ++kb) {
+                    ok = block(4, gather || (wgrad && t.valid - kb * 64 < 64), false);
                 }
                 if (ok) {
                     if (accumulate != 0) {
@@ -480,7 +481,7 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
         __syncwarp();
     } else if (warp >= Cfg::kFirstLoader) {
         // Loaders, one warp per stage as in the single-CTA kernel; a stage is handed to the leader.
-        const detail::Loader load(ring + static_cast<uint32_t>(warp - Cfg::kFirstLoader) * Cfg::kStageBytes, lane);
+        const detail::Loader<8> load(ring + static_cast<uint32_t>(warp - Cfg::kFirstLoader) * Cfg::kStageBytes, lane);
         const int own = warp - Cfg::kFirstLoader;
         uint32_t it = 0;     // blocks so far, whoever owns their stage
         uint32_t phase = 0;  // of the own stage
@@ -515,6 +516,23 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                         src[q] = at < p.a_count ? at : -1;
                     }
                 }
+                const int before = detail::for_adapter_blocks<kExt>(
+                    p, table, t, ext_blocks, 0, 0x7fffffff,
+                    [&](int part, int, const detail::Span& span, int eb, bool) -> bool {
+                        if (static_cast<int>(it++ % kStages) != own) {
+                            return true;
+                        }
+                        if (!acquire()) {
+                            return false;
+                        }
+                        load.adapter_rows(Cfg::kColsBytes, p, t.p0 + first_row, rows, span.lo, span.hi, part, eb * 64);
+                        hand_over();
+                        return true;
+                    });
+                if (before < 0) {
+                    ok = false;
+                    break;
+                }
                 for (int kb = 0; kb < t.k_blocks; ++kb, ++it) {
                     if (!gather || static_cast<int>(it % kStages) != own) {
                         continue;
@@ -525,22 +543,6 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                     }
                     load.rows128(Cfg::kColsBytes, p.a, p.lda, src, rows, kb * 64, p.k);
                     hand_over();
-                }
-                for (int g = t.ext_first; ok && g < t.ext_last; ++g) {
-                    const detail::Span span = detail::adapter_span(table, t, g);
-                    for (int eb = 0; span.lo < span.hi && eb < ext_blocks; ++eb, ++it) {
-                        if (static_cast<int>(it % kStages) != own) {
-                            continue;
-                        }
-                        if (!acquire()) {
-                            ok = false;
-                            break;
-                        }
-                        const int part = eb >= ext_blocks / 2 ? 1 : 0;
-                        load.adapter_rows(Cfg::kColsBytes, p, t.p0 + first_row, rows, span.lo, span.hi, part,
-                                          (eb - part * (ext_blocks / 2)) * 64);
-                        hand_over();
-                    }
                 }
             } else {
                 const int first = (own - static_cast<int>(it % kStages) + kStages) % kStages;
@@ -643,7 +645,7 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
             };
             // Whole runs of 32 consecutive rows leave by TMA, which clips at the edge of C; in a weight
             // gradient it clips rows as well.
-            const bool flagged = detail::has_flagged(table, t);
+            const bool flagged = kExt && detail::has_flagged(table, t);
             const int by_tma = p.c_tma == 0 || flagged ? 0 : wgrad ? (rows + 31) / 32 * 32 : rows / 32 * 32;
             int j0 = 0;
             if (sizeof(Elem) == 2 && p.beta == 0.0f && p.c_vec != 0 && !flagged) {

@@ -388,8 +388,9 @@ int ckl_moe_combine_backward_ex(int y_dtype, const void* y, const int* positions
  * (rank x n, ldlb), y: m x n of any type.  offsets (adapters + 1) and rows (a permutation of
  * 0 .. m-1, NULL: the identity) are what ckl_group_rows makes of the rows' adapter ids: position p
  * is row rows[p]; positions behind offsets[adapters] use no adapter.  scales NULL: 1.  The
- * product x A_g is held as the sum of two operand-type values (16 bits of BF16, 22 of FP16), so it
- * has the operand type's range.  rank <= 128, adapters <= 1024; operands 16-byte aligned with
+ * product scales[g] * x A_g is held in 32 bits, two words of the operand type: with BF16 16 significant
+ * bits; with FP16 21 from 2^-25 up to FP16's largest number, 65504, above which it is infinite, and to
+ * 2^-46 below.  rank <= 128, adapters <= 1024; operands 16-byte aligned with
  * leading dimensions and strides multiples of 8, else CKL_ERR_UNSUPPORTED.  The workspace holds
  * ckl_gemm_lora_workspace_bytes(m, rank, 0) bytes on a 256-byte boundary and is free again when
  * the call's work on the stream has run. */

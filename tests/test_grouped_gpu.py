@@ -853,3 +853,100 @@ def test_lora_rows_in_place_many_times(ckl):
             mag[sel] += ta @ b[i].double().abs()
             extra[sel] = TWO_PART["bf16"] * (t.abs() @ b[i].double().abs())
         check(first, ref, mag, 2 * k + 2 * r + 10, "f32", extra)
+
+
+
+@pytest.mark.parametrize("m,g,k,n,r", [(5, 3, 40, 24, 8), (300, 4, 40, 24, 24), (3000, 6, 72, 1032, 16)],
+                         ids=["few", "single", "pairs"])
+@pytest.mark.parametrize("size", [1e-4, 1e-5])
+def test_lora_small_values(ckl, m, g, k, n, r, size):
+    """FP16 adapters early in training: the second factor is almost zero and so is what passes through it,
+    far below FP16's smallest normal number, while FP32 gradients hold it.  The intermediate is two FP16
+    words: the first leaves 2^-11 of a value, the second, whose last bit says in which unit the words
+    are, 2^-10 of that: 2^-21 = 4 * 2^-23, which the 10 steps on top count.  The last unit is 2^-22, FP16's
+    smallest step 2^-24: 2^-46 at most is left of a value that both words are too coarse for.
+
+    Operands that are themselves subnormal: the tensor core multiplies significands as they stand and
+    aligns the products by their exponent fields, and a subnormal's field is 2^-14's.  An addition is
+    then off by up to 2^-23 of the sum that the same operands raised to 2^-14 would have, so that is the
+    sum of absolute values that counts (zeros stay zeros)."""
+
+    def raised(v):
+        return torch.where(v == 0, 0.0, v.abs().clamp(min=2.0 ** -14))
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    ids = torch.randint(-1, g, (m,), generator=gen, device="cuda", dtype=torch.int32)
+    ids[0], ids[1] = 0, 1
+    m, x, w, a, b, s, offs, rows = lora_case(ckl, ids, g, k, n, r, "f16", 110)
+    w = (w * 2.0 ** -10).contiguous()
+    b = rand((g, r, n), torch.float16, 111, 1e-4)
+    dy = rand((m, n), torch.float16, 112, size)
+    xs_small = (x.float() * size).half()  # and forward: a small T under a second factor of ordinary size
+    b_big = rand((g, r, n), torch.float16, 113, 1.0)
+    bytes_ = ckl.gemm_lora_workspace_bytes(m, r, True)
+    ws = torch.full((bytes_,), 255, dtype=torch.uint8, device="cuda")
+    y, dx = torch.empty(m, n, device="cuda"), torch.empty(m, k, device="cuda")
+    da, db = torch.empty(g, k, r, device="cuda"), torch.empty(g, r, n, device="cuda")
+    small_a = rand((g, k, r), torch.float16, 114, 1e-3)
+    ckl.gemm_lora(ckl.F16, xs_small, w, small_a, b_big, s, y, ckl.F32, offs, rows, g, m, n, k, r, ws, bytes_)
+    ckl.gemm_lora_backward(ckl.F16, dy, xs_small, w, small_a, b, s, dx, ckl.F32, da, db, ckl.F32, offs, rows, g, m, n,
+                           k, r, ws, bytes_)
+    torch.cuda.synchronize()
+    tiny = 2.0 ** -46
+    for i in range(-1, g):
+        sel = ids == i
+        v, d, ww = xs_small[sel].double(), dy[sel].double(), w.double()
+        ref, mag, extra = v @ ww, raised(v) @ raised(ww), 0.0
+        dref, dmag, dextra = d @ ww.t(), raised(d) @ raised(ww).t(), 0.0
+        if i >= 0:
+            f, aa, b0, b1 = s[i].double(), small_a[i].double(), b[i].double(), b_big[i].double()
+            t, ta = f * (v @ aa), f * (raised(v) @ raised(aa))
+            u, ua = f * (d @ b0.t()), f * (raised(d) @ raised(b0).t())
+            ref, mag, extra = ref + t @ b1, mag + ta @ raised(b1), tiny * b1.abs().sum(0)
+            dref, dmag, dextra = dref + u @ aa.t(), dmag + ua @ raised(aa).t(), tiny * aa.abs().sum(1)
+            count = int(sel.sum())
+            check(da[i], v.t() @ u, raised(v).t() @ ua, n + 3 * count + 10, "f32", tiny * v.abs().sum(0).unsqueeze(1))
+            check(db[i], t.t() @ d, ta.t() @ raised(d), k + 3 * count + 10, "f32", tiny * d.abs().sum(0).unsqueeze(0))
+        check(y[sel], ref, mag, 2 * k + 3 * r + 10, "f32", extra)
+        check(dx[sel], dref, dmag, 2 * n + 3 * r + 10, "f32", dextra)
+
+
+@pytest.mark.parametrize("m,n", [(600, 200), (3000, 1040)], ids=["single", "pairs"])
+@pytest.mark.parametrize("trans", [False, True], ids=["forward", "dx"])
+def test_lora_intermediate_holds_its_digits(ckl, m, n, trans):
+    """Nothing but the intermediate, in every binary order of magnitude from 2^-45 to 2^15: one rank with a 1
+    behind it and no shared weights.  Left of it: 2^-21 of its value (two words, the second one with a bit
+    less), 2^-46 (the last word's step), the FP32 result's own rounding, and 2^-23 of 2^-25, the least that
+    the tensor core takes a word in the middle unit for: 2^-48."""
+    k, r, g = 64, 24, 2
+    if trans:
+        k, n = n, k
+    x = torch.zeros(m, n if trans else k, dtype=torch.float16, device="cuda")
+    e = torch.randint(-24, 16, (m,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    x[:, 0] = (rand((m,), torch.float32, 2) * 2.0 ** e).clamp(-65504, 65504).half()
+    x[5, 0], x[6, 0] = 0.0, 2.0 ** -14
+    w = torch.zeros(k, n, dtype=torch.float16, device="cuda")
+    a, b = (torch.zeros(g, *s, dtype=torch.float16, device="cuda") for s in ((k, r), (r, n)))
+    small = torch.tensor([1.0, 1.375 * 2.0 ** -21], dtype=torch.float64)
+    s = torch.tensor([1.0, 2.0 ** -10], device="cuda")
+    first, second = (b, a) if trans else (a, b)
+    second.fill_(0.0)
+    for i in range(g):
+        first[i, 0, 0] = small[i] * 2.0 ** 10 if i else small[i]
+        if trans:
+            second[i, :, 0] = 1.0
+        else:
+            second[i, 0] = 1.0
+    ids = torch.arange(m, device="cuda", dtype=torch.int32) % g
+    offs, rows, _ = plan(ckl, ids, g)
+    size = ckl.gemm_lora_workspace_bytes(m, r, True)
+    ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    out = torch.full((m, k if trans else n), float("nan"), device="cuda")
+    if trans:
+        ckl.gemm_lora_backward(ckl.F16, x, None, w, a, b, s, out, ckl.F32, None, None, ckl.F32, offs, rows, g, m, n, k, r,
+                               ws, size)
+    else:
+        ckl.gemm_lora(ckl.F16, x, w, a, b, s, out, ckl.F32, offs, rows, g, m, n, k, r, ws, size)
+    t = x[:, 0].double() * torch.stack([first[i, 0, 0].double() * s[i].double() for i in range(g)])[ids.long()]
+    err = (out.double() - t.unsqueeze(1)).abs()
+    assert (err <= (t.abs() * (2.0 ** -21 + 2.0 ** -23) + 2.0 ** -46 + 2.0 ** -48).unsqueeze(1)).all()
+    assert (out[5] == 0).all()
