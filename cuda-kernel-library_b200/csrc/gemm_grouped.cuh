@@ -9,7 +9,7 @@
 //
 // kFormRows may be "extended": one B for all positions (a shared projection), and for the rows of
 // adapter g (offsets are then the adapters') T[p] * op(E_g) besides.
-//   kExtBlocks  before the k blocks of the product a tile runs, for each adapter whose rows it holds,
+//   kExtBlocks  besides the k blocks of the product a tile runs, for each adapter whose rows it holds,
 //               those of T and E_g into the same accumulator, the rows of other adapters read as
 //               zeros: no second pass over C, and no tiles cut at the borders of requests (which
 //               reads the shared weights again for each: 2000 rows, 30 adapters, 4096 x 4096:
@@ -153,7 +153,7 @@ struct GroupedTile {
     int cols;       // columns of the tile that exist
     int k_blocks;   // 64-wide blocks of the main product
     int ext_first, ext_last;  // kExtBlocks: adapters [first, last) that may have rows in the tile
-    int begin, end;  // this CTA's share of the tile's blocks (adapters, then the main product)
+    int begin, end;  // this CTA's share of the tile's blocks, in the order of for_blocks
     int finer;       // part in whose unit the share's sum ends up (FP16 passes), 0: the result's
 };
 
@@ -451,34 +451,55 @@ __device__ __forceinline__ uint4 layer_of(const uint4& a, const uint4& b, int pa
                       layer_of(a.w, b.w, part));
 }
 
-// Walks the blocks of a tile's adapters that fall into the share [begin, end): one pass per part, the
-// finest first, and in each the adapters that have rows in the tile, `per` blocks each.
-// f(part, adapter, span, block, first of its pass) returns false to stop.  Returns the number of
-// adapters' blocks of the whole tile, which the main product's follow, or -1 where f stopped.
+// Walks the blocks of a kFormRows tile that fall into the share [begin, end): main(kb) for those of the
+// product, ext(part, adapter, span, block, first of its pass) for those of the adapters that have rows in
+// the tile, `per` blocks each, one pass per part.  Either returns false to stop.
+// FP16 adapters come before the product and the finest part first, because each pass shifts what was
+// summed before it.  BF16 ones come behind it: an addition loses 2^-24 or so of what has been
+// summed, which at the beginning is little (4096 x 4096, rank 64: twice as many results rounded the
+// other way with the adapters in front).
 // (Kernels for products without adapters have kAdapters off and none of this.)
-template <bool kAdapters, typename Tile, typename F>
-__device__ __forceinline__ int for_adapter_blocks(const GroupedParams& p, const GroupedTable& table, const Tile& t,
-                                                  int per, int begin, int end, F&& f) {
+template <bool kAdapters, typename Tile, typename Ext, typename Main>
+__device__ __forceinline__ bool for_blocks(const GroupedParams& p, const GroupedTable& table, const Tile& t, int per,
+                                           int begin, int end, Ext&& ext, Main&& main) {
+    if constexpr (!kAdapters) {
+        for (int kb = begin; kb < min(end, t.k_blocks); ++kb) {
+            if (!main(kb)) {
+                return false;
+            }
+        }
+        return true;
+    }
     int at = 0;
-    if (kAdapters && t.ext_first < t.ext_last) {
-        for (int part = p.parts - 1; part >= 0; --part) {
-            bool first = true;
-            for (int g = t.ext_first; g < t.ext_last; ++g) {
-                const Span span = adapter_span(table, t, g);
-                if (span.lo >= span.hi) {
-                    continue;
+    const bool ext_first = p.fmt == 0;
+    for (int turn = 0; turn < 2; ++turn) {
+        if ((turn == 0) != ext_first) {
+            for (int kb = max(0, begin - at); kb < min(t.k_blocks, end - at); ++kb) {
+                if (!main(kb)) {
+                    return false;
                 }
-                for (int eb = max(0, begin - at); eb < min(per, end - at); ++eb) {
-                    if (!f(part, g, span, eb, first)) {
-                        return -1;
+            }
+            at += t.k_blocks;
+        } else if (t.ext_first < t.ext_last) {
+            for (int part = p.parts - 1; part >= 0; --part) {
+                bool first = true;
+                for (int g = t.ext_first; g < t.ext_last; ++g) {
+                    const Span span = adapter_span(table, t, g);
+                    if (span.lo >= span.hi) {
+                        continue;
                     }
-                    first = false;
+                    for (int eb = max(0, begin - at); eb < min(per, end - at); ++eb) {
+                        if (!ext(part, g, span, eb, first)) {
+                            return false;
+                        }
+                        first = false;
+                    }
+                    at += per;
                 }
-                at += per;
             }
         }
     }
-    return at;
+    return true;
 }
 
 // One 16-byte unit of row c_row of C: `have` of its columns exist, v holds the raw sums.
@@ -1020,7 +1041,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                 };
                 if (p.form == kFormRows) {
                     const int group = kAdapters || table.whole ? 0 : t.group;
-                    const int before = detail::for_adapter_blocks<kAdapters>(
+                    ok = detail::for_blocks<kAdapters>(
                         p, table, t, ext_blocks, t.begin, t.end,
                         [&](int, int g, const detail::Span&, int eb, bool) -> bool {
                             if (!acquire_stage(b_bytes, !every)) {
@@ -1030,25 +1051,21 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                                    eb * 64, g);
                             advance();
                             return true;
+                        },
+                        [&](int kb) -> bool {
+                            if (!acquire_stage(b_bytes + (gather_a ? 0u : Cfg::kABytes), false)) {
+                                return false;
+                            }
+                            const uint32_t a_dst = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
+                            if (!gather_a) {
+                                // Rows behind the tile's last one belong to the next group (or lie
+                                // outside A): computed with and not stored.
+                                ptx::tma_load_2d(a_dst, &tmap_a_box, full_bar(stage), kb * 64, t.p0);
+                            }
+                            load_b(a_dst + Cfg::kABytes, &tmap_b_box, kb * 64, group);
+                            advance();
+                            return true;
                         });
-                    if (before < 0) {
-                        ok = false;
-                        break;
-                    }
-                    for (int kb = max(0, t.begin - before); kb < min(t.k_blocks, t.end - before); ++kb) {
-                        if (!acquire_stage(b_bytes + (gather_a ? 0u : Cfg::kABytes), false)) {
-                            ok = false;
-                            break;
-                        }
-                        const uint32_t a_dst = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
-                        if (!gather_a) {
-                            // Rows behind the tile's last one belong to the next group (or lie
-                            // outside A): computed with and not stored.
-                            ptx::tma_load_2d(a_dst, &tmap_a_box, full_bar(stage), kb * 64, t.p0);
-                        }
-                        load_b(a_dst + Cfg::kABytes, &tmap_b_box, kb * 64, group);
-                        advance();
-                    }
                 } else {
                     // Weight gradient: 64 positions per block, both operands MN-major.
                     const int row_blocks = (t.valid + 63) / 64;
@@ -1174,16 +1191,16 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                     return true;
                 };
                 const int row_blocks = a_mn ? (t.valid + 63) / 64 : 0;
-                const int before = detail::for_adapter_blocks<kAdapters>(
-                    p, table, t, ext_blocks, t.begin, t.end, [&](int, int, const detail::Span&, int eb, bool first) {
+                ok = detail::for_blocks<kAdapters>(
+                    p, table, t, ext_blocks, t.begin, t.end,
+                    [&](int, int, const detail::Span&, int eb, bool first) {
                         return block(min(4, (p.ext_cols - eb * 64) / 16), true, shifts && first);
+                    },
+                    [&](int kb) {
+                        const int in_pass = a_mn ? kb - pass_of(kb, row_blocks) * row_blocks : 0;
+                        const bool tail = a_mn && (t.valid & 63) != 0 && in_pass + 1 == row_blocks;
+                        return block(4, gather_a || gather_b || tail, a_mn && shifts && in_pass == 0);
                     });
-                ok = before >= 0;
-                for (int kb = max(0, t.begin - before); ok && kb < min(t.k_blocks, t.end - before); ++kb) {
-                    const int in_pass = a_mn ? kb - pass_of(kb, row_blocks) * row_blocks : 0;
-                    const bool tail = a_mn && (t.valid & 63) != 0 && in_pass + 1 == row_blocks;
-                    ok = block(4, gather_a || gather_b || tail, a_mn && shifts && in_pass == 0);
-                }
                 if (ok) {
                     if (accumulate != 0) {
                         ptx::umma_commit(acc_full_bar(acc));
@@ -1264,7 +1281,7 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         src[q] = at < p.a_count ? at : -1;
                     }
                 }
-                const int before = detail::for_adapter_blocks<kAdapters>(
+                ok = detail::for_blocks<kAdapters>(
                     p, table, t, ext_blocks, t.begin, t.end,
                     [&](int part, int, const detail::Span& span, int eb, bool) -> bool {
                         if (static_cast<int>(it++ % kStages) != own) {
@@ -1276,22 +1293,20 @@ grouped_gemm_kernel(const __grid_constant__ GroupedProblems problems) {
                         load.adapter_rows(0, p, t.p0, t.valid, span.lo, span.hi, part, eb * 64);
                         hand_over();
                         return true;
+                    },
+                    [&](int kb) -> bool {
+                        const bool mine = gather_a && static_cast<int>(it % kStages) == own;
+                        ++it;
+                        if (!mine) {
+                            return true;
+                        }
+                        if (!acquire()) {
+                            return false;
+                        }
+                        load.rows128(0, p.a, p.lda, src, t.valid, kb * 64, p.k);
+                        hand_over();
+                        return true;
                     });
-                if (before < 0) {
-                    ok = false;
-                    break;
-                }
-                for (int kb = max(0, t.begin - before); kb < min(t.k_blocks, t.end - before); ++kb, ++it) {
-                    if (!gather_a || static_cast<int>(it % kStages) != own) {
-                        continue;
-                    }
-                    if (!acquire()) {
-                        ok = false;
-                        break;
-                    }
-                    load.rows128(0, p.a, p.lda, src, t.valid, kb * 64, p.k);
-                    hand_over();
-                }
             } else {
                 const int row_blocks = (t.valid + 63) / 64;
                 const int a_boxes = (min(128, p.m - t.m0) + 63) / 64;

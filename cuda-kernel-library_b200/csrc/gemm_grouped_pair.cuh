@@ -283,7 +283,7 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                     const int row0 = t.p0 + static_cast<int>(rank) * t.half;
                     const int row_boxes = gather ? 0 : (t.half + 63) / 64;
                     const uint32_t rows_bytes = 2u * static_cast<uint32_t>(row_boxes) * Cfg::kBoxBytes;
-                    const int before = detail::for_adapter_blocks<kExt>(
+                    ok = detail::for_blocks<kExt>(
                         p, table, t, ext_blocks, 0, 0x7fffffff,
                         [&](int, int g, const detail::Span&, int eb, bool) -> bool {
                             if (!acquire_stage(cols_bytes, !gather)) {
@@ -292,28 +292,24 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                             load_cols(ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes, &tmap_ext, eb * 64, g);
                             advance();
                             return true;
-                        });
-                    if (before < 0) {
-                        ok = false;
-                        break;
-                    }
-                    for (int kb = 0; kb < t.k_blocks; ++kb) {
-                        if (!acquire_stage(cols_bytes + rows_bytes, false)) {
-                            ok = false;
-                            break;
-                        }
-                        const uint32_t dst = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
-                        load_cols(dst, &tmap_cols, kb * 64, group);
-                        // rows behind the tile's last are another tile's, or zeros: not stored
-#pragma unroll
-                        for (int b = 0; b < 2; ++b) {
-                            if (b < row_boxes) {
-                                ptx::tma_load_2d_pair(dst + Cfg::kColsBytes + b * Cfg::kBoxBytes, &tmap_rows, bar,
-                                                      kb * 64, row0 + b * 64);
+                        },
+                        [&](int kb) -> bool {
+                            if (!acquire_stage(cols_bytes + rows_bytes, false)) {
+                                return false;
                             }
-                        }
-                        advance();
-                    }
+                            const uint32_t dst = ring + static_cast<uint32_t>(stage) * Cfg::kStageBytes;
+                            load_cols(dst, &tmap_cols, kb * 64, group);
+                            // rows behind the tile's last are another tile's, or zeros: not stored
+#pragma unroll
+                            for (int b = 0; b < 2; ++b) {
+                                if (b < row_boxes) {
+                                    ptx::tma_load_2d_pair(dst + Cfg::kColsBytes + b * Cfg::kBoxBytes, &tmap_rows, bar,
+                                                          kb * 64, row0 + b * 64);
+                                }
+                            }
+                            advance();
+                            return true;
+                        });
                 } else {
                     const int row0 = t.r0 + static_cast<int>(rank) * t.half;
                     // boxes of 64 rows of W_g (columns of A) that exist, of this CTA and of both
@@ -434,14 +430,12 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                     }
                     return true;
                 };
-                ok = detail::for_adapter_blocks<kExt>(
-                         p, table, t, ext_blocks, 0, 0x7fffffff,
-                         [&](int, int, const detail::Span&, int eb, bool first) {
-                             return block(min(4, (p.ext_cols - eb * 64) / 16), true, shifts && first);
-                         }) >= 0;
-                for (int kb = 0; ok && kb < t.k_blocks; ++kb) {
-                    ok = block(4, gather || (wgrad && t.valid - kb * 64 < 64), false);
-                }
+                ok = detail::for_blocks<kExt>(
+                    p, table, t, ext_blocks, 0, 0x7fffffff,
+                    [&](int, int, const detail::Span&, int eb, bool first) {
+                        return block(min(4, (p.ext_cols - eb * 64) / 16), true, shifts && first);
+                    },
+                    [&](int kb) { return block(4, gather || (wgrad && t.valid - kb * 64 < 64), false); });
                 if (ok) {
                     if (accumulate != 0) {
                         ptx::umma_commit_pair_both(acc_full_bar(acc));
@@ -516,7 +510,7 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                         src[q] = at < p.a_count ? at : -1;
                     }
                 }
-                const int before = detail::for_adapter_blocks<kExt>(
+                ok = detail::for_blocks<kExt>(
                     p, table, t, ext_blocks, 0, 0x7fffffff,
                     [&](int part, int, const detail::Span& span, int eb, bool) -> bool {
                         if (static_cast<int>(it++ % kStages) != own) {
@@ -528,22 +522,20 @@ grouped_pair_kernel(const __grid_constant__ GroupedProblem problem) {
                         load.adapter_rows(Cfg::kColsBytes, p, t.p0 + first_row, rows, span.lo, span.hi, part, eb * 64);
                         hand_over();
                         return true;
+                    },
+                    [&](int kb) -> bool {
+                        const bool mine = gather && static_cast<int>(it % kStages) == own;
+                        ++it;
+                        if (!mine) {
+                            return true;
+                        }
+                        if (!acquire()) {
+                            return false;
+                        }
+                        load.rows128(Cfg::kColsBytes, p.a, p.lda, src, rows, kb * 64, p.k);
+                        hand_over();
+                        return true;
                     });
-                if (before < 0) {
-                    ok = false;
-                    break;
-                }
-                for (int kb = 0; kb < t.k_blocks; ++kb, ++it) {
-                    if (!gather || static_cast<int>(it % kStages) != own) {
-                        continue;
-                    }
-                    if (!acquire()) {
-                        ok = false;
-                        break;
-                    }
-                    load.rows128(Cfg::kColsBytes, p.a, p.lda, src, rows, kb * 64, p.k);
-                    hand_over();
-                }
             } else {
                 const int first = (own - static_cast<int>(it % kStages) + kStages) % kStages;
                 int next[2];
