@@ -827,21 +827,30 @@ def test_grouped_pairs_half_a_tile_of_columns(ckl):
         check(first[o[g]:o[g + 1]], x @ w, x.abs() @ w.abs(), k, "f32")
 
 
-def test_lora_rows_in_place_many_times(ckl):
-    """Rows already in adapter order: only the adapters' blocks pass through the loader warps."""
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_lora_rows_in_place_many_times(ckl, dt):
+    """Rows already in adapter order: only the adapters' blocks pass through the loader warps.  The gradients
+    have the bits that an explicit order gives."""
     g, r = 5, 24
     for m, k, n in ((300, 1032, 328), (3000, 1032, 1040)):
         ids = torch.sort(torch.randint(0, g, (m,), device="cuda", dtype=torch.int32)).values.int()
-        m, x, w, a, b, s, offs, _ = lora_case(ckl, ids, g, k, n, r, "bf16", 140)
-        size = ckl.gemm_lora_workspace_bytes(m, r)
+        m, x, w, a, b, s, offs, order = lora_case(ckl, ids, g, k, n, r, dt, 140)
+        assert torch.equal(order, torch.arange(m, dtype=torch.int32, device="cuda"))
+        size = ckl.gemm_lora_workspace_bytes(m, r, True)
         ws = torch.empty(size, dtype=torch.uint8, device="cuda")
         first, y = (torch.empty(m, n, device="cuda") for _ in range(2))
         same = torch.ones((), dtype=torch.bool, device="cuda")
         for i in range(200):
             out = y if i else first
-            ckl.gemm_lora(ckl.BF16, x, w, a, b, s, out, ckl.F32, offs, None, g, m, n, k, r, ws, size)
+            ckl.gemm_lora(code(ckl, dt), x, w, a, b, s, out, ckl.F32, offs, None, g, m, n, k, r, ws, size)
             same &= (out == first).all()
         assert bool(same)
+        dy = rand((m, n), DT[dt], 145)
+        grads = [[torch.empty(t.shape, device="cuda") for t in (x, a, b)] for _ in range(2)]
+        for (dx, da, db), rows in zip(grads, (None, order)):
+            ckl.gemm_lora_backward(code(ckl, dt), dy, x, w, a, b, s, dx, ckl.F32, da, db, ckl.F32, offs, rows, g, m, n, k,
+                                   r, ws, size)
+        assert all(torch.equal(p, q) for p, q in zip(*grads))
         f = s[ids.long()].double().unsqueeze(1)
         t, ta = torch.zeros(m, r, dtype=torch.float64, device="cuda"), torch.zeros(m, r, dtype=torch.float64, device="cuda")
         ref, mag = x.double() @ w.double(), x.double().abs() @ w.double().abs()
@@ -851,7 +860,7 @@ def test_lora_rows_in_place_many_times(ckl):
             t, ta = f[sel] * (x[sel].double() @ a[i].double()), f[sel] * (x[sel].double().abs() @ a[i].double().abs())
             ref[sel] += t @ b[i].double()
             mag[sel] += ta @ b[i].double().abs()
-            extra[sel] = TWO_PART["bf16"] * (t.abs() @ b[i].double().abs())
+            extra[sel] = TWO_PART[dt] * (t.abs() @ b[i].double().abs())
         check(first, ref, mag, 2 * k + 2 * r + 10, "f32", extra)
 
 
