@@ -959,3 +959,26 @@ def test_lora_intermediate_holds_its_digits(ckl, m, n, trans):
     err = (out.double() - t.unsqueeze(1)).abs()
     assert (err <= (t.abs() * (2.0 ** -21 + 2.0 ** -23) + 2.0 ** -46 + 2.0 ** -48).unsqueeze(1)).all()
     assert (out[5] == 0).all()
+
+
+@pytest.mark.parametrize("gather", [False, True], ids=["rows", "gather"])
+def test_wait_that_runs_out_is_reported_by_pairs(ckl, gather):
+    """A stage that never fills: both CTAs of every pair leave, the status says so, and the next call is right."""
+    sizes, n, k = [300, 5, 256, 1000] * 10, 296, 264
+    offs, rows = offsets_of(sizes), sum(sizes)
+    a, b = rand((rows, k), torch.float16, 1), rand((40, k, n), torch.float16, 2, k ** -0.5)
+    idx = torch.arange(rows, dtype=torch.int32, device="cuda") if gather else None
+    c = torch.empty(rows, n, device="cuda")
+    args = (ckl.F16, a, b, c, ckl.F32, offs, 40, rows, n, k)
+    torch.cuda.synchronize()
+    ckl.arm_wait_fault(1, 50_000_000)
+    ckl.gemm_grouped(*args, a_rows=idx, a_count=rows)
+    with pytest.raises(ckl.CklError) as e:
+        ckl.device_status()
+    assert e.value.status == ckl.ERR_DEVICE
+    ckl.gemm_grouped(*args, a_rows=idx, a_count=rows)
+    torch.cuda.synchronize()
+    o = offs.tolist()
+    for g in range(40):
+        x, w = a[o[g]:o[g + 1]].double(), b[g].double()
+        check(c[o[g]:o[g + 1]], x @ w, x.abs() @ w.abs(), k, "f32")
