@@ -19,6 +19,7 @@ LIB = os.path.join(HERE, "libckl_gemm.so")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",
+    "--threads", "0",  # the sources side by side: the routed products alone take two minutes
     "-Xcompiler", "-fPIC", "-shared",
 ]
 

@@ -565,7 +565,7 @@ __device__ __forceinline__ void store_unit(const GroupedParams& p,
 // eight lanes a row, kBatch rows a lane in flight.
 template <int kBatch>
 __device__ __forceinline__ void store_layer(uint32_t dst, const unsigned short* from, int ld, int second, int row0,
-                                         int rows, int lo, int hi, int units, int part) {
+                                            int rows, int lo, int hi, int units, int part) {
     const int lane = static_cast<int>(threadIdx.x & 31);
     const int shift = units <= 2 ? 1 : units <= 4 ? 2 : 3;
     const int unit = lane & ((1 << shift) - 1), sub = lane >> shift, step = 32 >> shift;
@@ -599,6 +599,8 @@ __device__ __forceinline__ void store_layer(uint32_t dst, const unsigned short* 
 // 16-byte unit), four rows per instruction; a unit's place under the 128-byte swizzle depends on
 // the row modulo 8.  Shuffles and copies go in batches of eight: one after the other each pair
 // would cost its full latency (110 cycles).
+// kBatch: rows of a two-word matrix that a lane has in flight; 4 in the split kernel, whose warps have 128
+// registers a thread.
 template <int kBatch>
 struct Loader {
     uint32_t stage;      // shared address
@@ -672,8 +674,8 @@ struct Loader {
         const int col = k0 + unit * 8;
         const bool exists = col < p.ext_cols;
         if (p.fmt == 0) {
-            store_layer<kBatch>(stage + offset, static_cast<const unsigned short*>(p.t) + k0, p.ldt, p.ext_cols, pos0,
-                        (rows + 31) / 32 * 32, lo, hi, min(8, (p.ext_cols - k0) / 8), part);
+            store_layer<kBatch>(stage + offset, static_cast<const unsigned short*>(p.t) + k0, p.ldt, p.ext_cols,
+                                pos0, (rows + 31) / 32 * 32, lo, hi, min(8, (p.ext_cols - k0) / 8), part);
             return;
         }
         const char* base = static_cast<const char*>(p.t) +
@@ -700,8 +702,8 @@ struct Loader {
                                               int boxes, int col0, int part_cols, int part) const {
         for (int box = 0; box < boxes; ++box) {
             const int col = col0 + box * 64;
-            store_layer<kBatch>(stage + offset + box * 8192u, static_cast<const unsigned short*>(from) + col, ld, part_cols,
-                        row0, 64, row0, row0 + left, min(8, (part_cols - col) / 8), part);
+            store_layer<kBatch>(stage + offset + box * 8192u, static_cast<const unsigned short*>(from) + col, ld,
+                                part_cols, row0, 64, row0, row0 + left, min(8, (part_cols - col) / 8), part);
         }
     }
 
