@@ -234,7 +234,10 @@ int describe(Product& q, GroupedProblem* out) {
         const int bytes = size_of(q.c_dtype);
         p.c_vec = !misaligned(p.c, 16) && (static_cast<long long>(p.ldc) * bytes) % 16 == 0 &&
                   (p.c_stride * bytes) % 16 == 0;
-        p.c_tma = p.c_vec && p.beta == 0.0f && p.c_rows == nullptr && p.split == 1;
+        // A TMA store writes whole 16-byte units: columns that end inside one would take what lies
+        // behind them along (measured: up to 7 columns of zeros in a wider matrix).
+        p.c_tma = p.c_vec && (static_cast<long long>(p.n) * bytes) % 16 == 0 && p.beta == 0.0f &&
+                  p.c_rows == nullptr && p.split == 1;
         if (p.c_tma) {
             GRP_TRY(encode_operand(&out->c, q.c_dtype, p.c, p.n, wgrad ? p.m : p.rows, p.ldc, wgrad ? p.groups : 1,
                                    wgrad ? p.c_stride : static_cast<long long>(p.ldc) * p.rows,

@@ -982,3 +982,52 @@ def test_wait_that_runs_out_is_reported_by_pairs(ckl, gather):
     for g in range(40):
         x, w = a[o[g]:o[g + 1]].double(), b[g].double()
         check(c[o[g]:o[g + 1]], x @ w, x.abs() @ w.abs(), k, "f32")
+
+
+@pytest.mark.parametrize("out", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [57, 62, 257, 611])
+def test_columns_that_end_inside_16_bytes(ckl, out, n):
+    """Results in a wider matrix whose rows begin on 16-byte boundaries: the columns behind them stay."""
+    ldn = (n + 7) // 8 * 8 + 8
+    for sizes, k in (([300, 5, 64], 72), ([300, 5, 256, 1000] * 10, 136), ([40], 2048)):
+        g, rows, offs = len(sizes), sum(sizes), offsets_of(sizes)
+        a, b = rand((rows, k), DT["f16"], 1), rand((g, k, ldn), DT["f16"], 2, k ** -0.5)
+        c = torch.full((rows, ldn), 7.0, dtype=DT[out], device="cuda")
+        ckl.gemm_grouped(ckl.F16, a, b, c, code(ckl, out), offs, g, rows, n, k, ldb=ldn, ldc=ldn)
+        assert (c[:, n:] == 7.0).all()
+        o = offs.tolist()
+        for i in range(g):
+            x, w = a[o[i]:o[i + 1]].double(), b[i, :, :n].double()
+            check(c[o[i]:o[i + 1], :n], x @ w, x.abs() @ w.abs(), k + 10, out)
+        for m in (72, 520):
+            x, d = rand((rows, m), DT["f16"], 3), rand((rows, ldn), DT["f16"], 4)
+            dw = torch.full((g, m, ldn), 7.0, dtype=DT[out], device="cuda")
+            ckl.gemm_grouped_wgrad(ckl.F16, x, d, dw, code(ckl, out), offs, g, rows, m, n, ldg=ldn, lddw=ldn)
+            assert (dw[:, :, n:] == 7.0).all()
+            for i in range(g):
+                u, v = x[o[i]:o[i + 1]].double(), d[o[i]:o[i + 1], :n].double()
+                check(dw[i, :, :n], u.t() @ v, u.abs().t() @ v.abs(), sizes[i] + 10, out)
+
+
+@pytest.mark.parametrize("m", [5, 300, 3000])
+def test_adapters_that_end_inside_16_bytes(ckl, m):
+    """The same of the adapters' outputs: y, the gradient of x, and gradients of rank 13."""
+    g, k, n, r = 4, 131, 611, 13
+    ids = torch.arange(m, device="cuda", dtype=torch.int32) % g
+    offs, rows, _ = plan(ckl, ids, g)
+    ldk, ldn, ldr = 136, 616, 16
+    x, w, dy = rand((m, ldk), DT["bf16"], 1), rand((k, ldn), DT["bf16"], 2), rand((m, ldn), DT["bf16"], 3)
+    a, b = rand((g, k, ldr), DT["bf16"], 4), rand((g, r, ldn), DT["bf16"], 5)
+    y, dx = torch.full((m, ldn), 7.0, device="cuda"), torch.full((m, ldk), 7.0, device="cuda")
+    da, db = torch.full((g, k, ldr), 7.0, device="cuda"), torch.full((g, r, ldn), 7.0, device="cuda")
+    size = ckl.gemm_lora_workspace_bytes(m, r, True)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    ld = dict(ldx=ldk, ldw=ldn, ldla=ldr, ldlb=ldn)
+    for order in (rows, None):
+        ckl.gemm_lora(ckl.BF16, x, w, a, b, None, y, ckl.F32, offs, order, g, m, n, k, r, ws, size, ldy=ldn, **ld)
+        ckl.gemm_lora_backward(ckl.BF16, dy, x, w, a, b, None, dx, ckl.F32, da, db, ckl.F32, offs, order, g, m, n, k, r, ws,
+                               size, lddy=ldn, lddx=ldk, ldda=ldr, lddb=ldn, **ld)
+        assert (y[:, n:] == 7.0).all() and (dx[:, k:] == 7.0).all()
+        assert (da[:, :, r:] == 7.0).all() and (db[:, :, n:] == 7.0).all()
+        for t, end in ((y, n), (dx, k), (da, r), (db, n)):
+            assert torch.isfinite(t[..., :end]).all() and not (t[..., :end] == 7.0).all()
