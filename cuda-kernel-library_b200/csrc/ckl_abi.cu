@@ -859,13 +859,16 @@ int gemm_impl(int ab_dtype, const void* a, const void* b, void* c, int c_dtype, 
 
     // Operands TMA cannot describe travel through aligned copies in this stream's scratch
     // (grown on demand, reused by later calls on the stream: stream order keeps a later copy
-    // from overwriting what an earlier GEMM still reads).  The same goes for a C whose base or
-    // pitch rules out 16-byte accesses on a large problem: the kernel writes an aligned copy
+    // from overwriting what an earlier GEMM still reads).  The same goes for a C whose base, pitch
+    // or last column rules out 16-byte accesses on a large problem: the kernel writes an aligned copy
     // through its TMA epilogue and one pass copies it out, instead of the register-store
     // epilogue's 2-byte stores (C_in is copied in first when it is read).
     const size_t csz = dtype_size(c_dtype);
-    const bool c_aligned =
-        reinterpret_cast<uintptr_t>(c) % 16 == 0 && (static_cast<size_t>(ldc) * csz) % 16 == 0;
+    // A TMA store writes whole 16-byte units: columns that end inside one would take up to 7 columns
+    // of a wider matrix along.
+    const bool whole_units = (static_cast<size_t>(n) * csz) % 16 == 0;
+    const bool c_aligned = whole_units && reinterpret_cast<uintptr_t>(c) % 16 == 0 &&
+                           (static_cast<size_t>(ldc) * csz) % 16 == 0;
     const bool stage_c = algo == CKL_ALGO_AUTO && !c_aligned &&
                          static_cast<long long>(m) * n * static_cast<long long>(k) >= kRepackMinMacs;
     void* c_user = c;
@@ -951,10 +954,11 @@ int gemm_impl(int ab_dtype, const void* a, const void* b, void* c, int c_dtype, 
                   : 0;
     p.epi_mode = epi;
     // The coalesced epilogue moves C through TMA (32-row x 128-byte boxes); it needs the
-    // same alignment as the vector path.  Otherwise the kernel stores from registers.
+    // same alignment as the vector path, and rows that end with a unit or in a copy, whose padding is
+    // nobody's.  Otherwise the kernel stores from registers.
     CUtensorMap tc;
     std::memset(&tc, 0, sizeof tc);
-    p.c_tma = p.c_vec;
+    p.c_tma = p.c_vec != 0 && (whole_units || stage_c) ? 1 : 0;
     if (p.c_tma) {
         if (const int rc = encode_2d(ctx, &tc, c_dtype, c, static_cast<uint64_t>(n),
                                      static_cast<uint64_t>(m), static_cast<uint64_t>(ldc),

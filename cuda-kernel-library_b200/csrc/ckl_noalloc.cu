@@ -255,7 +255,8 @@ int ckl_gemm_streamk_noalloc(int ab_dtype, const void* a, const void* b, void* c
     p.c_vec = (reinterpret_cast<uintptr_t>(c) % 16 == 0 && (static_cast<size_t>(ldc) * csz) % 16 == 0)
                   ? 1
                   : 0;
-    p.c_tma = p.c_vec;
+    // (a TMA store writes whole 16-byte units, also behind the last column)
+    p.c_tma = p.c_vec != 0 && (static_cast<size_t>(n) * csz) % 16 == 0 ? 1 : 0;
     if (p.c_tma) {
         if (int rc = encode(*st, &tc, c_dtype, c, static_cast<uint64_t>(n), static_cast<uint64_t>(m),
                             static_cast<uint64_t>(ldc), static_cast<uint32_t>(128 / csz), 32);
